@@ -611,6 +611,102 @@ int lc_jit_pointwise(const void *image, size_t image_size, const lc_pw_program *
 int lc_jit_rowprog(const void *image, size_t image_size, const lc_pw_program *program,
                    const lc_rp_layout *layout, void *const *buffers, void *stream);
 
+/* ---------------------------------------------------------------- serving
+ * Attention of prompts and of single new tokens, and the page operations of the
+ * key-value cache between them.  No reference counterpart (its attention
+ * packages are whole, unmasked and without a cache).
+ *
+ * A query at position p sees key j when j <= p and (window == 0, or
+ * j > p - window, or j < sinks): causal, with an optional sliding window and
+ * `sinks` first tokens that stay visible.  A row that sees nothing has output 0
+ * and log-sum-exp -infinity.  dtype is LC_F16 or LC_BF16 (operands and output;
+ * softmax statistics and sums are f32).  q_heads is a multiple of kv_heads:
+ * query head h reads key-value head h / (q_heads / kv_heads).  Head sizes up to
+ * 256; the innermost axis is contiguous, `strides` are host arrays of element
+ * (attention) or byte (page operations) strides.  lse may be null; it is f32
+ * and contiguous.  What masked or absent tokens hold does not matter (infinities
+ * and NaN included). */
+
+/* o[b, i, h, :] = sum_j softmax_j(scale q[b, i, h] . k[b, j, h / g]) v[b, j, h / g, :].
+ * Sequence b has q_lens[b] queries (null: s_q) and kv_lens[b] keys (null: s_kv),
+ * at the start of their rows of the buffers; query i is at position
+ * kv_lens[b] - q_lens[b] + i.  Rows from q_lens[b] on are written as empty.
+ * lse is [batch, q_heads, s_q].  strides: batch, token and head of q, of k, of v
+ * and of o (12 values). */
+int lc_window_attention(int dtype, const void *q, const void *k, const void *v, void *o, float *lse,
+                        const int32_t *q_lens, const int32_t *kv_lens, int64_t batch, int64_t s_q,
+                        int64_t s_kv, int64_t q_heads, int64_t kv_heads, int64_t d,
+                        const int64_t *strides, int64_t window, int64_t sinks, float scale,
+                        void *stream);
+
+/* One new token per slot: q[slots, q_heads, d] at position lens[slot] - 1 over the
+ * slot's lens[slot] cached tokens (its own among them).  Token j is row
+ * j % page_size of page table[slot, j / page_size]; lens beyond width * page_size
+ * are cut there, table entries outside [0, pages) count as not visible.
+ * lse is [slots, q_heads].  strides: q slot, head; k page, head, token; v page,
+ * head, token; o slot, head; table slot (11 values). */
+int lc_paged_decode(int dtype, const void *q, const void *k, const void *v, void *o, float *lse,
+                    const int32_t *table, const int32_t *lens, int64_t slots, int64_t width,
+                    int64_t pages, int64_t page_size, int64_t q_heads, int64_t kv_heads, int64_t d,
+                    const int64_t *strides, int64_t window, int64_t sinks, float scale, void *stream);
+
+/* The maps of a cache: table[slots, width] (contiguous; -1: no page), lens[slots],
+ * refs[pages] (how many sequences hold the page; 0: free).  The operations below
+ * read one set of maps and write another, which may be the same one except for
+ * lc_cache_fork.  status[0]: 0, or -1 (an argument out of range), or how many
+ * pages were missing; where it is not 0 the maps are those before.  status[1]:
+ * the pages free afterwards. */
+
+/* Room for add[i] >= 0 more tokens in slot i: the lowest-numbered free pages, in
+ * slot order and then in order of position; lens grow by add. */
+int lc_cache_extend(const int32_t *table_in, int32_t *table_out, const int32_t *lens_in,
+                    int32_t *lens_out, const int32_t *refs_in, int32_t *refs_out, const int32_t *add,
+                    int32_t *status, int64_t slots, int64_t width, int64_t pages, int64_t page_size,
+                    void *stream);
+
+/* Writes the keys and values of the newest add[i] <= most tokens of each slot
+ * (k, v [slots, most, kv_heads, row_bytes]) to positions lens[i] - add[i] and on.
+ * Tokens without a page are skipped.  strides, in bytes: slot, token, head of k
+ * and of v; page, head, token of k_pages and of v_pages (12 values). */
+int lc_cache_write(const void *k, const void *v, void *k_pages, void *v_pages, const int32_t *table,
+                   const int32_t *lens, const int32_t *add, int64_t slots, int64_t most, int64_t width,
+                   int64_t pages, int64_t page_size, int64_t kv_heads, int64_t row_bytes,
+                   const int64_t *strides, void *stream);
+
+/* Slot i continues as slot parent[i] was (-1: it is dropped).  Full pages are
+ * shared; a last page that is not full stays with the lowest slot of its parent,
+ * the others get the lowest-numbered free page, in slot order, with the tokens
+ * held.  pool: `planes` x pages x kv_heads x page_size x token_bytes, tokens of a
+ * head contiguous; strides, in bytes: plane, page, head (3 values). */
+int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes,
+                  const int64_t *strides, const int32_t *table_in, int32_t *table_out,
+                  const int32_t *lens_in, int32_t *lens_out, const int32_t *refs_in, int32_t *refs_out,
+                  const int32_t *parent, int32_t *status, int64_t slots, int64_t width, int64_t pages,
+                  int64_t page_size, void *stream);
+
+/* Gives pages back, in place: of every slot with gone[i] != 0, which is empty
+ * afterwards; or, gone null, the pages that no position from lens[i] on sees
+ * under this window and sinks (their table entries become -1). */
+int lc_cache_release(int32_t *table, int32_t *lens, int32_t *refs, const int32_t *gone, int64_t window,
+                     int64_t sinks, int32_t *status, int64_t slots, int64_t width, int64_t pages,
+                     int64_t page_size, void *stream);
+
+/* Moves the pages in use onto the lowest numbers: with U in use, the r-th page in
+ * use from number U on moves into the r-th free one below U; tables and refs
+ * follow.  Pool and strides as in lc_cache_fork. */
+int lc_cache_compact(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes,
+                     const int64_t *strides, const int32_t *table_in, int32_t *table_out,
+                     const int32_t *lens_in, int32_t *lens_out, const int32_t *refs_in,
+                     int32_t *refs_out, int32_t *status, int64_t slots, int64_t width, int64_t pages,
+                     int64_t page_size, void *stream);
+
+/* Copies page src[i] to page dst[i] in every plane, i < n (device arrays; no page
+ * may be a destination twice, or both source and destination).  Pairs outside
+ * [0, pages) are skipped. */
+int lc_cache_copy(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes,
+                  const int64_t *strides, const int32_t *src, const int32_t *dst, int64_t n,
+                  int64_t pages, int64_t page_size, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -72,6 +72,14 @@ SIGNATURES = {
     "lc_selftest_bounded_wait": [_I64, _P],
     "lc_sdpa_f16": [_P, _P, _P, _P, _I64, _I64, _I64, _I64, ctypes.c_float, _P],
     "lc_sdpa_path": [_P, _P, _P, _P, _I64, _I64, _I64],
+    "lc_window_attention": [_INT] + [_P] * 7 + [_I64] * 6 + [_P, _I64, _I64, ctypes.c_float, _P],
+    "lc_paged_decode": [_INT] + [_P] * 7 + [_I64] * 7 + [_P, _I64, _I64, ctypes.c_float, _P],
+    "lc_cache_extend": [_P] * 8 + [_I64] * 4 + [_P],
+    "lc_cache_write": [_P] * 7 + [_I64] * 7 + [_P, _P],
+    "lc_cache_fork": [_P, _I64, _I64, _I64, _P] + [_P] * 8 + [_I64] * 4 + [_P],
+    "lc_cache_release": [_P] * 4 + [_I64, _I64, _P] + [_I64] * 4 + [_P],
+    "lc_cache_compact": [_P, _I64, _I64, _I64, _P] + [_P] * 7 + [_I64] * 4 + [_P],
+    "lc_cache_copy": [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P],
 }
 
 # pointwise programs (include/lazyb200.h lc_pw_program)
