@@ -102,6 +102,18 @@ __device__ __forceinline__ void store_row(const RowState &st, T *o, float *lse, 
   if (lse && lane == 0) *lse = st.l == 0.f ? -INFINITY : (st.m + log2f(st.l)) * kLn2;
 }
 
+// The same row for a kernel whose own sums came out infinite or NaN in some
+// columns: those alone are written, the others keep their bits.
+template <class T>
+__device__ __forceinline__ void mend_row(const RowState &st, T *o, int d, int lane) {
+  const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
+#pragma unroll
+  for (int i = 0; i < kMaxHead / 32; ++i) {
+    const int c = lane + 32 * i;
+    if (c < d && !isfinite(Elem<T>::to_float(o[c]))) o[c] = Elem<T>::from_float(st.acc[i] * inv);
+  }
+}
+
 // Joins the states of the WARPS warps of a CTA, which each took a share of one
 // row's keys, in warp order; warp 0 receives the row.
 template <int WARPS>

@@ -85,7 +85,7 @@ int reduce_workspace(cudaStream_t stream, ReduceWorkspace *out) {
   return LC_OK;
 }
 
-int scratch_buffer(cudaStream_t stream, int slot, size_t bytes, void **out) {
+static int scratch_of(cudaStream_t stream, int slot, size_t bytes, bool zeroed, void **out) {
   int dev = 0;
   if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
   std::lock_guard<std::mutex> lock(g_mutex);
@@ -103,11 +103,26 @@ int scratch_buffer(cudaStream_t stream, int slot, size_t bytes, void **out) {
       cudaGetLastError();
       return fail(LC_ERR_NOMEM, "scratch: cudaMalloc(%zu) failed", bytes);
     }
+    // a synchronous memset: the zeros are there before any kernel of any stream reads them
+    if (zeroed) {
+      if (int rc = check_cuda(cudaMemset(mem, 0, bytes), "scratch: memset")) {
+        cudaFree(mem);
+        return rc;
+      }
+    }
     sc.ptr = mem;
     sc.bytes = bytes;
   }
   *out = sc.ptr;
   return LC_OK;
+}
+
+int scratch_buffer(cudaStream_t stream, int slot, size_t bytes, void **out) {
+  return scratch_of(stream, slot, bytes, false, out);
+}
+
+int zeroed_buffer(cudaStream_t stream, int slot, size_t bytes, void **out) {
+  return scratch_of(stream, slot, bytes, true, out);
 }
 
 int device_error_word(int **out) {

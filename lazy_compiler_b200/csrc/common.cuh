@@ -62,6 +62,9 @@ int gemm_mixed(int mma_type, int a_type, int b_type, int c_type, int b_layout, i
 // grown (never shrunk) on demand with cudaMalloc.  Growing synchronises the
 // device, so it must not happen inside stream capture.
 int scratch_buffer(cudaStream_t stream, int slot, size_t bytes, void **out);
+// The same, all zero when it is created or grown (for counters that each kernel
+// leaves at zero).
+int zeroed_buffer(cudaStream_t stream, int slot, size_t bytes, void **out);
 
 // Per-device error word that kernels with bounded waits write when a wait
 // gives up (zero-initialised; read and cleared by lc_device_status).

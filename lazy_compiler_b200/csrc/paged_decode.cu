@@ -26,8 +26,11 @@ __device__ __forceinline__ int cached_tokens(const DecodeParams &p, int slot) {
   return n < most ? n : (int)most;
 }
 
+constexpr int kPartialsSlot = 41, kArrivedSlot = 42;  // scratch_buffer slots
+
 // ---------------------------------------------------------------- plain form
-// One CTA of eight warps per (slot, query head), the keys dealt to the warps.
+// One CTA of eight warps per (slot, query head), the keys dealt to the warps: what
+// the tensor-core form below does not take (odd head sizes and alignments).
 constexpr int kRowWarps = 8;
 
 template <class T>
@@ -57,6 +60,633 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
   if (warp == 0)
     store_row(st, static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1],
               p.lse ? p.lse + (int64_t)slot * p.q_heads + h : nullptr, p.d, lane);
+}
+
+// ---------------------------------------------------------------- tensor-core form
+// Reading the cache is all the work (4 flops per element and query head), so the
+// kernel is built around keeping loads in flight.
+//
+// Work is cut by length, not by sequence: all (slot, key-value head, group of 8 NT
+// query heads) segments are laid end to end as tiles of 64 keys, and each CTA takes
+// an equal contiguous run of them, so a batch of unequal lengths and a single long
+// sequence both fill the GPU.  A segment that spans CTAs leaves an unnormalised
+// (O, m, l) per CTA in the workspace; the CTA that arrives last joins them in CTA
+// order (the run boundaries depend on the lengths alone, so results repeat).
+//
+// In a CTA each warp takes 16 keys of every tile and is on its own until the
+// segment ends: it copies its keys' rows (cp.async, 16 bytes per lane, zeros where
+// a key is not visible, so what an unused row holds never enters a product) through
+// a private ring of STAGES tiles, and computes
+//   S^T[16 keys, 8 heads] = K Q^T          (mma.sync m16n8k16, Q in registers)
+//   O^T[D, 8 heads] += V^T P^T             (P^T by movmatrix from S^T's registers)
+// with the heads along N: 8 query heads of a group fill the instruction, and a
+// thread holds the same two heads in S^T and O^T, so rescaling needs no exchange.
+// tcgen05 has no use here: its 128-row tiles would be 1/16 full, and the tensor
+// pipe is idle most of the time as it is.
+// P is split into two 16-bit parts (value and remainder) and multiplied twice: the
+// extra products hide behind the loads and keep P to 16 bits or more.
+constexpr int kDecodeWarps = 4;
+constexpr int kTileKeys = 16;
+constexpr int kMinTiles = 2;  // CTA tiles below which a segment is not cut further
+
+template <class T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// 16 bytes to shared memory; zeros, and no read, where `bytes` is 0.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <class T>
+__device__ __forceinline__ float round_to(float v) {
+  return Elem<T>::to_float(Elem<T>::from_float(v));
+}
+
+// One slot's tiles of 16 keys: those of the sinks, then those from the window's
+// start on (a tile both reach counts once).
+struct SlotTiles {
+  int n, sink_end, lo;       // keys, and the visible ones: j < sink_end or j >= lo
+  int sink_tiles, first, tiles;  // tile x is keys 16 (x < sink_tiles ? x : x - sink_tiles + first)
+};
+__device__ __forceinline__ SlotTiles slot_tiles(const DecodeParams &p, int slot) {
+  SlotTiles t;
+  t.n = cached_tokens(p, slot);
+  const Visible see = visible(t.n - 1, p.window, p.sinks);
+  t.sink_end = see.sink_end;
+  t.lo = see.lo;
+  t.sink_tiles = (t.sink_end + kTileKeys - 1) / kTileKeys;
+  t.first = max(t.lo / kTileKeys, t.sink_tiles);
+  t.tiles = t.n <= 0 ? 0 : t.sink_tiles + (t.n + kTileKeys - 1) / kTileKeys - t.first;
+  return t;
+}
+__device__ __forceinline__ int cta_tiles(const SlotTiles &t) { return (t.tiles + kDecodeWarps - 1) / kDecodeWarps; }
+
+// A place in the sequence of all tiles.
+struct Cursor {
+  SlotTiles tiles;
+  int slot, part, t, count;  // part: (head, group) of the slot; t of count CTA tiles
+};
+__device__ __forceinline__ void advance(Cursor &c, const DecodeParams &p, int parts) {
+  if (++c.t < c.count) return;
+  c.t = 0;
+  if (++c.part < parts) return;
+  c.part = 0;
+  do {
+    if (++c.slot >= p.slots) return;
+    c.tiles = slot_tiles(p, c.slot);
+    c.count = cta_tiles(c.tiles);
+  } while (c.count == 0);
+}
+
+struct DecodeWork {
+  float *partials;    // [CTA][2][rows][DP + 4]: of a segment that began before the CTA, of one that began in it
+  unsigned *arrived;  // [slots * parts], zero between launches
+};
+
+template <class T, int DP, int NT, int STAGES>
+struct DecodeLayout {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kRowBytes = DP * 2;
+  static constexpr int kStageBytes = 2 * kTileKeys * kRowBytes;  // K and V of 16 keys
+  static constexpr int kBytes = kDecodeWarps * STAGES * kStageBytes;
+  static_assert(kRows * DP * 4 <= kStageBytes, "a warp's sums are joined in its last stage");
+};
+
+// PAGED16: a tile of 16 keys lies in one page (page_size is a multiple of 16).
+template <class T, int DP, int NT, int STAGES, bool PAGED16>
+__global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_kernel(DecodeParams p, DecodeWork work) {
+  using L = DecodeLayout<T, DP, NT, STAGES>;
+  constexpr int kRows = L::kRows;
+  constexpr int kChunks = DP / 8;                   // 16-byte pieces of a row
+  constexpr int kRowsPerCopy = 32 / (kChunks < 32 ? kChunks : 32);
+  constexpr int kCopies = kTileKeys / kRowsPerCopy;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ unsigned masks[kDecodeWarps][STAGES];  // the visible keys of each warp's staged tiles
+  __shared__ float scratch[kDecodeWarps * (kMaxHead + 2)];  // the plain form's joins
+  __shared__ float merge_m[kDecodeWarps][kRows], merge_l[kDecodeWarps][kRows], merge_w[kDecodeWarps][kRows];
+  __shared__ float row_m[kRows], row_l[kRows];
+  __shared__ long long sums[kDecodeWarps];
+  __shared__ int start_slot;
+  __shared__ long long start_tile;
+  __shared__ unsigned ticket;
+
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = p.q_heads / p.kv_heads;
+  const int chunks = (group + kRows - 1) / kRows;
+  const int parts = p.kv_heads * chunks;
+
+  // ---- this CTA's run of tiles
+  const int per = (p.slots + kDecodeWarps * 32 - 1) / (kDecodeWarps * 32);
+  const int s0 = min(p.slots, tid * per), s1 = min(p.slots, s0 + per);
+  long long own = 0;
+  for (int s = s0; s < s1; ++s) own += (long long)cta_tiles(slot_tiles(p, s)) * parts;
+  long long inc = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  long long before = inc - own, total = 0;
+#pragma unroll
+  for (int w = 0; w < kDecodeWarps; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  const long long useful = (total + kMinTiles - 1) / kMinTiles;
+  const long long ctas = useful < (long long)gridDim.x ? useful : (long long)gridDim.x;
+  const bool works = blockIdx.x < ctas;
+  const long long begin = works ? blockIdx.x * total / ctas : 0, end = works ? (blockIdx.x + 1) * total / ctas : 0;
+  if (works && begin >= before && begin < before + own) {
+    long long at = before;
+    int s = s0;
+    for (;; ++s) {
+      const long long here = (long long)cta_tiles(slot_tiles(p, s)) * parts;
+      if (begin < at + here) break;
+      at += here;
+    }
+    start_slot = s;
+    start_tile = begin - at;
+  }
+  // slots with nothing to see
+  for (int s = blockIdx.x; s < p.slots; s += gridDim.x) {
+    if (slot_tiles(p, s).tiles != 0) continue;
+    for (int i = tid; i < p.q_heads * p.d; i += blockDim.x) {
+      const int h = i / p.d;
+      static_cast<T *>(p.o)[s * p.os[0] + h * p.os[1] + (i - h * p.d)] = Elem<T>::from_float(0.f);
+    }
+    if (p.lse)
+      for (int h = tid; h < p.q_heads; h += blockDim.x) p.lse[(int64_t)s * p.q_heads + h] = -INFINITY;
+  }
+  __syncthreads();
+  if (!works) return;
+
+  Cursor load;
+  load.slot = start_slot;
+  load.tiles = slot_tiles(p, load.slot);
+  load.count = cta_tiles(load.tiles);
+  load.part = (int)(start_tile / load.count);
+  load.t = (int)(start_tile % load.count);
+  Cursor use = load;
+  const int steps = (int)(end - begin);
+  int64_t seg_begin = begin - use.t;  // first tile of the current segment in the sequence of all
+
+  // ---- loading: lane l copies piece l % kChunks of rows l / kChunks, ...
+  const int piece = lane % kChunks, piece_row = lane / kChunks;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * STAGES * L::kStageBytes;
+  const bool piece_real = piece * 8 < p.d;
+  int page = -1;  // of the tile the load cursor is at (PAGED16), or of its key `lane`
+  auto key_of_tile = [&](const Cursor &c) {
+    const int x = c.t * kDecodeWarps + warp;
+    return x < c.tiles.tiles ? kTileKeys * (x < c.tiles.sink_tiles ? x : x - c.tiles.sink_tiles + c.tiles.first) : -1;
+  };
+  auto find_page = [&]() {
+    const int key = key_of_tile(load);
+    page = -1;
+    if (key < 0) return;
+    if (PAGED16) {
+      page = p.table[load.slot * p.ts + key / p.page_size];
+    } else {
+      const int j = key + (lane & 15);
+      if (j < load.tiles.n) page = p.table[load.slot * p.ts + j / p.page_size];
+    }
+  };
+  auto issue = [&](int stage) {
+    const int key = key_of_tile(load);
+    const int j = key + (lane & 15);
+    const bool sees = key >= 0 && (unsigned)page < (unsigned)p.pages && j < load.tiles.n &&
+                      (j >= load.tiles.lo || j < load.tiles.sink_end);
+    const unsigned mask = __ballot_sync(0xffffffffu, sees) & 0xffffu;
+    if (lane == 0) masks[warp][stage] = mask;
+    if (mask) {
+      const int head = load.part / chunks;
+      const uint32_t k_dst = ring + stage * L::kStageBytes, v_dst = k_dst + kTileKeys * L::kRowBytes;
+      int64_t k_off, v_off;
+      if (PAGED16) {
+        const int r = key % p.page_size;
+        k_off = page * p.ks[0] + head * p.ks[1] + (r + piece_row) * p.ks[2] + piece * 8;
+        v_off = page * p.vs[0] + head * p.vs[1] + (r + piece_row) * p.vs[2] + piece * 8;
+      } else {
+        const int r = j % p.page_size;
+        k_off = page * p.ks[0] + head * p.ks[1] + r * p.ks[2];
+        v_off = page * p.vs[0] + head * p.vs[1] + r * p.vs[2];
+      }
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int row = i * kRowsPerCopy + piece_row;
+        const int bytes = (mask >> row & 1) && piece_real ? 16 : 0;
+        int64_t ko, vo;
+        if (PAGED16) {
+          ko = k_off + (int64_t)(i * kRowsPerCopy) * p.ks[2];
+          vo = v_off + (int64_t)(i * kRowsPerCopy) * p.vs[2];
+        } else {
+          ko = __shfl_sync(0xffffffffu, k_off, row) + piece * 8;
+          vo = __shfl_sync(0xffffffffu, v_off, row) + piece * 8;
+        }
+        const uint32_t at = row * L::kRowBytes + ((piece ^ (row & 7)) << 4);
+        copy_async16(k_dst + at, static_cast<const T *>(p.k) + (bytes ? ko : 0), bytes);
+        copy_async16(v_dst + at, static_cast<const T *>(p.v) + (bytes ? vo : 0), bytes);
+      }
+    }
+  };
+
+  // ---- computing
+  uint32_t q[NT][DP / 16][2];
+  float o[NT][DP / 16][4];
+  float m[NT][2], l[NT][2];
+  const int g = lane >> 2, c2 = (lane & 3) * 2;
+  auto start_segment = [&]() {
+    const int head = use.part / chunks, first = head * group + use.part % chunks * kRows;
+    const int live = min(kRows, (head + 1) * group - first);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const T *row = static_cast<const T *>(p.q) + use.slot * p.qs[0] + (first + nt * 8 + g) * p.qs[1];
+      const bool real = nt * 8 + g < live;
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int c = k * 16 + x * 8 + c2;
+          q[nt][k][x] = real && c < p.d ? *reinterpret_cast<const uint32_t *>(row + c) : 0u;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[nt][k][x] = 0.f;
+      }
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+  };
+  auto compute = [&](int stage) {
+    const unsigned mask = masks[warp][stage];
+    if (!mask) return;
+    const uint32_t k_src = ring + stage * L::kStageBytes, v_src = k_src + kTileKeys * L::kRowBytes;
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    // K: rows 0-7, 8-15 of pieces 2k, then 2k + 1
+    const int k_row = lane & 15, k_half = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      uint32_t a[4];
+      ldmatrix4(a, k_src + k_row * L::kRowBytes + (((2 * k + k_half) ^ (k_row & 7)) << 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[nt], a, q[nt][k][0], q[nt][k][1]);
+    }
+    uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      // s: (key g, heads c2, c2 + 1), (key g + 8, the same heads)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[nt][x] = mask >> (g + (x >> 1) * 8) & 1 ? s[nt][x] * p.scale_log2 : -INFINITY;
+      float top[2] = {fmaxf(s[nt][0], s[nt][2]), fmaxf(s[nt][1], s[nt][3])};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
+      }
+      const bool grew = top[0] > m[nt][0] || top[1] > m[nt][1];
+      if (__any_sync(0xffffffffu, grew)) {
+        float alpha[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float m_new = fmaxf(m[nt][x], top[x]);
+          alpha[x] = exp2f(m[nt][x] - (m_new == -INFINITY ? 0.f : m_new));
+          m[nt][x] = m_new;
+          l[nt][x] *= alpha[x];
+        }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          o[nt][k][0] *= alpha[0];
+          o[nt][k][1] *= alpha[1];
+          o[nt][k][2] *= alpha[0];
+          o[nt][k][3] *= alpha[1];
+        }
+      }
+      const float base[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0], m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
+      float e[4], r[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        e[x] = exp2f(s[nt][x] - base[x & 1]);
+        l[nt][x & 1] += e[x];
+        r[x] = round_to<T>(e[x]);
+      }
+      hi[nt][0] = movmatrix_trans(pack<T>(r[0], r[1]));
+      hi[nt][1] = movmatrix_trans(pack<T>(r[2], r[3]));
+      lo[nt][0] = movmatrix_trans(pack<T>(e[0] - r[0], e[1] - r[1]));
+      lo[nt][1] = movmatrix_trans(pack<T>(e[2] - r[2], e[3] - r[3]));
+    }
+    // V^T: (keys 0-7, pieces 2k, 2k + 1), then keys 8-15
+    const int v_row = (lane & 7) + (lane >> 4) * 8, v_half = lane >> 3 & 1;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      uint32_t a[4];
+      ldmatrix4_trans(a, v_src + v_row * L::kRowBytes + (((2 * k + v_half) ^ (v_row & 7)) << 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma16816<T>(o[nt][k], a, hi[nt][0], hi[nt][1]);
+        mma16816<T>(o[nt][k], a, lo[nt][0], lo[nt][1]);
+      }
+    }
+  };
+
+  // ---- ending a segment: the warps' states joined, and the CTAs' where there are several
+  constexpr int kPartial = kRows * (DP + 4);  // floats; m and l at DP, DP + 1 of a row
+  // a thread's share of the rows x DP sums: columns col + 128 y of rows first_row + kSplit x
+  constexpr int kCols = DP < 128 ? DP : 128, kSplit = kDecodeWarps * 32 / kCols, kRpt = kRows / kSplit, kCpt = DP / kCols;
+  const int col = tid % kCols, first_row = tid / kCols;
+  auto write_rows = [&](const float (&values)[kRpt][kCpt]) {  // O / l and the log-sum-exp; whether all is finite
+    const int head = use.part / chunks, first = head * group + use.part % chunks * kRows;
+    const int live = min(kRows, (head + 1) * group - first);
+    bool odd = false;
+#pragma unroll
+    for (int x = 0; x < kRpt; ++x) {
+      const int row = first_row + kSplit * x;
+      if (row >= live) continue;
+      const float sum = row_l[row], inv = sum == 0.f ? 0.f : 1.f / sum;
+      T *out = static_cast<T *>(p.o) + use.slot * p.os[0] + (first + row) * p.os[1];
+#pragma unroll
+      for (int y = 0; y < kCpt; ++y) {
+        const float v = values[x][y] * inv;
+        if (col + kCols * y < p.d) {
+          odd |= !isfinite(v);
+          out[col + kCols * y] = Elem<T>::from_float(v);
+        }
+      }
+    }
+    if (p.lse && tid < live)
+      p.lse[(int64_t)use.slot * p.q_heads + first + tid] = row_l[tid] == 0.f ? -INFINITY : (row_m[tid] + log2f(row_l[tid])) * kLn2;
+    return odd;
+  };
+  // What came out infinite or NaN is computed again one key at a time: the
+  // remainder's products can turn an infinite value into NaN.
+  auto plain_rows = [&]() {
+    const int head = use.part / chunks, first = head * group + use.part % chunks * kRows;
+    const int live = min(kRows, (head + 1) * group - first);
+    const int *row = p.table + use.slot * p.ts;
+    auto at = [&](int j, const T *&k, const T *&v) {
+      const int pg = row[j / p.page_size], r = j % p.page_size;
+      if ((unsigned)pg >= (unsigned)p.pages) return false;
+      k = static_cast<const T *>(p.k) + pg * p.ks[0] + head * p.ks[1] + r * p.ks[2];
+      v = static_cast<const T *>(p.v) + pg * p.vs[0] + head * p.vs[1] + r * p.vs[2];
+      return true;
+    };
+    for (int x = 0; x < live; ++x) {
+      float qv[kMaxHead / 32];
+      load_row(qv, static_cast<const T *>(p.q) + use.slot * p.qs[0] + (first + x) * p.qs[1], p.d, lane, p.scale_log2);
+      RowState st;
+      attend_keys<T>(st, qv, p.d, lane, warp, use.tiles.sink_end, kDecodeWarps, at);
+      attend_keys<T>(st, qv, p.d, lane, use.tiles.lo + warp, use.tiles.n, kDecodeWarps, at);
+      __syncthreads();
+      join_warps<kDecodeWarps>(st, scratch);
+      if (warp == 0) mend_row(st, static_cast<T *>(p.o) + use.slot * p.os[0] + (first + x) * p.os[1], p.d, lane);
+    }
+  };
+  auto end_segment = [&](long long seg_end, int stage) {
+    // The stage just used is free until the next copies: each warp leaves its sums
+    // there, column c of heads 2 t, 2 t + 1 at c ^ 8 t, off each other's banks.
+    auto sums_of = [&](int w) { return reinterpret_cast<float *>(smem + (w * STAGES + stage) * L::kStageBytes); };
+    float *mine = sums_of(warp);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float sum = l[nt][x];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g == 0) {
+          merge_m[warp][nt * 8 + c2 + x] = m[nt][x];
+          merge_l[warp][nt * 8 + c2 + x] = sum;
+        }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          float *row = mine + (nt * 8 + c2 + x) * DP;
+          row[(k * 16 + g) ^ (c2 << 2)] = o[nt][k][x];
+          row[(k * 16 + g + 8) ^ (c2 << 2)] = o[nt][k][2 + x];
+        }
+      }
+    }
+    __syncthreads();
+    if (tid < kRows) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kDecodeWarps; ++w) top = fmaxf(top, merge_m[w][tid]);
+#pragma unroll
+      for (int w = 0; w < kDecodeWarps; ++w) {
+        const float weight = exp2f(merge_m[w][tid] - (top == -INFINITY ? 0.f : top));
+        merge_w[w][tid] = weight;
+        sum = fmaf(merge_l[w][tid], weight, sum);
+      }
+      row_m[tid] = top;
+      row_l[tid] = sum;
+    }
+    __syncthreads();
+    float values[kRpt][kCpt];
+#pragma unroll
+    for (int x = 0; x < kRpt; ++x) {
+      const int row = first_row + kSplit * x;
+#pragma unroll
+      for (int y = 0; y < kCpt; ++y) {
+        values[x][y] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kDecodeWarps; ++w)
+          values[x][y] = fmaf(sums_of(w)[row * DP + ((col + kCols * y) ^ ((row & 6) << 2))], merge_w[w][row], values[x][y]);
+      }
+    }
+    bool odd = false;
+    if (seg_begin >= begin && seg_end <= end) {
+      odd = write_rows(values);
+    } else {
+      float *partial = work.partials + ((int64_t)blockIdx.x * 2 + (seg_begin >= begin)) * kPartial;
+#pragma unroll
+      for (int x = 0; x < kRpt; ++x)
+#pragma unroll
+        for (int y = 0; y < kCpt; ++y) partial[(first_row + kSplit * x) * (DP + 4) + col + kCols * y] = values[x][y];
+      if (tid < kRows) {
+        partial[tid * (DP + 4) + DP] = row_m[tid];
+        partial[tid * (DP + 4) + DP + 1] = row_l[tid];
+      }
+      // the CTAs whose runs hold the segment's first and last tile
+      const int first = (int)(((seg_begin + 1) * ctas - 1) / total), last = (int)((seg_end * ctas - 1) / total);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        unsigned *count = work.arrived + (int64_t)use.slot * parts + use.part;
+        ticket = atomicAdd(count, 1u);
+        if (ticket == (unsigned)(last - first)) *count = 0;  // for the next launch
+      }
+      __syncthreads();
+      if (ticket != (unsigned)(last - first)) return;
+      __threadfence();
+      // CTA c's share: the segment began in CTA `first` and before every other
+      auto share = [&](int c) { return work.partials + ((int64_t)c * 2 + (c == first)) * kPartial; };
+      float top[kRpt];
+#pragma unroll
+      for (int x = 0; x < kRpt; ++x) top[x] = -INFINITY;
+#pragma unroll 2
+      for (int c = first; c <= last; ++c)
+#pragma unroll
+        for (int x = 0; x < kRpt; ++x) top[x] = fmaxf(top[x], __ldcg(share(c) + (first_row + kSplit * x) * (DP + 4) + DP));
+      float sum[kRpt];
+#pragma unroll
+      for (int x = 0; x < kRpt; ++x) {
+        sum[x] = 0.f;
+#pragma unroll
+        for (int y = 0; y < kCpt; ++y) values[x][y] = 0.f;
+      }
+#pragma unroll 2
+      for (int c = first; c <= last; ++c) {
+        const float *from = share(c);
+#pragma unroll
+        for (int x = 0; x < kRpt; ++x) {
+          const float *row = from + (first_row + kSplit * x) * (DP + 4);
+          const float weight = exp2f(__ldcg(row + DP) - (top[x] == -INFINITY ? 0.f : top[x]));
+          sum[x] = fmaf(__ldcg(row + DP + 1), weight, sum[x]);
+#pragma unroll
+          for (int y = 0; y < kCpt; ++y) values[x][y] = fmaf(__ldcg(row + col + kCols * y), weight, values[x][y]);
+        }
+      }
+      if (col == 0) {
+#pragma unroll
+        for (int x = 0; x < kRpt; ++x) {
+          row_m[first_row + kSplit * x] = top[x];
+          row_l[first_row + kSplit * x] = sum[x];
+        }
+      }
+      __syncthreads();
+      odd = write_rows(values);
+    }
+    if (__syncthreads_or(odd)) plain_rows();  // (the sums have been read, too)
+  };
+
+  find_page();
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (i < steps) {
+      issue(i);
+      advance(load, p, parts);
+      if (i + 1 < steps) find_page();
+    }
+    copy_commit();
+  }
+  start_segment();
+  int stage = 0;
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    copy_wait<STAGES - 2>();
+    __syncwarp();  // this stage has landed, and the one before has been read, in every lane
+    if (i + STAGES - 1 < steps) {
+      issue(stage == 0 ? STAGES - 1 : stage - 1);
+      advance(load, p, parts);
+      if (i + STAGES < steps) find_page();
+    }
+    copy_commit();
+    compute(stage);
+    if (use.t + 1 == use.count || i + 1 == steps) {
+      end_segment(seg_begin + use.count, stage);
+      seg_begin += use.count;
+      if (i + 1 < steps) {
+        use.t = use.count - 1;
+        advance(use, p, parts);
+        start_segment();
+      }
+    } else {
+      ++use.t;
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+}
+
+template <class T, int DP, int NT, int STAGES, bool PAGED16>
+int launch_decode(const DecodeParams &p, cudaStream_t s) {
+  using L = DecodeLayout<T, DP, NT, STAGES>;
+  auto *kernel = decode_kernel<T, DP, NT, STAGES, PAGED16>;
+  static int configured[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "decode shared memory"))
+      return rc;
+    if (dev >= 0 && dev < 64) configured[dev] = 1;
+  }
+  const int ctas = sm_count() * (DP == 256 ? 1 : 2);
+  const int group = p.q_heads / p.kv_heads;
+  const int64_t parts = (int64_t)p.kv_heads * ((group + L::kRows - 1) / L::kRows);
+  DecodeWork w;
+  void *mem = nullptr;
+  if (int rc = scratch_buffer(s, kPartialsSlot, (size_t)ctas * 2 * L::kRows * (DP + 4) * 4, &mem)) return rc;
+  w.partials = static_cast<float *>(mem);
+  if (int rc = zeroed_buffer(s, kArrivedSlot, (size_t)(p.slots * parts * 4), &mem)) return rc;
+  w.arrived = static_cast<unsigned *>(mem);
+  return check_cuda(launch_pdl(kernel, dim3(ctas), dim3(kDecodeWarps * 32), L::kBytes, s, p, w), "lc_paged_decode");
+}
+
+template <class T, bool PAGED16>
+int launch_sized(const DecodeParams &p, cudaStream_t s) {
+  // NT: 8 or 16 query heads of a group in one pass over its keys (a group of 9 to 16
+  // read twice, 8 heads at a time, would take the loads twice; larger groups are cut in sixteens)
+  const bool wide = p.q_heads / p.kv_heads > 8;
+  if (p.d <= 64) return wide ? launch_decode<T, 64, 2, 6, PAGED16>(p, s) : launch_decode<T, 64, 1, 6, PAGED16>(p, s);
+  if (p.d <= 128) return wide ? launch_decode<T, 128, 2, 3, PAGED16>(p, s) : launch_decode<T, 128, 1, 3, PAGED16>(p, s);
+  return wide ? launch_decode<T, 256, 2, 3, PAGED16>(p, s) : launch_decode<T, 256, 1, 3, PAGED16>(p, s);
+}
+
+// The tensor-core form takes 16-byte pieces of keys and values and pairs of the query.
+bool decode_tensor(const DecodeParams &p) {
+  bool ok = p.d % 8 == 0 && aligned(p.k, 16) && aligned(p.v, 16) && aligned(p.q, 4) && p.pages > 0 && p.width > 0;
+  for (int i = 0; i < 3; ++i) ok = ok && p.ks[i] % 8 == 0 && p.vs[i] % 8 == 0;
+  for (int i = 0; i < 2; ++i) ok = ok && p.qs[i] % 2 == 0;
+  return ok;
 }
 
 }  // namespace
@@ -92,6 +722,10 @@ extern "C" int lc_paged_decode(int dtype, const void *q, const void *k, const vo
   p.sinks = (int)(sinks < most ? sinks : most);
   p.scale_log2 = scale * attend::kLog2e;
   cudaStream_t s = as_stream(stream);
+  if (decode_tensor(p)) {
+    if (dtype == LC_F16) return page_size % 16 == 0 ? launch_sized<__half, true>(p, s) : launch_sized<__half, false>(p, s);
+    return page_size % 16 == 0 ? launch_sized<__nv_bfloat16, true>(p, s) : launch_sized<__nv_bfloat16, false>(p, s);
+  }
   const dim3 grid((unsigned)slots, (unsigned)q_heads);
   if (dtype == LC_F16)
     decode_row_kernel<__half><<<grid, kRowWarps * 32, 0, s>>>(p);
