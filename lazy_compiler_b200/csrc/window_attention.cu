@@ -5,6 +5,7 @@
 // heads: query head h reads key-value head h / (q_heads / kv_heads).
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "attend.cuh"
@@ -78,10 +79,15 @@ __global__ void __launch_bounds__(kRowWarps * 32) window_row_kernel(WindowParams
 //           against the window plus 256 with one head per tile;
 //   keys    an item (two tiles of one sequence and key-value head) visits the blocks
 //           of the sinks and then blocks from the first key that its first token
-//           sees on (a TMA box may start at any row), nothing else; only blocks that
-//           cross a bound of some row are masked, by four 32-bit words per row;
-//   bounds  lengths come from the device; items run longest first, so that the causal
-//           triangle's tail is made of short ones;
+//           sees on (a TMA box may start at any row), nothing else; where the last of
+//           them is half empty, its second half takes the sinks instead; only blocks
+//           that cross a bound of some row are masked, by four 32-bit words per row;
+//   cuts    lengths come from the device.  With many items each CTA takes every
+//           gridDim-th one, longest first, so that the causal triangle's tail is made
+//           of short ones.  With few, or ragged ones, all items' blocks are laid end to
+//           end and each CTA takes an equal run of them; what a run holds of an item
+//           without holding it all goes to the workspace in f32, and join_kernel
+//           adds it up in CTA order;
 //   values  0 x infinity is NaN, so the rows of V beyond a sequence's end are cleared
 //           in shared memory, and a row whose sums come out infinite or NaN is
 //           computed again key by key (it may hold a value that its mask hides).
@@ -94,7 +100,15 @@ constexpr int kRows = 128;     // of a query tile
 constexpr int kTiles = 2;      // per CTA
 constexpr int kKeys = 128;     // of a block
 constexpr int kStages = 2;
-constexpr int kThreads = 64 + kTiles * 128;
+constexpr int kMinRun = 6;     // units of a run: a shorter one costs more to join than it saves
+constexpr int kCutUnits = 4;   // units that the join costs
+constexpr int kMaxCutItems = 2048;
+constexpr int kSpansSlot = 43, kSumsSlot = 44, kStatsSlot = 45;  // scratch_buffer slots
+constexpr int kThreads = 128 + kTiles * 128;
+// Registers per thread after the split: the softmax warpgroups' rows of 128 scores
+// need more than the 168 that 384 threads are launched with (spills otherwise);
+// 88 x 128 + 208 x 256 = 168 x 384.
+constexpr int kFewRegs = 88, kManyRegs = 208;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;             // O of tile t at kOCol + t * DP; S of tile t at t * 128
 constexpr float kRescale = 8.0f;            // log2 units a row's maximum may lag behind
@@ -113,6 +127,12 @@ struct TensorParams {
   int k_head, k_batch, v_head, v_batch;  // 0 where the axis is broadcast (stride 0), else 1
   int o_vec;                // output rows by 32-byte (2) or 16-byte (1) stores
   int *err;
+  // runs of blocks (cut): the item that began in a CTA and goes on after it, or -1, and that
+  // item's last CTA; a CTA's shares of the item that began before it, and of that one
+  int cut;
+  int2 *spans;
+  float *sums;              // [CTA][2][tile][row][DP]
+  float2 *stats;            // [CTA][2][tile][row]: m and l
 };
 
 // One item: its tokens and the key blocks that they see.
@@ -120,6 +140,7 @@ struct Item {
   int b, hk, i0;            // first token of tile 0
   int n_q, n_kv, base;      // token i is at position base + i
   int n, n_sink, start, sinks;  // blocks; the first n_sink hold keys 0 .. sinks - 1, the others start at key `start`
+  bool sink_half;               // the last block's rows from 64 on hold the keys from 0 on
 };
 
 __device__ __forceinline__ int first_seen(int p, int window) { return window == 0 ? 0 : max(0, p - window + 1); }
@@ -138,18 +159,55 @@ __device__ __forceinline__ Item item_of(const WindowParams &p, const TensorParam
   const int p_first = max(0, it.base + it.i0), p_last = it.base + last;
   it.n = it.n_sink = it.start = 0;
   it.sinks = p.sinks;
+  it.sink_half = false;
   if (last < it.i0 || p_last < 0) return it;
   const int lo = first_seen(p_first, p.window);
+  int keys = p_last + 1;
   if (lo > p.sinks) {  // a gap, or nothing, between the sinks and the windows
-    it.n_sink = (p.sinks + kKeys - 1) / kKeys;
     it.start = lo;
+    keys -= lo;
+    const int rest = keys % kKeys;
+    it.sink_half = p.sinks > 0 && p.sinks <= kKeys / 2 && rest > 0 && rest <= kKeys / 2;
+    it.n_sink = it.sink_half ? 0 : (p.sinks + kKeys - 1) / kKeys;
   }
-  it.n = it.n_sink + (p_last + 1 - it.start + kKeys - 1) / kKeys;
+  it.n = it.n_sink + (keys + kKeys - 1) / kKeys;
   return it;
 }
 __device__ __forceinline__ int block_key(const Item &it, int j) {
   return j < it.n_sink ? j * kKeys : it.start + (j - it.n_sink) * kKeys;
 }
+
+// What a CTA works on: blocks [j0, j1) of an item after the other.  A run is measured
+// in units of a block's time; beginning and ending an item costs some more of them,
+// which count as lying before its first block.
+constexpr int kItemUnits = 2;
+__host__ __device__ __forceinline__ int units_of(int blocks) { return blocks > 0 ? blocks + kItemUnits : 0; }
+
+struct Piece {
+  Item it;
+  int index, j0, j1;
+};
+struct Pieces {
+  int index, skip, left;  // skip: units of the first item that lie before the run; left: the run's units (cut)
+  __device__ __forceinline__ bool next(const WindowParams &p, const TensorParams &t, Piece &out) {
+    for (;;) {
+      if (index >= t.items || (t.cut && left <= 0)) return false;
+      out.it = item_of(p, t, index);
+      out.index = index;
+      out.j0 = 0;
+      out.j1 = out.it.n;
+      index += t.cut ? 1 : gridDim.x;
+      if (t.cut) {
+        const int end = min(units_of(out.it.n), skip + left);
+        out.j0 = max(0, skip - kItemUnits);
+        out.j1 = max(0, end - kItemUnits);
+        left -= end - skip;
+        skip = 0;
+      }
+      if (out.j1 > out.j0) return true;
+    }
+  }
+};
 
 // 5-D and 4-D tiled TMA loads (c0 innermost).
 __device__ __forceinline__ void tma_load_5d(void *dst, const CUtensorMap *map, uint64_t *bar, int32_t c0, int32_t c1,
@@ -246,6 +304,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t s_full[kTiles], p_full[kTiles], o_done[kTiles], o_empty[kTiles];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
+  __shared__ int warp_blocks[kThreads / 32];
+  __shared__ Pieces run;
+  __shared__ int run_end, run_total, run_ctas;
   volatile int *abort = &abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -282,17 +343,61 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_base;
   pdl_wait();
   pdl_trigger();
+  if (!tp.cut) {
+    if (threadIdx.x == 0) run = {(int)blockIdx.x, 0, 0};
+  } else {
+    // this CTA's run: unit blockIdx.x * total / ctas of all items' units on
+    const int per = (tp.items + kThreads - 1) / kThreads;
+    const int first = min(tp.items, (int)threadIdx.x * per), last = min(tp.items, first + per);
+    int own = 0;
+    for (int i = first; i < last; ++i) own += units_of(item_of(p, tp, i).n);
+    int inc = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) warp_blocks[warp] = inc;
+    if (threadIdx.x == 0) run = {tp.items, 0, 0};
+    __syncthreads();
+    int before = inc - own, total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += warp_blocks[w];
+      total += warp_blocks[w];
+    }
+    const int ctas = min((int)gridDim.x, (total + kMinRun - 1) / kMinRun);
+    const int begin = ctas ? (int)((int64_t)blockIdx.x * total / ctas) : 0;
+    const int end = ctas ? (int)((int64_t)(blockIdx.x + 1) * total / ctas) : 0;
+    if ((int)blockIdx.x < ctas && begin >= before && begin < before + own) {
+      int at = before, i = first;
+      for (;; ++i) {
+        const int n = units_of(item_of(p, tp, i).n);
+        if (begin < at + n) break;
+        at += n;
+      }
+      run = {i, begin - at, end - begin};
+    }
+    if (threadIdx.x == 0) {
+      run_end = end;
+      run_total = total;
+      run_ctas = ctas;
+      tp.spans[blockIdx.x] = make_int2(-1, -1);
+    }
+  }
+  __syncthreads();
+  Pieces pieces = run;
+  Piece piece;
   // Every barrier phase counts over all blocks of the CTA's items: block g (over all
   // items) uses stage g & 1, and s_full / p_full / o_done complete once per block.
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+    if (warp == 0 && lane == 0) {
       int g = 0, local = 0;
       bool ok = true;
       const uint32_t q_bytes = kTiles * DP / 64 * tp.group * tp.tokens * 128;
-      for (int index = blockIdx.x; ok && index < tp.items; index += gridDim.x) {
-        const Item it = item_of(p, tp, index);
-        if (it.n == 0) continue;
+      while (ok && pieces.next(p, tp, piece)) {
+        const Item &it = piece.it;
         // Q of the previous item is free once its last S products completed
         if (local > 0 && !mbar_wait(&q_empty, (local - 1) & 1, abort)) {
           give_up(tp, abort, kErrTimeoutProducer);
@@ -303,8 +408,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = 0; t < kTiles; ++t)
           for (int c = 0; c < DP / 64; ++c)
             tma_load_5d(q_s + t * kTile + c * kChunkBytes, &tma_q, &q_full, c * 64, 0, it.i0 + t * tp.tokens, it.hk, it.b);
-        for (int j = 0; j < it.n; ++j, ++g) {
+        for (int j = piece.j0; j < piece.j1; ++j, ++g) {
           const int st = g & 1, key = block_key(it, j);
+          const int half_key = it.sink_half && j + 1 == it.n ? 0 : key + kKeys / 2;
           const uint32_t ph = (g >> 1) & 1;
           uint8_t *k_s = kv_s + st * 2 * kTile, *v_s = k_s + kTile;
           if (!mbar_wait(&k_empty[st], ph ^ 1, abort)) {
@@ -313,21 +419,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           mbar_expect_tx(&k_full[st], kTile);
-          for (int c = 0; c < DP / 64; ++c)
+          for (int c = 0; c < DP / 64; ++c) {
             tma_load_4d(k_s + c * kChunkBytes, &tma_k, &k_full[st], c * 64, key, it.hk * tp.k_head, it.b * tp.k_batch);
+            tma_load_4d(k_s + c * kChunkBytes + kChunkBytes / 2, &tma_k, &k_full[st], c * 64, half_key, it.hk * tp.k_head, it.b * tp.k_batch);
+          }
           if (!mbar_wait(&v_empty[st], ph ^ 1, abort)) {
             give_up(tp, abort, kErrTimeoutProducer);
             ok = false;
             break;
           }
           mbar_expect_tx(&v_full[st], kTile);
-          for (int c = 0; c < DP / 64; ++c)
+          for (int c = 0; c < DP / 64; ++c) {
             tma_load_4d(v_s + c * kChunkBytes, &tma_v, &v_full[st], c * 64, key, it.hk * tp.v_head, it.b * tp.v_batch);
+            tma_load_4d(v_s + c * kChunkBytes + kChunkBytes / 2, &tma_v, &v_full[st], c * 64, half_key, it.hk * tp.v_head, it.b * tp.v_batch);
+          }
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
+    } else if (warp == 1 && lane == 0) {
       constexpr uint32_t idesc_s = idesc_f16(kBf16, false, false, kRows, kKeys);
       constexpr uint32_t idesc_o = idesc_f16(kBf16, false, true, kRows, DP);
       const uint64_t q_desc = smem_desc_sw128(smem_u32(q_s), 16, 1024);
@@ -353,9 +461,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int g0 = 0, local = 0;
       bool ok = true;
-      for (int index = blockIdx.x; ok && index < tp.items; index += gridDim.x) {
-        const int n = item_of(p, tp, index).n;
-        if (n == 0) continue;
+      while (ok && pieces.next(p, tp, piece)) {
+        const int n = piece.j1 - piece.j0;
         ok = mbar_wait(&q_full, local & 1, abort) && mbar_wait(&k_full[g0 & 1], (g0 >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
@@ -392,7 +499,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) give_up(tp, abort, kErrTimeoutMma);
     }
   } else {
-    const int t = (warp - 2) >> 2;  // query tile of this warpgroup
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
+    const int t = (warp - 4) >> 2;  // query tile of this warpgroup
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -401,14 +509,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int token = row / tp.group, head = row - token * tp.group;
     int g0 = 0;
     bool ok = true;
-    for (int index = blockIdx.x; ok && index < tp.items; index += gridDim.x) {
+    // items that see nothing: zeros
+    for (int index = blockIdx.x; index < tp.items; index += gridDim.x) {
       const Item it = item_of(p, tp, index);
+      const int i = it.i0 + t * tp.tokens + token, h = it.hk * tp.group + head;
+      if (it.n > 0 || !in_tile || i >= p.s_q) continue;
+      T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
+      for (int c = 0; c < p.d; c += 8) *reinterpret_cast<uint4 *>(out + c) = make_uint4(0, 0, 0, 0);
+      if (p.lse) p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = -INFINITY;
+    }
+    __syncwarp();
+    while (ok && pieces.next(p, tp, piece)) {
+      const Item &it = piece.it;
+      const int n = piece.j1 - piece.j0;
       const int i = it.i0 + t * tp.tokens + token, h = it.hk * tp.group + head;
       const int pos = it.base + i;
       const int p_low = it.base + it.i0 + t * tp.tokens, p_high = p_low + tp.tokens - 1;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < it.n; ++j) {
-        const int g = g0 + j, key = block_key(it, j);
+      for (int x = 0; x < n; ++x) {
+        const int g = g0 + x, j = piece.j0 + x, key = block_key(it, j);
         if (!wait_all(&s_full[t], g & 1, abort, tp, kErrTimeoutSoftmax)) {
           ok = false;
           break;
@@ -431,13 +550,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           sunk = min(it.sinks - key, to);
           whole = key + kKeys - 1 <= p_low && key >= first_seen(p_high, p.window);
         }
+        const bool sink_half = it.sink_half && j + 1 == it.n;
+        int sunk_from = 0;
+        if (sink_half) {  // keys 0 .. sinks - 1 are rows 64 on
+          whole = false;
+          to = min(to, kKeys / 2);
+          sunk_from = kKeys / 2;
+          sunk = kKeys / 2 + it.sinks;
+        }
         if (!whole) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const uint32_t sees = bits_between(from - c * 32, to - c * 32) | bits_between(0, sunk - c * 32);
+            const uint32_t sees = bits_between(from - c * 32, to - c * 32) | bits_between(sunk_from - c * 32, sunk - c * 32);
 #pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (!(sees >> x & 1)) sr[c][x] = __float_as_uint(-INFINITY);
+            for (int y = 0; y < 32; ++y)
+              if (!(sees >> y & 1)) sr[c][y] = __float_as_uint(-INFINITY);
           }
         }
         if (key + kKeys > it.n_kv && it.n_kv < p.s_kv) {
@@ -446,10 +573,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          if (key + row >= it.n_kv) {
+          if ((sink_half && row >= kKeys / 2 ? row - kKeys / 2 : key + row) >= it.n_kv) {
             uint8_t *v_row = kv_s + (g & 1) * 2 * kTile + kTile + row * 128;
             for (int c = 0; c < DP / 64; ++c)
-              for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4 *>(v_row + c * kChunkBytes + x * 16) = make_uint4(0, 0, 0, 0);
+              for (int y = 0; y < 8; ++y) *reinterpret_cast<uint4 *>(v_row + c * kChunkBytes + y * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_async_shared();
         }
@@ -460,8 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int x = 0; x < 32; x += 2)
-            mx8[(x >> 1) & 7] = max3(mx8[(x >> 1) & 7], __uint_as_float(sr[c][x]), __uint_as_float(sr[c][x + 1]));
+          for (int y = 0; y < 32; y += 2)
+            mx8[(y >> 1) & 7] = max3(mx8[(y >> 1) & 7], __uint_as_float(sr[c][y]), __uint_as_float(sr[c][y + 1]));
         const float mx = max3(max3(mx8[0], mx8[1], mx8[2]), max3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])) * p.scale_log2;
         const float m_new = fmaxf(m, mx);
         const bool need = m_new > m + kRescale;
@@ -471,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             l *= alpha;
             m = m_new;
           }
-          if (j > 0) {
+          if (x > 0) {
             if (!wait_all(&o_done[t], (g - 1) & 1, abort, tp, kErrTimeoutCorrection)) {
               ok = false;
               break;
@@ -483,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_ld16(o_at + c * 16, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
               tmem_st16(o_at + c * 16, o);
             }
             tmem_wait_st();
@@ -497,18 +624,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 4; ++c) {
           uint32_t packed[16];
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const uint64_t x2 = ffma2(pack2(__uint_as_float(sr[c][2 * x]), __uint_as_float(sr[c][2 * x + 1])), scale2, base2);
+          for (int y = 0; y < 16; ++y) {
+            const uint64_t x2 = ffma2(pack2(__uint_as_float(sr[c][2 * y]), __uint_as_float(sr[c][2 * y + 1])), scale2, base2);
             uint64_t p2;
-            if ((x + 1) * POLY / 16 > x * POLY / 16) {
+            if ((y + 1) * POLY / 16 > y * POLY / 16) {
               p2 = ex2_poly2<true>(x2);
             } else {
               const float2 xx = unpack2(x2);
               p2 = pack2(ex2(xx.x), ex2(xx.y));
             }
-            part2[x & 3] = fadd2(part2[x & 3], p2);
+            part2[y & 3] = fadd2(part2[y & 3], p2);
             const float2 pp = unpack2(p2);
-            packed[x] = pack16<T>(pp.x, pp.y);
+            packed[y] = pack16<T>(pp.x, pp.y);
           }
           tmem_st16(s_at + c * 16, packed);
         }
@@ -520,29 +647,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
       if (!ok) break;
+      if (!wait_all(&o_done[t], (g0 + n - 1) & 1, abort, tp, kErrTimeoutSoftmax)) break;
+      tc_fence_after();
+      if (n < it.n) {  // a share of the item: unnormalised, for join_kernel
+        const int64_t at = (((int64_t)blockIdx.x * 2 + (piece.j0 == 0)) * kTiles + t) * kRows + row;
+        tp.stats[at] = make_float2(m, l);
+        if (piece.j0 == 0 && t == 0 && row == 0) {  // the run's last piece: it goes on in the next CTA's
+          const int64_t last_unit = run_end - (piece.j1 + kItemUnits) + units_of(it.n);
+          tp.spans[blockIdx.x] = make_int2(piece.index, (int)((last_unit * run_ctas - 1) / run_total));
+        }
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(o_at + c * 32, o);
+          tmem_wait_ld();
+          if (c == DP / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[t]);
+          }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) st_global_v8_b32(tp.sums + at * DP + c * 32 + y * 8, o + y * 8);
+          __syncwarp();
+        }
+        g0 += n;
+        continue;
+      }
       const bool stored = in_tile && i < p.s_q;
       const bool live = stored && i < it.n_q && pos >= 0 && m != -INFINITY;  // sees something
       T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
       if (p.lse && stored)
         p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = live || isnan(l) && i < it.n_q ? (m + log2f(l)) * kLn2 : -INFINITY;
-      if (it.n > 0) {
-        if (!wait_all(&o_done[t], (g0 + it.n - 1) & 1, abort, tp, kErrTimeoutSoftmax)) break;
-        tc_fence_after();
-      }
       const bool some = live || (stored && i < it.n_q && isnan(l));
       const float inv = some ? 1.0f / l : 0.f;
       bool odd = false;
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t o[32];
-        if (it.n > 0) {
-          tmem_ld32(o_at + c * 32, o);
-          tmem_wait_ld();
-          if (c == DP / 32 - 1) {  // O may now be overwritten by the next item's first product
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_empty[t]);
-          }
+        tmem_ld32(o_at + c * 32, o);
+        tmem_wait_ld();
+        if (c == DP / 32 - 1) {  // O may now be overwritten by the next item's first product
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[t]);
         }
         if (stored) {
           uint32_t packed[16];
@@ -568,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       if (__any_sync(0xffffffffu, odd)) mend_rows<T>(p, odd, it.b, it.hk, pos, i, h);
-      g0 += it.n;
+      g0 += n;
     }
   }
 
@@ -578,6 +725,63 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
+}
+
+// Adds up the items that several CTAs share: 8 rows per CTA, a warp each.
+constexpr int kJoinRows = 8;
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kJoinRows * 32) join_kernel(const __grid_constant__ WindowParams p, const __grid_constant__ TensorParams tp) {
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = blockIdx.x, t = blockIdx.y / (kRows / kJoinRows);
+  const int row = blockIdx.y % (kRows / kJoinRows) * kJoinRows + warp;
+  const int2 span = tp.spans[first];
+  if (span.x < 0 || row >= tp.group * tp.tokens) return;
+  const Item it = item_of(p, tp, span.x);
+  constexpr int kCols = DP / 32;  // a lane's columns: lane * kCols on
+  const int token = row / tp.group, h = it.hk * tp.group + row - token * tp.group;
+  const int i = it.i0 + t * tp.tokens + token, pos = it.base + i;
+  if (i >= p.s_q) return;
+  // CTA c's share: the item began in CTA `first`, before every other
+  auto share = [&](int c) { return (((int64_t)c * 2 + (c == first)) * kTiles + t) * kRows + row; };
+  float m = -INFINITY;
+  for (int c = first + lane; c <= span.y; c += 32) m = fmaxf(m, __ldcg(tp.stats + share(c)).x);
+  m = warp_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[kCols];
+#pragma unroll
+  for (int x = 0; x < kCols; ++x) o[x] = 0.f;
+#pragma unroll 4
+  for (int c = first; c <= span.y; ++c) {
+    const float2 st = __ldcg(tp.stats + share(c));
+    const float weight = exp2f(st.x - base);
+    // a share that saw nothing of the row counts nothing, whatever its sums hold
+    const bool none = st.x == -INFINITY && !isnan(st.y);
+    l = none ? l : fmaf(st.y, weight, l);
+    const float *from = tp.sums + share(c) * DP + lane * kCols;
+#pragma unroll
+    for (int x = 0; x < kCols; x += 2) {
+      const float2 two = __ldcg(reinterpret_cast<const float2 *>(from + x));
+      o[x] = none ? o[x] : fmaf(two.x, weight, o[x]);
+      o[x + 1] = none ? o[x + 1] : fmaf(two.y, weight, o[x + 1]);
+    }
+  }
+  const bool some = i < it.n_q && pos >= 0 && (m != -INFINITY || isnan(l));
+  const float inv = some ? 1.0f / l : 0.f;
+  T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
+  bool odd = false;
+#pragma unroll
+  for (int x = 0; x < kCols; x += 2) {
+    const float a = some ? o[x] * inv : 0.f, b = some ? o[x + 1] * inv : 0.f;
+    if (lane * kCols + x < p.d) {
+      odd |= !isfinite(a) || !isfinite(b);
+      *reinterpret_cast<uint32_t *>(out + lane * kCols + x) = pack16<T>(a, b);
+    }
+  }
+  if (p.lse && lane == 0) p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
+  if (__any_sync(0xffffffffu, odd)) mend_rows<T>(p, lane == 0, it.b, it.hk, pos, i, h);
 }
 
 // ---------------------------------------------------------------- host side
@@ -637,7 +841,7 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
   using L = WindowLayout<DP>;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   auto *kernel = window_kernel<T, DP, POLY>;
-  TensorParams t;
+  TensorParams t = {};
   t.group = p.q_heads / p.kv_heads;
   t.tokens = kRows / t.group;
   CUtensorMap tq, tk, tv;
@@ -645,7 +849,7 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
   const int64_t q_strides[5] = {1, p.qs[2], p.qs[1], p.qs[2] * t.group, p.qs[0]};
   const int q_box[5] = {64, t.group, t.tokens, 1, 1};
   if (int rc = make_map(&tq, kBf16, p.q, 5, q_sizes, q_strides, q_box)) return rc;
-  const int kv_box[4] = {64, kKeys, 1, 1};
+  const int kv_box[4] = {64, kKeys / 2, 1, 1};  // a block's halves may come from two places
   auto keys_map = [&](CUtensorMap *map, const void *base, const int64_t *st, int *head, int *batch) {
     *head = st[2] != 0;
     *batch = st[0] != 0;
@@ -671,8 +875,40 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
       return rc;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const int grid = t.items < sm_count() ? t.items : sm_count();
-  return check_cuda(launch_pdl(kernel, dim3(grid), dim3(kThreads), L::kBytes, s, tq, tk, tv, p, t), "lc_window_attention");
+  // Whole items, or runs of blocks: where the most loaded CTA (the first one: items come longest
+  // first) has kCutUnits units more than its share.  Lengths on the device are not known here;
+  // the items may be short or empty then, and the longest is all that is left to go by.
+  const int sms = sm_count();
+  t.cut = 0;
+  if (items <= kMaxCutItems) {
+    const int heads = p.batch * p.kv_heads;
+    auto units = [&](int qb) {
+      const int64_t keys = (int64_t)p.s_kv - p.s_q + (int64_t)(qb + 1) * kTiles * t.tokens;
+      const int64_t reach = p.window ? (int64_t)p.window + kTiles * t.tokens + p.sinks : p.s_kv;
+      const int64_t seen = std::min(std::min(keys, reach), (int64_t)p.s_kv);
+      return seen <= 0 ? 0 : units_of((int)((seen + kKeys - 1) / kKeys));
+    };
+    int64_t total = 0, most = 0;
+    for (int qb = 0; qb < t.q_blocks; ++qb) total += (int64_t)units(qb) * heads;
+    for (int64_t i = 0; i < items; i += sms) most += units(t.q_blocks - 1 - (int)(i / heads));
+    const bool ragged = p.q_lens || p.kv_lens;
+    t.cut = total < (1 << 30) && (ragged ? units(t.q_blocks - 1) > kMinRun + kItemUnits : most - total / sms > kCutUnits);
+  }
+  int grid = t.items < sms ? t.items : sms;
+  if (t.cut) {
+    grid = sms;
+    void *mem = nullptr;
+    const size_t rows = (size_t)sms * 2 * kTiles * kRows;
+    if (int rc = scratch_buffer(s, kSpansSlot, sms * sizeof(int2), &mem)) return rc;
+    t.spans = static_cast<int2 *>(mem);
+    if (int rc = scratch_buffer(s, kSumsSlot, rows * 128 * sizeof(float), &mem)) return rc;
+    t.sums = static_cast<float *>(mem);
+    if (int rc = scratch_buffer(s, kStatsSlot, rows * sizeof(float2), &mem)) return rc;
+    t.stats = static_cast<float2 *>(mem);
+  }
+  if (int rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(kThreads), L::kBytes, s, tq, tk, tv, p, t), "lc_window_attention")) return rc;
+  if (!t.cut) return LC_OK;
+  return check_cuda(launch_pdl(join_kernel<T, DP>, dim3(sms, kTiles * kRows / kJoinRows), dim3(kJoinRows * 32), 0, s, p, t), "lc_window_attention (join)");
 }
 
 template <class T>
