@@ -71,8 +71,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) window_row_kernel(WindowParams
 // ---------------------------------------------------------------- tensor-core form
 // Flash attention on tcgen05, the schedule of sdpa.cu: per CTA two query tiles of
 // 128 rows share every block of 128 keys; warp 0 loads (TMA), one thread of warp 1
-// issues the products (S = Q K^T and O += P V, P from tensor memory), and a
-// warpgroup per tile does the softmax, one row per thread.  What is different:
+// issues the products (S = Q K^T and O += P V, P from tensor memory), a warpgroup per
+// tile does the softmax, one row per thread.  Under a window an item is only a few
+// blocks long, so its end must not stop the others: warp 2 works out the coming items
+// and leaves them in a ring, and a fourth warpgroup divides and stores the finished
+// tiles while the softmax is at the next item.  What else is different:
 //   rows    a tile's 128 rows are G heads of a group x 128 / G tokens (one 5-D TMA
 //           box), so a key block is loaded once for the whole group, and a tile spans
 //           few tokens: the keys that two tiles see are the window plus 2 x 128 / G,
@@ -104,11 +107,14 @@ constexpr int kMinRun = 6;     // units of a run: a shorter one costs more to jo
 constexpr int kCutUnits = 4;   // units that the join costs
 constexpr int kMaxCutItems = 2048;
 constexpr int kSpansSlot = 43, kSumsSlot = 44, kStatsSlot = 45;  // scratch_buffer slots
-constexpr int kThreads = 128 + kTiles * 128;
+constexpr int kThreads = 128 + kTiles * 128 + 128;  // loads and products, softmax, output
 // Registers per thread after the split: the softmax warpgroups' rows of 128 scores
-// need more than the 168 that 384 threads are launched with (spills otherwise);
-// 88 x 128 + 208 x 256 = 168 x 384.
-constexpr int kFewRegs = 88, kManyRegs = 208;
+// need more than the 128 that 512 threads are launched with, the others less;
+// 72 x 256 + 184 x 256 = 128 x 512.
+constexpr int kLaunchRegs = 128, kFewRegs = 72, kManyRegs = 184;
+constexpr int kLensHeld = 256;  // sequences whose lengths are kept in shared memory
+constexpr int kRing = 4;        // pieces of work known ahead
+constexpr int kReaders = 2 + 8 + 4;  // of a piece: loads, products, the softmax's and the output's warps
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;             // O of tile t at kOCol + t * DP; S of tile t at t * 128
 constexpr float kRescale = 8.0f;            // log2 units a row's maximum may lag behind
@@ -129,9 +135,9 @@ struct TensorParams {
   int *err;
   // runs of blocks (cut): the item that began in a CTA and goes on after it, or -1, and that
   // item's last CTA; a CTA's shares of the item that began before it, and of that one
-  int cut;
+  int cut, ctas;
   int2 *spans;
-  float *sums;              // [CTA][2][tile][row][DP]
+  float *sums;              // [CTA][2][tile][DP / 8][row][8]: 8 columns of a warp's rows lie together
   float2 *stats;            // [CTA][2][tile][row]: m and l
 };
 
@@ -145,15 +151,20 @@ struct Item {
 
 __device__ __forceinline__ int first_seen(int p, int window) { return window == 0 ? 0 : max(0, p - window + 1); }
 
-__device__ __forceinline__ Item item_of(const WindowParams &p, const TensorParams &t, int index) {
+// The lengths, from shared memory where they fit.
+struct Lens {
+  const int *q, *kv;
+};
+
+__device__ __forceinline__ Item item_of(const WindowParams &p, const TensorParams &t, const Lens &lens, int index) {
   Item it;
   const int heads = p.batch * p.kv_heads;
   const int qb = t.q_blocks - 1 - index / heads, bh = index % heads;
   it.b = bh / p.kv_heads;
   it.hk = bh - it.b * p.kv_heads;
   it.i0 = qb * kTiles * t.tokens;
-  it.n_q = length_of(p.q_lens, it.b, p.s_q);
-  it.n_kv = length_of(p.kv_lens, it.b, p.s_kv);
+  it.n_q = length_of(lens.q, it.b, p.s_q);
+  it.n_kv = length_of(lens.kv, it.b, p.s_kv);
   it.base = it.n_kv - it.n_q;
   const int last = min(it.i0 + kTiles * t.tokens, it.n_q) - 1;  // the last token that exists
   const int p_first = max(0, it.base + it.i0), p_last = it.base + last;
@@ -189,10 +200,10 @@ struct Piece {
 };
 struct Pieces {
   int index, skip, left;  // skip: units of the first item that lie before the run; left: the run's units (cut)
-  __device__ __forceinline__ bool next(const WindowParams &p, const TensorParams &t, Piece &out) {
+  __device__ __forceinline__ bool next(const WindowParams &p, const TensorParams &t, const Lens &lens, Piece &out) {
     for (;;) {
       if (index >= t.items || (t.cut && left <= 0)) return false;
-      out.it = item_of(p, t, index);
+      out.it = item_of(p, t, lens, index);
       out.index = index;
       out.j0 = 0;
       out.j1 = out.it.n;
@@ -226,6 +237,38 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
       : "memory");
 }
+// The products and their commits as issued by a whole warp: descriptors stay in uniform
+// registers, and `leader` (one lane, by elect.sync) issues.  From a branch that one lane
+// enters, every operand is moved there first, which takes longer than the product.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t leader;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
+  return leader;
+}
+__device__ __forceinline__ void warp_mma(uint32_t leader, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void warp_mma_tmem_a(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void warp_commit(uint32_t leader, uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Bits [lo, hi) of a 32-bit word (either bound may lie outside it).
@@ -286,6 +329,21 @@ __device__ __noinline__ void mend_rows(const WindowParams &p, bool odd, int b, i
   }
 }
 
+// The rows of a finished item, a lane each (row 0 .. 255 of its two tiles).
+template <class T>
+__device__ __noinline__ void mend_piece(const WindowParams &p, const TensorParams &tp, const Item &it, int tile_row) {
+  const int t = tile_row / kRows, row = tile_row % kRows;
+  const int token = row / tp.group, h = it.hk * tp.group + row - token * tp.group;
+  const int i = it.i0 + t * tp.tokens + token, pos = it.base + i;
+  bool odd = false;
+  if (row < tp.group * tp.tokens && i < it.n_q && pos >= 0) {
+    const T *out = static_cast<const T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
+    for (int c = 0; c < p.d; ++c) odd |= !isfinite(Elem<T>::to_float(out[c]));
+  }
+  __syncwarp();
+  if (__any_sync(0xffffffffu, odd)) mend_rows<T>(p, odd, it.b, it.hk, pos, i, h);
+}
+
 // POLY: of sixteen pairs of exponentials, how many go to the FMA pipe.
 template <class T, int DP, int POLY>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -301,16 +359,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *kv_s = smem + L::kQBytes;
   __shared__ __align__(8) uint64_t q_full, q_empty;
   __shared__ __align__(8) uint64_t k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
-  __shared__ __align__(8) uint64_t s_full[kTiles], p_full[kTiles], o_done[kTiles], o_empty[kTiles];
+  __shared__ __align__(8) uint64_t s_full[kTiles], p_full[kTiles], o_done[kTiles], o_empty[kTiles], stat_full[kTiles];
+  __shared__ float2 stat[kTiles][kRows];  // m and l of a tile's rows, from the softmax to the output warps
+  __shared__ int held_lens[2][kLensHeld];
   __shared__ uint32_t tmem_base;
-  __shared__ int abort_flag;
+  __shared__ int abort_flag, any_odd;
   __shared__ int warp_blocks[kThreads / 32];
   __shared__ Pieces run;
   __shared__ int run_end, run_total, run_ctas;
+  __shared__ Piece ring[kRing];
+  __shared__ __align__(8) uint64_t piece_full[kRing], piece_empty[kRing];
   volatile int *abort = &abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    for (int r = 0; r < kRing; ++r) {
+      mbar_init(&piece_full[r], 1);
+      mbar_init(&piece_empty[r], kReaders);
+    }
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 1);
     for (int s = 0; s < kStages; ++s) {
@@ -324,8 +390,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
       mbar_init(&o_empty[t], 4);
+      mbar_init(&stat_full[t], 4);
     }
     abort_flag = 0;
+    any_odd = 0;
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -343,6 +411,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_base;
   pdl_wait();
   pdl_trigger();
+  Lens lens = {p.q_lens, p.kv_lens};
+  if (p.batch <= kLensHeld && (lens.q || lens.kv)) {
+    for (int b = threadIdx.x; b < p.batch; b += kThreads) {
+      held_lens[0][b] = length_of(p.q_lens, b, p.s_q);
+      held_lens[1][b] = length_of(p.kv_lens, b, p.s_kv);
+    }
+    lens = {held_lens[0], held_lens[1]};
+    __syncthreads();
+  }
   if (!tp.cut) {
     if (threadIdx.x == 0) run = {(int)blockIdx.x, 0, 0};
   } else {
@@ -350,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int per = (tp.items + kThreads - 1) / kThreads;
     const int first = min(tp.items, (int)threadIdx.x * per), last = min(tp.items, first + per);
     int own = 0;
-    for (int i = first; i < last; ++i) own += units_of(item_of(p, tp, i).n);
+    for (int i = first; i < last; ++i) own += units_of(item_of(p, tp, lens, i).n);
     int inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -371,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if ((int)blockIdx.x < ctas && begin >= before && begin < before + own) {
       int at = before, i = first;
       for (;; ++i) {
-        const int n = units_of(item_of(p, tp, i).n);
+        const int n = units_of(item_of(p, tp, lens, i).n);
         if (begin < at + n) break;
         at += n;
       }
@@ -385,19 +462,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncthreads();
-  Pieces pieces = run;
-  Piece piece;
   // Every barrier phase counts over all blocks of the CTA's items: block g (over all
   // items) uses stage g & 1, and s_full / p_full / o_done complete once per block.
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
-    if (warp == 0 && lane == 0) {
+    if (warp == 2 && lane == 0) {
+      Pieces pieces = run;
+      Piece piece;
+      for (int k = 0;; ++k) {
+        const int r = k % kRing;
+        const bool more = pieces.next(p, tp, lens, piece);
+        if (!more) piece.j0 = piece.j1 = 0;  // the end
+        if (k >= kRing && !mbar_wait(&piece_empty[r], (k / kRing - 1) & 1, abort)) {
+          give_up(tp, abort, kErrTimeoutProducer);
+          break;
+        }
+        ring[r] = piece;
+        mbar_arrive(&piece_full[r]);
+        if (!more) break;
+      }
+    } else if (warp == 0 && lane == 0) {
       int g = 0, local = 0;
       bool ok = true;
       const uint32_t q_bytes = kTiles * DP / 64 * tp.group * tp.tokens * 128;
-      while (ok && pieces.next(p, tp, piece)) {
+      while (ok) {
+        const int r = local % kRing;
+        if (!mbar_wait(&piece_full[r], local / kRing & 1, abort)) {
+          give_up(tp, abort, kErrTimeoutProducer);
+          break;
+        }
+        const Piece piece = ring[r];
         const Item &it = piece.it;
+        mbar_arrive(&piece_empty[r]);
+        if (piece.j1 == 0) break;
         // Q of the previous item is free once its last S products completed
         if (local > 0 && !mbar_wait(&q_empty, (local - 1) & 1, abort)) {
           give_up(tp, abort, kErrTimeoutProducer);
@@ -435,7 +533,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
+      const uint32_t leader = elect_one();
       constexpr uint32_t idesc_s = idesc_f16(kBf16, false, false, kRows, kKeys);
       constexpr uint32_t idesc_o = idesc_f16(kBf16, false, true, kRows, DP);
       const uint64_t q_desc = smem_desc_sw128(smem_u32(q_s), 16, 1024);
@@ -448,82 +547,98 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t off = ((k >> 2) * kChunkBytes + (k & 3) * 32) / 16;
-          mma_f16(tmem + t * kKeys, qd + off, kd + off, idesc_s, k > 0);
+          warp_mma(leader, tmem + t * kKeys, qd + off, kd + off, idesc_s, k > 0);
         }
-        mma_commit(&s_full[t]);
+        warp_commit(leader, &s_full[t]);
       };
       auto issue_pv = [&](int t, int g, bool first) {  // O_t (+)= P_t V(block g), P_t over S_t
         const uint64_t vd = v_desc + (uint64_t)((g & 1) * kStageStep);
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
-          mma_f16_tmem_a(tmem + kOCol + t * DP, tmem + t * kKeys + k * 8, vd + (uint64_t)(k * 2048 / 16), idesc_o, !(first && k == 0));
-        mma_commit(&o_done[t]);
+          warp_mma_tmem_a(leader, tmem + kOCol + t * DP, tmem + t * kKeys + k * 8, vd + (uint64_t)(k * 2048 / 16), idesc_o, !(first && k == 0));
+        warp_commit(leader, &o_done[t]);
       };
-      int g0 = 0, local = 0;
+      // One order over all pieces: PV_0(g), S_0(g + 1), PV_1(g), S_1(g + 1), where block
+      // g + 1 may be the next piece's first.
+      int g = 0, local = 0, n = 0, next_n = 0;
       bool ok = true;
-      while (ok && pieces.next(p, tp, piece)) {
-        const int n = piece.j1 - piece.j0;
-        ok = mbar_wait(&q_full, local & 1, abort) && mbar_wait(&k_full[g0 & 1], (g0 >> 1) & 1, abort);
-        if (!ok) break;
-        tc_fence_after();
-        for (int t = 0; t < kTiles; ++t) issue_s(t, g0);
-        mma_commit(&k_empty[g0 & 1]);
-        if (n == 1) mma_commit(&q_empty);
-        for (int j = 0; ok && j < n; ++j) {
-          const int g = g0 + j, st = g & 1;
-          const uint32_t ph = (g >> 1) & 1;
-          const bool next = j + 1 < n;
+      auto blocks = [&](int k) {  // of the k-th piece; 0: there is none
+        const int r = k % kRing;
+        if (!mbar_wait(&piece_full[r], k / kRing & 1, abort)) {
+          ok = false;
+          return 0;
+        }
+        const int count = ring[r].j1 - ring[r].j0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&piece_empty[r]);
+        return count;
+      };
+      n = blocks(0);
+      if (n > 0) {
+        ok = mbar_wait(&q_full, 0, abort) && mbar_wait(&k_full[0], 0, abort);
+        if (ok) {
+          tc_fence_after();
+          for (int t = 0; t < kTiles; ++t) issue_s(t, 0);
+          warp_commit(leader, &k_empty[0]);
+          if (n == 1) warp_commit(leader, &q_empty);
+        }
+      }
+      while (ok && n > 0) {
+        next_n = blocks(local + 1);
+        for (int j = 0; ok && j < n; ++j, ++g) {
+          const int st = g & 1;
+          const bool last = j + 1 == n, more = !last || next_n > 0;
           for (int t = 0; t < kTiles; ++t) {
-            if ((t == 0 && !mbar_wait(&v_full[st], ph, abort)) ||
-                (t == 0 && next && !mbar_wait(&k_full[(g + 1) & 1], ((g + 1) >> 1) & 1, abort)) ||
+            if ((t == 0 && !mbar_wait(&v_full[st], (g >> 1) & 1, abort)) ||
                 (j == 0 && local > 0 && !mbar_wait(&o_empty[t], (local - 1) & 1, abort)) ||
+                (t == 0 && !last && !mbar_wait(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort)) ||
                 !mbar_wait(&p_full[t], g & 1, abort)) {
               ok = false;
               break;
             }
             tc_fence_after();
             issue_pv(t, g, j == 0);
-            if (t == kTiles - 1) mma_commit(&v_empty[st]);
-            if (next) {
+            if (t == kTiles - 1) warp_commit(leader, &v_empty[st]);
+            if (more) {
+              if (t == 0 && last) {
+                if (!mbar_wait(&q_full, (local + 1) & 1, abort) || !mbar_wait(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+              }
               issue_s(t, g + 1);
               if (t == kTiles - 1) {
-                mma_commit(&k_empty[(g + 1) & 1]);
-                if (j + 2 == n) mma_commit(&q_empty);  // the item's last S products
+                warp_commit(leader, &k_empty[st ^ 1]);
+                if (last ? next_n == 1 : j + 2 == n) warp_commit(leader, &q_empty);  // a piece's last S products
               }
             }
           }
         }
         ++local;
-        g0 += n;
+        n = next_n;
       }
-      if (!ok) give_up(tp, abort, kErrTimeoutMma);
+      if (!ok && lane == 0) give_up(tp, abort, kErrTimeoutMma);
     }
-  } else {
+  } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
     const int t = (warp - 4) >> 2;  // query tile of this warpgroup
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_at = tmem + lane_base + t * kKeys, o_at = tmem + lane_base + kOCol + t * DP;
-    const bool in_tile = row < tp.group * tp.tokens;
-    const int token = row / tp.group, head = row - token * tp.group;
-    int g0 = 0;
+    const int token = row / tp.group;
+    int g0 = 0, local = 0;
     bool ok = true;
-    // items that see nothing: zeros
-    for (int index = blockIdx.x; index < tp.items; index += gridDim.x) {
-      const Item it = item_of(p, tp, index);
-      const int i = it.i0 + t * tp.tokens + token, h = it.hk * tp.group + head;
-      if (it.n > 0 || !in_tile || i >= p.s_q) continue;
-      T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
-      for (int c = 0; c < p.d; c += 8) *reinterpret_cast<uint4 *>(out + c) = make_uint4(0, 0, 0, 0);
-      if (p.lse) p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = -INFINITY;
-    }
-    __syncwarp();
-    while (ok && pieces.next(p, tp, piece)) {
+    while (ok) {
+      if (!wait_all(&piece_full[local % kRing], local / kRing & 1, abort, tp, kErrTimeoutSoftmax)) break;
+      const Piece piece = ring[local % kRing];
       const Item &it = piece.it;
       const int n = piece.j1 - piece.j0;
-      const int i = it.i0 + t * tp.tokens + token, h = it.hk * tp.group + head;
-      const int pos = it.base + i;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&piece_empty[local % kRing]);
+      if (n == 0) break;
+      const int pos = it.base + it.i0 + t * tp.tokens + token;
       const int p_low = it.base + it.i0 + t * tp.tokens, p_high = p_low + tp.tokens - 1;
       float m = -INFINITY, l = 0.f;
       for (int x = 0; x < n; ++x) {
@@ -562,9 +677,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t sees = bits_between(from - c * 32, to - c * 32) | bits_between(sunk_from - c * 32, sunk - c * 32);
+            if (sees != 0xffffffffu) {
 #pragma unroll
-            for (int y = 0; y < 32; ++y)
-              if (!(sees >> y & 1)) sr[c][y] = __float_as_uint(-INFINITY);
+              for (int y = 0; y < 32; ++y)
+                if (!(sees >> y & 1)) sr[c][y] = __float_as_uint(-INFINITY);
+            }
           }
         }
         if (key + kKeys > it.n_kv && it.n_kv < p.s_kv) {
@@ -647,74 +764,116 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
       if (!ok) break;
-      if (!wait_all(&o_done[t], (g0 + n - 1) & 1, abort, tp, kErrTimeoutSoftmax)) break;
-      tc_fence_after();
-      if (n < it.n) {  // a share of the item: unnormalised, for join_kernel
-        const int64_t at = (((int64_t)blockIdx.x * 2 + (piece.j0 == 0)) * kTiles + t) * kRows + row;
-        tp.stats[at] = make_float2(m, l);
-        if (piece.j0 == 0 && t == 0 && row == 0) {  // the run's last piece: it goes on in the next CTA's
-          const int64_t last_unit = run_end - (piece.j1 + kItemUnits) + units_of(it.n);
-          tp.spans[blockIdx.x] = make_int2(piece.index, (int)((last_unit * run_ctas - 1) / run_total));
+      // the output warps have read the piece before's
+      if (local > 0 && !wait_all(&o_empty[t], (local - 1) & 1, abort, tp, kErrTimeoutSoftmax)) break;
+      stat[t][row] = make_float2(m, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&stat_full[t]);
+      ++local;
+      g0 += n;
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const bool in_tile = row < tp.group * tp.tokens;
+    const int token = row / tp.group, head = row - token * tp.group;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    int g0 = 0, local = 0;
+    bool ok = true;
+    // items that see nothing: zeros
+    for (int index = blockIdx.x; index < tp.items; index += gridDim.x) {
+      const Item it = item_of(p, tp, lens, index);
+      if (it.n > 0 || !in_tile) continue;
+      for (int t = 0; t < kTiles; ++t) {
+        const int i = it.i0 + t * tp.tokens + token, h = it.hk * tp.group + head;
+        if (i >= p.s_q) continue;
+        T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
+        for (int c = 0; c < p.d; c += 8) *reinterpret_cast<uint4 *>(out + c) = make_uint4(0, 0, 0, 0);
+        if (p.lse) p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = -INFINITY;
+      }
+    }
+    __syncwarp();
+    while (ok) {
+      if (!wait_all(&piece_full[local % kRing], local / kRing & 1, abort, tp, kErrTimeoutEpilogue)) break;
+      const Piece piece = ring[local % kRing];
+      const Item &it = piece.it;
+      const int n = piece.j1 - piece.j0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&piece_empty[local % kRing]);
+      if (n == 0) break;
+      for (int t = 0; t < kTiles; ++t) {
+        const uint32_t o_at = tmem + lane_base + kOCol + t * DP;
+        const int i = it.i0 + t * tp.tokens + token, h = it.hk * tp.group + head;
+        if (!wait_all(&stat_full[t], local & 1, abort, tp, kErrTimeoutEpilogue) ||
+            !wait_all(&o_done[t], (g0 + n - 1) & 1, abort, tp, kErrTimeoutEpilogue)) {
+          ok = false;
+          break;
         }
+        tc_fence_after();
+        const float m = stat[t][row].x, l = stat[t][row].y;
+        if (n < it.n) {  // a share of the item: unnormalised, for join_kernel
+          const int64_t at = (((int64_t)blockIdx.x * 2 + (piece.j0 == 0)) * kTiles + t) * kRows + row;
+          tp.stats[at] = make_float2(m, l);
+          if (piece.j0 == 0 && t == 0 && row == 0) {  // the run's last piece: it goes on in the next CTA's
+            const int64_t last_unit = run_end - (piece.j1 + kItemUnits) + units_of(it.n);
+            tp.spans[blockIdx.x] = make_int2(piece.index, (int)((last_unit * run_ctas - 1) / run_total));
+          }
 #pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(o_at + c * 32, o);
-          tmem_wait_ld();
-          if (c == DP / 32 - 1) {
-            tc_fence_before();
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_at + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 4; ++y) st_global_v8_b32(tp.sums + (at - row) * DP + ((c * 4 + y) * kRows + row) * 8, o + y * 8);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&o_empty[t]);
           }
-#pragma unroll
-          for (int y = 0; y < 4; ++y) st_global_v8_b32(tp.sums + at * DP + c * 32 + y * 8, o + y * 8);
-          __syncwarp();
-        }
-        g0 += n;
-        continue;
-      }
-      const bool stored = in_tile && i < p.s_q;
-      const bool live = stored && i < it.n_q && pos >= 0 && m != -INFINITY;  // sees something
-      T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
-      if (p.lse && stored)
-        p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = live || isnan(l) && i < it.n_q ? (m + log2f(l)) * kLn2 : -INFINITY;
-      const bool some = live || (stored && i < it.n_q && isnan(l));
-      const float inv = some ? 1.0f / l : 0.f;
-      bool odd = false;
+        } else {
+          const bool stored = in_tile && i < p.s_q;
+          // sees something (a row of NaN scores has no maximum)
+          const bool some = stored && i < it.n_q && it.base + i >= 0 && (m != -INFINITY || isnan(l));
+          const float inv = some ? 1.0f / l : 0.f;
+          const uint64_t inv2 = pack2(inv, inv);
+          T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
+          if (p.lse && stored) p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
+          bool odd = false;
 #pragma unroll 1
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(o_at + c * 32, o);
-        tmem_wait_ld();
-        if (c == DP / 32 - 1) {  // O may now be overwritten by the next item's first product
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_empty[t]);
-        }
-        if (stored) {
-          uint32_t packed[16];
-          float top = 0.f;
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_at + c * 32, o);
+            tmem_wait_ld();
+            if (stored) {
+              uint32_t packed[16];
+              uint64_t zero[2] = {0ull, 0ull};  // NaN once a value is infinite or NaN
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const float a = some ? __uint_as_float(o[2 * x]) * inv : 0.f, b = some ? __uint_as_float(o[2 * x + 1]) * inv : 0.f;
-            top = max_nan(top, max_nan(fabsf(a), fabsf(b)));
-            packed[x] = pack16<T>(a, b);
-          }
-          odd |= !isfinite(top) && c * 32 < p.d;
-          T *to = out + c * 32;
-          if (tp.o_vec == 2) {
-            if (c * 32 + 16 <= p.d) st_global_v8_b32(to, packed);
-            if (c * 32 + 32 <= p.d) st_global_v8_b32(to + 16, packed + 8);
-          } else {
+              for (int x = 0; x < 16; ++x) {
+                const uint64_t two = ffma2(pack2(__uint_as_float(o[2 * x]), __uint_as_float(o[2 * x + 1])), inv2, 0ull);
+                zero[x & 1] = ffma2(two, 0ull, zero[x & 1]);
+                const float2 ab = unpack2(two);
+                packed[x] = some ? pack16<T>(ab.x, ab.y) : 0u;
+              }
+              const float2 z = unpack2(fadd2(zero[0], zero[1]));
+              odd |= some && !(z.x + z.y == 0.f);
+              T *to = out + c * 32;
+              if (tp.o_vec == 2) {
+                if (c * 32 + 16 <= p.d) st_global_v8_b32(to, packed);
+                if (c * 32 + 32 <= p.d) st_global_v8_b32(to + 16, packed + 8);
+              } else {
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (c * 32 + x * 8 + 8 <= p.d)
-                reinterpret_cast<uint4 *>(to)[x] = make_uint4(packed[4 * x], packed[4 * x + 1], packed[4 * x + 2], packed[4 * x + 3]);
+                for (int x = 0; x < 4; ++x)
+                  if (c * 32 + x * 8 + 8 <= p.d)
+                    reinterpret_cast<uint4 *>(to)[x] = make_uint4(packed[4 * x], packed[4 * x + 1], packed[4 * x + 2], packed[4 * x + 3]);
+              }
+            }
+            __syncwarp();
           }
+          if (odd) any_odd = 1;
         }
+        tc_fence_before();
         __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[t]);  // O and the tile's m and l are free
       }
-      if (__any_sync(0xffffffffu, odd)) mend_rows<T>(p, odd, it.b, it.hk, pos, i, h);
+      ++local;
       g0 += n;
     }
   }
@@ -725,63 +884,135 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
+  if (any_odd && !abort_flag) {
+    // Some row of some whole item holds an infinite or NaN output (a rare case: it is not
+    // kept which): look at all of them.
+    if (warp >= 4 && warp < 12)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));
+    else
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));
+    Pieces pieces = run;
+    Piece piece;
+    while (pieces.next(p, tp, lens, piece)) {
+      if (piece.j1 - piece.j0 < piece.it.n) continue;
+      for (int first = warp * 32; first < kTiles * kRows; first += kThreads)
+        mend_piece<T>(p, tp, piece.it, first + lane);
+    }
+  }
 }
 
-// Adds up the items that several CTAs share: 8 rows per CTA, a warp each.
-constexpr int kJoinRows = 8;
-
-template <class T, int DP>
-__global__ void __launch_bounds__(kJoinRows * 32) join_kernel(const __grid_constant__ WindowParams p, const __grid_constant__ TensorParams tp) {
+// Adds up the items that several CTAs share.  A warp takes 8 rows, four lanes each, so
+// that a load instruction reads 256 bytes together and a part's 16 of them are in
+// flight at once.  DEEP (few items, many parts of each): the CTA's warps share 8 rows
+// and deal the parts among themselves; blockIdx.x counts the shared items.  Else each
+// warp has rows of its own, and blockIdx.x is the CTA that an item began in; most find
+// nothing and leave.  19 parts of 8 items: 5 us against 16 us with rows of its own.
+template <class T, int DP, bool DEEP>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ WindowParams p, const __grid_constant__ TensorParams tp) {
+  constexpr int kSums = DEEP ? 8 : 1;
+  __shared__ float warp_m[kSums][32], warp_l[kSums][32];
+  __shared__ float2 warp_o[kSums][DP / 8][32];
+  __shared__ int found;
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = blockIdx.x, t = blockIdx.y / (kRows / kJoinRows);
-  const int row = blockIdx.y % (kRows / kJoinRows) * kJoinRows + warp;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int first = blockIdx.x;
+  if (DEEP) {  // the CTA in which the blockIdx.x-th shared item began
+    if (threadIdx.x == 0) found = -1;
+    __syncthreads();
+    if (warp == 0) {
+      int left = blockIdx.x;
+      for (int base = 0; base < tp.ctas; base += 32) {
+        const unsigned some = __ballot_sync(0xffffffffu, base + lane < tp.ctas && tp.spans[base + lane].x >= 0);
+        const int here = __popc(some);
+        if (left < here) {
+          if ((some >> lane & 1) && __popc(some & ((1u << lane) - 1)) == left) found = base + lane;
+          break;
+        }
+        left -= here;
+      }
+    }
+    __syncthreads();
+    first = found;
+    if (first < 0) return;
+  }
   const int2 span = tp.spans[first];
-  if (span.x < 0 || row >= tp.group * tp.tokens) return;
-  const Item it = item_of(p, tp, span.x);
-  constexpr int kCols = DP / 32;  // a lane's columns: lane * kCols on
+  if (span.x < 0) return;
+  const Item it = item_of(p, tp, {p.q_lens, p.kv_lens}, span.x);
+  const int tile_row = (DEEP ? blockIdx.y : blockIdx.y * 8 + warp) * 8 + (lane >> 2), t = tile_row / kRows, row = tile_row % kRows;
   const int token = row / tp.group, h = it.hk * tp.group + row - token * tp.group;
   const int i = it.i0 + t * tp.tokens + token, pos = it.base + i;
-  if (i >= p.s_q) return;
+  const bool stored = row < tp.group * tp.tokens && i < p.s_q;
+  if (!__any_sync(0xffffffffu, stored)) return;  // (the same rows in every warp where DEEP)
   // CTA c's share: the item began in CTA `first`, before every other
-  auto share = [&](int c) { return (((int64_t)c * 2 + (c == first)) * kTiles + t) * kRows + row; };
-  float m = -INFINITY;
-  for (int c = first + lane; c <= span.y; c += 32) m = fmaxf(m, __ldcg(tp.stats + share(c)).x);
-  m = warp_max(m);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[kCols];
-#pragma unroll
-  for (int x = 0; x < kCols; ++x) o[x] = 0.f;
+  auto share = [&](int c) { return ((int64_t)c * 2 + (c == first)) * kTiles + t; };
+  const int begin = first + (DEEP ? warp : 0), step = DEEP ? 8 : 1;
+  float m = -INFINITY, l = 0.f;
 #pragma unroll 4
-  for (int c = first; c <= span.y; ++c) {
-    const float2 st = __ldcg(tp.stats + share(c));
+  for (int c = begin; c <= span.y; c += step) m = fmaxf(m, __ldcg(tp.stats + share(c) * kRows + row).x);
+  const float base = m == -INFINITY ? 0.f : m;
+  float2 o[DP / 8];  // columns 8 y + 2 (lane % 4) on
+#pragma unroll
+  for (int y = 0; y < DP / 8; ++y) o[y] = make_float2(0.f, 0.f);
+#pragma unroll 2
+  for (int c = begin; c <= span.y; c += step) {
+    const float2 st = __ldcg(tp.stats + share(c) * kRows + row);
     const float weight = exp2f(st.x - base);
     // a share that saw nothing of the row counts nothing, whatever its sums hold
     const bool none = st.x == -INFINITY && !isnan(st.y);
     l = none ? l : fmaf(st.y, weight, l);
-    const float *from = tp.sums + share(c) * DP + lane * kCols;
+    const float *from = tp.sums + (share(c) * DP * kRows + row * 8) + (lane & 3) * 2;
 #pragma unroll
-    for (int x = 0; x < kCols; x += 2) {
-      const float2 two = __ldcg(reinterpret_cast<const float2 *>(from + x));
-      o[x] = none ? o[x] : fmaf(two.x, weight, o[x]);
-      o[x + 1] = none ? o[x + 1] : fmaf(two.y, weight, o[x + 1]);
+    for (int y = 0; y < DP / 8; ++y) {
+      const float2 two = __ldcg(reinterpret_cast<const float2 *>(from + y * kRows * 8));
+      o[y].x = none ? o[y].x : fmaf(two.x, weight, o[y].x);
+      o[y].y = none ? o[y].y : fmaf(two.y, weight, o[y].y);
     }
   }
-  const bool some = i < it.n_q && pos >= 0 && (m != -INFINITY || isnan(l));
+  constexpr int kMine = DP / 8 / kSums;  // columns' groups that this warp writes
+  if (DEEP) {
+    warp_m[warp][lane] = m;
+    warp_l[warp][lane] = l;
+#pragma unroll
+    for (int y = 0; y < DP / 8; ++y) warp_o[warp][y][lane] = o[y];
+    __syncthreads();
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSums; ++w) m = fmaxf(m, warp_m[w][lane]);
+    const float all = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int y = 0; y < kMine; ++y) o[y] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kSums; ++w) {
+      const float weight = exp2f(warp_m[w][lane] - all);
+      l = fmaf(warp_l[w][lane], weight, l);  // (a warp without parts has sums of zero)
+#pragma unroll
+      for (int y = 0; y < kMine; ++y) {
+        const float2 two = warp_o[w][warp * kMine + y][lane];
+        o[y].x = fmaf(two.x, weight, o[y].x);
+        o[y].y = fmaf(two.y, weight, o[y].y);
+      }
+    }
+  }
+  const int col = (DEEP ? warp * kMine : 0) * 8 + (lane & 3) * 2;
+  const bool some = stored && i < it.n_q && pos >= 0 && (m != -INFINITY || isnan(l));
   const float inv = some ? 1.0f / l : 0.f;
   T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
   bool odd = false;
 #pragma unroll
-  for (int x = 0; x < kCols; x += 2) {
-    const float a = some ? o[x] * inv : 0.f, b = some ? o[x + 1] * inv : 0.f;
-    if (lane * kCols + x < p.d) {
+  for (int y = 0; y < kMine; ++y) {
+    const float a = some ? o[y].x * inv : 0.f, b = some ? o[y].y * inv : 0.f;
+    if (stored && col + y * 8 < p.d) {
       odd |= !isfinite(a) || !isfinite(b);
-      *reinterpret_cast<uint32_t *>(out + lane * kCols + x) = pack16<T>(a, b);
+      *reinterpret_cast<uint32_t *>(out + col + y * 8) = pack16<T>(a, b);
     }
   }
-  if (p.lse && lane == 0) p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
-  if (__any_sync(0xffffffffu, odd)) mend_rows<T>(p, lane == 0, it.b, it.hk, pos, i, h);
+  if (p.lse && stored && (lane & 3) == 0 && (!DEEP || warp == 0))
+    p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
+  if (DEEP) __syncthreads();  // the other warps' columns are there: mended once or more, but alike
+  const unsigned odd_lanes = __ballot_sync(0xffffffffu, odd);
+  if (odd_lanes) mend_rows<T>(p, (lane & 3) == 0 && (odd_lanes >> lane & 0xf) != 0, it.b, it.hk, pos, i, h);
 }
 
 // ---------------------------------------------------------------- host side
@@ -896,7 +1127,7 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
   }
   int grid = t.items < sms ? t.items : sms;
   if (t.cut) {
-    grid = sms;
+    grid = t.ctas = sms;
     void *mem = nullptr;
     const size_t rows = (size_t)sms * 2 * kTiles * kRows;
     if (int rc = scratch_buffer(s, kSpansSlot, sms * sizeof(int2), &mem)) return rc;
@@ -908,7 +1139,10 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
   }
   if (int rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(kThreads), L::kBytes, s, tq, tk, tv, p, t), "lc_window_attention")) return rc;
   if (!t.cut) return LC_OK;
-  return check_cuda(launch_pdl(join_kernel<T, DP>, dim3(sms, kTiles * kRows / kJoinRows), dim3(kJoinRows * 32), 0, s, p, t), "lc_window_attention (join)");
+  const bool deep = items * 4 <= sms;  // an item then spans four CTAs or more
+  const cudaError_t err = deep ? launch_pdl(join_kernel<T, DP, true>, dim3(t.items, kTiles * kRows / 8), dim3(256), 0, s, p, t)
+                               : launch_pdl(join_kernel<T, DP, false>, dim3(sms, kTiles * kRows / 64), dim3(256), 0, s, p, t);
+  return check_cuda(err, "lc_window_attention (join)");
 }
 
 template <class T>
