@@ -3,7 +3,9 @@
 Every ``csrc/*.cu`` file is compiled to an object in ``_build/`` (in
 parallel, skipped when the object is newer than its sources) and linked into
 ``lazy_compiler_b200/liblazyb200.so`` with the CUDA runtime linked
-statically, so the library only needs the driver at run time.
+statically, so the library only needs the driver at run time.  The Python
+side of the serving operators, ``csrc/serving_ext.cpp``, becomes the extension
+module ``_serving`` beside it (against the installed torch's headers).
 ``python -m lazy_compiler_b200.build`` runs it from the command line.
 """
 from __future__ import annotations
@@ -21,6 +23,7 @@ CSRC = PACKAGE / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIBRARY = PACKAGE / "liblazyb200.so"
+EXTENSION = PACKAGE / "_serving.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -54,15 +57,37 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _build_extension(force: bool) -> None:
+    src = CSRC / "serving_ext.cpp"
+    newest = max(p.stat().st_mtime for p in (src, *INCLUDE.glob("*.h")))
+    if EXTENSION.exists() and EXTENSION.stat().st_mtime >= newest and not force:
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    includes = [INCLUDE, *include_paths(), Path(nvcc()).resolve().parents[1] / "include", sysconfig.get_paths()["include"]]
+    tmp = EXTENSION.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in includes), str(src), "-o", str(tmp),
+           *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode:
+        raise RuntimeError(f"{cmd[0]} failed on {src.name}:\n{result.stderr}")
+    os.replace(tmp, EXTENSION)
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
-    """Compile every kernel source and link the shared library; returns its path."""
+    """Compile every kernel source, link the shared library and the extension module; returns the library's path."""
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     if force:
         for obj in BUILD.glob("*.o"):
             obj.unlink()
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        extension = pool.submit(_build_extension, force)
         objects = list(pool.map(lambda s: _compile(s, verbose), sources))
+        extension.result()
     newest = max(o.stat().st_mtime for o in objects)
     if not LIBRARY.exists() or LIBRARY.stat().st_mtime < newest or force:
         tmp = LIBRARY.with_suffix(".so.tmp")

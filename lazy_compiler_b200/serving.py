@@ -15,18 +15,40 @@ needs the host: a decode step can be captured in a CUDA graph.  Operations on ma
 given ones, which may be the same (not for :func:`cache_fork`).  :class:`PagedCache` keeps a pool with its maps.
 
 A tensor used on another stream than the one it was made on needs ``record_stream`` or an event, as any torch tensor.
+The library's workspaces belong to a stream and grow on its first calls: before a capture, run the step once on the
+stream that will capture it.
 """
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import NamedTuple
 
 import torch
 
 from . import runtime
 
-_DTYPES = {torch.float16: runtime.LC_F16, torch.bfloat16: runtime.LC_BF16}
+# the order in which csrc/serving_ext.cpp takes the entry points
+_ENTRIES = ("lc_window_attention", "lc_paged_decode", "lc_cache_extend", "lc_cache_write", "lc_cache_fork", "lc_cache_release",
+            "lc_cache_compact", "lc_cache_copy")
+
+
+def _extension():
+    """The extension module, bound to the loaded library.  There is no other path: unbuilt, this raises."""
+    library = runtime.library()
+    try:
+        from . import _serving
+    except ImportError as e:
+        raise RuntimeError("the extension module _serving is not built; run `python -m lazy_compiler_b200.build`") from e
+    _serving.bind(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in _ENTRIES))
+    return _serving
+
+
+_ext = _extension()
+
+
+def _failed(name: str, status: int):
+    """The error of a C-ABI call."""
+    return runtime.LcError(name, status, runtime.last_error())
 
 
 class CacheMaps(NamedTuple):
@@ -40,49 +62,6 @@ class CacheMaps(NamedTuple):
     status: torch.Tensor | None = None
 
 
-def _stream(stream, device) -> int:
-    return stream if stream is not None else torch.cuda.current_stream(device).cuda_stream
-
-
-def _call(name: str, device, *args) -> None:
-    """Calls the entry point with ``device`` current."""
-    if device.index == torch.cuda.current_device():
-        runtime.call(name, *args)
-    else:
-        with torch.cuda.device(device):
-            runtime.call(name, *args)
-
-
-def _check(t: torch.Tensor, what: str, device, dtype, shape: tuple) -> None:
-    if t.dtype != dtype or t.device != device:
-        raise ValueError(f"{what}: {t.dtype} on {t.device}, expected {dtype} on {device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
-
-
-def _check_ints(t: torch.Tensor, what: str, device, shape: tuple) -> None:
-    _check(t, what, device, torch.int32, shape)
-    if not t.is_contiguous():
-        raise ValueError(f"{what}: must be contiguous")
-
-
-def _attention_dtype(q: torch.Tensor, what: str) -> int:
-    if q.dtype not in _DTYPES:
-        raise ValueError(f"{what}: {q.dtype} is not float16 or bfloat16")
-    if not q.is_cuda:
-        raise ValueError(f"{what}: on {q.device}, the kernels run on CUDA devices only")
-    return _DTYPES[q.dtype]
-
-
-def _inner(t: torch.Tensor, what: str) -> None:
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what}: the last axis must be contiguous")
-
-
-def _scale(scale, d: int) -> float:
-    return 1.0 / math.sqrt(d) if scale is None else float(scale)
-
-
 def window_attention(q, k, v, *, window: int = 0, sinks: int = 0, scale: float | None = None, q_lens=None, kv_lens=None,
                      out=None, return_lse: bool = False, stream: int | None = None):
     """Causal attention of ``q[batch, s_q, q_heads, d]`` over ``k, v[batch, s_kv, kv_heads, d]`` (f16 or bf16).
@@ -93,30 +72,10 @@ def window_attention(q, k, v, *, window: int = 0, sinks: int = 0, scale: float |
     where given), with ``return_lse`` also the log-sum-exp of the scaled scores, f32 ``[batch, q_heads, s_q]``.  Rows
     that see nothing, and rows from ``q_lens[b]`` on, are 0 and -inf.  Any strides with a contiguous last axis.
     """
-    dtype = _attention_dtype(q, "q")
-    if q.dim() != 4 or k.dim() != 4:
-        raise ValueError(f"q and k have 4 axes, got {q.dim()} and {k.dim()}")
-    batch, s_q, q_heads, d = q.shape
-    s_kv, kv_heads = k.shape[1], k.shape[2]
-    dev = q.device
-    _check(k, "k", dev, q.dtype, (batch, s_kv, kv_heads, d))
-    _check(v, "v", dev, q.dtype, (batch, s_kv, kv_heads, d))
-    if out is None:
-        out = torch.empty((batch, s_q, q_heads, d), dtype=q.dtype, device=dev)
-    else:
-        _check(out, "out", dev, q.dtype, (batch, s_q, q_heads, d))
-    for t, what in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        _inner(t, what)
-    for t, what in ((q_lens, "q_lens"), (kv_lens, "kv_lens")):
-        if t is not None:
-            _check_ints(t, what, dev, (batch,))
-    lse = torch.empty((batch, q_heads, s_q), dtype=torch.float32, device=dev) if return_lse else None
-    strides = (ctypes.c_int64 * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
-    _call("lc_window_attention", dev, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-          lse.data_ptr() if return_lse else None, q_lens.data_ptr() if q_lens is not None else None,
-          kv_lens.data_ptr() if kv_lens is not None else None, batch, s_q, s_kv, q_heads, kv_heads, d, strides, window,
-          sinks, _scale(scale, d), _stream(stream, dev))
-    return (out, lse) if return_lse else out
+    r = _ext.window_attention(q, k, v, window, sinks, scale, q_lens, kv_lens, out, return_lse, stream)
+    if type(r) is int:
+        raise _failed("lc_window_attention", r)
+    return r
 
 
 def paged_decode(q, k_pages, v_pages, table, lens, *, window: int = 0, sinks: int = 0, scale: float | None = None, out=None,
@@ -127,69 +86,15 @@ def paged_decode(q, k_pages, v_pages, table, lens, *, window: int = 0, sinks: in
     as in :class:`CacheMaps`; ``lens`` counts the new token, whose key and value are in the cache already.  The rest
     is as in :func:`window_attention`, of which this is the single-token form; the log-sum-exp is ``[slots, q_heads]``.
     """
-    dtype = _attention_dtype(q, "q")
-    if q.dim() != 3 or k_pages.dim() != 4 or table.dim() != 2:
-        raise ValueError(f"q, k_pages and table have 3, 4 and 2 axes, got {q.dim()}, {k_pages.dim()} and {table.dim()}")
-    slots, q_heads, d = q.shape
-    pages, kv_heads, page_size, _ = k_pages.shape
-    dev = q.device
-    _check(k_pages, "k_pages", dev, q.dtype, (pages, kv_heads, page_size, d))
-    _check(v_pages, "v_pages", dev, q.dtype, (pages, kv_heads, page_size, d))
-    _check(table, "table", dev, torch.int32, (slots, table.shape[1]))
-    _check_ints(lens, "lens", dev, (slots,))
-    if out is None:
-        out = torch.empty((slots, q_heads, d), dtype=q.dtype, device=dev)
-    else:
-        _check(out, "out", dev, q.dtype, (slots, q_heads, d))
-    for t, what in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (out, "out"), (table, "table")):
-        _inner(t, what)
-    lse = torch.empty((slots, q_heads), dtype=torch.float32, device=dev) if return_lse else None
-    strides = (ctypes.c_int64 * 11)(*q.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3], *out.stride()[:2],
-                                    table.stride(0))
-    _call("lc_paged_decode", dev, dtype, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
-          lse.data_ptr() if return_lse else None, table.data_ptr(), lens.data_ptr(), slots, table.shape[1], pages, page_size,
-          q_heads, kv_heads, d, strides, window, sinks, _scale(scale, d), _stream(stream, dev))
-    return (out, lse) if return_lse else out
+    r = _ext.paged_decode(q, k_pages, v_pages, table, lens, window, sinks, scale, out, return_lse, stream)
+    if type(r) is int:
+        raise _failed("lc_paged_decode", r)
+    return r
 
 
 # ---------------------------------------------------------------- pages
 
-def _maps(maps: CacheMaps, what: str = "maps") -> tuple:
-    """(device, slots, width, pages) of checked maps."""
-    if maps.table.dim() != 2 or maps.refs.dim() != 1:
-        raise ValueError(f"{what}: table and refs have 2 and 1 axes")
-    dev, (slots, width), pages = maps.table.device, maps.table.shape, maps.refs.shape[0]
-    if not maps.table.is_cuda:
-        raise ValueError(f"{what}: on {dev}, the kernels run on CUDA devices only")
-    _check_ints(maps.table, f"{what}.table", dev, (slots, width))
-    _check_ints(maps.lens, f"{what}.lens", dev, (slots,))
-    _check_ints(maps.refs, f"{what}.refs", dev, (pages,))
-    if maps.status is not None:
-        _check_ints(maps.status, f"{what}.status", dev, (2,))
-    return dev, slots, width, pages
-
-
-def _into(maps: CacheMaps, into: CacheMaps | None) -> CacheMaps:
-    """The maps an operation writes: new ones, or the given ones with a status."""
-    if into is None:
-        return CacheMaps(torch.empty_like(maps.table), torch.empty_like(maps.lens), torch.empty_like(maps.refs),
-                         torch.empty(2, dtype=torch.int32, device=maps.table.device))
-    if _maps(into, "into") != _maps(maps):
-        raise ValueError("into: other sizes or another device than the maps")
-    return into if into.status is not None else into._replace(status=torch.empty(2, dtype=torch.int32, device=into.table.device))
-
-
-def _pool(pool, dev, pages: int) -> tuple:
-    """The pool's arguments of the page operations: pointer, planes, heads, bytes of a token, strides; and page_size."""
-    if pool.dim() != 5 or pool.device != dev or pool.shape[1] != pages:
-        raise ValueError(f"pool: {tuple(pool.shape)} on {pool.device}, expected [planes, {pages}, kv_heads, page_size, d] on {dev}")
-    planes, _, heads, page_size, d = pool.shape
-    _inner(pool, "pool")
-    if page_size > 1 and pool.stride(3) != d:
-        raise ValueError("pool: the tokens of a head must be contiguous")
-    size = pool.element_size()
-    strides = (ctypes.c_int64 * 3)(*(s * size for s in pool.stride()[:3]))
-    return (pool.data_ptr(), planes, heads, d * size, strides), page_size
+_NONE = (None, None, None, None)
 
 
 def cache_extend(maps: CacheMaps, add, *, page_size: int, into: CacheMaps | None = None, stream: int | None = None) -> CacheMaps:
@@ -197,35 +102,19 @@ def cache_extend(maps: CacheMaps, add, *, page_size: int, into: CacheMaps | None
 
     All or nothing: where pages or table columns are missing, the maps stay as they are and ``status`` says so.
     """
-    dev, slots, width, pages = _maps(maps)
-    _check_ints(add, "add", dev, (slots,))
-    new = _into(maps, into)
-    _call("lc_cache_extend", dev, maps.table.data_ptr(), new.table.data_ptr(), maps.lens.data_ptr(), new.lens.data_ptr(),
-          maps.refs.data_ptr(), new.refs.data_ptr(), add.data_ptr(), new.status.data_ptr(), slots, width, pages, page_size,
-          _stream(stream, dev))
-    return new
+    r = _ext.cache_extend(*maps, add, page_size, *(into or _NONE), stream)
+    if type(r) is int:
+        raise _failed("lc_cache_extend", r)
+    return CacheMaps(*r)
 
 
 def cache_write(k, v, k_pages, v_pages, maps: CacheMaps, add, *, stream: int | None = None) -> None:
     """Writes the newest ``add[i]`` tokens of every slot, ``k, v[slots, most, kv_heads, d]``, to the positions
     ``lens[i] - add[i]`` and on (``maps`` as :func:`cache_extend` left them).  ``k_pages, v_pages[pages, kv_heads,
     page_size, d]`` are planes of the pool; any element type."""
-    dev, slots, width, pages = _maps(maps)
-    _check_ints(add, "add", dev, (slots,))
-    if k.dim() != 4 or k_pages.dim() != 4:
-        raise ValueError(f"k and k_pages have 4 axes, got {k.dim()} and {k_pages.dim()}")
-    _, most, heads, d = k.shape
-    page_size, size = k_pages.shape[2], k.element_size()
-    for t, what in ((k, "k"), (v, "v")):
-        _check(t, what, dev, k.dtype, (slots, most, heads, d))
-        _inner(t, what)
-    for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        _check(t, what, dev, k.dtype, (pages, heads, page_size, d))
-        _inner(t, what)
-    strides = (ctypes.c_int64 * 12)(*(s * size for t in (k, v, k_pages, v_pages) for s in t.stride()[:3]))
-    _call("lc_cache_write", dev, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), maps.table.data_ptr(),
-          maps.lens.data_ptr(), add.data_ptr(), slots, most, width, pages, page_size, heads, d * size, strides,
-          _stream(stream, dev))
+    status = _ext.cache_write(k, v, k_pages, v_pages, *maps, add, stream)
+    if status:
+        raise _failed("lc_cache_write", status)
 
 
 def cache_fork(pool, maps: CacheMaps, parent, *, into: CacheMaps | None = None, stream: int | None = None) -> CacheMaps:
@@ -235,25 +124,17 @@ def cache_fork(pool, maps: CacheMaps, parent, *, into: CacheMaps | None = None, 
     page of their own (the lowest free ones, in slot order) with its tokens.  All or nothing, as :func:`cache_extend`;
     the new maps may not be the old ones.
     """
-    dev, slots, width, pages = _maps(maps)
-    _check_ints(parent, "parent", dev, (slots,))
-    args, page_size = _pool(pool, dev, pages)
-    new = _into(maps, into)
-    _call("lc_cache_fork", dev, *args, maps.table.data_ptr(), new.table.data_ptr(), maps.lens.data_ptr(), new.lens.data_ptr(),
-          maps.refs.data_ptr(), new.refs.data_ptr(), parent.data_ptr(), new.status.data_ptr(), slots, width, pages, page_size,
-          _stream(stream, dev))
-    return new
+    r = _ext.cache_fork(pool, *maps, parent, *(into or _NONE), stream)
+    if type(r) is int:
+        raise _failed("lc_cache_fork", r)
+    return CacheMaps(*r)
 
 
 def _release(maps, gone, window, sinks, page_size, stream) -> CacheMaps:
-    dev, slots, width, pages = _maps(maps)
-    if gone is not None:
-        _check_ints(gone, "gone", dev, (slots,))
-    maps = _into(maps, maps)
-    _call("lc_cache_release", dev, maps.table.data_ptr(), maps.lens.data_ptr(), maps.refs.data_ptr(),
-          gone.data_ptr() if gone is not None else None, window, sinks, maps.status.data_ptr(), slots, width, pages, page_size,
-          _stream(stream, dev))
-    return maps
+    r = _ext.cache_release(*maps, gone, window, sinks, page_size, stream)
+    if type(r) is int:
+        raise _failed("lc_cache_release", r)
+    return CacheMaps(*r)
 
 
 def cache_release(maps: CacheMaps, gone, *, page_size: int, stream: int | None = None) -> CacheMaps:
@@ -268,25 +149,18 @@ def cache_trim(maps: CacheMaps, *, window: int, sinks: int = 0, page_size: int, 
 
 def cache_compact(pool, maps: CacheMaps, *, into: CacheMaps | None = None, stream: int | None = None) -> CacheMaps:
     """Moves the pages in use onto the lowest numbers (``pages - status[1]`` of them); tables and refs follow."""
-    dev, slots, width, pages = _maps(maps)
-    args, page_size = _pool(pool, dev, pages)
-    new = _into(maps, into)
-    _call("lc_cache_compact", dev, *args, maps.table.data_ptr(), new.table.data_ptr(), maps.lens.data_ptr(),
-          new.lens.data_ptr(), maps.refs.data_ptr(), new.refs.data_ptr(), new.status.data_ptr(), slots, width, pages, page_size,
-          _stream(stream, dev))
-    return new
+    r = _ext.cache_compact(pool, *maps, *(into or _NONE), stream)
+    if type(r) is int:
+        raise _failed("lc_cache_compact", r)
+    return CacheMaps(*r)
 
 
 def cache_copy(pool, src, dst, *, stream: int | None = None) -> None:
     """Copies page ``src[i]`` onto page ``dst[i]`` in every plane (int32 on the device).  No page may be a destination
     twice, or a destination and a source."""
-    dev, pages = pool.device, pool.shape[1]
-    if not pool.is_cuda:
-        raise ValueError(f"pool: on {dev}, the kernels run on CUDA devices only")
-    _check_ints(src, "src", dev, (src.numel(),))
-    _check_ints(dst, "dst", dev, (src.numel(),))
-    args, page_size = _pool(pool, dev, pages)
-    _call("lc_cache_copy", dev, *args, src.data_ptr(), dst.data_ptr(), src.numel(), pages, page_size, _stream(stream, dev))
+    status = _ext.cache_copy(pool, src, dst, stream)
+    if status:
+        raise _failed("lc_cache_copy", status)
 
 
 class PagedCache:
