@@ -2,7 +2,10 @@
 // (the single-token form of window_attention.cu): slot s has lens[s] cached
 // tokens, its query is the last of them, and token j is row j % page_size of
 // page table[s][j / page_size].
+#include <algorithm>
+
 #include "attend.cuh"
+#include "softmax.cuh"
 
 namespace lc {
 namespace {
@@ -18,7 +21,13 @@ struct DecodeParams {
   int64_t qs[2], ks[3], vs[3], os[2], ts;  // element strides: q, o slot and head; k, v page, head, token; table slot
   int window, sinks;
   float scale_log2;
+  int page_shift;  // page_size is 1 << page_shift, or -1
+  int dense;       // a head's tokens follow each other in k and v, without padding
 };
+
+__device__ __forceinline__ int page_index(const DecodeParams &p, int key) {
+  return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+}
 
 __device__ __forceinline__ int cached_tokens(const DecodeParams &p, int slot) {
   const int64_t most = (int64_t)p.width * p.page_size;
@@ -26,40 +35,45 @@ __device__ __forceinline__ int cached_tokens(const DecodeParams &p, int slot) {
   return n < most ? n : (int)most;
 }
 
-constexpr int kPartialsSlot = 41, kArrivedSlot = 42;  // scratch_buffer slots
+constexpr int kPartialsSlot = 41, kArrivedSlot = 42, kSpansSlot = 46;  // scratch_buffer slots
 
 // ---------------------------------------------------------------- plain form
-// One CTA of eight warps per (slot, query head), the keys dealt to the warps: what
-// the tensor-core form below does not take (odd head sizes and alignments).
+// One row key by key, by the WARPS warps of a CTA; warp 0 receives it.
+template <class T, int WARPS>
+__device__ __forceinline__ void plain_row(const DecodeParams &p, int slot, int h, int head, RowState &st, float *scratch) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = cached_tokens(p, slot);
+  float q[kMaxHead / 32];
+  load_row(q, static_cast<const T *>(p.q) + slot * p.qs[0] + h * p.qs[1], p.d, lane, p.scale_log2);
+  const int *row = p.table + slot * p.ts;
+  auto at = [&](int j, const T *&k, const T *&v) {
+    const int page = row[page_index(p, j)], r = j - page_index(p, j) * p.page_size;
+    if ((unsigned)page >= (unsigned)p.pages) return false;
+    k = static_cast<const T *>(p.k) + page * p.ks[0] + head * p.ks[1] + r * p.ks[2];
+    v = static_cast<const T *>(p.v) + page * p.vs[0] + head * p.vs[1] + r * p.vs[2];
+    return true;
+  };
+  if (n > 0) {
+    const Visible see = visible(n - 1, p.window, p.sinks);
+    attend_keys<T>(st, q, p.d, lane, warp, see.sink_end, WARPS, at);
+    attend_keys<T>(st, q, p.d, lane, see.lo + warp, n, WARPS, at);
+  }
+  join_warps<WARPS>(st, scratch);
+}
+
+// One CTA of eight warps per (slot, query head): what the tensor-core form below does
+// not take (odd head sizes and alignments).
 constexpr int kRowWarps = 8;
 
 template <class T>
 __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams p) {
   __shared__ float scratch[kRowWarps * (kMaxHead + 2)];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = blockIdx.x, h = blockIdx.y;
-  const int hk = h / (p.q_heads / p.kv_heads);
-  const int n = cached_tokens(p, slot);
   RowState st;
-  if (n > 0) {
-    float q[kMaxHead / 32];
-    load_row(q, static_cast<const T *>(p.q) + slot * p.qs[0] + h * p.qs[1], p.d, lane, p.scale_log2);
-    const int *row = p.table + slot * p.ts;
-    auto at = [&](int j, const T *&k, const T *&v) {
-      const int page = row[j / p.page_size], r = j % p.page_size;
-      if ((unsigned)page >= (unsigned)p.pages) return false;
-      k = static_cast<const T *>(p.k) + page * p.ks[0] + hk * p.ks[1] + r * p.ks[2];
-      v = static_cast<const T *>(p.v) + page * p.vs[0] + hk * p.vs[1] + r * p.vs[2];
-      return true;
-    };
-    const Visible see = visible(n - 1, p.window, p.sinks);
-    attend_keys<T>(st, q, p.d, lane, warp, see.sink_end, kRowWarps, at);
-    attend_keys<T>(st, q, p.d, lane, see.lo + warp, n, kRowWarps, at);
-  }
-  join_warps<kRowWarps>(st, scratch);
-  if (warp == 0)
+  plain_row<T, kRowWarps>(p, slot, h, h / (p.q_heads / p.kv_heads), st, scratch);
+  if (threadIdx.x < 32)
     store_row(st, static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1],
-              p.lse ? p.lse + (int64_t)slot * p.q_heads + h : nullptr, p.d, lane);
+              p.lse ? p.lse + (int64_t)slot * p.q_heads + h : nullptr, p.d, threadIdx.x);
 }
 
 // ---------------------------------------------------------------- tensor-core form
@@ -71,7 +85,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // an equal contiguous run of them, so a batch of unequal lengths and a single long
 // sequence both fill the GPU.  A segment that spans CTAs leaves an unnormalised
 // (O, m, l) per CTA in the workspace; the CTA that arrives last joins them in CTA
-// order (the run boundaries depend on the lengths alone, so results repeat).
+// order (the run boundaries depend on the lengths alone, so results repeat), or,
+// where a segment may span kDeepParts of them or more, a second kernel with a CTA per row
+// (one sequence of 131072 with one key-value head, 444 parts: 29 us; 167 us with the last
+// CTA, which reads 1.9 MB alone).
 //
 // In a CTA each warp takes 16 keys of every tile and is on its own until the
 // segment ends: it copies its keys' rows (cp.async, 16 bytes per lane, zeros where
@@ -87,6 +104,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // extra products hide behind the loads and keep P to 16 bits or more.
 constexpr int kDecodeWarps = 4;
 constexpr int kTileKeys = 16;
+constexpr int kDeepParts = 16;
 constexpr int kMinTiles = 2;  // CTA tiles below which a segment is not cut further
 
 template <class T>
@@ -121,6 +139,9 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // 16 bytes to shared memory; zeros, and no read, where `bytes` is 0.
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void *src, int bytes) {
@@ -187,6 +208,10 @@ __device__ __forceinline__ void advance(Cursor &c, const DecodeParams &p, int pa
 struct DecodeWork {
   float *partials;    // [CTA][2][rows][DP + 4]: of a segment that began before the CTA, of one that began in it
   unsigned *arrived;  // [slots * parts], zero between launches
+  // deep: segments span so many CTAs that decode_join_kernel joins them; the segment
+  // (slot * parts + part) that began in a CTA and goes on after it, or -1, and its last CTA
+  int deep, ctas;
+  int2 *spans;
 };
 
 template <class T, int DP, int NT, int STAGES>
@@ -199,8 +224,8 @@ struct DecodeLayout {
 };
 
 // PAGED16: a tile of 16 keys lies in one page (page_size is a multiple of 16).
-template <class T, int DP, int NT, int STAGES, bool PAGED16>
-__global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_kernel(DecodeParams p, DecodeWork work) {
+template <class T, int DP, int NT, int STAGES, int CTAS, bool PAGED16>
+__global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeParams p, DecodeWork work) {
   using L = DecodeLayout<T, DP, NT, STAGES>;
   constexpr int kRows = L::kRows;
   constexpr int kChunks = DP / 8;                   // 16-byte pieces of a row
@@ -267,6 +292,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
     if (p.lse)
       for (int h = tid; h < p.q_heads; h += blockDim.x) p.lse[(int64_t)s * p.q_heads + h] = -INFINITY;
   }
+  if (work.deep && tid == 0) work.spans[blockIdx.x] = make_int2(-1, -1);
   __syncthreads();
   if (!works) return;
 
@@ -294,10 +320,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
     page = -1;
     if (key < 0) return;
     if (PAGED16) {
-      page = p.table[load.slot * p.ts + key / p.page_size];
+      page = p.table[load.slot * p.ts + page_index(p, key)];
     } else {
       const int j = key + (lane & 15);
-      if (j < load.tiles.n) page = p.table[load.slot * p.ts + j / p.page_size];
+      if (j < load.tiles.n) page = p.table[load.slot * p.ts + page_index(p, j)];
     }
   };
   auto issue = [&](int stage) {
@@ -307,16 +333,28 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
                       (j >= load.tiles.lo || j < load.tiles.sink_end);
     const unsigned mask = __ballot_sync(0xffffffffu, sees) & 0xffffu;
     if (lane == 0) masks[warp][stage] = mask;
-    if (mask) {
+    // Piece x of row r lies at x ^ (r & 7).  A lane's rows are i * kRowsPerCopy + piece_row, whose
+    // two parts share no bit, so the i-th address differs from the first by constants.
+    const uint32_t dst = ring + stage * L::kStageBytes + piece_row * L::kRowBytes + ((piece ^ (piece_row & 7)) << 4);
+    auto dst_of = [&](int i) { return (dst ^ ((i * kRowsPerCopy & 7) << 4)) + i * kRowsPerCopy * L::kRowBytes; };
+    constexpr uint32_t kV = kTileKeys * L::kRowBytes;  // V behind K
+    if (PAGED16 && mask == 0xffffu && p.dense) {  // one run of memory each
+      const int head = load.part / chunks, r = key - page_index(p, key) * p.page_size;
+      const T *k = static_cast<const T *>(p.k) + page * p.ks[0] + head * p.ks[1] + r * DP + lane * 8;
+      const T *v = static_cast<const T *>(p.v) + page * p.vs[0] + head * p.vs[1] + r * DP + lane * 8;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) copy_async16(dst_of(i), k + i * 256);
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) copy_async16(dst_of(i) + kV, v + i * 256);
+    } else if (mask) {
       const int head = load.part / chunks;
-      const uint32_t k_dst = ring + stage * L::kStageBytes, v_dst = k_dst + kTileKeys * L::kRowBytes;
       int64_t k_off, v_off;
       if (PAGED16) {
-        const int r = key % p.page_size;
+        const int r = key - page_index(p, key) * p.page_size;
         k_off = page * p.ks[0] + head * p.ks[1] + (r + piece_row) * p.ks[2] + piece * 8;
         v_off = page * p.vs[0] + head * p.vs[1] + (r + piece_row) * p.vs[2] + piece * 8;
       } else {
-        const int r = j % p.page_size;
+        const int r = j - page_index(p, j) * p.page_size;
         k_off = page * p.ks[0] + head * p.ks[1] + r * p.ks[2];
         v_off = page * p.vs[0] + head * p.vs[1] + r * p.vs[2];
       }
@@ -332,9 +370,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
           ko = __shfl_sync(0xffffffffu, k_off, row) + piece * 8;
           vo = __shfl_sync(0xffffffffu, v_off, row) + piece * 8;
         }
-        const uint32_t at = row * L::kRowBytes + ((piece ^ (row & 7)) << 4);
-        copy_async16(k_dst + at, static_cast<const T *>(p.k) + (bytes ? ko : 0), bytes);
-        copy_async16(v_dst + at, static_cast<const T *>(p.v) + (bytes ? vo : 0), bytes);
+        copy_async16(dst_of(i), static_cast<const T *>(p.k) + (bytes ? ko : 0), bytes);
+        copy_async16(dst_of(i) + kV, static_cast<const T *>(p.v) + (bytes ? vo : 0), bytes);
       }
     }
   };
@@ -373,11 +410,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
     // K: rows 0-7, 8-15 of pieces 2k, then 2k + 1
-    const int k_row = lane & 15, k_half = lane >> 4;
+    const int k_row = lane & 15;
+    const uint32_t k_at = k_src + k_row * L::kRowBytes + (((lane >> 4) ^ (k_row & 7)) << 4);
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
       uint32_t a[4];
-      ldmatrix4(a, k_src + k_row * L::kRowBytes + (((2 * k + k_half) ^ (k_row & 7)) << 4));
+      ldmatrix4(a, (k_at ^ ((2 * k & 7) << 4)) + (2 * k >> 3) * 128);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[nt], a, q[nt][k][0], q[nt][k][1]);
     }
@@ -386,7 +424,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
     for (int nt = 0; nt < NT; ++nt) {
       // s: (key g, heads c2, c2 + 1), (key g + 8, the same heads)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[nt][x] = mask >> (g + (x >> 1) * 8) & 1 ? s[nt][x] * p.scale_log2 : -INFINITY;
+      for (int x = 0; x < 4; ++x) s[nt][x] *= p.scale_log2;
+      if (mask != 0xffffu) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (!(mask >> (g + (x >> 1) * 8) & 1)) s[nt][x] = -INFINITY;
+      }
       float top[2] = {fmaxf(s[nt][0], s[nt][2]), fmaxf(s[nt][1], s[nt][3])};
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -400,7 +443,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const float m_new = fmaxf(m[nt][x], top[x]);
-          alpha[x] = exp2f(m[nt][x] - (m_new == -INFINITY ? 0.f : m_new));
+          alpha[x] = softmax::ex2(m[nt][x] - (m_new == -INFINITY ? 0.f : m_new));
           m[nt][x] = m_new;
           l[nt][x] *= alpha[x];
         }
@@ -416,7 +459,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
       float e[4], r[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        e[x] = exp2f(s[nt][x] - base[x & 1]);
+        e[x] = softmax::ex2(s[nt][x] - base[x & 1]);
         l[nt][x & 1] += e[x];
         r[x] = round_to<T>(e[x]);
       }
@@ -426,11 +469,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
       lo[nt][1] = movmatrix_trans(pack<T>(e[2] - r[2], e[3] - r[3]));
     }
     // V^T: (keys 0-7, pieces 2k, 2k + 1), then keys 8-15
-    const int v_row = (lane & 7) + (lane >> 4) * 8, v_half = lane >> 3 & 1;
+    const int v_row = (lane & 7) + (lane >> 4) * 8;
+    const uint32_t v_at = v_src + v_row * L::kRowBytes + (((lane >> 3 & 1) ^ (v_row & 7)) << 4);
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
       uint32_t a[4];
-      ldmatrix4_trans(a, v_src + v_row * L::kRowBytes + (((2 * k + v_half) ^ (v_row & 7)) << 4));
+      ldmatrix4_trans(a, (v_at ^ ((2 * k & 7) << 4)) + (2 * k >> 3) * 128);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         mma16816<T>(o[nt][k], a, hi[nt][0], hi[nt][1]);
@@ -472,22 +516,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
   auto plain_rows = [&]() {
     const int head = use.part / chunks, first = head * group + use.part % chunks * kRows;
     const int live = min(kRows, (head + 1) * group - first);
-    const int *row = p.table + use.slot * p.ts;
-    auto at = [&](int j, const T *&k, const T *&v) {
-      const int pg = row[j / p.page_size], r = j % p.page_size;
-      if ((unsigned)pg >= (unsigned)p.pages) return false;
-      k = static_cast<const T *>(p.k) + pg * p.ks[0] + head * p.ks[1] + r * p.ks[2];
-      v = static_cast<const T *>(p.v) + pg * p.vs[0] + head * p.vs[1] + r * p.vs[2];
-      return true;
-    };
     for (int x = 0; x < live; ++x) {
-      float qv[kMaxHead / 32];
-      load_row(qv, static_cast<const T *>(p.q) + use.slot * p.qs[0] + (first + x) * p.qs[1], p.d, lane, p.scale_log2);
       RowState st;
-      attend_keys<T>(st, qv, p.d, lane, warp, use.tiles.sink_end, kDecodeWarps, at);
-      attend_keys<T>(st, qv, p.d, lane, use.tiles.lo + warp, use.tiles.n, kDecodeWarps, at);
       __syncthreads();
-      join_warps<kDecodeWarps>(st, scratch);
+      plain_row<T, kDecodeWarps>(p, use.slot, first + x, head, st, scratch);
       if (warp == 0) mend_row(st, static_cast<T *>(p.o) + use.slot * p.os[0] + (first + x) * p.os[1], p.d, lane);
     }
   };
@@ -558,6 +590,11 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
       }
       // the CTAs whose runs hold the segment's first and last tile
       const int first = (int)(((seg_begin + 1) * ctas - 1) / total), last = (int)((seg_end * ctas - 1) / total);
+      if (work.deep) {
+        if (seg_begin >= begin && tid == 0) work.spans[blockIdx.x] = make_int2(use.slot * parts + use.part, last);
+        __syncthreads();  // the sums have been read
+        return;
+      }
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -570,39 +607,63 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
       __threadfence();
       // CTA c's share: the segment began in CTA `first` and before every other
       auto share = [&](int c) { return work.partials + ((int64_t)c * 2 + (c == first)) * kPartial; };
-      float top[kRpt];
+      // Weights first, 64 parts at a time into the free stage of warp 0; then the sums, 16 bytes
+      // a thread and eight parts in flight: an SM reads them at the rate its loads arrive.
+      constexpr int kThreads = kDecodeWarps * 32, kGroups = kThreads / kRows, kChunk = 64;
+      float *weights = sums_of(0), *joined = sums_of(1);
+      const int wrow = tid % kRows, wgroup = tid / kRows;
+      float top = -INFINITY;
+#pragma unroll 4
+      for (int c = first + wgroup; c <= last; c += kGroups) top = fmaxf(top, __ldcg(share(c) + wrow * (DP + 4) + DP));
+      weights[wgroup * kRows + wrow] = top;
+      __syncthreads();
+      for (int x = 0; x < kGroups; ++x) top = fmaxf(top, weights[x * kRows + wrow]);
+      const float base = top == -INFINITY ? 0.f : top;
+      constexpr int kVecs = kRows * DP / 4 / kThreads;  // 16-byte pieces of the rows that a thread adds up
+      float4 sum4[kVecs];
 #pragma unroll
-      for (int x = 0; x < kRpt; ++x) top[x] = -INFINITY;
-#pragma unroll 2
-      for (int c = first; c <= last; ++c)
+      for (int x = 0; x < kVecs; ++x) sum4[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+      for (int from = first; from <= last; from += kChunk) {
+        const int parts_here = min(kChunk, last + 1 - from);
+        __syncthreads();
+        for (int c = wgroup; c < parts_here; c += kGroups) {
+          const float2 ml = __ldcg(reinterpret_cast<const float2 *>(share(from + c) + wrow * (DP + 4) + DP));
+          const float weight = softmax::ex2(ml.x - base);
+          sum = fmaf(ml.y, weight, sum);
+          weights[c * kRows + wrow] = weight;
+        }
+        __syncthreads();
+#pragma unroll 8
+        for (int c = 0; c < parts_here; ++c) {
+          const float *part = share(from + c);
 #pragma unroll
-        for (int x = 0; x < kRpt; ++x) top[x] = fmaxf(top[x], __ldcg(share(c) + (first_row + kSplit * x) * (DP + 4) + DP));
-      float sum[kRpt];
-#pragma unroll
-      for (int x = 0; x < kRpt; ++x) {
-        sum[x] = 0.f;
-#pragma unroll
-        for (int y = 0; y < kCpt; ++y) values[x][y] = 0.f;
-      }
-#pragma unroll 2
-      for (int c = first; c <= last; ++c) {
-        const float *from = share(c);
-#pragma unroll
-        for (int x = 0; x < kRpt; ++x) {
-          const float *row = from + (first_row + kSplit * x) * (DP + 4);
-          const float weight = exp2f(__ldcg(row + DP) - (top[x] == -INFINITY ? 0.f : top[x]));
-          sum[x] = fmaf(__ldcg(row + DP + 1), weight, sum[x]);
-#pragma unroll
-          for (int y = 0; y < kCpt; ++y) values[x][y] = fmaf(__ldcg(row + col + kCols * y), weight, values[x][y]);
+          for (int x = 0; x < kVecs; ++x) {
+            const int vec = tid + x * kThreads, row = vec / (DP / 4);
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + row * (DP + 4) + vec % (DP / 4) * 4));
+            const float weight = weights[c * kRows + row];
+            sum4[x].x = fmaf(v.x, weight, sum4[x].x);
+            sum4[x].y = fmaf(v.y, weight, sum4[x].y);
+            sum4[x].z = fmaf(v.z, weight, sum4[x].z);
+            sum4[x].w = fmaf(v.w, weight, sum4[x].w);
+          }
         }
       }
-      if (col == 0) {
+      __syncthreads();
+      weights[wgroup * kRows + wrow] = sum;
 #pragma unroll
-        for (int x = 0; x < kRpt; ++x) {
-          row_m[first_row + kSplit * x] = top[x];
-          row_l[first_row + kSplit * x] = sum[x];
-        }
+      for (int x = 0; x < kVecs; ++x) reinterpret_cast<float4 *>(joined)[tid + x * kThreads] = sum4[x];
+      __syncthreads();
+      if (wgroup == 0) {
+        sum = 0.f;
+        for (int x = 0; x < kGroups; ++x) sum += weights[x * kRows + wrow];
+        row_m[wrow] = top;
+        row_l[wrow] = sum;
       }
+#pragma unroll
+      for (int x = 0; x < kRpt; ++x)
+#pragma unroll
+        for (int y = 0; y < kCpt; ++y) values[x][y] = joined[(first_row + kSplit * x) * DP + col + kCols * y];
       __syncthreads();
       odd = write_rows(values);
     }
@@ -647,10 +708,90 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DP == 256 ? 1 : 2) decode_k
   }
 }
 
-template <class T, int DP, int NT, int STAGES, bool PAGED16>
+// Joins the segments that span CTAs: blockIdx.x counts them, blockIdx.y is a row; the
+// parts are dealt to eight warps.
+constexpr int kJoinWarps = 8;
+
+template <class T, int DP, int NT>
+__global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodeParams p, DecodeWork work) {
+  constexpr int kRows = 8 * NT, kCols = DP / 32;
+  __shared__ float scratch[kJoinWarps * (kMaxHead + 2)];
+  __shared__ int found;
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) found = -1;
+  __syncthreads();
+  if (warp == 0) {
+    int left = blockIdx.x;
+    for (int base = 0; base < work.ctas; base += 32) {
+      const unsigned some = __ballot_sync(0xffffffffu, base + lane < work.ctas && work.spans[base + lane].x >= 0);
+      const int here = __popc(some);
+      if (left < here) {
+        if ((some >> lane & 1) && __popc(some & ((1u << lane) - 1)) == left) found = base + lane;
+        break;
+      }
+      left -= here;
+    }
+  }
+  __syncthreads();
+  const int first = found, row = blockIdx.y;
+  if (first < 0) return;
+  const int2 span = work.spans[first];
+  const int group = p.q_heads / p.kv_heads, chunks = (group + kRows - 1) / kRows, parts = p.kv_heads * chunks;
+  const int slot = span.x / parts, part = span.x % parts, head = part / chunks, h = head * group + part % chunks * kRows + row;
+  if (h >= (head + 1) * group) return;
+  // CTA c's share of the row: the segment began in CTA `first` and before every other
+  auto share = [&](int c) { return work.partials + ((int64_t)c * 2 + (c == first)) * kRows * (DP + 4) + row * (DP + 4); };
+  float top = -INFINITY;
+  for (int c = first + tid; c <= span.y; c += kJoinWarps * 32) top = fmaxf(top, __ldcg(share(c) + DP));
+  top = block_max(top, scratch);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, o[kCols];
+#pragma unroll
+  for (int x = 0; x < kCols; ++x) o[x] = 0.f;
+#pragma unroll 8
+  for (int c = first + warp; c <= span.y; c += kJoinWarps) {
+    const float *from = share(c);
+    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from + DP));
+    const float weight = softmax::ex2(ml.x - base);
+    sum = fmaf(ml.y, weight, sum);
+#pragma unroll
+    for (int x = 0; x < kCols; x += 2) {
+      const float2 two = __ldcg(reinterpret_cast<const float2 *>(from + lane * kCols + x));
+      o[x] = fmaf(two.x, weight, o[x]);
+      o[x + 1] = fmaf(two.y, weight, o[x + 1]);
+    }
+  }
+  __syncthreads();  // block_max's scratch has been read
+#pragma unroll
+  for (int x = 0; x < kCols; ++x) scratch[warp * (kMaxHead + 2) + lane * kCols + x] = o[x];
+  if (lane == 0) scratch[warp * (kMaxHead + 2) + kMaxHead] = sum;
+  __syncthreads();
+  sum = 0.f;
+  for (int w = 0; w < kJoinWarps; ++w) sum += scratch[w * (kMaxHead + 2) + kMaxHead];
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T *out = static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1];
+  bool odd = false;
+  if (tid < p.d) {
+    float v = 0.f;
+    for (int w = 0; w < kJoinWarps; ++w) v += scratch[w * (kMaxHead + 2) + tid];
+    v *= inv;
+    odd = !isfinite(v);
+    out[tid] = Elem<T>::from_float(v);
+  }
+  if (p.lse && tid == 0) p.lse[(int64_t)slot * p.q_heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  if (__syncthreads_or(odd)) {  // as in decode_kernel
+    RowState st;
+    plain_row<T, kJoinWarps>(p, slot, h, head, st, scratch);
+    if (warp == 0) mend_row(st, out, p.d, lane);
+  }
+}
+
+template <class T, int DP, int NT, int STAGES, int CTAS, bool PAGED16>
 int launch_decode(const DecodeParams &p, cudaStream_t s) {
   using L = DecodeLayout<T, DP, NT, STAGES>;
-  auto *kernel = decode_kernel<T, DP, NT, STAGES, PAGED16>;
+  auto *kernel = decode_kernel<T, DP, NT, STAGES, CTAS, PAGED16>;
   static int configured[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -659,16 +800,28 @@ int launch_decode(const DecodeParams &p, cudaStream_t s) {
       return rc;
     if (dev >= 0 && dev < 64) configured[dev] = 1;
   }
-  const int ctas = sm_count() * (DP == 256 ? 1 : 2);
+  const int ctas = sm_count() * CTAS;
   const int group = p.q_heads / p.kv_heads;
   const int64_t parts = (int64_t)p.kv_heads * ((group + L::kRows - 1) / L::kRows);
-  DecodeWork w;
+  DecodeWork w = {};
   void *mem = nullptr;
   if (int rc = scratch_buffer(s, kPartialsSlot, (size_t)ctas * 2 * L::kRows * (DP + 4) * 4, &mem)) return rc;
   w.partials = static_cast<float *>(mem);
   if (int rc = zeroed_buffer(s, kArrivedSlot, (size_t)(p.slots * parts * 4), &mem)) return rc;
   w.arrived = static_cast<unsigned *>(mem);
-  return check_cuda(launch_pdl(kernel, dim3(ctas), dim3(kDecodeWarps * 32), L::kBytes, s, p, w), "lc_paged_decode");
+  w.ctas = ctas;
+  // the CTAs that a segment may span, if every slot's cache is as long as it can be
+  const int64_t most = (int64_t)p.width * p.page_size, reach = p.window ? (int64_t)p.window + p.sinks : most;
+  const int64_t cuts = (std::min(most, reach) / (kTileKeys * kDecodeWarps) + kMinTiles) / kMinTiles;
+  w.deep = std::min<int64_t>(cuts, ctas / (p.slots * parts)) >= kDeepParts;
+  if (w.deep) {
+    if (int rc = scratch_buffer(s, kSpansSlot, ctas * sizeof(int2), &mem)) return rc;
+    w.spans = static_cast<int2 *>(mem);
+  }
+  if (int rc = check_cuda(launch_pdl(kernel, dim3(ctas), dim3(kDecodeWarps * 32), L::kBytes, s, p, w), "lc_paged_decode")) return rc;
+  if (!w.deep) return LC_OK;
+  return check_cuda(launch_pdl(decode_join_kernel<T, DP, NT>, dim3((unsigned)(p.slots * parts), L::kRows), dim3(kJoinWarps * 32), 0, s, p, w),
+                    "lc_paged_decode (join)");
 }
 
 template <class T, bool PAGED16>
@@ -676,9 +829,9 @@ int launch_sized(const DecodeParams &p, cudaStream_t s) {
   // NT: 8 or 16 query heads of a group in one pass over its keys (a group of 9 to 16
   // read twice, 8 heads at a time, would take the loads twice; larger groups are cut in sixteens)
   const bool wide = p.q_heads / p.kv_heads > 8;
-  if (p.d <= 64) return wide ? launch_decode<T, 64, 2, 6, PAGED16>(p, s) : launch_decode<T, 64, 1, 6, PAGED16>(p, s);
-  if (p.d <= 128) return wide ? launch_decode<T, 128, 2, 3, PAGED16>(p, s) : launch_decode<T, 128, 1, 3, PAGED16>(p, s);
-  return wide ? launch_decode<T, 256, 2, 3, PAGED16>(p, s) : launch_decode<T, 256, 1, 3, PAGED16>(p, s);
+  if (p.d <= 64) return wide ? launch_decode<T, 64, 2, 6, 2, PAGED16>(p, s) : launch_decode<T, 64, 1, 4, 3, PAGED16>(p, s);
+  if (p.d <= 128) return wide ? launch_decode<T, 128, 2, 3, 2, PAGED16>(p, s) : launch_decode<T, 128, 1, 2, 3, PAGED16>(p, s);
+  return wide ? launch_decode<T, 256, 2, 3, 1, PAGED16>(p, s) : launch_decode<T, 256, 1, 3, 1, PAGED16>(p, s);
 }
 
 // The tensor-core form takes 16-byte pieces of keys and values and pairs of the query.
@@ -721,8 +874,13 @@ extern "C" int lc_paged_decode(int dtype, const void *q, const void *k, const vo
   p.window = window >= most ? 0 : (int)window;  // a window the cache cannot outgrow is no window
   p.sinks = (int)(sinks < most ? sinks : most);
   p.scale_log2 = scale * attend::kLog2e;
+  p.page_shift = -1;
+  for (int x = 0; x < 21; ++x)
+    if (page_size == 1ll << x) p.page_shift = x;
   cudaStream_t s = as_stream(stream);
   if (decode_tensor(p)) {
+    const int padded = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+    p.dense = d == padded && p.ks[2] == d && p.vs[2] == d;
     if (dtype == LC_F16) return page_size % 16 == 0 ? launch_sized<__half, true>(p, s) : launch_sized<__half, false>(p, s);
     return page_size % 16 == 0 ? launch_sized<__nv_bfloat16, true>(p, s) : launch_sized<__nv_bfloat16, false>(p, s);
   }
