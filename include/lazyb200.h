@@ -676,7 +676,7 @@ int lc_cache_write(const void *k, const void *v, void *k_pages, void *v_pages, c
 /* Slot i continues as slot parent[i] was (-1: it is dropped).  Full pages are
  * shared; a last page that is not full stays with the lowest slot of its parent,
  * the others get the lowest-numbered free page, in slot order, with the tokens
- * held.  pool: `planes` x pages x kv_heads x page_size x token_bytes, tokens of a
+ * held.  At most 8192 slots.  pool: `planes` x pages x kv_heads x page_size x token_bytes, tokens of a
  * head contiguous; strides, in bytes: plane, page, head (3 values). */
 int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes,
                   const int64_t *strides, const int32_t *table_in, int32_t *table_out,

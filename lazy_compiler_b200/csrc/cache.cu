@@ -13,12 +13,16 @@
 //   compact  moves the pages in use onto the lowest numbers
 //   copy     copies listed pages
 //
-// The map kernels run as one cluster of 8 CTAs: what they touch is a few hundred
-// kilobytes, one SM alone reads that at some 100 GB/s, and a cluster barrier
-// (about a microsecond) separates the phases where a grid would need another
-// launch.  Every result is independent of scheduling: ranks come from scans in
-// index order, and atomics only count.
+// A map kernel is one cluster, whose barrier separates the phases where a grid would
+// need another launch.  It is a chain of some six dependent reads, each as long as an
+// L2 access takes, so its size goes by the table's and refs' entries: one CTA of 256
+// threads up to 2048 of them, 8 of 512 up to 65536, 8 of 1024 beyond (compact, 312
+// entries: 6.6, 9.2 us; extend, 12662: 12.1, 9.1, 9.6 us; 200652: 55, 19.5, 14.3 us).
+// Every result is independent of scheduling: ranks come from scans in index order, and
+// atomics only count.
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 
@@ -27,16 +31,17 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kCtas = 8;
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMostCtas = 8;
+constexpr int kMostThreads = 1024;
+constexpr int kMostWarps = kMostThreads / 32;
+constexpr int kItems = 4;  // consecutive items of a thread in the scans, independent ones elsewhere
 constexpr int kScratchSlot = 40;  // scratch_buffer slot of the page operations
 
 // Exclusive prefix of v over the CTA's threads, and the CTA's total.
 struct BlockScan {
-  int warp_sums[kWarps + 1];
+  int warp_sums[kMostWarps + 1];
   __device__ __forceinline__ int exclusive(int v, int &total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -47,18 +52,19 @@ struct BlockScan {
     if (lane == 31) warp_sums[warp] = inc;
     __syncthreads();
     if (warp == 0) {
-      const int own = warp_sums[lane];
+      const int own = lane < warps ? warp_sums[lane] : 0;
       int sum = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += up;
       }
-      warp_sums[lane] = sum - own;
-      if (lane == 31) warp_sums[kWarps] = sum;
+      __syncwarp();
+      if (lane < warps) warp_sums[lane] = sum - own;
+      if (lane == 31) warp_sums[kMostWarps] = sum;
     }
     __syncthreads();
-    total = warp_sums[kWarps];
+    total = warp_sums[kMostWarps];
     return warp_sums[warp] + inc - v;
   }
 };
@@ -71,10 +77,23 @@ __device__ __forceinline__ int pages_of(int tokens, int page_size) {
 struct Share {
   int begin, end;
 };
-__device__ __forceinline__ Share share_of(int n, int rank) {
-  const int per = (n + kCtas - 1) / kCtas;
+__device__ __forceinline__ Share share_of(int n, int rank, int ctas) {
+  const int per = (n + ctas - 1) / ctas;
   const int begin = min(n, rank * per);
   return {begin, min(n, begin + per)};
+}
+
+// How many of share [begin, end) of refs are free.
+__device__ __forceinline__ int count_free(const int *refs, const Share &share) {
+  int n = 0;
+  for (int i = share.begin + threadIdx.x; i < share.end; i += kItems * blockDim.x) {
+    int r[kItems];
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) r[x] = i + x * (int)blockDim.x < share.end ? refs[i + x * blockDim.x] : 1;
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) n += r[x] == 0;
+  }
+  return n;
 }
 
 // Adds v over the CTA and leaves the sum for the cluster in *mine; after the
@@ -87,7 +106,7 @@ __device__ __forceinline__ void publish(int v, BlockScan &scan, int *mine) {
 __device__ __forceinline__ void before_and_total(cg::cluster_group &cluster, int *mine, int &before, int &total) {
   before = total = 0;
   const int rank = (int)cluster.block_rank();
-  for (int r = 0; r < kCtas; ++r) {
+  for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
     const int x = *cluster.map_shared_rank(mine, r);
     if (r < rank) before += x;
     total += x;
@@ -103,14 +122,16 @@ struct ExtendParams {
   int slots, width, pages, page_size;
 };
 
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) extend_kernel(ExtendParams p) {
+__global__ void __launch_bounds__(kMostThreads, 1) extend_kernel(ExtendParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ BlockScan scan;
   __shared__ int free_here;
-  const int rank = (int)cluster.block_rank(), tid = threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), threads = blockDim.x, warps = threads >> 5, tid = threadIdx.x;
   // every CTA adds up the demand of all slots; CTA 0 keeps each slot's offset
   int need = 0, wide = 0;
-  for (int base = 0; base < p.slots; base += kThreads) {
+  for (int base = 0; base < p.slots; base += threads) {
     const int i = base + tid;
     int n = 0;
     if (i < p.slots) {
@@ -130,31 +151,34 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) ext
   }
   wide = __syncthreads_or(wide);
   // count the free pages of this CTA's share
-  const Share mine = share_of(p.pages, rank);
-  int n_free = 0;
-  for (int i = mine.begin + tid; i < mine.end; i += kThreads) n_free += p.refs_in[i] == 0;
-  publish(n_free, scan, &free_here);
+  const Share mine = share_of(p.pages, rank, ctas);
+  publish(count_free(p.refs_in, mine), scan, &free_here);
   cluster.sync();
   int before, total_free;
   before_and_total(cluster, &free_here, before, total_free);
   const bool fits = !wide && need <= total_free;
   const int take = fits ? need : 0;
   // take the lowest `take` free pages
-  for (int base = mine.begin; base < mine.end; base += kThreads) {
-    const int i = base + tid;
-    const int refs = i < mine.end ? p.refs_in[i] : 1;
-    int total = 0, at = 0;
-    if (before < take) {  // uniform: all lower pages are accounted for
-      at = scan.exclusive(refs == 0, total);
-      at += before;
+  for (int base = mine.begin; base < mine.end; base += kItems * threads) {
+    const int i = base + tid * kItems;
+    int refs[kItems], n = 0, total = 0, at = 0;
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) {
+      refs[x] = i + x < mine.end ? p.refs_in[i + x] : 1;
+      n += refs[x] == 0;
     }
-    const bool taken = before < take && refs == 0 && at < take;
-    if (i < mine.end) p.refs_out[i] = taken ? 1 : refs;
-    if (taken) p.list[at] = i;
+    if (before < take) at = before + scan.exclusive(n, total);  // uniform: all lower pages are accounted for
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) {
+      const bool taken = before < take && refs[x] == 0 && at < take;
+      if (i + x < mine.end) p.refs_out[i + x] = taken ? 1 : refs[x];
+      if (taken) p.list[at] = i + x;
+      at += refs[x] == 0;
+    }
     before += total;
   }
   cluster.sync();  // the list and the offsets are complete, and no CTA reads another's shared memory any more
-  for (int i = rank * kWarps + (tid >> 5); i < p.slots; i += kCtas * kWarps) {
+  for (int i = rank * warps + (tid >> 5); i < p.slots; i += ctas * warps) {
     const int lane = tid & 31;
     const int len = max(p.lens_in[i], 0), more = fits ? p.add[i] : 0;
     const int held = pages_of(len, p.page_size), want = pages_of(len + more, p.page_size);
@@ -180,33 +204,36 @@ struct CopyList {  // pages to copy, written by a map kernel and read by copy_ke
   int *src, *dst, *tokens;
 };
 
+constexpr int kMostForkSlots = 8192;
+
 struct ForkParams {
   const int *table_in, *lens_in, *refs_in, *parent;
   int *table_out, *lens_out, *refs_out, *status;
-  int *lowest, *list;  // scratch: the lowest slot of each parent; the pages taken
+  int *list;  // scratch: the pages taken
   CopyList copies;
   int slots, width, pages, page_size;
 };
 
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) fork_kernel(ForkParams p) {
+__global__ void __launch_bounds__(kMostThreads, 1) fork_kernel(ForkParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ BlockScan scan;
-  __shared__ int free_here;
+  __shared__ int free_here, lowest[kMostForkSlots];  // the lowest slot of each parent
+  pdl_wait();
   pdl_trigger();  // copy_kernel may be scheduled; it waits for this kernel's end
-  const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31;
-  const Share mine = share_of(p.pages, rank);
-  const Share own = share_of(p.slots, rank);
-  for (int i = mine.begin + tid; i < mine.end; i += kThreads) p.refs_out[i] = 0;
-  for (int i = own.begin + tid; i < own.end; i += kThreads) p.lowest[i] = 0x7fffffff;
-  cluster.sync();
-  for (int i = own.begin + tid; i < own.end; i += kThreads) {
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), threads = blockDim.x, warps = threads >> 5, tid = threadIdx.x, lane = tid & 31;
+  const Share mine = share_of(p.pages, rank, ctas);
+  const Share own = share_of(p.slots, rank, ctas);
+  for (int i = mine.begin + tid; i < mine.end; i += threads) p.refs_out[i] = 0;
+  for (int i = tid; i < p.slots; i += threads) lowest[i] = 0x7fffffff;
+  __syncthreads();
+  for (int i = tid; i < p.slots; i += threads) {
     const int from = p.parent[i];
-    if (from >= 0 && from < p.slots) atomicMin(p.lowest + from, i);
+    if (from >= 0 && from < p.slots) atomicMin(lowest + from, i);
   }
-  cluster.sync();
+  __syncthreads();
   // demand: every CTA counts all slots' copies (the same result in each)
   int need = 0, bad = 0;
-  for (int base = 0; base < p.slots; base += kThreads) {
+  for (int base = 0; base < p.slots; base += threads) {
     const int i = base + tid;
     int n = 0;
     if (i < p.slots) {
@@ -215,7 +242,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) for
         bad = 1;
       else if (from >= 0) {
         const int len = max(p.lens_in[from], 0);
-        n = len % p.page_size != 0 && p.lowest[from] != i && len / p.page_size < p.width;
+        n = len % p.page_size != 0 && lowest[from] != i && len / p.page_size < p.width;
       }
     }
     int total;
@@ -229,11 +256,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) for
     need += total;
   }
   bad = __syncthreads_or(bad);
+  cluster.sync();  // refs_out is zero
   // the new rows, and how often each page is held
-  for (int i = rank * kWarps + (tid >> 5); i < p.slots; i += kCtas * kWarps) {
+  for (int i = rank * warps + (tid >> 5); i < p.slots; i += ctas * warps) {
     const int from = bad ? -1 : p.parent[i];
     const int len = from >= 0 ? max(p.lens_in[from], 0) : 0;
-    const int own_page = from >= 0 && len % p.page_size != 0 && p.lowest[from] != i ? len / p.page_size : -1;
+    const int own_page = from >= 0 && len % p.page_size != 0 && lowest[from] != i ? len / p.page_size : -1;
     const int *in = p.table_in + (int64_t)(from >= 0 ? from : 0) * p.width;
     int *out = p.table_out + (int64_t)i * p.width;
     for (int j = lane; j < p.width; j += 32) {
@@ -244,28 +272,35 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) for
     if (lane == 0) p.lens_out[i] = from >= 0 ? p.lens_in[from] : 0;
   }
   cluster.sync();
-  int n_free = 0;
-  for (int i = mine.begin + tid; i < mine.end; i += kThreads) n_free += p.refs_out[i] == 0;
-  publish(n_free, scan, &free_here);
+  publish(count_free(p.refs_out, mine), scan, &free_here);
   cluster.sync();
   int before, total_free;
   before_and_total(cluster, &free_here, before, total_free);
   const bool fits = !bad && need <= total_free;
   const int short_by = need - total_free;
   if (fits) {
-    for (int base = mine.begin; base < mine.end && before < need; base += kThreads) {
-      const int i = base + tid;
-      const bool is_free = i < mine.end && p.refs_out[i] == 0;
-      int total;
-      const int at = before + scan.exclusive(is_free, total);
-      if (is_free && at < need) {
-        p.refs_out[i] = 1;
-        p.list[at] = i;
+    for (int base = mine.begin; base < mine.end && before < need; base += kItems * threads) {
+      const int i = base + tid * kItems;
+      bool is_free[kItems];
+      int n = 0, total;
+#pragma unroll
+      for (int x = 0; x < kItems; ++x) {
+        is_free[x] = i + x < mine.end && p.refs_out[i + x] == 0;
+        n += is_free[x];
+      }
+      int at = before + scan.exclusive(n, total);
+#pragma unroll
+      for (int x = 0; x < kItems; ++x) {
+        if (is_free[x] && at < need) {
+          p.refs_out[i + x] = 1;
+          p.list[at] = i + x;
+        }
+        at += is_free[x];
       }
       before += total;
     }
     cluster.sync();
-    for (int i = rank * kThreads + tid; i < need; i += kCtas * kThreads) {
+    for (int i = rank * threads + tid; i < need; i += ctas * threads) {
       const int slot = p.copies.dst[i], page = p.list[i];
       const int from = p.parent[slot];
       p.table_out[(int64_t)slot * p.width + p.lens_in[from] / p.page_size] = page;
@@ -273,14 +308,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) for
     }
   } else {  // nothing changes
     int count = 0;
-    for (int i = mine.begin + tid; i < mine.end; i += kThreads) {
+    for (int i = mine.begin + tid; i < mine.end; i += threads) {
       const int refs = p.refs_in[i];
       p.refs_out[i] = refs;
       count += refs == 0;
     }
-    for (int i = own.begin + tid; i < own.end; i += kThreads) p.lens_out[i] = p.lens_in[i];
+    for (int i = own.begin + tid; i < own.end; i += threads) p.lens_out[i] = p.lens_in[i];
     const int64_t cells = (int64_t)p.slots * p.width;
-    for (int64_t i = rank * kThreads + tid; i < cells; i += kCtas * kThreads) p.table_out[i] = p.table_in[i];
+    for (int64_t i = rank * threads + tid; i < cells; i += ctas * threads) p.table_out[i] = p.table_in[i];
     cluster.sync();  // every CTA has read free_here
     publish(count, scan, &free_here);
     cluster.sync();
@@ -303,12 +338,14 @@ struct ReleaseParams {
   int slots, width, pages, page_size;
 };
 
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) release_kernel(ReleaseParams p) {
+__global__ void __launch_bounds__(kMostThreads, 1) release_kernel(ReleaseParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ BlockScan scan;
   __shared__ int free_here;
-  const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31;
-  for (int i = rank * kWarps + (tid >> 5); i < p.slots; i += kCtas * kWarps) {
+  pdl_wait();
+  pdl_trigger();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), threads = blockDim.x, warps = threads >> 5, tid = threadIdx.x, lane = tid & 31;
+  for (int i = rank * warps + (tid >> 5); i < p.slots; i += ctas * warps) {
     const int len = max(p.lens[i], 0);
     int begin = 0, end = min(pages_of(len, p.page_size), p.width);
     if (p.gone) {
@@ -328,10 +365,8 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) rel
     if (p.gone && lane == 0) p.lens[i] = 0;
   }
   cluster.sync();
-  const Share mine = share_of(p.pages, rank);
-  int n_free = 0;
-  for (int i = mine.begin + tid; i < mine.end; i += kThreads) n_free += p.refs[i] == 0;
-  publish(n_free, scan, &free_here);
+  const Share mine = share_of(p.pages, rank, ctas);
+  publish(count_free(p.refs, mine), scan, &free_here);
   cluster.sync();
   int before, total;
   before_and_total(cluster, &free_here, before, total);
@@ -355,31 +390,40 @@ struct CompactParams {
 // With U pages in use, L(p) of them below page p: a free page p < U is hole
 // p - L(p), and the pages in use from U on have the ranks L = U - holes .. U - 1;
 // the r-th of them moves into hole r.  No source is a destination.
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) compact_kernel(CompactParams p) {
+__global__ void __launch_bounds__(kMostThreads, 1) compact_kernel(CompactParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ BlockScan scan;
   __shared__ int used_here, holes_here;
+  pdl_wait();
   pdl_trigger();  // copy_kernel may be scheduled; it waits for this kernel's end
-  const int rank = (int)cluster.block_rank(), tid = threadIdx.x;
-  const Share mine = share_of(p.pages, rank);
-  int n = 0;
-  for (int i = mine.begin + tid; i < mine.end; i += kThreads) n += p.refs_in[i] != 0;
-  publish(n, scan, &used_here);
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), threads = blockDim.x, warps = threads >> 5, tid = threadIdx.x;
+  const Share mine = share_of(p.pages, rank, ctas);
+  publish((tid == 0 ? mine.end - mine.begin : 0) - count_free(p.refs_in, mine), scan, &used_here);
   cluster.sync();
   int below, used;
   before_and_total(cluster, &used_here, below, used);
   int holes = 0;
-  for (int base = mine.begin; base < mine.end; base += kThreads) {
-    const int i = base + tid;
-    const bool live = i < mine.end && p.refs_in[i] != 0;
-    int total;
-    const int at = below + scan.exclusive(live, total);
-    if (i < mine.end) {
-      if (i >= used) p.rank_of[i] = live ? at : -1;
-      if (!live && i < used) {
-        p.copies.dst[i - at] = i;
-        ++holes;
+  for (int base = mine.begin; base < mine.end; base += kItems * threads) {
+    const int i = base + tid * kItems;
+    bool live[kItems];
+    int n = 0, total;
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) {
+      live[x] = i + x < mine.end && p.refs_in[i + x] != 0;
+      n += live[x];
+    }
+    int at = below + scan.exclusive(n, total);
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) {
+      const int page = i + x;
+      if (page < mine.end) {
+        if (page >= used) p.rank_of[page] = live[x] ? at : -1;
+        if (!live[x] && page < used) {
+          p.copies.dst[page - at] = page;
+          ++holes;
+        }
       }
+      at += live[x];
     }
     below += total;
   }
@@ -388,7 +432,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) com
   int before, total_holes;
   before_and_total(cluster, &holes_here, before, total_holes);
   const int first = used - total_holes;  // the lowest rank that moves
-  for (int i = mine.begin + tid; i < mine.end; i += kThreads) {
+  for (int i = mine.begin + tid; i < mine.end; i += threads) {
     const int refs = p.refs_in[i];
     if (i >= used) {
       if (refs != 0) {
@@ -402,14 +446,23 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 1) com
     }
   }
   const int64_t cells = (int64_t)p.slots * p.width;
-  for (int64_t i = rank * kThreads + tid; i < cells; i += kCtas * kThreads) {
-    const int page = p.table_in[i];
-    const int r = page >= used && page < p.pages ? p.rank_of[page] : -1;
-    p.table_out[i] = r >= first ? p.copies.dst[r - first] : page;
+  const int64_t stride = (int64_t)ctas * threads;
+  for (int64_t i = rank * threads + tid; i < cells; i += kItems * stride) {
+    int page[kItems], r[kItems];
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) page[x] = i + x * stride < cells ? p.table_in[i + x * stride] : -1;
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) r[x] = page[x] >= used && page[x] < p.pages ? p.rank_of[page[x]] : -1;
+#pragma unroll
+    for (int x = 0; x < kItems; ++x)
+      if (r[x] >= first) page[x] = p.copies.dst[r[x] - first];
+#pragma unroll
+    for (int x = 0; x < kItems; ++x)
+      if (i + x * stride < cells) p.table_out[i + x * stride] = page[x];
   }
-  const Share own = share_of(p.slots, rank);
+  const Share own = share_of(p.slots, rank, ctas);
   if (p.lens_in != p.lens_out)
-    for (int i = own.begin + tid; i < own.end; i += kThreads) p.lens_out[i] = p.lens_in[i];
+    for (int i = own.begin + tid; i < own.end; i += threads) p.lens_out[i] = p.lens_in[i];
   if (rank == 0 && tid == 0) {
     p.status[0] = 0;
     p.status[1] = p.pages - used;
@@ -432,37 +485,44 @@ struct CopyParams {
   int n;
 };
 
-// One item is one page of one plane: `heads` runs of tokens * token_bytes.  Pure
-// traffic; four 16-byte loads in flight per thread before the first store.
+__device__ __forceinline__ uint4 load_once(const uint4 *p) { return ld_stream_u4(p); }
+__device__ __forceinline__ uint8_t load_once(const uint8_t *p) { return *p; }
+__device__ __forceinline__ void store_once(uint4 *p, uint4 v) { st_stream_u4(p, v); }
+__device__ __forceinline__ void store_once(uint8_t *p, uint8_t v) { *p = v; }
+
+// A warp moves up to 8 x 32 vectors (4 KB) of one run at a time: a head's tokens of one
+// page of one plane, or the whole page where its heads lie together.  Eight loads are in
+// flight before the first store, whatever the pages' size.
 template <class Vec>
 __global__ void __launch_bounds__(256) copy_kernel(CopyParams p) {
   pdl_wait();
-  const int n = p.count ? *p.count : p.n;
-  const int64_t items = (int64_t)n * p.pool.planes;
-  constexpr int V = sizeof(Vec), U = 4;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int pair = (int)(item / p.pool.planes), plane = (int)(item % p.pool.planes);
+  pdl_trigger();
+  constexpr int V = sizeof(Vec), U = 8;
+  const int n = p.count ? *p.count : p.n, lane = threadIdx.x & 31;
+  const bool together = !p.tokens && p.pool.head == p.pool.page_size * p.pool.token_bytes;
+  const unsigned runs = together ? 1 : p.pool.heads;
+  const int64_t most = p.pool.page_size * p.pool.token_bytes * (together ? p.pool.heads : 1);
+  const unsigned pieces = (unsigned)((most + U * 32 * V - 1) / (U * 32 * V));
+  const unsigned per_plane = runs * pieces;
+  const int64_t units = (int64_t)n * p.pool.planes * per_plane;
+  for (int64_t unit = blockIdx.x * 8 + (threadIdx.x >> 5); unit < units; unit += gridDim.x * 8) {
+    const int64_t page = unit / per_plane;  // (pair, plane)
+    const unsigned in_plane = (unsigned)(unit - page * per_plane), head = in_plane / pieces, piece = in_plane - head * pieces;
+    const int pair = (int)(page / p.pool.planes), plane = (int)(page - (int64_t)pair * p.pool.planes);
     const int src = p.src[pair], dst = p.dst[pair];
     if (src < 0 || src >= p.pool.pages || dst < 0 || dst >= p.pool.pages || src == dst) continue;
-    const int tokens = p.tokens ? p.tokens[pair] : p.pool.page_size;
-    const char *from = p.pool.pool + plane * p.pool.plane + src * p.pool.page;
-    char *to = p.pool.pool + plane * p.pool.plane + dst * p.pool.page;
-    const int run = (int)(tokens * p.pool.token_bytes / V);
-    const int all = run * p.pool.heads;
-    for (int base = threadIdx.x; base < all; base += 256 * U) {
-      Vec v[U];
-      int64_t at[U];
+    const int64_t bytes = p.tokens ? p.tokens[pair] * p.pool.token_bytes : most;
+    const int64_t at = plane * p.pool.plane + head * p.pool.head + ((int64_t)piece * U * 32 + lane) * V;
+    const int left = (int)((bytes - ((int64_t)piece * U * 32 + lane) * V + V - 1) / V);  // of this lane's vectors on
+    const Vec *from = reinterpret_cast<const Vec *>(p.pool.pool + at + src * p.pool.page);
+    Vec *to = reinterpret_cast<Vec *>(p.pool.pool + at + dst * p.pool.page);
+    Vec v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = base + u * 256;
-        const int head = i / run;
-        at[u] = head * p.pool.head + (int64_t)(i - head * run) * V;
-        if (i < all) v[u] = *reinterpret_cast<const Vec *>(from + at[u]);
-      }
+    for (int u = 0; u < U; ++u)
+      if (u * 32 < left) v[u] = load_once(from + u * 32);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (base + u * 256 < all) *reinterpret_cast<Vec *>(to + at[u]) = v[u];
-    }
+    for (int u = 0; u < U; ++u)
+      if (u * 32 < left) store_once(to + u * 32, v[u]);
   }
 }
 
@@ -484,6 +544,8 @@ constexpr int kWriteTokens = 8;
 
 template <class Vec>
 __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
+  pdl_wait();
+  pdl_trigger();
   const int slot = blockIdx.y;
   const int add = min(max(p.add[slot], 0), p.most);
   const int first = blockIdx.x * kWriteTokens;
@@ -512,6 +574,23 @@ __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
 
 // ---------------------------------------------------------------- host side
 
+template <class Params>
+int launch_maps(const char *me, void (*kernel)(Params), int64_t cells, cudaStream_t s, const Params &p) {
+  const unsigned ctas = cells <= 2048 ? 1 : kMostCtas, threads = cells <= 2048 ? 256 : cells <= 65536 ? 512 : kMostThreads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {ctas, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), me);
+}
+
 int check_maps(const char *me, int64_t slots, int64_t width, int64_t pages, int64_t page_size) {
   if (slots < 0 || width < 0 || pages < 0 || page_size < 1) return fail(LC_ERR_INVALID, "%s: negative or zero size", me);
   if (slots > (1 << 20) || pages > (1 << 30) || page_size > (1 << 20) || width > (1 << 24) || width * page_size > (1ll << 30))
@@ -536,10 +615,14 @@ bool all_multiple(const int64_t *v, int n, int64_t of) {
   return true;
 }
 
-int launch_copy(const char *me, const CopyParams &p, cudaStream_t s) {
+int launch_copy(const char *me, const CopyParams &p, int64_t most_pairs, cudaStream_t s) {
   const int64_t sizes[4] = {p.pool.token_bytes, p.pool.plane, p.pool.page, p.pool.head};
   const bool wide = aligned(p.pool.pool, 16) && all_multiple(sizes, 4, 16);
-  const unsigned grid = (unsigned)sm_count() * 8;
+  // as many CTAs as there can be units of 4 KB for, up to 32 per SM (whole pages,
+  // 1.1 GB: 195 us with 8, 182 with 32, 180 with 64; where fewer move than could, the rest leave at once)
+  const int64_t page_bytes = p.pool.heads * p.pool.page_size * p.pool.token_bytes;
+  const int64_t units = most_pairs * p.pool.planes * std::max<int64_t>(p.pool.heads, (page_bytes + 4095) / 4096);
+  const unsigned grid = (unsigned)std::min<int64_t>(sm_count() * 32, (units + 7) / 8);
   const cudaError_t err = wide ? launch_pdl(copy_kernel<uint4>, dim3(grid), dim3(256), 0, s, p)
                                : launch_pdl(copy_kernel<uint8_t>, dim3(grid), dim3(256), 0, s, p);
   return check_cuda(err, me);
@@ -563,8 +646,7 @@ extern "C" int lc_cache_extend(const int32_t *table_in, int32_t *table_out, cons
   int *ints = static_cast<int *>(scratch);
   const ExtendParams p = {table_in, lens_in, refs_in, add, table_out, lens_out, refs_out, status, ints, ints + slots,
                           (int)slots, (int)width, (int)pages, (int)page_size};
-  extend_kernel<<<kCtas, kThreads, 0, s>>>(p);
-  return check_launch(me);
+  return launch_maps(me, extend_kernel, slots * width + pages, s, p);
 }
 
 extern "C" int lc_cache_write(const void *k, const void *v, void *k_pages, void *v_pages, const int32_t *table,
@@ -587,11 +669,7 @@ extern "C" int lc_cache_write(const void *k, const void *v, void *k_pages, void 
                     row_bytes % 16 == 0 && all_multiple(strides, 12, 16);
   const dim3 grid((unsigned)((most + kWriteTokens - 1) / kWriteTokens), (unsigned)slots);
   cudaStream_t s = as_stream(stream);
-  if (wide)
-    write_kernel<uint4><<<grid, 256, 0, s>>>(p);
-  else
-    write_kernel<uint8_t><<<grid, 256, 0, s>>>(p);
-  return check_launch(me);
+  return check_cuda(wide ? launch_pdl(write_kernel<uint4>, grid, dim3(256), 0, s, p) : launch_pdl(write_kernel<uint8_t>, grid, dim3(256), 0, s, p), me);
 }
 
 extern "C" int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes, const int64_t *strides,
@@ -606,20 +684,20 @@ extern "C" int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64
   if (!status || (slots > 0 && (!lens_in || !lens_out || !parent || (width > 0 && (!table_in || !table_out)))) ||
       (pages > 0 && (!refs_in || !refs_out)))
     return fail(LC_ERR_INVALID, "%s: null buffer", me);
+  if (slots > kMostForkSlots) return fail(LC_ERR_UNSUPPORTED, "%s: %lld slots, at most %d", me, (long long)slots, kMostForkSlots);
   if ((slots > 0 && (lens_in == lens_out || (width > 0 && table_in == table_out))) || (pages > 0 && refs_in == refs_out))
     return fail(LC_ERR_INVALID, "%s: the new maps may not overwrite the old ones", me);
   cudaStream_t s = as_stream(stream);
   void *scratch = nullptr;
-  if (int rc = scratch_buffer(s, kScratchSlot, (size_t)(5 * slots + 1) * 4, &scratch)) return rc;
+  if (int rc = scratch_buffer(s, kScratchSlot, (size_t)(4 * slots + 1) * 4, &scratch)) return rc;
   int *ints = static_cast<int *>(scratch);
-  ForkParams p = {table_in, lens_in, refs_in, parent, table_out, lens_out, refs_out, status, ints + 1, ints + 1 + slots,
-                  {ints, ints + 1 + 2 * slots, ints + 1 + 3 * slots, ints + 1 + 4 * slots},
+  ForkParams p = {table_in, lens_in, refs_in, parent, table_out, lens_out, refs_out, status, ints + 1,
+                  {ints, ints + 1 + slots, ints + 1 + 2 * slots, ints + 1 + 3 * slots},
                   (int)slots, (int)width, (int)pages, (int)page_size};
-  fork_kernel<<<kCtas, kThreads, 0, s>>>(p);
-  if (int rc = check_launch(me)) return rc;
+  if (int rc = launch_maps(me, fork_kernel, slots * width + pages, s, p)) return rc;
   if (planes == 0 || pages == 0 || slots == 0) return LC_OK;
   c.src = p.copies.src, c.dst = p.copies.dst, c.tokens = p.copies.tokens, c.count = p.copies.count;
-  return launch_copy(me, c, s);
+  return launch_copy(me, c, slots, s);
 }
 
 extern "C" int lc_cache_release(int32_t *table, int32_t *lens, int32_t *refs, const int32_t *gone, int64_t window,
@@ -634,8 +712,7 @@ extern "C" int lc_cache_release(int32_t *table, int32_t *lens, int32_t *refs, co
   const int64_t most = 1ll << 30;
   const ReleaseParams p = {table, lens, refs, status, gone, (int)(window < most ? window : most), (int)(sinks < most ? sinks : most),
                            (int)slots, (int)width, (int)pages, (int)page_size};
-  release_kernel<<<kCtas, kThreads, 0, as_stream(stream)>>>(p);
-  return check_launch(me);
+  return launch_maps(me, release_kernel, slots * width + pages, as_stream(stream), p);
 }
 
 extern "C" int lc_cache_compact(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes,
@@ -657,11 +734,10 @@ extern "C" int lc_cache_compact(void *pool, int64_t planes, int64_t kv_heads, in
   int *ints = static_cast<int *>(scratch);
   const CompactParams p = {table_in, lens_in, refs_in, table_out, lens_out, refs_out, status, ints + 1,
                            {ints, ints + 1 + pages, ints + 1 + 2 * pages, nullptr}, (int)slots, (int)width, (int)pages};
-  compact_kernel<<<kCtas, kThreads, 0, s>>>(p);
-  if (int rc = check_launch(me)) return rc;
+  if (int rc = launch_maps(me, compact_kernel, slots * width + pages, s, p)) return rc;
   if (planes == 0 || pages == 0) return LC_OK;
   c.src = p.copies.src, c.dst = p.copies.dst, c.count = p.copies.count;
-  return launch_copy(me, c, s);
+  return launch_copy(me, c, (pages + 1) / 2, s);
 }
 
 extern "C" int lc_cache_copy(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes, const int64_t *strides,
@@ -677,5 +753,5 @@ extern "C" int lc_cache_copy(void *pool, int64_t planes, int64_t kv_heads, int64
   if (n == 0 || planes == 0 || pages == 0) return LC_OK;
   if (!src || !dst) return fail(LC_ERR_INVALID, "%s: null buffer", me);
   c.src = src, c.dst = dst, c.n = (int)n;
-  return launch_copy(me, c, as_stream(stream));
+  return launch_copy(me, c, n, as_stream(stream));
 }

@@ -63,6 +63,7 @@ def test_invalid_arguments(case):
 UNSUPPORTED = [
     lambda: window(d=264), lambda: window(batch=1 << 17), lambda: window(s_q=1 << 31), lambda: decode(d=257), lambda: decode(width=1 << 30),
     lambda: decode(slots=1 << 21), lambda: fork(token=1 << 20),
+    lambda: runtime.call("lc_cache_fork", P, 1, 1, 16, strides(3), P, P, P, P, P, P, P, P, 8193, 4, 4, 16, NULL),
     lambda: runtime.call("lc_cache_extend", P, P, P, P, P, P, P, P, 1 << 24, 4, 4, 16, NULL),
 ]
 
