@@ -41,61 +41,96 @@ __host__ __device__ __forceinline__ Visible visible(int p, int window, int sinks
   return {sinks < lo ? sinks : lo, lo};
 }
 
-// Running softmax of one query row spread over the lanes of a warp: lane c
-// holds output elements c, c + 32, ...
+// Running softmax of one query row of up to 32 NC columns spread over the lanes of a
+// warp: lane c holds output elements c, c + 32, ...
+template <int NC>
 struct RowState {
   float m = -INFINITY, l = 0.f;
-  float acc[kMaxHead / 32];
+  float acc[NC];
   __device__ __forceinline__ RowState() {
 #pragma unroll
-    for (int i = 0; i < kMaxHead / 32; ++i) acc[i] = 0.f;
+    for (int i = 0; i < NC; ++i) acc[i] = 0.f;
   }
 };
 
-template <class T>
-__device__ __forceinline__ void load_row(float (&q)[kMaxHead / 32], const T *src, int d, int lane, float factor) {
+template <class T, int NC>
+__device__ __forceinline__ void load_row(float (&q)[NC], const T *src, int d, int lane, float factor) {
 #pragma unroll
-  for (int i = 0; i < kMaxHead / 32; ++i) {
+  for (int i = 0; i < NC; ++i) {
     const int c = lane + 32 * i;
     q[i] = c < d ? Elem<T>::to_float(src[c]) * factor : 0.f;
   }
 }
 
-// Takes the keys j = begin, begin + step, ... < end into the row; `at(j, k, v)`
-// sets the rows of key j, or returns false where there is none.
-template <class T, class At>
-__device__ __forceinline__ void attend_keys(RowState &st, const float (&q)[kMaxHead / 32], int d, int lane, int begin,
-                                            int end, int step, const At &at) {
-  for (int j = begin; j < end; j += step) {
-    const T *k, *v;
-    if (!at(j, k, v)) continue;
-    float dot = 0.f;
+// Takes the keys j = begin, begin + step, ... < end into the row; `at(j, k, v)` sets
+// the rows of key j, or readable ones in their place, and says whether key j counts.
+// Four keys at a time, and every load unconditional in the key, so that the loads
+// and the lanes' sums overlap.
+template <class T, int NC, class At>
+__device__ __forceinline__ void attend_keys(RowState<NC> &st, const float (&q)[NC], int d, int lane, int begin, int end, int step,
+                                            const At &at) {
+  constexpr int U = 4;
+  for (int j = begin; j < end; j += U * step) {
+    bool real[U];
+    const T *kr[U], *vr[U];
 #pragma unroll
-    for (int i = 0; i < kMaxHead / 32; ++i) {
-      const int c = lane + 32 * i;
-      if (c < d) dot = fmaf(q[i], Elem<T>::to_float(k[c]), dot);
+    for (int u = 0; u < U; ++u) {
+      const int key = j + u * step;
+      real[u] = at(key < end ? key : j, kr[u], vr[u]) && key < end;
     }
-    dot = warp_sum(dot);
-    const float m_new = fmaxf(st.m, dot);
-    const float base = m_new == -INFINITY ? 0.f : m_new;  // a row of -inf scores so far
-    const float alpha = exp2f(st.m - base), w = exp2f(dot - base);
-    st.m = m_new;
-    st.l = st.l * alpha + w;
+    T kv[U][NC], vv[U][NC];
 #pragma unroll
-    for (int i = 0; i < kMaxHead / 32; ++i) {
+    for (int i = 0; i < NC; ++i) {
       const int c = lane + 32 * i;
-      if (c < d) st.acc[i] = fmaf(w, Elem<T>::to_float(v[c]), st.acc[i] * alpha);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        kv[u][i] = vv[u][i] = Elem<T>::from_float(0.f);
+        if (c < d) {
+          kv[u][i] = kr[u][c];
+          vv[u][i] = vr[u][c];
+        }
+      }
+    }
+    float s[U], v[U][NC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        s[u] = fmaf(q[i], Elem<T>::to_float(kv[u][i]), s[u]);
+        v[u][i] = Elem<T>::to_float(vv[u][i]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = warp_sum(s[u]);
+    float m_new = st.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (real[u]) m_new = fmaxf(m_new, s[u]);
+    const float base = m_new == -INFINITY ? 0.f : m_new;  // a row of -inf scores so far
+    const float alpha = exp2f(st.m - base);
+    st.m = m_new;
+    st.l *= alpha;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) st.acc[i] *= alpha;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!real[u]) continue;
+      const float w = exp2f(s[u] - base);
+      st.l += w;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) st.acc[i] = fmaf(w, v[u][i], st.acc[i]);
     }
   }
 }
 
 // Writes a row whose sums are complete: O / l, and the log-sum-exp.  A row
 // that saw nothing (or only scores of -inf) is 0 and -inf.
-template <class T>
-__device__ __forceinline__ void store_row(const RowState &st, T *o, float *lse, int d, int lane) {
+template <class T, int NC>
+__device__ __forceinline__ void store_row(const RowState<NC> &st, T *o, float *lse, int d, int lane) {
   const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
 #pragma unroll
-  for (int i = 0; i < kMaxHead / 32; ++i) {
+  for (int i = 0; i < NC; ++i) {
     const int c = lane + 32 * i;
     if (c < d) o[c] = Elem<T>::from_float(st.acc[i] * inv);
   }
@@ -104,11 +139,11 @@ __device__ __forceinline__ void store_row(const RowState &st, T *o, float *lse, 
 
 // The same row for a kernel whose own sums came out infinite or NaN in some
 // columns: those alone are written, the others keep their bits.
-template <class T>
-__device__ __forceinline__ void mend_row(const RowState &st, T *o, int d, int lane) {
+template <class T, int NC>
+__device__ __forceinline__ void mend_row(const RowState<NC> &st, T *o, int d, int lane) {
   const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
 #pragma unroll
-  for (int i = 0; i < kMaxHead / 32; ++i) {
+  for (int i = 0; i < NC; ++i) {
     const int c = lane + 32 * i;
     if (c < d && !isfinite(Elem<T>::to_float(o[c]))) o[c] = Elem<T>::from_float(st.acc[i] * inv);
   }
@@ -116,35 +151,30 @@ __device__ __forceinline__ void mend_row(const RowState &st, T *o, int d, int la
 
 // Joins the states of the WARPS warps of a CTA, which each took a share of one
 // row's keys, in warp order; warp 0 receives the row.
-template <int WARPS>
-__device__ __forceinline__ void join_warps(RowState &st, float *scratch /* WARPS * (kMaxHead + 2) */) {
+template <int WARPS, int NC>
+__device__ __forceinline__ void join_warps(RowState<NC> &st, float *scratch /* WARPS * (32 * NC + 2) */) {
+  constexpr int kWide = 32 * NC;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float *mine = scratch + warp * (kMaxHead + 2);
+  float *mine = scratch + warp * (kWide + 2);
 #pragma unroll
-  for (int i = 0; i < kMaxHead / 32; ++i) mine[lane + 32 * i] = st.acc[i];
+  for (int i = 0; i < NC; ++i) mine[lane + 32 * i] = st.acc[i];
   if (lane == 0) {
-    mine[kMaxHead] = st.m;
-    mine[kMaxHead + 1] = st.l;
+    mine[kWide] = st.m;
+    mine[kWide + 1] = st.l;
   }
   __syncthreads();
   if (warp != 0) return;
   float m = -INFINITY;
-  bool nan = false;
-  for (int w = 0; w < WARPS; ++w) {
-    m = fmaxf(m, scratch[w * (kMaxHead + 2) + kMaxHead]);
-    nan |= isnan(scratch[w * (kMaxHead + 2) + kMaxHead + 1]);
-  }
-  RowState sum;
+  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, scratch[w * (kWide + 2) + kWide]);
+  RowState<NC> sum;
   sum.m = m;
-  if (nan || m != -INFINITY) {
-    for (int w = 0; w < WARPS; ++w) {
-      const float *s = scratch + w * (kMaxHead + 2);
-      if (s[kMaxHead + 1] == 0.f) continue;  // no keys: its sums are zero
-      const float a = exp2f(s[kMaxHead] - (m == -INFINITY ? 0.f : m));
-      sum.l = fmaf(s[kMaxHead + 1], a, sum.l);
+  for (int w = 0; w < WARPS; ++w) {
+    const float *s = scratch + w * (kWide + 2);
+    if (s[kWide + 1] == 0.f) continue;  // no keys: its sums are zero
+    const float a = exp2f(s[kWide] - (m == -INFINITY ? 0.f : m));
+    sum.l = fmaf(s[kWide + 1], a, sum.l);
 #pragma unroll
-      for (int i = 0; i < kMaxHead / 32; ++i) sum.acc[i] = fmaf(s[lane + 32 * i], a, sum.acc[i]);
-    }
+    for (int i = 0; i < NC; ++i) sum.acc[i] = fmaf(s[lane + 32 * i], a, sum.acc[i]);
   }
   st = sum;
 }

@@ -39,21 +39,22 @@ constexpr int kPartialsSlot = 41, kArrivedSlot = 42, kSpansSlot = 46;  // scratc
 
 // ---------------------------------------------------------------- plain form
 // One row key by key, by the WARPS warps of a CTA; warp 0 receives it.
-template <class T, int WARPS>
-__device__ __forceinline__ void plain_row(const DecodeParams &p, int slot, int h, int head, RowState &st, float *scratch) {
+template <class T, int WARPS, int NC>
+__device__ __forceinline__ void plain_row(const DecodeParams &p, int slot, int h, int head, RowState<NC> &st, float *scratch) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = cached_tokens(p, slot);
-  float q[kMaxHead / 32];
+  float q[NC];
   load_row(q, static_cast<const T *>(p.q) + slot * p.qs[0] + h * p.qs[1], p.d, lane, p.scale_log2);
   const int *row = p.table + slot * p.ts;
   auto at = [&](int j, const T *&k, const T *&v) {
-    const int page = row[page_index(p, j)], r = j - page_index(p, j) * p.page_size;
-    if ((unsigned)page >= (unsigned)p.pages) return false;
+    const int entry = row[page_index(p, j)], r = j - page_index(p, j) * p.page_size;
+    const bool held = (unsigned)entry < (unsigned)p.pages;
+    const int64_t page = held ? entry : 0;
     k = static_cast<const T *>(p.k) + page * p.ks[0] + head * p.ks[1] + r * p.ks[2];
     v = static_cast<const T *>(p.v) + page * p.vs[0] + head * p.vs[1] + r * p.vs[2];
-    return true;
+    return held;
   };
-  if (n > 0) {
+  if (n > 0 && p.pages > 0) {
     const Visible see = visible(n - 1, p.window, p.sinks);
     attend_keys<T>(st, q, p.d, lane, warp, see.sink_end, WARPS, at);
     attend_keys<T>(st, q, p.d, lane, see.lo + warp, n, WARPS, at);
@@ -61,15 +62,17 @@ __device__ __forceinline__ void plain_row(const DecodeParams &p, int slot, int h
   join_warps<WARPS>(st, scratch);
 }
 
-// One CTA of eight warps per (slot, query head): what the tensor-core form below does
-// not take (odd head sizes and alignments).
+// One CTA of eight warps per (slot, query head): few keys, and what the tensor-core form
+// below does not take (odd head sizes and alignments).
 constexpr int kRowWarps = 8;
 
-template <class T>
+template <class T, int NC>
 __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams p) {
-  __shared__ float scratch[kRowWarps * (kMaxHead + 2)];
+  __shared__ float scratch[kRowWarps * (32 * NC + 2)];
+  pdl_wait();
+  pdl_trigger();
   const int slot = blockIdx.x, h = blockIdx.y;
-  RowState st;
+  RowState<NC> st;
   plain_row<T, kRowWarps>(p, slot, h, h / (p.q_heads / p.kv_heads), st, scratch);
   if (threadIdx.x < 32)
     store_row(st, static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1],
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   constexpr int kCopies = kTileKeys / kRowsPerCopy;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ unsigned masks[kDecodeWarps][STAGES];  // the visible keys of each warp's staged tiles
-  __shared__ float scratch[kDecodeWarps * (kMaxHead + 2)];  // the plain form's joins
+  __shared__ float scratch[kDecodeWarps * (DP + 2)];  // the plain form's joins
   __shared__ float merge_m[kDecodeWarps][kRows], merge_l[kDecodeWarps][kRows], merge_w[kDecodeWarps][kRows];
   __shared__ float row_m[kRows], row_l[kRows];
   __shared__ long long sums[kDecodeWarps];
@@ -517,7 +520,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
     const int head = use.part / chunks, first = head * group + use.part % chunks * kRows;
     const int live = min(kRows, (head + 1) * group - first);
     for (int x = 0; x < live; ++x) {
-      RowState st;
+      RowState<DP / 32> st;
       __syncthreads();
       plain_row<T, kDecodeWarps>(p, use.slot, first + x, head, st, scratch);
       if (warp == 0) mend_row(st, static_cast<T *>(p.o) + use.slot * p.os[0] + (first + x) * p.os[1], p.d, lane);
@@ -715,7 +718,7 @@ constexpr int kJoinWarps = 8;
 template <class T, int DP, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodeParams p, DecodeWork work) {
   constexpr int kRows = 8 * NT, kCols = DP / 32;
-  __shared__ float scratch[kJoinWarps * (kMaxHead + 2)];
+  __shared__ float scratch[kJoinWarps * (DP + 2)];
   __shared__ int found;
   pdl_wait();
   pdl_trigger();
@@ -765,24 +768,24 @@ __global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodePara
   }
   __syncthreads();  // block_max's scratch has been read
 #pragma unroll
-  for (int x = 0; x < kCols; ++x) scratch[warp * (kMaxHead + 2) + lane * kCols + x] = o[x];
-  if (lane == 0) scratch[warp * (kMaxHead + 2) + kMaxHead] = sum;
+  for (int x = 0; x < kCols; ++x) scratch[warp * (DP + 2) + lane * kCols + x] = o[x];
+  if (lane == 0) scratch[warp * (DP + 2) + DP] = sum;
   __syncthreads();
   sum = 0.f;
-  for (int w = 0; w < kJoinWarps; ++w) sum += scratch[w * (kMaxHead + 2) + kMaxHead];
+  for (int w = 0; w < kJoinWarps; ++w) sum += scratch[w * (DP + 2) + DP];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T *out = static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1];
   bool odd = false;
   if (tid < p.d) {
     float v = 0.f;
-    for (int w = 0; w < kJoinWarps; ++w) v += scratch[w * (kMaxHead + 2) + tid];
+    for (int w = 0; w < kJoinWarps; ++w) v += scratch[w * (DP + 2) + tid];
     v *= inv;
     odd = !isfinite(v);
     out[tid] = Elem<T>::from_float(v);
   }
   if (p.lse && tid == 0) p.lse[(int64_t)slot * p.q_heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
   if (__syncthreads_or(odd)) {  // as in decode_kernel
-    RowState st;
+    RowState<DP / 32> st;
     plain_row<T, kJoinWarps>(p, slot, h, head, st, scratch);
     if (warp == 0) mend_row(st, out, p.d, lane);
   }
@@ -842,6 +845,23 @@ bool decode_tensor(const DecodeParams &p) {
   return ok;
 }
 
+// Few rows of few keys, by what any slot can see: as in window_attention.cu (1 x 8 rows
+// of 68 keys: 4.7 against 5.5 us, 16 x 8: 5.1 against 6.4; 64 x 8 of 68: 9.4 against 6.6, 1 x 8 of 128: 6.2 against 5.5).
+bool few_keys(const DecodeParams &p) {
+  const int64_t most = (int64_t)p.width * p.page_size;
+  const int64_t reach = p.window ? std::min<int64_t>((int64_t)p.window + p.sinks, most) : most;
+  return reach <= 96 && (int64_t)p.slots * p.q_heads * reach <= 16384;
+}
+
+template <class T>
+int launch_rows(const DecodeParams &p, cudaStream_t s) {
+  const dim3 grid((unsigned)p.slots, (unsigned)p.q_heads), block(kRowWarps * 32);
+  return check_cuda(p.d <= 64    ? launch_pdl(decode_row_kernel<T, 2>, grid, block, 0, s, p)
+                    : p.d <= 128 ? launch_pdl(decode_row_kernel<T, 4>, grid, block, 0, s, p)
+                                 : launch_pdl(decode_row_kernel<T, 8>, grid, block, 0, s, p),
+                    "lc_paged_decode (rows)");
+}
+
 }  // namespace
 }  // namespace lc
 
@@ -878,16 +898,11 @@ extern "C" int lc_paged_decode(int dtype, const void *q, const void *k, const vo
   for (int x = 0; x < 21; ++x)
     if (page_size == 1ll << x) p.page_shift = x;
   cudaStream_t s = as_stream(stream);
-  if (decode_tensor(p)) {
+  if (!few_keys(p) && decode_tensor(p)) {
     const int padded = d <= 64 ? 64 : d <= 128 ? 128 : 256;
     p.dense = d == padded && p.ks[2] == d && p.vs[2] == d;
     if (dtype == LC_F16) return page_size % 16 == 0 ? launch_sized<__half, true>(p, s) : launch_sized<__half, false>(p, s);
     return page_size % 16 == 0 ? launch_sized<__nv_bfloat16, true>(p, s) : launch_sized<__nv_bfloat16, false>(p, s);
   }
-  const dim3 grid((unsigned)slots, (unsigned)q_heads);
-  if (dtype == LC_F16)
-    decode_row_kernel<__half><<<grid, kRowWarps * 32, 0, s>>>(p);
-  else
-    decode_row_kernel<__nv_bfloat16><<<grid, kRowWarps * 32, 0, s>>>(p);
-  return check_launch(me);
+  return dtype == LC_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s);
 }

@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -105,6 +106,11 @@ void *stream_of(PyObject *o, const at::Tensor &t) {
   if (o == Py_None) return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
   return reinterpret_cast<void *>(static_cast<intptr_t>(integer(o)));
 }
+// An uninitialised tensor on the device of `like`, without the dispatcher's way there.
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Tensor &like) {
+  return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
+}
+
 template <class T = void>
 T *ptr(const at::Tensor *t) {
   return t ? static_cast<T *>(t->data_ptr()) : nullptr;
@@ -153,8 +159,8 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (kv_lens) check_ints(*kv_lens, "kv_lens", q, {batch});
   if (given) check(*given, "out", q, q.scalar_type(), {batch, s_q, heads, d});
   const c10::cuda::CUDAGuard guard(q.device());
-  const at::Tensor out = given ? *given : at::empty({batch, s_q, heads, d}, q.options());
-  const at::Tensor lse = a[9] == Py_True ? at::empty({batch, heads, s_q}, q.options().dtype(at::kFloat)) : at::Tensor();
+  const at::Tensor out = given ? *given : fresh({batch, s_q, heads, d}, q.scalar_type(), q);
+  const at::Tensor lse = a[9] == Py_True ? fresh({batch, heads, s_q}, at::kFloat, q) : at::Tensor();
   const at::Tensor *views[4] = {&q, &k, &v, &out};
   const char *names[4] = {"q", "k", "v", "out"};
   int64_t strides[12];
@@ -189,8 +195,8 @@ PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const at::Tensor *given = maybe(a[8], "out");
   if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d});
   const c10::cuda::CUDAGuard guard(q.device());
-  const at::Tensor out = given ? *given : at::empty({slots, heads, d}, q.options());
-  const at::Tensor lse = a[9] == Py_True ? at::empty({slots, heads}, q.options().dtype(at::kFloat)) : at::Tensor();
+  const at::Tensor out = given ? *given : fresh({slots, heads, d}, q.scalar_type(), q);
+  const at::Tensor lse = a[9] == Py_True ? fresh({slots, heads}, at::kFloat, q) : at::Tensor();
   check_inner(q, "q");
   check_inner(k, "k_pages");
   check_inner(v, "v_pages");
@@ -233,16 +239,16 @@ Maps maps_of(PyObject *const *a, const char *what) {
 Maps into_of(const Maps &m, PyObject *const *a) {
   Maps to = m;
   if (a[0] == Py_None) {
-    to.table = at::empty_like(m.table);
-    to.lens = at::empty_like(m.lens);
-    to.refs = at::empty_like(m.refs);
+    to.table = fresh({m.slots, m.width}, at::kInt, m.table);
+    to.lens = fresh({m.slots}, at::kInt, m.table);
+    to.refs = fresh({m.pages}, at::kInt, m.table);
     to.status = at::Tensor();
   } else {
     to = maps_of(a, "into");
     if (to.slots != m.slots || to.width != m.width || to.pages != m.pages || to.table.device() != m.table.device())
       refuse("into: other sizes or another device than the maps");
   }
-  if (!to.status.defined()) to.status = at::empty({2}, m.lens.options());
+  if (!to.status.defined()) to.status = fresh({2}, at::kInt, m.table);
   return to;
 }
 PyObject *wrapped(const Maps &m) {

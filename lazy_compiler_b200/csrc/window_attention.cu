@@ -35,21 +35,23 @@ __device__ __forceinline__ int length_of(const int *lens, int b, int most) {
 
 // ---------------------------------------------------------------- plain form
 // One CTA of four warps per (row, query head), the row's keys dealt to the
-// warps: what the tensor-core form does not take (head sizes over 128 or not a
-// multiple of 8, odd alignments, groups of over 128 heads).
+// warps: few rows of few keys, and what the tensor-core form does not take (head
+// sizes over 128 or not a multiple of 8, odd alignments, groups of over 128 heads).
 constexpr int kRowWarps = 4;
 
-template <class T>
+template <class T, int NC>
 __global__ void __launch_bounds__(kRowWarps * 32) window_row_kernel(WindowParams p) {
-  __shared__ float scratch[kRowWarps * (kMaxHead + 2)];
+  __shared__ float scratch[kRowWarps * (32 * NC + 2)];
+  pdl_wait();
+  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int hk = h / (p.q_heads / p.kv_heads);
   const int n_q = length_of(p.q_lens, b, p.s_q), n_kv = length_of(p.kv_lens, b, p.s_kv);
   const int pos = n_kv - n_q + i;
-  RowState st;
+  RowState<NC> st;
   if (i < n_q && pos >= 0) {
-    float q[kMaxHead / 32];
+    float q[NC];
     load_row(q, static_cast<const T *>(p.q) + b * p.qs[0] + i * p.qs[1] + h * p.qs[2], p.d, lane, p.scale_log2);
     const T *k0 = static_cast<const T *>(p.k) + b * p.ks[0] + hk * p.ks[2];
     const T *v0 = static_cast<const T *>(p.v) + b * p.vs[0] + hk * p.vs[2];
@@ -304,7 +306,7 @@ __device__ __forceinline__ bool wait_all(uint64_t *bar, uint32_t parity, volatil
 
 // Rows of this warp (a lane each, `odd` where it holds one) whose output came out
 // infinite or NaN, key by key; the columns that came out finite keep their bits.
-template <class T>
+template <class T, int NC>
 __device__ __noinline__ void mend_rows(const WindowParams &p, bool odd, int b, int hk, int pos, int i, int h) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
@@ -312,8 +314,8 @@ __device__ __noinline__ void mend_rows(const WindowParams &p, bool odd, int b, i
     const int from = __ffs(left) - 1;
     const int row_pos = __shfl_sync(0xffffffffu, pos, from), row_i = __shfl_sync(0xffffffffu, i, from),
               row_h = __shfl_sync(0xffffffffu, h, from);
-    RowState st;
-    float q[kMaxHead / 32];
+    RowState<NC> st;
+    float q[NC];
     load_row(q, static_cast<const T *>(p.q) + b * p.qs[0] + row_i * p.qs[1] + row_h * p.qs[2], p.d, lane, p.scale_log2);
     const T *k0 = static_cast<const T *>(p.k) + b * p.ks[0] + hk * p.ks[2];
     const T *v0 = static_cast<const T *>(p.v) + b * p.vs[0] + hk * p.vs[2];
@@ -330,7 +332,7 @@ __device__ __noinline__ void mend_rows(const WindowParams &p, bool odd, int b, i
 }
 
 // The rows of a finished item, a lane each (row 0 .. 255 of its two tiles).
-template <class T>
+template <class T, int NC>
 __device__ __noinline__ void mend_piece(const WindowParams &p, const TensorParams &tp, const Item &it, int tile_row) {
   const int t = tile_row / kRows, row = tile_row % kRows;
   const int token = row / tp.group, h = it.hk * tp.group + row - token * tp.group;
@@ -341,7 +343,7 @@ __device__ __noinline__ void mend_piece(const WindowParams &p, const TensorParam
     for (int c = 0; c < p.d; ++c) odd |= !isfinite(Elem<T>::to_float(out[c]));
   }
   __syncwarp();
-  if (__any_sync(0xffffffffu, odd)) mend_rows<T>(p, odd, it.b, it.hk, pos, i, h);
+  if (__any_sync(0xffffffffu, odd)) mend_rows<T, NC>(p, odd, it.b, it.hk, pos, i, h);
 }
 
 // POLY: of sixteen pairs of exponentials, how many go to the FMA pipe.
@@ -896,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (pieces.next(p, tp, lens, piece)) {
       if (piece.j1 - piece.j0 < piece.it.n) continue;
       for (int first = warp * 32; first < kTiles * kRows; first += kThreads)
-        mend_piece<T>(p, tp, piece.it, first + lane);
+        mend_piece<T, DP / 32>(p, tp, piece.it, first + lane);
     }
   }
 }
@@ -1012,7 +1014,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Windo
     p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
   if (DEEP) __syncthreads();  // the other warps' columns are there: mended once or more, but alike
   const unsigned odd_lanes = __ballot_sync(0xffffffffu, odd);
-  if (odd_lanes) mend_rows<T>(p, (lane & 3) == 0 && (odd_lanes >> lane & 0xf) != 0, it.b, it.hk, pos, i, h);
+  if (odd_lanes) mend_rows<T, DP / 32>(p, (lane & 3) == 0 && (odd_lanes >> lane & 0xf) != 0, it.b, it.hk, pos, i, h);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1150,6 +1152,24 @@ int window_sized(const WindowParams &p, cudaStream_t s) {
   return p.d <= 64 ? launch_window<T, 64, 1>(p, s) : launch_window<T, 128, 1>(p, s);
 }
 
+// Few rows of few keys: a CTA per row is done before the tensor-core form has set up its
+// barriers, tensor memory and copies (19 rows x 8 heads of 19 keys: 2.7 against 6.7 us,
+// 16 x 32 of 64: 6.0 against 7.7; 64 x 32 of 64: 12.2 against 8.9, 1 x 8 of 256: 10.8
+// against 8.0).
+bool few_keys(const WindowParams &p) {
+  const int64_t reach = p.window ? std::min<int64_t>((int64_t)p.window + p.sinks, p.s_kv) : p.s_kv;
+  return reach <= 128 && (int64_t)p.batch * p.s_q * p.q_heads * reach <= 32768;
+}
+
+template <class T>
+int launch_rows(const WindowParams &p, cudaStream_t s) {
+  const dim3 grid((unsigned)p.s_q, (unsigned)p.q_heads, (unsigned)p.batch), block(kRowWarps * 32);
+  return check_cuda(p.d <= 64    ? launch_pdl(window_row_kernel<T, 2>, grid, block, 0, s, p)
+                    : p.d <= 128 ? launch_pdl(window_row_kernel<T, 4>, grid, block, 0, s, p)
+                                 : launch_pdl(window_row_kernel<T, 8>, grid, block, 0, s, p),
+                    "lc_window_attention (rows)");
+}
+
 }  // namespace
 }  // namespace lc
 
@@ -1181,11 +1201,6 @@ extern "C" int lc_window_attention(int dtype, const void *q, const void *k, cons
   p.sinks = (int)(sinks < s_kv ? sinks : s_kv);
   p.scale_log2 = scale * attend::kLog2e;
   cudaStream_t s = as_stream(stream);
-  if (window_tensor(p)) return dtype == LC_F16 ? window_sized<__half>(p, s) : window_sized<__nv_bfloat16>(p, s);
-  const dim3 grid((unsigned)s_q, (unsigned)q_heads, (unsigned)batch);
-  if (dtype == LC_F16)
-    window_row_kernel<__half><<<grid, kRowWarps * 32, 0, s>>>(p);
-  else
-    window_row_kernel<__nv_bfloat16><<<grid, kRowWarps * 32, 0, s>>>(p);
-  return check_launch(me);
+  if (!few_keys(p) && window_tensor(p)) return dtype == LC_F16 ? window_sized<__half>(p, s) : window_sized<__nv_bfloat16>(p, s);
+  return dtype == LC_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s);
 }

@@ -78,6 +78,43 @@ def test_prompt(case, dtype, cuda_device):
     prompt(dtype, *case, seed=sum(case))
 
 
+# The same edges with enough rows that they are not taken one by one.
+MANY_ROWS = [
+    (1, 129, 129, 16, 4, 128, 9, 0), (2, 200, 333, 8, 2, 128, 100, 7), (1, 300, 300, 12, 4, 128, 17, 40), (1, 150, 420, 10, 2, 64, 20, 130),
+    (1, 520, 520, 8, 8, 128, 1, 0), (1, 500, 900, 8, 1, 64, 2, 1), (1, 400, 400, 2, 1, 8, 64, 4), (1, 140, 140, 32, 2, 128, 12, 2),
+    (1, 130, 165, 48, 1, 64, 30, 3), (1, 257, 700, 7, 7, 96, 65, 64), (1, 257, 700, 6, 2, 128, 63, 63), (1, 70, 400, 100, 1, 64, 24, 5),
+    (1, 130, 700, 6, 2, 128, 300, 65), (1, 65, 1200, 20, 4, 64, 600, 300),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", MANY_ROWS)
+def test_prompt_many_rows(case, dtype, cuda_device):
+    prompt(dtype, *case, seed=sum(case))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompt_few_rows_of_many_keys(dtype, cuda_device):
+    """The keys of a few rows are cut over the SMs and joined."""
+    prompt(dtype, 1, 3, 5000, 4, 1, 128, 0, 0, seed=20)
+    prompt(dtype, 2, 5, 3000, 4, 2, 64, 2500, 9, q_lens=[5, 2], kv_lens=[2900, 1500], seed=21, poison=True)
+    prompt(dtype, 1, 130, 2000, 3, 1, 96, 1100, 200, seed=22)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_joined_rows_keep_infinite_values_to_themselves(d, cuda_device):
+    import torch
+    from lazy_compiler_b200 import serving as S
+    q, k, v, clean, lse = prompt("f16", 1, 6, 4000, 4, 2, d, 0, 0, seed=23)
+    v[0, 3997, 1, 3] = float("inf")  # seen by the last three queries
+    o, lse2 = S.window_attention(q, k, v, return_lse=True)
+    assert torch.equal(o[:, :, :2], clean[:, :, :2]) and torch.equal(lse, lse2)
+    assert torch.isposinf(o[0, 3:, 2:, 3]).all()
+    u = R.U["f16"]
+    near = (o[0, :3, 2:].float() - clean[0, :3, 2:].float()).abs() <= 4 * u * (1 + clean[0, :3, 2:].float().abs())
+    assert near.all() and torch.isfinite(o[0, 3:, 2:, 4:]).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [64, 128, 24])
 def test_prompt_ragged_and_empty_rows(d, dtype, cuda_device):
@@ -263,6 +300,33 @@ TOKENS = [
 @pytest.mark.parametrize("case", TOKENS)
 def test_token(case, dtype, cuda_device):
     decode(dtype, *case, seed=sum(case[0]))
+
+
+# The same edges with enough slots that they are not taken row by row.
+MANY_TOKENS = [
+    ([0, 1, 2, 15, 16, 17] * 20, 16, 8, 2, 128, 0, 0), ([1] * 200, 16, 4, 1, 64, 0, 0), ([301, 2, 40] * 12, 16, 8, 2, 64, 64, 4),
+    ([90, 30] * 10, 5, 12, 4, 96, 50, 7), ([64, 129] * 8, 128, 16, 1, 64, 33, 200), ([40, 14] * 16, 16, 24, 1, 128, 20, 1),
+    ([70] * 40, 16, 8, 8, 8, 0, 0), ([48, 97] * 30, 16, 4, 4, 128, 1, 1), ([25] * 12, 8, 32, 2, 192, 0, 0), ([20000], 32, 5, 1, 128, 0, 0),
+    ([9000, 11], 64, 20, 1, 64, 8000, 30), ([6000], 16, 4, 2, 256, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", range(len(MANY_TOKENS)))
+def test_token_more(case, dtype, cuda_device):
+    decode(dtype, *MANY_TOKENS[case], seed=case)
+
+
+def test_token_joined_rows_keep_infinite_values_to_themselves(cuda_device):
+    import torch
+    from lazy_compiler_b200 import serving as S
+    k, v, table = cache("f16", [9000], 16, 2, 128, 1, 24)
+    q = normal((1, 4, 128), "f16", 25)
+    clean = S.paged_decode(q, k, v, ints(table), ints([9000]))
+    v[table[0, 300], 1, 2, 7] = float("inf")
+    o = S.paged_decode(q, k, v, ints(table), ints([9000]))
+    keep = torch.arange(128, device="cuda") != 7
+    assert torch.equal(o[:, :2], clean[:, :2]) and torch.isposinf(o[:, 2:, 7]).all() and torch.equal(o[:, 2:][..., keep], clean[:, 2:][..., keep])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
