@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kMostThreads, 1) compact_kernel(CompactParams 
   __shared__ int used_here, holes_here;
   pdl_wait();
   pdl_trigger();  // copy_kernel may be scheduled; it waits for this kernel's end
-  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), threads = blockDim.x, warps = threads >> 5, tid = threadIdx.x;
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), threads = blockDim.x, tid = threadIdx.x;
   const Share mine = share_of(p.pages, rank, ctas);
   publish((tid == 0 ? mine.end - mine.begin : 0) - count_free(p.refs_in, mine), scan, &used_here);
   cluster.sync();

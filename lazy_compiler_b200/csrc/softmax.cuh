@@ -54,12 +54,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 // 2^x for a pair on the FMA pipe, for a share of the exponentials so the MUFU
 // unit is not the limiter.  Range reduction: x = n + f with n = round(x) taken
 // from the low mantissa bits of x + 1.5*2^23 and f in [-0.5, 0.5]; 2^f from a
@@ -67,12 +61,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN where eithe
 // relative error on [-0.5, 0.5] (max relative error 7.5e-5, below half an f16
 // ulp); 2^n is added to the exponent field.  x is clamped at -125 so the
 // exponent stays normal; the caller's x never exceeds 8.
-// KEEP_NAN: a NaN stays one (the plain form loses it at the clamp).
-template <bool KEEP_NAN = false>
 __device__ __forceinline__ uint64_t ex2_poly2(uint64_t x2) {
   const float2 x = unpack2(x2);
-  const uint64_t xc = KEEP_NAN ? pack2(max_nan(x.x, -125.0f), max_nan(x.y, -125.0f))
-                               : pack2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
+  const uint64_t xc = pack2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
   const uint64_t magic = pack2(12582912.0f, 12582912.0f);
   const uint64_t t = fadd2(xc, magic);
   const uint64_t f = fsub2(xc, fsub2(t, magic));
@@ -80,9 +71,8 @@ __device__ __forceinline__ uint64_t ex2_poly2(uint64_t x2) {
   q = ffma2(q, f, pack2(0.693260968f, 0.693260968f));
   q = ffma2(q, f, pack2(0.999928057f, 0.999928057f));
   const float2 qq = unpack2(q), tt = unpack2(t);
-  const uint64_t r = pack2(__int_as_float(__float_as_int(qq.x) + (__float_as_int(tt.x) << 23)),
-                           __int_as_float(__float_as_int(qq.y) + (__float_as_int(tt.y) << 23)));
-  return KEEP_NAN ? ffma2(xc, 0ull, r) : r;
+  return pack2(__int_as_float(__float_as_int(qq.x) + (__float_as_int(tt.x) << 23)),
+               __int_as_float(__float_as_int(qq.y) + (__float_as_int(tt.y) << 23)));
 }
 
 }  // namespace softmax

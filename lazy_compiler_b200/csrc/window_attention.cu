@@ -90,9 +90,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) window_row_kernel(WindowParams
 //   cuts    lengths come from the device.  With many items each CTA takes every
 //           gridDim-th one, longest first, so that the causal triangle's tail is made
 //           of short ones.  With few, or ragged ones, all items' blocks are laid end to
-//           end and each CTA takes an equal run of them; what a run holds of an item
-//           without holding it all goes to the workspace in f32, and join_kernel
-//           adds it up in CTA order;
+//           end and each CTA takes an equal run of them: of whole items where that is
+//           nearly as even, else cut anywhere; then what a run holds of an item without
+//           holding it all goes to the workspace in f32, and join_kernel adds it up in
+//           CTA order;
 //   values  0 x infinity is NaN, so the rows of V beyond a sequence's end are cleared
 //           in shared memory, and a row whose sums come out infinite or NaN is
 //           computed again key by key (it may hold a value that its mask hides).
@@ -107,6 +108,8 @@ constexpr int kKeys = 128;     // of a block
 constexpr int kStages = 2;
 constexpr int kMinRun = 6;     // units of a run: a shorter one costs more to join than it saves
 constexpr int kCutUnits = 4;   // units that the join costs
+constexpr int kJoinUnits = 3;  // that whole items may take beyond a CTA's share
+constexpr int kMostCtas = 256;
 constexpr int kMaxCutItems = 2048;
 constexpr int kSpansSlot = 43, kSumsSlot = 44, kStatsSlot = 45;  // scratch_buffer slots
 constexpr int kThreads = 128 + kTiles * 128 + 128;  // loads and products, softmax, output
@@ -346,8 +349,7 @@ __device__ __noinline__ void mend_piece(const WindowParams &p, const TensorParam
   if (__any_sync(0xffffffffu, odd)) mend_rows<T, NC>(p, odd, it.b, it.hk, pos, i, h);
 }
 
-// POLY: of sixteen pairs of exponentials, how many go to the FMA pipe.
-template <class T, int DP, int POLY>
+template <class T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     window_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                   const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ WindowParams p,
@@ -361,14 +363,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *kv_s = smem + L::kQBytes;
   __shared__ __align__(8) uint64_t q_full, q_empty;
   __shared__ __align__(8) uint64_t k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
-  __shared__ __align__(8) uint64_t s_full[kTiles], p_full[kTiles], o_done[kTiles], o_empty[kTiles], stat_full[kTiles];
+  __shared__ __align__(8) uint64_t s_full[kTiles], p_half[kTiles], p_full[kTiles], o_done[kTiles], o_empty[kTiles], stat_full[kTiles];
   __shared__ float2 stat[kTiles][kRows];  // m and l of a tile's rows, from the softmax to the output warps
   __shared__ int held_lens[2][kLensHeld];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag, any_odd;
   __shared__ int warp_blocks[kThreads / 32];
   __shared__ Pieces run;
-  __shared__ int run_end, run_total, run_ctas;
+  __shared__ int run_end, run_total, run_ctas, first_item;
+  __shared__ int load[kMostCtas];  // units of each CTA, with whole items
   __shared__ Piece ring[kRing];
   __shared__ __align__(8) uint64_t piece_full[kRing], piece_empty[kRing];
   volatile int *abort = &abort_flag;
@@ -389,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int t = 0; t < kTiles; ++t) {
       mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
       mbar_init(&o_empty[t], 4);
@@ -445,9 +449,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       total += warp_blocks[w];
     }
     const int ctas = min((int)gridDim.x, (total + kMinRun - 1) / kMinRun);
+    // Whole items, each in the run that its middle falls in, where no CTA gets much more than
+    // its share by that: shares of items are 128 KB a tile to write and to read again.
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) load[i] = 0;
+    if (threadIdx.x == 0) first_item = tp.items;
+    __syncthreads();
+    int middle = before;
+    for (int i = first; i < last; ++i) {
+      const int n = units_of(item_of(p, tp, lens, i).n);
+      if (n > 0) {
+        const int cta = (int)((int64_t)(middle + n / 2) * ctas / total);
+        atomicAdd(load + cta, n);
+        if (cta == (int)blockIdx.x) atomicMin(&first_item, i);
+      }
+      middle += n;
+    }
+    __syncthreads();
+    int heaviest = 0;
+    for (int i = threadIdx.x; i < ctas; i += kThreads) heaviest = max(heaviest, load[i]);
+    const bool whole = !__syncthreads_or(heaviest > total / max(1, ctas) + kJoinUnits);
     const int begin = ctas ? (int)((int64_t)blockIdx.x * total / ctas) : 0;
     const int end = ctas ? (int)((int64_t)(blockIdx.x + 1) * total / ctas) : 0;
-    if ((int)blockIdx.x < ctas && begin >= before && begin < before + own) {
+    if (whole) {
+      if (threadIdx.x == 0 && (int)blockIdx.x < ctas && load[blockIdx.x] > 0) run = {first_item, 0, load[blockIdx.x]};
+    } else if ((int)blockIdx.x < ctas && begin >= before && begin < before + own) {
       int at = before, i = first;
       for (;; ++i) {
         const int n = units_of(item_of(p, tp, lens, i).n);
@@ -553,12 +578,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         warp_commit(leader, &s_full[t]);
       };
-      auto issue_pv = [&](int t, int g, bool first) {  // O_t (+)= P_t V(block g), P_t over S_t
+      auto issue_pv = [&](int t, int g, bool first, int half) {  // O_t (+)= P_t V(block g), P_t over S_t
         const uint64_t vd = v_desc + (uint64_t)((g & 1) * kStageStep);
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
+        for (int k = half * kKeys / 32; k < (half + 1) * kKeys / 32; ++k)
           warp_mma_tmem_a(leader, tmem + kOCol + t * DP, tmem + t * kKeys + k * 8, vd + (uint64_t)(k * 2048 / 16), idesc_o, !(first && k == 0));
-        warp_commit(leader, &o_done[t]);
+        if (half) warp_commit(leader, &o_done[t]);
       };
       // One order over all pieces: PV_0(g), S_0(g + 1), PV_1(g), S_1(g + 1), where block
       // g + 1 may be the next piece's first.
@@ -594,12 +619,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             if ((t == 0 && !mbar_wait(&v_full[st], (g >> 1) & 1, abort)) ||
                 (j == 0 && local > 0 && !mbar_wait(&o_empty[t], (local - 1) & 1, abort)) ||
                 (t == 0 && !last && !mbar_wait(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort)) ||
-                !mbar_wait(&p_full[t], g & 1, abort)) {
+                !mbar_wait(&p_half[t], g & 1, abort)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            issue_pv(t, g, j == 0);
+            issue_pv(t, g, j == 0, 0);
+            if (!mbar_wait(&p_full[t], g & 1, abort)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            issue_pv(t, g, false, 1);
             if (t == kTiles - 1) warp_commit(leader, &v_empty[st]);
             if (more) {
               if (t == 0 && last) {
@@ -645,15 +676,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int x = 0; x < n; ++x) {
         const int g = g0 + x, j = piece.j0 + x, key = block_key(it, j);
-        if (!wait_all(&s_full[t], g & 1, abort, tp, kErrTimeoutSoftmax)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        uint32_t sr[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, sr[c]);
-        tmem_wait_ld();
         // the block's keys that this row sees: [from, to) and [0, sunk)
         int from, to, sunk;
         bool whole;  // every row of the tile sees every key
@@ -675,15 +697,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           sunk_from = kKeys / 2;
           sunk = kKeys / 2 + it.sinks;
         }
-        if (!whole) {
+        if (!wait_all(&s_full[t], g & 1, abort, tp, kErrTimeoutSoftmax)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        // The row's scores, the second half's load under the first half's mask and maximum
+        // (of the raw scores, as 8 independent chains).
+        uint32_t sr[4][32];
+        float mx8[8];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t sees = bits_between(from - c * 32, to - c * 32) | bits_between(sunk_from - c * 32, sunk - c * 32);
-            if (sees != 0xffffffffu) {
+        for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
+        tmem_ld32(s_at, sr[0]);
+        tmem_ld32(s_at + 32, sr[1]);
+        tmem_wait_ld();
 #pragma unroll
-              for (int y = 0; y < 32; ++y)
-                if (!(sees >> y & 1)) sr[c][y] = __float_as_uint(-INFINITY);
+        for (int half = 0; half < 2; ++half) {
+          if (half == 0) {
+            tmem_ld32(s_at + 64, sr[2]);
+            tmem_ld32(s_at + 96, sr[3]);
+          } else {
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int c = half * 2; c < half * 2 + 2; ++c) {
+            if (!whole) {
+              const uint32_t sees = bits_between(from - c * 32, to - c * 32) | bits_between(sunk_from - c * 32, sunk - c * 32);
+              if (sees != 0xffffffffu) {
+#pragma unroll
+                for (int y = 0; y < 32; ++y)
+                  if (!(sees >> y & 1)) sr[c][y] = __float_as_uint(-INFINITY);
+              }
             }
+#pragma unroll
+            for (int y = 0; y < 32; y += 2)
+              mx8[(y >> 1) & 7] = max3(mx8[(y >> 1) & 7], __uint_as_float(sr[c][y]), __uint_as_float(sr[c][y + 1]));
           }
         }
         if (key + kKeys > it.n_kv && it.n_kv < p.s_kv) {
@@ -699,15 +747,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_async_shared();
         }
-        // max of the raw scores, as 8 independent chains
-        float mx8[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int y = 0; y < 32; y += 2)
-            mx8[(y >> 1) & 7] = max3(mx8[(y >> 1) & 7], __uint_as_float(sr[c][y]), __uint_as_float(sr[c][y + 1]));
         const float mx = max3(max3(mx8[0], mx8[1], mx8[2]), max3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])) * p.scale_log2;
         const float m_new = fmaxf(m, mx);
         const bool need = m_new > m + kRescale;
@@ -735,6 +774,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_st();
           }
         }
+        // All exponentials on the MUFU unit: one pair in sixteen on the FMA pipe, as in sdpa.cu,
+        // measured the same, one in eight 3% slower.
         uint64_t part2[4] = {0ull, 0ull, 0ull, 0ull};
         const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
         const float base = m == -INFINITY ? 0.f : -m;  // nothing seen so far: all weights are 2^-inf
@@ -745,16 +786,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
             const uint64_t x2 = ffma2(pack2(__uint_as_float(sr[c][2 * y]), __uint_as_float(sr[c][2 * y + 1])), scale2, base2);
-            uint64_t p2;
-            if ((y + 1) * POLY / 16 > y * POLY / 16) {
-              p2 = ex2_poly2<true>(x2);
-            } else {
-              const float2 xx = unpack2(x2);
-              p2 = pack2(ex2(xx.x), ex2(xx.y));
-            }
+            const float2 xx = unpack2(x2);
+            const uint64_t p2 = pack2(ex2(xx.x), ex2(xx.y));
             part2[y & 3] = fadd2(part2[y & 3], p2);
             const float2 pp = unpack2(p2);
             packed[y] = pack16<T>(pp.x, pp.y);
+          }
+          if (c == 2) {  // the first half of P was stored some time ago: its products may begin
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[t]);
           }
           tmem_st16(s_at + c * 16, packed);
         }
@@ -1069,11 +1111,11 @@ bool window_tensor(const WindowParams &p) {
   return ok;
 }
 
-template <class T, int DP, int POLY>
+template <class T, int DP>
 int launch_window(const WindowParams &p, cudaStream_t s) {
   using L = WindowLayout<DP>;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
-  auto *kernel = window_kernel<T, DP, POLY>;
+  auto *kernel = window_kernel<T, DP>;
   TensorParams t = {};
   t.group = p.q_heads / p.kv_heads;
   t.tokens = kRows / t.group;
@@ -1111,7 +1153,7 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
   // Whole items, or runs of blocks: where the most loaded CTA (the first one: items come longest
   // first) has kCutUnits units more than its share.  Lengths on the device are not known here;
   // the items may be short or empty then, and the longest is all that is left to go by.
-  const int sms = sm_count();
+  const int sms = std::min(sm_count(), kMostCtas);
   t.cut = 0;
   if (items <= kMaxCutItems) {
     const int heads = p.batch * p.kv_heads;
@@ -1149,7 +1191,7 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
 
 template <class T>
 int window_sized(const WindowParams &p, cudaStream_t s) {
-  return p.d <= 64 ? launch_window<T, 64, 1>(p, s) : launch_window<T, 128, 1>(p, s);
+  return p.d <= 64 ? launch_window<T, 64>(p, s) : launch_window<T, 128>(p, s);
 }
 
 // Few rows of few keys: a CTA per row is done before the tensor-core form has set up its
