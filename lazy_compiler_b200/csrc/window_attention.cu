@@ -1094,11 +1094,12 @@ int make_map(CUtensorMap *map, bool bf16, const void *base, int rank, const int6
 }
 
 // What the TMA loads and the row stores take: head sizes up to 128 in pieces of 8,
-// a group that fits a tile, 16-byte alignment, strides that a tensor map holds (a
-// broadcast batch or head of K and V becomes an axis of one).
+// a group that fits a tile, 16-byte alignment, strides that a tensor map holds (below
+// 2^40 bytes; a broadcast batch or head of K and V becomes an axis of one).
 bool window_tensor(const WindowParams &p) {
+  constexpr int64_t kMostStride = 1ll << 38;
   const int group = p.q_heads / p.kv_heads;
-  bool ok = p.d <= 128 && p.d % 8 == 0 && group <= kRows && p.s_kv > 0 && aligned(p.q, 16) && aligned(p.k, 16) &&
+  bool ok = p.d <= 128 && p.d % 8 == 0 && group <= kRows && (group == 1 || p.qs[2] < kMostStride / group) && p.s_kv > 0 && aligned(p.q, 16) && aligned(p.k, 16) &&
             aligned(p.v, 16) && aligned(p.o, 16);
   const int sizes[4][3] = {{p.batch, p.s_q, p.q_heads}, {p.batch, p.s_kv, p.kv_heads}, {p.batch, p.s_kv, p.kv_heads}, {p.batch, p.s_q, p.q_heads}};
   const int64_t *strides[4] = {p.qs, p.ks, p.vs, p.os};
@@ -1106,7 +1107,7 @@ bool window_tensor(const WindowParams &p) {
     for (int a = 0; a < 3; ++a) {
       const bool repeats = (x == 1 || x == 2) && a != 1;  // may have a stride of zero
       const int64_t s = strides[x][a];
-      ok = ok && (sizes[x][a] == 1 || (s % 8 == 0 && (s > 0 || (s == 0 && repeats)) && s < (1ll << 38)));
+      ok = ok && (sizes[x][a] == 1 || (s % 8 == 0 && (s > 0 || (s == 0 && repeats)) && s < kMostStride));
     }
   return ok;
 }

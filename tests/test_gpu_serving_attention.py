@@ -422,3 +422,33 @@ def test_streams_and_graph_capture(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(other, S.paged_decode(q, k, v, table, ints([333, 0])))
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """Sequences four billion elements into their buffers: pages at the end of a long pool, a batch far apart."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    pages, page, h, d = 270000, 16, 8, 128  # 4.4e9 elements a plane
+    k = torch.zeros((pages, h, page, d), dtype=torch.float16, device="cuda")
+    v = torch.zeros_like(k)
+    table = np.array([[pages - 1, pages - 40, pages - 7], [3, pages - 2, 0]])
+    for x, seed in ((k, 26), (v, 27)):
+        x[torch.from_numpy(table.ravel()).cuda()] = normal((6, h, page, d), "f16", seed)
+    q, lens = normal((2, 8, d), "f16", 28), [45, 33]
+    small = [x[torch.from_numpy(table.ravel()).cuda()] for x in (k, v)]
+    ref = R.paged_decode(f64(q), f64(small[0]), f64(small[1]), np.arange(6).reshape(2, 3), lens, d ** -0.5, 0, 0)
+    for repeat in (1, 40):  # row by row, and by tiles
+        o, lse = S.paged_decode(q.repeat(repeat, 1, 1), k, v, ints(table).repeat(repeat, 1), ints(lens).repeat(repeat), return_lse=True)
+        for r in (0, repeat - 1):
+            R.check_attention(f64(o[2 * r:2 * r + 2]), f64(lse[2 * r:2 * r + 2]), ref, "f16")
+    far = (1 << 32) + 64
+    flat = k.view(-1)
+    qs, ks, vs, outs = (flat[i * 10 ** 7:].as_strided((2, 200, n, d), (far, n * d, d, 1)) for i, n in enumerate((4, 2, 2, 4)))
+    for i, x in enumerate((qs, ks, vs)):
+        x.copy_(normal(x.shape, "f16", 30 + i))
+    ref = R.window_attention(f64(qs), f64(ks), f64(vs), d ** -0.5, 150, 3, [200] * 2, [200] * 2)
+    o, lse = S.window_attention(qs, ks, vs, window=150, sinks=3, out=outs, return_lse=True)
+    R.check_attention(f64(o), f64(lse), ref, "f16")
+    o, lse = S.window_attention(qs[:, :, :, :125], ks[:, :, :, :125], vs[:, :, :, :125], window=150, sinks=3, scale=d ** -0.5, return_lse=True)
+    ref = R.window_attention(f64(qs[..., :125]), f64(ks[..., :125]), f64(vs[..., :125]), d ** -0.5, 150, 3, [200] * 2, [200] * 2)
+    R.check_attention(f64(o), f64(lse), ref, "f16")

@@ -262,3 +262,27 @@ def test_paged_cache_steps_in_a_graph(cuda_device):
     with pytest.raises(RuntimeError, match="40 pages are missing"):
         cache.extend(ints([page * width] * 3))
         cache.check()
+
+
+def test_pages_beyond_32_bit_offsets(cuda_device):
+    """Copies, forks, compaction and writes four billion bytes and elements into the pool."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    pages, page, h, d = 40000, 16, 8, 64
+    pool = torch.zeros((14, pages, h, page, d), dtype=torch.float16, device="cuda")  # 4.6e9 elements
+    last = torch.randn((14, 2, h, page, d), device="cuda").half()
+    pool[:, pages - 2:] = last
+    S.cache_copy(pool, ints([pages - 2]), ints([5]))
+    assert torch.equal(pool[:, 5], last[:, 0]) and pool[:, 4].eq(0).all()
+    refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    refs[pages - 2:] = 1
+    maps = S.CacheMaps(ints([[pages - 1, pages - 2], [-1, -1]]), ints([20, 0]), refs)
+    new = S.cache_fork(pool, maps, ints([0, 0]))
+    assert new.table.tolist() == [[pages - 1, pages - 2], [pages - 1, 0]] and torch.equal(pool[:, 0, :, :4], last[:, 0, :, :4])
+    new = S.cache_compact(pool, new)
+    assert new.table.tolist() == [[2, 1], [2, 0]] and torch.equal(pool[:, 1], last[:, 0]) and torch.equal(pool[:, 2], last[:, 1])
+    k = torch.randn((2, 3, h, d), device="cuda").half()
+    maps = S.CacheMaps(ints([[pages - 3, -1], [1, pages - 5]]), ints([3, 18]), refs)
+    S.cache_write(k, k, pool[12], pool[13], maps, ints([3, 2]))
+    for plane in (12, 13):
+        assert torch.equal(pool[plane, pages - 3, :, :3], k[0].transpose(0, 1)) and torch.equal(pool[plane, pages - 5, :, :2], k[1, :2].transpose(0, 1))
