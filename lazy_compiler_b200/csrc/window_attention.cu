@@ -107,8 +107,11 @@ constexpr int kTiles = 2;      // per CTA
 constexpr int kKeys = 128;     // of a block
 constexpr int kStages = 2;
 constexpr int kMinRun = 6;     // units of a run: a shorter one costs more to join than it saves
-constexpr int kCutUnits = 4;   // units that the join costs
-constexpr int kJoinUnits = 3;  // that whole items may take beyond a CTA's share
+// Units that cutting costs: few items (deep: 64 queries of 8 key-value heads over 1024 keys,
+// 4 units saved: 20.8 us whole, 23.3 cut; over 1500, 8 saved: 28.0, 23.6) or shares of the
+// first and last item of every CTA (2 x 2048 tokens, 9 saved: 83, 92; 4096, 13: 148, 140);
+// and what whole items may take beyond a CTA's share before the kernel cuts them.
+constexpr int kDeepCut = 6, kWideCut = 11, kDeepSlack = 3, kWideSlack = 5;
 constexpr int kMostCtas = 256;
 constexpr int kMaxCutItems = 2048;
 constexpr int kSpansSlot = 43, kSumsSlot = 44, kStatsSlot = 45;  // scratch_buffer slots
@@ -140,7 +143,7 @@ struct TensorParams {
   int *err;
   // runs of blocks (cut): the item that began in a CTA and goes on after it, or -1, and that
   // item's last CTA; a CTA's shares of the item that began before it, and of that one
-  int cut, ctas;
+  int cut, deep, ctas;
   int2 *spans;
   float *sums;              // [CTA][2][tile][DP / 8][row][8]: 8 columns of a warp's rows lie together
   float2 *stats;            // [CTA][2][tile][row]: m and l
@@ -430,10 +433,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) run = {(int)blockIdx.x, 0, 0};
   } else {
     // this CTA's run: unit blockIdx.x * total / ctas of all items' units on
-    const int per = (tp.items + kThreads - 1) / kThreads;
-    const int first = min(tp.items, (int)threadIdx.x * per), last = min(tp.items, first + per);
-    int own = 0;
-    for (int i = first; i < last; ++i) own += units_of(item_of(p, tp, lens, i).n);
+    constexpr int kPer = kMaxCutItems / kThreads;  // a thread's items, or fewer
+    const int per = (tp.items + kThreads - 1) / kThreads, first = threadIdx.x * per;
+    int units[kPer], own = 0;
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+      units[x] = x < per && first + x < tp.items ? units_of(item_of(p, tp, lens, first + x).n) : 0;
+      own += units[x];
+    }
     int inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -441,7 +448,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane >= o) inc += up;
     }
     if (lane == 31) warp_blocks[warp] = inc;
-    if (threadIdx.x == 0) run = {tp.items, 0, 0};
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) load[i] = 0;
+    if (threadIdx.x == 0) {
+      run = {tp.items, 0, 0};
+      first_item = tp.items;
+    }
     __syncthreads();
     int before = inc - own, total = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
@@ -451,35 +462,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int ctas = min((int)gridDim.x, (total + kMinRun - 1) / kMinRun);
     // Whole items, each in the run that its middle falls in, where no CTA gets much more than
     // its share by that: shares of items are 128 KB a tile to write and to read again.
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) load[i] = 0;
-    if (threadIdx.x == 0) first_item = tp.items;
-    __syncthreads();
-    int middle = before;
-    for (int i = first; i < last; ++i) {
-      const int n = units_of(item_of(p, tp, lens, i).n);
-      if (n > 0) {
-        const int cta = (int)((int64_t)(middle + n / 2) * ctas / total);
-        atomicAdd(load + cta, n);
-        if (cta == (int)blockIdx.x) atomicMin(&first_item, i);
+    int at = before;
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+      if (units[x] > 0) {
+        const int cta = (int)((int64_t)(at + units[x] / 2) * ctas / total);
+        atomicAdd(load + cta, units[x]);
+        if (cta == (int)blockIdx.x) atomicMin(&first_item, first + x);
       }
-      middle += n;
+      at += units[x];
     }
     __syncthreads();
     int heaviest = 0;
     for (int i = threadIdx.x; i < ctas; i += kThreads) heaviest = max(heaviest, load[i]);
-    const bool whole = !__syncthreads_or(heaviest > total / max(1, ctas) + kJoinUnits);
+    const bool whole = !__syncthreads_or(heaviest > total / max(1, ctas) + (tp.deep ? kDeepSlack : kWideSlack));
     const int begin = ctas ? (int)((int64_t)blockIdx.x * total / ctas) : 0;
     const int end = ctas ? (int)((int64_t)(blockIdx.x + 1) * total / ctas) : 0;
     if (whole) {
       if (threadIdx.x == 0 && (int)blockIdx.x < ctas && load[blockIdx.x] > 0) run = {first_item, 0, load[blockIdx.x]};
     } else if ((int)blockIdx.x < ctas && begin >= before && begin < before + own) {
-      int at = before, i = first;
-      for (;; ++i) {
-        const int n = units_of(item_of(p, tp, lens, i).n);
-        if (begin < at + n) break;
-        at += n;
+      at = before;
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) {
+        if (begin >= at && begin < at + units[x]) run = {first + x, begin - at, end - begin};
+        at += units[x];
       }
-      run = {i, begin - at, end - begin};
     }
     if (threadIdx.x == 0) {
       run_end = end;
@@ -849,13 +856,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = 0; t < kTiles; ++t) {
         const uint32_t o_at = tmem + lane_base + kOCol + t * DP;
         const int i = it.i0 + t * tp.tokens + token, h = it.hk * tp.group + head;
-        if (!wait_all(&stat_full[t], local & 1, abort, tp, kErrTimeoutEpilogue) ||
-            !wait_all(&o_done[t], (g0 + n - 1) & 1, abort, tp, kErrTimeoutEpilogue)) {
+        if (!wait_all(&stat_full[t], local & 1, abort, tp, kErrTimeoutEpilogue)) {
+          ok = false;
+          break;
+        }
+        const float m = stat[t][row].x, l = stat[t][row].y;
+        const bool stored = in_tile && i < p.s_q;
+        // sees something (a row of NaN scores has no maximum)
+        const bool some = stored && i < it.n_q && it.base + i >= 0 && (m != -INFINITY || isnan(l));
+        const float inv = some ? 1.0f / l : 0.f;
+        const uint64_t inv2 = pack2(inv, inv);
+        T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
+        if (p.lse && stored && n == it.n)
+          p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (!wait_all(&o_done[t], (g0 + n - 1) & 1, abort, tp, kErrTimeoutEpilogue)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const float m = stat[t][row].x, l = stat[t][row].y;
+        auto release = [&]() {  // O and the tile's m and l are read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[t]);
+        };
         if (n < it.n) {  // a share of the item: unnormalised, for join_kernel
           const int64_t at = (((int64_t)blockIdx.x * 2 + (piece.j0 == 0)) * kTiles + t) * kRows + row;
           tp.stats[at] = make_float2(m, l);
@@ -872,50 +895,43 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int y = 0; y < 4; ++y) st_global_v8_b32(tp.sums + (at - row) * DP + ((c * 4 + y) * kRows + row) * 8, o + y * 8);
             __syncwarp();
           }
+          release();
         } else {
-          const bool stored = in_tile && i < p.s_q;
-          // sees something (a row of NaN scores has no maximum)
-          const bool some = stored && i < it.n_q && it.base + i >= 0 && (m != -INFINITY || isnan(l));
-          const float inv = some ? 1.0f / l : 0.f;
-          const uint64_t inv2 = pack2(inv, inv);
-          T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
-          if (p.lse && stored) p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
-          bool odd = false;
-#pragma unroll 1
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_at + c * 32, o);
-            tmem_wait_ld();
-            if (stored) {
-              uint32_t packed[16];
-              uint64_t zero[2] = {0ull, 0ull};  // NaN once a value is infinite or NaN
+          // 16 columns at a time, the next ones' load under this ones' division and store
+          uint64_t zero[2] = {0ull, 0ull};  // NaN once a value is infinite or NaN
+          uint32_t o[2][16];
+          tmem_ld16(o_at, o[0]);
 #pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                const uint64_t two = ffma2(pack2(__uint_as_float(o[2 * x]), __uint_as_float(o[2 * x + 1])), inv2, 0ull);
+          for (int c = 0; c < DP / 16; ++c) {
+            tmem_wait_ld();
+            if (c + 1 < DP / 16) {
+              tmem_ld16(o_at + (c + 1) * 16, o[(c + 1) & 1]);
+            } else {
+              release();
+            }
+            if (stored) {
+              uint32_t packed[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const uint64_t two = ffma2(pack2(__uint_as_float(o[c & 1][2 * x]), __uint_as_float(o[c & 1][2 * x + 1])), inv2, 0ull);
                 zero[x & 1] = ffma2(two, 0ull, zero[x & 1]);
                 const float2 ab = unpack2(two);
                 packed[x] = some ? pack16<T>(ab.x, ab.y) : 0u;
               }
-              const float2 z = unpack2(fadd2(zero[0], zero[1]));
-              odd |= some && !(z.x + z.y == 0.f);
-              T *to = out + c * 32;
+              T *to = out + c * 16;
               if (tp.o_vec == 2) {
-                if (c * 32 + 16 <= p.d) st_global_v8_b32(to, packed);
-                if (c * 32 + 32 <= p.d) st_global_v8_b32(to + 16, packed + 8);
+                if (c * 16 < p.d) st_global_v8_b32(to, packed);
               } else {
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                  if (c * 32 + x * 8 + 8 <= p.d)
+                for (int x = 0; x < 2; ++x)
+                  if (c * 16 + x * 8 < p.d)
                     reinterpret_cast<uint4 *>(to)[x] = make_uint4(packed[4 * x], packed[4 * x + 1], packed[4 * x + 2], packed[4 * x + 3]);
               }
             }
-            __syncwarp();
           }
-          if (odd) any_odd = 1;
+          const float2 z = unpack2(fadd2(zero[0], zero[1]));
+          if (some && !(z.x + z.y == 0.f)) any_odd = 1;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&o_empty[t]);  // O and the tile's m and l are free
       }
       ++local;
       g0 += n;
@@ -1152,10 +1168,12 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   // Whole items, or runs of blocks: where the most loaded CTA (the first one: items come longest
-  // first) has kCutUnits units more than its share.  Lengths on the device are not known here;
-  // the items may be short or empty then, and the longest is all that is left to go by.
+  // first) has more units beyond a run's than cutting and joining cost.  With lengths on the
+  // device the items may be short or empty: several items a CTA are then left to the kernel,
+  // which cuts them only where whole ones would not be even.
   const int sms = std::min(sm_count(), kMostCtas);
   t.cut = 0;
+  t.deep = items * 4 <= sms;  // an item spans four CTAs or more, if it is cut
   if (items <= kMaxCutItems) {
     const int heads = p.batch * p.kv_heads;
     auto units = [&](int qb) {
@@ -1168,7 +1186,8 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
     for (int qb = 0; qb < t.q_blocks; ++qb) total += (int64_t)units(qb) * heads;
     for (int64_t i = 0; i < items; i += sms) most += units(t.q_blocks - 1 - (int)(i / heads));
     const bool ragged = p.q_lens || p.kv_lens;
-    t.cut = total < (1 << 30) && (ragged ? units(t.q_blocks - 1) > kMinRun + kItemUnits : most - total / sms > kCutUnits);
+    t.cut = total < (1 << 30) && (ragged && items > sms ? units(t.q_blocks - 1) > kMinRun
+                                                        : most - std::max<int64_t>(total / sms, kMinRun) > (t.deep ? kDeepCut : kWideCut));
   }
   int grid = t.items < sms ? t.items : sms;
   if (t.cut) {
@@ -1184,8 +1203,7 @@ int launch_window(const WindowParams &p, cudaStream_t s) {
   }
   if (int rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(kThreads), L::kBytes, s, tq, tk, tv, p, t), "lc_window_attention")) return rc;
   if (!t.cut) return LC_OK;
-  const bool deep = items * 4 <= sms;  // an item then spans four CTAs or more
-  const cudaError_t err = deep ? launch_pdl(join_kernel<T, DP, true>, dim3(t.items, kTiles * kRows / 8), dim3(256), 0, s, p, t)
+  const cudaError_t err = t.deep ? launch_pdl(join_kernel<T, DP, true>, dim3(t.items, kTiles * kRows / 8), dim3(256), 0, s, p, t)
                                : launch_pdl(join_kernel<T, DP, false>, dim3(sms, kTiles * kRows / 64), dim3(256), 0, s, p, t);
   return check_cuda(err, "lc_window_attention (join)");
 }
