@@ -105,6 +105,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // pipe is idle most of the time as it is.
 // P is split into two 16-bit parts (value and remainder) and multiplied twice: the
 // extra products hide behind the loads and keep P to 16 bits or more.
+// Bound by HBM.  Measured, 32/8 heads of 128, bf16: 64 sequences of 1 to 8192 tokens
+// in pages of 16: 169 us, 6370 GB/s, the rate of a copy; 64/8, f16, 100003 and 131072
+// tokens: 150 us, 6320 GB/s.  Three CTAs per SM of two stages against two of three:
+// the warps' own latency (a tile is a chain of some 500 instructions) needs 12 of them
+// (177 us with 8).
 constexpr int kDecodeWarps = 4;
 constexpr int kTileKeys = 16;
 constexpr int kDeepParts = 16;

@@ -97,8 +97,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) window_row_kernel(WindowParams
 //   values  0 x infinity is NaN, so the rows of V beyond a sequence's end are cleared
 //           in shared memory, and a row whose sums come out infinite or NaN is
 //           computed again key by key (it may hold a value that its mask hides).
-// P is rounded to the storage type for the second product: beside the output's own
-// rounding its error averages out over the keys.
+// P is rounded to the storage type for the second product: an error of the size of the
+// output's own rounding.
+// Bound by a tile's chain of softmax and products (3500 cycles a block of 128 keys, of
+// which the tensor pipe needs 2080 for both tiles), in long runs by the power cap.
+// Measured, f16, 32/8 heads of 128: 32768 tokens, window 4096: 1.75 ms, 1180 TFLOP/s;
+// bf16, 4 ragged chunks of up to 777 over 4001 keys, window 1024: 51 us, 685 TFLOP/s.
 using namespace sm100;
 using namespace softmax;
 
@@ -124,7 +128,11 @@ constexpr int kLensHeld = 256;  // sequences whose lengths are kept in shared me
 constexpr int kRing = 4;        // pieces of work known ahead
 constexpr int kReaders = 2 + 8 + 4;  // of a piece: loads, products, the softmax's and the output's warps
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kOCol = 256;             // O of tile t at kOCol + t * DP; S of tile t at t * 128
+// Tensor memory: S of tile t at t * 128, P over it, O of tile t at kOCol + t * DP.  (P of its
+// own, which a head size of 64 has room for, takes the products off the softmax's chain and
+// was slower, 8 x 4096 tokens of 16 heads: 590 against 483 us: both tiles' exponentials then
+// run at once.)
+constexpr uint32_t kOCol = 256;
 constexpr float kRescale = 8.0f;            // log2 units a row's maximum may lag behind
 constexpr int kChunkBytes = 128 * 64 * 2;   // 128 rows x 64 columns, one swizzle span
 
@@ -592,71 +600,64 @@ __global__ void __launch_bounds__(kThreads, 1)
           warp_mma_tmem_a(leader, tmem + kOCol + t * DP, tmem + t * kKeys + k * 8, vd + (uint64_t)(k * 2048 / 16), idesc_o, !(first && k == 0));
         if (half) warp_commit(leader, &o_done[t]);
       };
-      // One order over all pieces: PV_0(g), S_0(g + 1), PV_1(g), S_1(g + 1), where block
-      // g + 1 may be the next piece's first.
-      int g = 0, local = 0, n = 0, next_n = 0;
+      // PV_0(g), S_0(g + 1), PV_1(g), S_1(g + 1): block g + 1 may be the next piece's first.
       bool ok = true;
       auto blocks = [&](int k) {  // of the k-th piece; 0: there is none
-        const int r = k % kRing;
-        if (!mbar_wait(&piece_full[r], k / kRing & 1, abort)) {
+        if (!mbar_wait(&piece_full[k % kRing], k / kRing & 1, abort)) {
           ok = false;
           return 0;
         }
-        const int count = ring[r].j1 - ring[r].j0;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&piece_empty[r]);
-        return count;
+        return ring[k % kRing].j1 - ring[k % kRing].j0;
       };
-      n = blocks(0);
-      if (n > 0) {
+      auto leave = [&](int k) {  // its entry may be overwritten
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&piece_empty[k % kRing]);
+      };
+      auto products_pv = [&](int t, int g, bool first, int piece) {  // once P_t(g), V(g) and O_t are there
+        if (!mbar_wait(&v_full[g & 1], (g >> 1) & 1, abort) ||
+            (first && piece > 0 && !mbar_wait(&o_empty[t], (piece - 1) & 1, abort)) || !mbar_wait(&p_half[t], g & 1, abort))
+          return false;
+        tc_fence_after();
+        issue_pv(t, g, first, 0);
+        if (!mbar_wait(&p_full[t], g & 1, abort)) return false;
+        tc_fence_after();
+        issue_pv(t, g, false, 1);
+        if (t == kTiles - 1) warp_commit(leader, &v_empty[g & 1]);
+        return true;
+      };
+      const int n_first = blocks(0);
+      if (n_first > 0) {
         ok = mbar_wait(&q_full, 0, abort) && mbar_wait(&k_full[0], 0, abort);
         if (ok) {
           tc_fence_after();
           for (int t = 0; t < kTiles; ++t) issue_s(t, 0);
           warp_commit(leader, &k_empty[0]);
-          if (n == 1) warp_commit(leader, &q_empty);
+          if (n_first == 1) warp_commit(leader, &q_empty);
         }
       }
-      while (ok && n > 0) {
-        next_n = blocks(local + 1);
-        for (int j = 0; ok && j < n; ++j, ++g) {
-          const int st = g & 1;
-          const bool last = j + 1 == n, more = !last || next_n > 0;
-          for (int t = 0; t < kTiles; ++t) {
-            if ((t == 0 && !mbar_wait(&v_full[st], (g >> 1) & 1, abort)) ||
-                (j == 0 && local > 0 && !mbar_wait(&o_empty[t], (local - 1) & 1, abort)) ||
-                (t == 0 && !last && !mbar_wait(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort)) ||
-                !mbar_wait(&p_half[t], g & 1, abort)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            issue_pv(t, g, j == 0, 0);
-            if (!mbar_wait(&p_full[t], g & 1, abort)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            issue_pv(t, g, false, 1);
-            if (t == kTiles - 1) warp_commit(leader, &v_empty[st]);
-            if (more) {
-              if (t == 0 && last) {
-                if (!mbar_wait(&q_full, (local + 1) & 1, abort) || !mbar_wait(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort)) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after();
-              }
-              issue_s(t, g + 1);
-              if (t == kTiles - 1) {
-                warp_commit(leader, &k_empty[st ^ 1]);
-                if (last ? next_n == 1 : j + 2 == n) warp_commit(leader, &q_empty);  // a piece's last S products
-              }
-            }
-          }
+      struct Place {
+        int k, j, n;  // block j of the n blocks of piece k; n = 0: there is none
+      };
+      auto after = [&](const Place &a) { return a.j + 1 < a.n ? Place{a.k, a.j + 1, a.n} : Place{a.k + 1, 0, blocks(a.k + 1)}; };
+      auto products_s = [&](int t, int g, const Place &a) {
+        if ((t == 0 && a.j == 0 && !mbar_wait(&q_full, a.k & 1, abort)) || (t == 0 && !mbar_wait(&k_full[g & 1], (g >> 1) & 1, abort)))
+          return false;
+        tc_fence_after();
+        issue_s(t, g);
+        if (t == kTiles - 1) {
+          warp_commit(leader, &k_empty[g & 1]);
+          if (a.j + 1 == a.n) warp_commit(leader, &q_empty);  // a piece's last S products
         }
-        ++local;
-        n = next_n;
+        return true;
+      };
+      Place now = {0, 0, n_first};
+      for (int g = 0; ok && now.n > 0; ++g) {
+        const Place next = after(now);
+        const bool more = next.n > 0;
+        if (!ok) break;
+        for (int t = 0; ok && t < kTiles; ++t) ok = products_pv(t, g, now.j == 0, now.k) && (!more || products_s(t, g + 1, next));
+        if (now.j + 1 == now.n) leave(now.k);
+        now = next;
       }
       if (!ok && lane == 0) give_up(tp, abort, kErrTimeoutMma);
     }
