@@ -59,7 +59,7 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 def _build_extension(force: bool) -> None:
     src = CSRC / "serving_ext.cpp"
-    newest = max(p.stat().st_mtime for p in (src, *INCLUDE.glob("*.h")))
+    newest = max(p.stat().st_mtime for p in (src, Path(__file__), *INCLUDE.glob("*.h")))
     if EXTENSION.exists() and EXTENSION.stat().st_mtime >= newest and not force:
         return
     import sysconfig
@@ -68,9 +68,11 @@ def _build_extension(force: bool) -> None:
     from torch.utils.cpp_extension import include_paths, library_paths
     includes = [INCLUDE, *include_paths(), Path(nvcc()).resolve().parents[1] / "include", sysconfig.get_paths()["include"]]
     tmp = EXTENSION.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-shared", "-fPIC",
+    # the libstdc++ that torch has loaded, by name: a compiler that comes with the static one only would put a second
+    # copy into the module, half of its symbols shared, and writing a number to a stream then faults
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-shared", "-fPIC", "-nostdlib++",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in includes), str(src), "-o", str(tmp),
-           *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10"]
+           *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10", "-l:libstdc++.so.6"]
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode:
         raise RuntimeError(f"{cmd[0]} failed on {src.name}:\n{result.stderr}")

@@ -13,7 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
-#include <sstream>
+#include <string>
 
 #include "lazyb200.h"
 
@@ -32,11 +32,13 @@ struct Entries {
 } lib;
 constexpr int kEntries = sizeof(Entries) / sizeof(void *);
 
+std::string piece(const std::string &s) { return s; }
+std::string piece(const char *s) { return s; }
+std::string piece(int64_t v) { return std::to_string(v); }
+std::string piece(const at::Device &d) { return d.str(); }
 template <class... Parts>
 [[noreturn]] void refuse(const Parts &...parts) {
-  std::ostringstream text;
-  (text << ... << parts);
-  C10_THROW_ERROR(ValueError, text.str());
+  C10_THROW_ERROR(ValueError, (std::string() + ... + piece(parts)));
 }
 
 const at::Tensor &tensor(PyObject *o, const char *what) {
@@ -49,6 +51,11 @@ const at::Tensor *maybe(PyObject *o, const char *what) { return o == Py_None ? n
 int64_t integer(PyObject *o) {
   const long long v = PyLong_AsLongLong(o);
   if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+bool truth(PyObject *o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
   return v;
 }
 float scale_of(PyObject *o, int64_t d) {
@@ -71,11 +78,9 @@ const char *name_of(at::ScalarType t) {
 }
 
 std::string shape_text(at::IntArrayRef s) {
-  std::ostringstream text;
-  text << "(";
-  for (size_t i = 0; i < s.size(); ++i) text << (i ? ", " : "") << s[i];
-  text << ")";
-  return text.str();
+  std::string text = "(";
+  for (size_t i = 0; i < s.size(); ++i) text += (i ? ", " : "") + std::to_string(s[i]);
+  return text + ")";
 }
 
 void check(const at::Tensor &t, const char *what, const at::Tensor &like, at::ScalarType type, at::IntArrayRef shape) {
@@ -160,7 +165,7 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (given) check(*given, "out", q, q.scalar_type(), {batch, s_q, heads, d});
   const c10::cuda::CUDAGuard guard(q.device());
   const at::Tensor out = given ? *given : fresh({batch, s_q, heads, d}, q.scalar_type(), q);
-  const at::Tensor lse = a[9] == Py_True ? fresh({batch, heads, s_q}, at::kFloat, q) : at::Tensor();
+  const at::Tensor lse = truth(a[9]) ? fresh({batch, heads, s_q}, at::kFloat, q) : at::Tensor();
   const at::Tensor *views[4] = {&q, &k, &v, &out};
   const char *names[4] = {"q", "k", "v", "out"};
   int64_t strides[12];
@@ -196,7 +201,7 @@ PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d});
   const c10::cuda::CUDAGuard guard(q.device());
   const at::Tensor out = given ? *given : fresh({slots, heads, d}, q.scalar_type(), q);
-  const at::Tensor lse = a[9] == Py_True ? fresh({slots, heads}, at::kFloat, q) : at::Tensor();
+  const at::Tensor lse = truth(a[9]) ? fresh({slots, heads}, at::kFloat, q) : at::Tensor();
   check_inner(q, "q");
   check_inner(k, "k_pages");
   check_inner(v, "v_pages");

@@ -452,3 +452,41 @@ def test_offsets_beyond_32_bits(cuda_device):
     o, lse = S.window_attention(qs[:, :, :, :125], ks[:, :, :, :125], vs[:, :, :, :125], window=150, sinks=3, scale=d ** -0.5, return_lse=True)
     ref = R.window_attention(f64(qs[..., :125]), f64(ks[..., :125]), f64(vs[..., :125]), d ** -0.5, 150, 3, [200] * 2, [200] * 2)
     R.check_attention(f64(o), f64(lse), ref, "f16")
+
+
+def test_refusals_of_tensors(cuda_device):
+    """What does not fit is refused before anything is launched."""
+    import torch
+    from lazy_compiler_b200 import runtime
+    from lazy_compiler_b200 import serving as S
+    q, k = normal((2, 5, 4, 64), "f16", 0), normal((2, 7, 2, 64), "f16", 1)
+    pages, table, lens = normal((6, 2, 16, 64), "f16", 2), ints([[0, 1], [2, 3]]), ints([20, 9])
+    qt = q[:, 0]
+    refused = [
+        (lambda: S.window_attention(q, k, k[:, :6]), ValueError, "v: shape"),
+        (lambda: S.window_attention(q, k, k.bfloat16()), ValueError, "v: bfloat16"),
+        (lambda: S.window_attention(q.float(), k, k), ValueError, "q: float32"),
+        (lambda: S.window_attention(q, k.cpu(), k), ValueError, "k: float16 on cpu"),
+        (lambda: S.window_attention(q[0], k, k), ValueError, "3 axes"),
+        (lambda: S.window_attention(q.transpose(2, 3), k.transpose(2, 3), k.transpose(2, 3)), ValueError, "k: shape"),
+        (lambda: S.window_attention(k.mT, k.mT, k.mT), ValueError, "q: the last axis must be contiguous"),
+        (lambda: S.window_attention(q, k, k, q_lens=lens.long()), ValueError, "q_lens: int64"),
+        (lambda: S.window_attention(q, k, k, kv_lens=lens[:1]), ValueError, "kv_lens: shape"),
+        (lambda: S.window_attention(q, k, k, out=q[:, :4]), ValueError, "out: shape"),
+        (lambda: S.window_attention(q, k, k, window=1.5), TypeError, "integer"),
+        (lambda: S.window_attention(q, k, k, window=-1), runtime.LcError, "negative"),
+        (lambda: S.window_attention(q[:, :, :3], k, k), runtime.LcError, "3 query heads over 2"),
+        (lambda: S.window_attention(q, k, k, scale=0.0), runtime.LcError, "scale"),
+        (lambda: S.window_attention(None, k, k), ValueError, "q: expected a tensor"),
+        (lambda: S.paged_decode(qt, pages, pages[:5], table, lens), ValueError, "v_pages: shape"),
+        (lambda: S.paged_decode(qt, pages, pages, table[:1], lens), ValueError, "table: shape"),
+        (lambda: S.paged_decode(qt, pages, pages, table.long(), lens), ValueError, "table: int64"),
+        (lambda: S.paged_decode(qt, pages, pages, table, lens[::2]), ValueError, "lens: shape"),
+        (lambda: S.paged_decode(qt[:1], pages, pages, table, lens), ValueError, "table: shape"),
+        (lambda: S.paged_decode(normal((2, 4, 264), "f16", 3), *[normal((6, 2, 16, 264), "f16", 4)] * 2, table, lens), runtime.LcError, "over 256"),
+    ]
+    for call, kind, text in refused:
+        with pytest.raises(kind, match=text):
+            call()
+    o, lse = S.window_attention(q, k, k, return_lse=1)
+    assert o.shape == q.shape and lse.shape == (2, 4, 5)

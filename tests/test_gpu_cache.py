@@ -286,3 +286,35 @@ def test_pages_beyond_32_bit_offsets(cuda_device):
     S.cache_write(k, k, pool[12], pool[13], maps, ints([3, 2]))
     for plane in (12, 13):
         assert torch.equal(pool[plane, pages - 3, :, :3], k[0].transpose(0, 1)) and torch.equal(pool[plane, pages - 5, :, :2], k[1, :2].transpose(0, 1))
+
+
+def test_refusals_of_maps(cuda_device):
+    import torch
+    from lazy_compiler_b200 import runtime
+    from lazy_compiler_b200 import serving as S
+    pool = torch.zeros((2, 6, 2, 4, 8), device="cuda")
+    maps = S.CacheMaps(ints([[0, 1], [2, -1]]), ints([6, 3]), ints([1, 1, 1, 0, 0, 0]))
+    add, k = ints([1, 1]), torch.zeros((2, 1, 2, 8), device="cuda")
+    small = S.CacheMaps(maps.table[:1], maps.lens[:1], maps.refs)
+    refused = [
+        (lambda: S.cache_extend(maps, add[:1], page_size=4), ValueError, "add: shape"),
+        (lambda: S.cache_extend(maps, add.long(), page_size=4), ValueError, "add: int64"),
+        (lambda: S.cache_extend(maps, add, page_size=0), runtime.LcError, "size"),
+        (lambda: S.cache_extend(maps, add, page_size=4, into=small), ValueError, "into"),
+        (lambda: S.cache_extend(maps._replace(lens=maps.lens[:1]), add, page_size=4), ValueError, "maps: shape"),
+        (lambda: S.cache_extend(maps._replace(table=maps.table.t()), add, page_size=4), ValueError, "contiguous"),
+        (lambda: S.cache_extend(maps._replace(refs=maps.refs.cpu()), add, page_size=4), ValueError, "cpu"),
+        (lambda: S.cache_write(k, k, pool[0], pool[1, :5], maps, add), ValueError, "v_pages: shape"),
+        (lambda: S.cache_write(k, k.half(), pool[0], pool[1], maps, add), ValueError, "v: float16"),
+        (lambda: S.cache_write(k[:1], k[:1], pool[0], pool[1], maps, add), ValueError, "k: shape"),
+        (lambda: S.cache_fork(pool, maps, add, into=maps), runtime.LcError, "overwrite"),
+        (lambda: S.cache_fork(pool[:, :5], maps, add), ValueError, "pool"),
+        (lambda: S.cache_fork(pool.transpose(3, 4), maps, add), ValueError, "contiguous"),
+        (lambda: S.cache_compact(pool[0], maps), ValueError, "pool"),
+        (lambda: S.cache_trim(maps, window=0, page_size=4), runtime.LcError, "window"),
+        (lambda: S.cache_release(maps, add[:1], page_size=4), ValueError, "gone: shape"),
+        (lambda: S.cache_copy(pool, add, add[:1]), ValueError, "dst: shape"),
+    ]
+    for call, kind, text in refused:
+        with pytest.raises(kind, match=text):
+            call()

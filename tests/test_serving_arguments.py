@@ -103,3 +103,12 @@ def test_tensors_off_the_device_or_of_another_type():
         S.cache_extend(maps, maps.lens, page_size=16)
     with pytest.raises(ValueError, match="at least 1"):
         S.PagedCache(0, 1, 1, 1, 1, 1, 1)
+
+
+def test_numbers_in_the_refusals():
+    """The extension's messages hold sizes: with a libstdc++ of its own in the module, writing one faulted."""
+    from lazy_compiler_b200 import _serving
+    with pytest.raises(ValueError, match="expected 11 arguments, got 1"):
+        _serving.window_attention(1)
+    with pytest.raises(TypeError):
+        _serving.bind(*[1.5] * 8)
