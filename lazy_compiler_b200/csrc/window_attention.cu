@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) window_row_kernel(WindowParams
 }
 
 // ---------------------------------------------------------------- tensor-core form
-// Flash attention on tcgen05, the schedule of sdpa.cu: per CTA two query tiles of
+// Attention with a running softmax on tcgen05, the schedule of sdpa.cu: per CTA two query tiles of
 // 128 rows share every block of 128 keys; warp 0 loads (TMA), one thread of warp 1
 // issues the products (S = Q K^T and O += P V, P from tensor memory), a warpgroup per
 // tile does the softmax, one row per thread.  Under a window an item is only a few
