@@ -624,7 +624,7 @@ int lc_jit_rowprog(const void *image, size_t image_size, const lc_pw_program *pr
  * query head h reads key-value head h / (q_heads / kv_heads).  Head sizes up to
  * 256; the innermost axis is contiguous, `strides` are host arrays of element
  * (attention) or byte (page operations) strides.  lse may be null; it is f32
- * and contiguous.  What masked or absent tokens hold does not matter (infinities
+ * and contiguous.  Outputs overlap no input.  What masked or absent tokens hold does not matter (infinities
  * and NaN included). */
 
 /* o[b, i, h, :] = sum_j softmax_j(scale q[b, i, h] . k[b, j, h / g]) v[b, j, h / g, :].
@@ -655,7 +655,8 @@ int lc_paged_decode(int dtype, const void *q, const void *k, const void *v, void
  * read one set of maps and write another, which may be the same one except for
  * lc_cache_fork.  status[0]: 0, or -1 (an argument out of range), or how many
  * pages were missing; where it is not 0 the maps are those before.  status[1]:
- * the pages free afterwards. */
+ * the pages free afterwards.  Up to 2^31 - 1 table entries, 2^20 slots, 2^30
+ * tokens a slot. */
 
 /* Room for add[i] >= 0 more tokens in slot i: the lowest-numbered free pages, in
  * slot order and then in order of position; lens grow by add. */

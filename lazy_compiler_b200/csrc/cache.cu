@@ -595,7 +595,8 @@ int launch_maps(const char *me, void (*kernel)(Params), int64_t cells, cudaStrea
 
 int check_maps(const char *me, int64_t slots, int64_t width, int64_t pages, int64_t page_size) {
   if (slots < 0 || width < 0 || pages < 0 || page_size < 1) return fail(LC_ERR_INVALID, "%s: negative or zero size", me);
-  if (slots > (1 << 20) || pages > (1 << 30) || page_size > (1 << 20) || width > (1 << 24) || width * page_size > (1ll << 30))
+  if (slots > (1 << 20) || pages > (1 << 30) || page_size > (1 << 20) || width > (1 << 24) || width * page_size > (1ll << 30) ||
+      slots * width > INT32_MAX)  // the demand of all slots is an int, too
     return fail(LC_ERR_UNSUPPORTED, "%s: shape too large", me);
   return LC_OK;
 }

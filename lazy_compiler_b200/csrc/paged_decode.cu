@@ -881,7 +881,7 @@ extern "C" int lc_paged_decode(int dtype, const void *q, const void *k, const vo
     return fail(LC_ERR_INVALID, "%s: negative or zero size", me);
   if (q_heads % kv_heads) return fail(LC_ERR_INVALID, "%s: %lld query heads over %lld key-value heads", me, (long long)q_heads, (long long)kv_heads);
   if (!strides) return fail(LC_ERR_INVALID, "%s: null strides", me);
-  if (!(scale > 0.f) || scale > 3e38f) return fail(LC_ERR_INVALID, "%s: scale must be positive and finite", me);
+  if (!(scale > 0.f) || scale > 2e38f) return fail(LC_ERR_INVALID, "%s: scale must be positive and finite", me);
   if (d > attend::kMaxHead) return fail(LC_ERR_UNSUPPORTED, "%s: head size %lld is over 256", me, (long long)d);
   if (slots > (1 << 20) || q_heads > 65535 || pages > INT32_MAX || page_size > (1 << 20) || width * page_size > (1ll << 30))
     return fail(LC_ERR_UNSUPPORTED, "%s: shape too large", me);

@@ -95,6 +95,11 @@ void check_ints(const at::Tensor &t, const char *what, const at::Tensor &like, a
 void check_inner(const at::Tensor &t, const char *what) {
   if (t.dim() && t.size(-1) > 1 && t.stride(-1) != 1) refuse(what, ": the last axis must be contiguous");
 }
+// A tensor to write has every element at its own place, as far as strides of zero go.
+void check_out(const at::Tensor &t, const char *what) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) refuse(what, ": axis ", i, " is expanded, it cannot be written");
+}
 void check_cuda(const at::Tensor &t, const char *what) {
   if (!t.is_cuda()) refuse(what, ": on ", t.device(), ", the kernels run on CUDA devices only");
 }
@@ -162,7 +167,7 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const at::Tensor *q_lens = maybe(a[6], "q_lens"), *kv_lens = maybe(a[7], "kv_lens"), *given = maybe(a[8], "out");
   if (q_lens) check_ints(*q_lens, "q_lens", q, {batch});
   if (kv_lens) check_ints(*kv_lens, "kv_lens", q, {batch});
-  if (given) check(*given, "out", q, q.scalar_type(), {batch, s_q, heads, d});
+  if (given) check(*given, "out", q, q.scalar_type(), {batch, s_q, heads, d}), check_out(*given, "out");
   const c10::cuda::CUDAGuard guard(q.device());
   const at::Tensor out = given ? *given : fresh({batch, s_q, heads, d}, q.scalar_type(), q);
   const at::Tensor lse = truth(a[9]) ? fresh({batch, heads, s_q}, at::kFloat, q) : at::Tensor();
@@ -198,7 +203,7 @@ PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
   check(table, "table", q, at::kInt, {slots, width});
   check_ints(lens, "lens", q, {slots});
   const at::Tensor *given = maybe(a[8], "out");
-  if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d});
+  if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d}), check_out(*given, "out");
   const c10::cuda::CUDAGuard guard(q.device());
   const at::Tensor out = given ? *given : fresh({slots, heads, d}, q.scalar_type(), q);
   const at::Tensor lse = truth(a[9]) ? fresh({slots, heads}, at::kFloat, q) : at::Tensor();
@@ -271,6 +276,7 @@ Pool pool_of(const at::Tensor &t, const at::Tensor &like, int64_t pages) {
   if (t.dim() != 5 || t.device() != like.device() || t.size(1) != pages)
     refuse("pool: ", shape_text(t.sizes()), " on ", t.device(), ", expected [planes, ", pages, ", kv_heads, page_size, d] on ", like.device());
   check_inner(t, "pool");
+  check_out(t, "pool");
   if (t.size(3) > 1 && t.stride(3) != t.size(4)) refuse("pool: the tokens of a head must be contiguous");
   const int64_t size = t.element_size();
   return {ptr(t), t.size(0), t.size(2), t.size(3), t.size(4) * size, {t.stride(0) * size, t.stride(1) * size, t.stride(2) * size}};
@@ -307,6 +313,8 @@ PyObject *cache_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
   check(v, "v", m.table, k.scalar_type(), {m.slots, most, heads, d});
   check(kp, "k_pages", m.table, k.scalar_type(), {m.pages, heads, page_size, d});
   check(vp, "v_pages", m.table, k.scalar_type(), {m.pages, heads, page_size, d});
+  check_out(kp, "k_pages");
+  check_out(vp, "v_pages");
   const at::Tensor *views[4] = {&k, &v, &kp, &vp};
   const char *names[4] = {"k", "v", "k_pages", "v_pages"};
   int64_t strides[12];

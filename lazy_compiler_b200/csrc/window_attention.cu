@@ -1246,7 +1246,7 @@ extern "C" int lc_window_attention(int dtype, const void *q, const void *k, cons
     return fail(LC_ERR_INVALID, "%s: negative or zero size", me);
   if (q_heads % kv_heads) return fail(LC_ERR_INVALID, "%s: %lld query heads over %lld key-value heads", me, (long long)q_heads, (long long)kv_heads);
   if (!strides) return fail(LC_ERR_INVALID, "%s: null strides", me);
-  if (!(scale > 0.f) || scale > 3e38f) return fail(LC_ERR_INVALID, "%s: scale must be positive and finite", me);
+  if (!(scale > 0.f) || scale > 2e38f) return fail(LC_ERR_INVALID, "%s: scale must be positive and finite", me);
   if (d > attend::kMaxHead) return fail(LC_ERR_UNSUPPORTED, "%s: head size %lld is over 256", me, (long long)d);
   if (batch > 65535 || q_heads > 65535 || s_q > (1 << 30) || s_kv > (1 << 30) || batch * s_q > INT32_MAX)
     return fail(LC_ERR_UNSUPPORTED, "%s: shape too large", me);

@@ -70,7 +70,8 @@ def window_attention(q, k, v, *, window: int = 0, sinks: int = 0, scale: float |
     its query ``i`` is at position ``p = kv_lens[b] - q_lens[b] + i`` and sees key ``j <= p`` when ``window`` is 0,
     ``j > p - window`` or ``j < sinks``.  ``scale`` is ``1 / sqrt(d)`` by default.  Returns ``o`` like ``q`` (``out``
     where given), with ``return_lse`` also the log-sum-exp of the scaled scores, f32 ``[batch, q_heads, s_q]``.  Rows
-    that see nothing, and rows from ``q_lens[b]`` on, are 0 and -inf.  Any strides with a contiguous last axis.
+    that see nothing, and rows from ``q_lens[b]`` on, are 0 and -inf.  Any strides with a contiguous last axis; ``out``
+    overlaps no input.
     """
     r = _ext.window_attention(q, k, v, window, sinks, scale, q_lens, kv_lens, out, return_lse, stream)
     if type(r) is int:

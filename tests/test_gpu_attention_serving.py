@@ -473,6 +473,8 @@ def test_refusals_of_tensors(cuda_device):
         (lambda: S.window_attention(q, k, k, q_lens=lens.long()), ValueError, "q_lens: int64"),
         (lambda: S.window_attention(q, k, k, kv_lens=lens[:1]), ValueError, "kv_lens: shape"),
         (lambda: S.window_attention(q, k, k, out=q[:, :4]), ValueError, "out: shape"),
+        (lambda: S.window_attention(q, k, k, out=q[:1].expand(2, -1, -1, -1)), ValueError, "out: axis 0 is expanded"),
+        (lambda: S.paged_decode(qt, pages, pages, table, lens, out=qt[:, :1].expand(-1, 4, -1)), ValueError, "out: axis 1"),
         (lambda: S.window_attention(q, k, k, window=1.5), TypeError, "integer"),
         (lambda: S.window_attention(q, k, k, window=-1), runtime.LcError, "negative"),
         (lambda: S.window_attention(q[:, :, :3], k, k), runtime.LcError, "3 query heads over 2"),

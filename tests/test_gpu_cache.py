@@ -310,6 +310,8 @@ def test_refusals_of_maps(cuda_device):
         (lambda: S.cache_fork(pool, maps, add, into=maps), runtime.LcError, "overwrite"),
         (lambda: S.cache_fork(pool[:, :5], maps, add), ValueError, "pool"),
         (lambda: S.cache_fork(pool.transpose(3, 4), maps, add), ValueError, "contiguous"),
+        (lambda: S.cache_fork(pool[:, :1].expand(-1, 6, -1, -1, -1), maps, add), ValueError, "pool: axis 1 is expanded"),
+        (lambda: S.cache_write(k, k, pool[0], pool[1, :1].expand(6, -1, -1, -1), maps, add), ValueError, "v_pages: axis 0"),
         (lambda: S.cache_compact(pool[0], maps), ValueError, "pool"),
         (lambda: S.cache_trim(maps, window=0, page_size=4), runtime.LcError, "window"),
         (lambda: S.cache_release(maps, add[:1], page_size=4), ValueError, "gone: shape"),

@@ -105,6 +105,18 @@ def test_tensors_off_the_device_or_of_another_type():
         S.PagedCache(0, 1, 1, 1, 1, 1, 1)
 
 
+def test_limits_of_the_counts():
+    """A table whose entries, or a scale whose product with log2 e, would leave 32 bits."""
+    for call, status in [
+        (lambda: runtime.call("lc_cache_extend", P, P, P, P, P, P, P, P, 1 << 12, 1 << 19, 4, 16, NULL), -5),
+        (lambda: runtime.call("lc_cache_release", P, P, P, P, 0, 0, P, 1 << 20, 1 << 11, 4, 16, NULL), -5),
+        (lambda: window(scale=2.5e38), -1), (lambda: decode(scale=2.5e38), -1),
+    ]:
+        with pytest.raises(runtime.LcError) as err:
+            call()
+        assert err.value.status == status
+
+
 def test_numbers_in_the_refusals():
     """The extension's messages hold sizes: with a libstdc++ of its own in the module, writing one faulted."""
     from lazy_compiler_b200 import _serving
