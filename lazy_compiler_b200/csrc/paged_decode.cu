@@ -109,7 +109,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // in pages of 16: 169 us, 6370 GB/s, the rate of a copy; 64/8, f16, 100003 and 131072
 // tokens: 150 us, 6320 GB/s.  Three CTAs per SM of two stages against two of three:
 // the warps' own latency (a tile is a chain of some 500 instructions) needs 12 of them
-// (177 us with 8).
+// (177 us with 8).  Heads of 64, half the bytes a tile and nearly its instructions: four CTAs of
+// three stages (1 to 8192 tokens: 98 us; 105 with three of four, 98 with five of two, 111 with six;
+// groups of 16: 127, 161 with two of six).
 constexpr int kDecodeWarps = 4;
 constexpr int kTileKeys = 16;
 constexpr int kDeepParts = 16;
@@ -837,7 +839,7 @@ int launch_sized(const DecodeParams &p, cudaStream_t s) {
   // NT: 8 or 16 query heads of a group in one pass over its keys (a group of 9 to 16
   // read twice, 8 heads at a time, would take the loads twice; larger groups are cut in sixteens)
   const bool wide = p.q_heads / p.kv_heads > 8;
-  if (p.d <= 64) return wide ? launch_decode<T, 64, 2, 6, 2, PAGED16>(p, s) : launch_decode<T, 64, 1, 4, 3, PAGED16>(p, s);
+  if (p.d <= 64) return wide ? launch_decode<T, 64, 2, 3, 4, PAGED16>(p, s) : launch_decode<T, 64, 1, 3, 4, PAGED16>(p, s);
   if (p.d <= 128) return wide ? launch_decode<T, 128, 2, 3, 2, PAGED16>(p, s) : launch_decode<T, 128, 1, 2, 3, PAGED16>(p, s);
   return wide ? launch_decode<T, 256, 2, 3, 1, PAGED16>(p, s) : launch_decode<T, 256, 1, 3, 1, PAGED16>(p, s);
 }
