@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 //
 // Work is cut by length, not by sequence: all (slot, key-value head, group of 8 NT
 // query heads) segments are laid end to end as tiles of 64 keys, and each CTA takes
-// an equal contiguous run of them, so a batch of unequal lengths and a single long
+// an equal contiguous run of them (kEndUnits says how equal), so a batch of unequal lengths and a single long
 // sequence both fill the GPU.  A segment that spans CTAs leaves an unnormalised
 // (O, m, l) per CTA in the workspace; the CTA that arrives last joins them in CTA
 // order (the run boundaries depend on the lengths alone, so results repeat), or,
@@ -106,16 +106,21 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // P is split into two 16-bit parts (value and remainder) and multiplied twice: the
 // extra products hide behind the loads and keep P to 16 bits or more.
 // Bound by HBM.  Measured, 32/8 heads of 128, bf16: 64 sequences of 1 to 8192 tokens
-// in pages of 16: 169 us, 6370 GB/s, the rate of a copy; 64/8, f16, 100003 and 131072
-// tokens: 150 us, 6320 GB/s.  Three CTAs per SM of two stages against two of three:
+// in pages of 16: 167 us, 6440 GB/s, the rate of a copy; 64/8, f16, 100003 and 131072
+// tokens: 149 us, 6360 GB/s.  Three CTAs per SM of two stages against two of three:
 // the warps' own latency (a tile is a chain of some 500 instructions) needs 12 of them
 // (177 us with 8).  Heads of 64, half the bytes a tile and nearly its instructions: four CTAs of
-// three stages (1 to 8192 tokens: 98 us; 105 with three of four, 98 with five of two, 111 with six;
+// three stages (1 to 8192 tokens, before kEndUnits: 98 us; 105 with three of four, 98 with five of two, 111 with six of two;
 // groups of 16: 127, 161 with two of six).
 constexpr int kDecodeWarps = 4;
 constexpr int kTileKeys = 16;
 constexpr int kDeepParts = 16;
 constexpr int kMinTiles = 2;  // CTA tiles below which a segment is not cut further
+// Runs are cut into equal numbers of units, a tile's time each: a segment's end (the warps' sums
+// joined and written) counts as one too, or a CTA of nine segments of a tile each is done long after
+// the one beside it (64 sequences of 1 to 1000 tokens: 44.0 us without, 33.3 with one, 32.8 with
+// two, 33.0 with three; of 1 to 250: 18.7, 17.0, 17.7, 17.9; of 1 to 8192: 169, 168, 168, 170).
+constexpr int kEndUnits = 1;
 
 template <class T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -215,6 +220,11 @@ __device__ __forceinline__ void advance(Cursor &c, const DecodeParams &p, int pa
   } while (c.count == 0);
 }
 
+// a / b for counts: 32 bits where a has no more, which is a fifth of the instructions.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return (a >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
 struct DecodeWork {
   float *partials;    // [CTA][2][rows][DP + 4]: of a segment that began before the CTA, of one that began in it
   unsigned *arrived;  // [slots * parts], zero between launches
@@ -246,9 +256,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   __shared__ float scratch[kDecodeWarps * (DP + 2)];  // the plain form's joins
   __shared__ float merge_m[kDecodeWarps][kRows], merge_l[kDecodeWarps][kRows], merge_w[kDecodeWarps][kRows];
   __shared__ float row_m[kRows], row_l[kRows];
-  __shared__ long long sums[kDecodeWarps];
-  __shared__ int start_slot;
-  __shared__ long long start_tile;
+  __shared__ long long sums[kDecodeWarps], tile_sums[kDecodeWarps];
+  __shared__ int start_slot, start_part, start_t;
+  __shared__ long long tile_at[2];
   __shared__ unsigned ticket;
 
   pdl_wait();
@@ -261,36 +271,56 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   // ---- this CTA's run of tiles
   const int per = (p.slots + kDecodeWarps * 32 - 1) / (kDecodeWarps * 32);
   const int s0 = min(p.slots, tid * per), s1 = min(p.slots, s0 + per);
-  long long own = 0;
-  for (int s = s0; s < s1; ++s) own += (long long)cta_tiles(slot_tiles(p, s)) * parts;
-  long long inc = own;
+  // units: a segment's tiles and kEndUnits for its end
+  long long own = 0, own_tiles = 0;
+  auto units_of = [&](int count) { return (long long)(count ? count + kEndUnits : 0) * parts; };
+  for (int s = s0; s < s1; ++s) {
+    const int count = cta_tiles(slot_tiles(p, s));
+    own += units_of(count);
+    own_tiles += (long long)count * parts;
+  }
+  long long inc = own, inc_tiles = own_tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += up;
+    const long long up = __shfl_up_sync(0xffffffffu, inc, o), up_tiles = __shfl_up_sync(0xffffffffu, inc_tiles, o);
+    if (lane >= o) inc += up, inc_tiles += up_tiles;
   }
-  if (lane == 31) sums[warp] = inc;
+  if (lane == 31) sums[warp] = inc, tile_sums[warp] = inc_tiles;
   __syncthreads();
-  long long before = inc - own, total = 0;
+  long long before = inc - own, total = 0, before_tiles = inc_tiles - own_tiles, total_tiles = 0;
 #pragma unroll
   for (int w = 0; w < kDecodeWarps; ++w) {
-    if (w < warp) before += sums[w];
+    if (w < warp) before += sums[w], before_tiles += tile_sums[w];
     total += sums[w];
+    total_tiles += tile_sums[w];
   }
-  const long long useful = (total + kMinTiles - 1) / kMinTiles;
+  const long long useful = (total_tiles + kMinTiles - 1) / kMinTiles;
   const long long ctas = useful < (long long)gridDim.x ? useful : (long long)gridDim.x;
   const bool works = blockIdx.x < ctas;
-  const long long begin = works ? blockIdx.x * total / ctas : 0, end = works ? (blockIdx.x + 1) * total / ctas : 0;
-  if (works && begin >= before && begin < before + own) {
-    long long at = before;
-    int s = s0;
-    for (;; ++s) {
-      const long long here = (long long)cta_tiles(slot_tiles(p, s)) * parts;
-      if (begin < at + here) break;
-      at += here;
+  const long long begin = works ? quotient(blockIdx.x * total, ctas) : 0, end = works ? quotient((blockIdx.x + 1) * total, ctas) : 0;
+  // where the run begins, and the numbers of its first tile and of the one behind it
+  if (works) {
+#pragma unroll 1
+    for (int x = 0; x < 2; ++x) {
+      const long long unit = x ? end : begin;
+      if (unit < before || unit >= before + own) continue;
+      long long at = before, at_tile = before_tiles;
+      int s = s0, count;
+      for (;; ++s) {
+        count = cta_tiles(slot_tiles(p, s));
+        if (unit < at + units_of(count)) break;
+        at += units_of(count);
+        at_tile += (long long)count * parts;
+      }
+      const long long in = unit - at, seg = quotient(in, count + kEndUnits), t = in - seg * (count + kEndUnits);
+      tile_at[x] = at_tile + seg * count + min(t, (long long)count);
+      if (x == 0) {
+        start_slot = s;
+        start_part = (int)seg;
+        start_t = (int)t;
+      }
     }
-    start_slot = s;
-    start_tile = begin - at;
+    if (end == total && tid == 0) tile_at[1] = total_tiles;
   }
   // slots with nothing to see
   for (int s = blockIdx.x; s < p.slots; s += gridDim.x) {
@@ -305,16 +335,22 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   if (work.deep && tid == 0) work.spans[blockIdx.x] = make_int2(-1, -1);
   __syncthreads();
   if (!works) return;
+  const int steps = (int)(tile_at[1] - tile_at[0]);
+  if (steps == 0) return;  // a run of a segment's end alone
 
   Cursor load;
   load.slot = start_slot;
   load.tiles = slot_tiles(p, load.slot);
   load.count = cta_tiles(load.tiles);
-  load.part = (int)(start_tile / load.count);
-  load.t = (int)(start_tile % load.count);
+  load.part = start_part;
+  load.t = start_t;
+  int64_t seg_begin = begin - load.t;  // unit of the current segment's first tile in the sequence of all
+  if (load.t >= load.count) {          // behind a segment's last tile: the next one
+    seg_begin += load.count + kEndUnits;
+    load.t = load.count - 1;
+    advance(load, p, parts);
+  }
   Cursor use = load;
-  const int steps = (int)(end - begin);
-  int64_t seg_begin = begin - use.t;  // first tile of the current segment in the sequence of all
 
   // ---- loading: lane l copies piece l % kChunks of rows l / kChunks, ...
   const int piece = lane % kChunks, piece_row = lane / kChunks;
@@ -599,7 +635,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
         partial[tid * (DP + 4) + DP + 1] = row_l[tid];
       }
       // the CTAs whose runs hold the segment's first and last tile
-      const int first = (int)(((seg_begin + 1) * ctas - 1) / total), last = (int)((seg_end * ctas - 1) / total);
+      const int first = (int)quotient((seg_begin + 1) * ctas - 1, total), last = (int)quotient(seg_end * ctas - 1, total);
       if (work.deep) {
         if (seg_begin >= begin && tid == 0) work.spans[blockIdx.x] = make_int2(use.slot * parts + use.part, last);
         __syncthreads();  // the sums have been read
@@ -705,7 +741,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
     compute(stage);
     if (use.t + 1 == use.count || i + 1 == steps) {
       end_segment(seg_begin + use.count, stage);
-      seg_begin += use.count;
+      seg_begin += use.count + kEndUnits;
       if (i + 1 < steps) {
         use.t = use.count - 1;
         advance(use, p, parts);
