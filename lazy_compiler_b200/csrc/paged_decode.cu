@@ -121,6 +121,11 @@ constexpr int kMinTiles = 2;  // CTA tiles below which a segment is not cut furt
 // the one beside it (64 sequences of 1 to 1000 tokens: 44.0 us without, 33.3 with one, 32.8 with
 // two, 33.0 with three; of 1 to 250: 18.7, 17.0, 17.7, 17.9; of 1 to 8192: 169, 168, 168, 170).
 constexpr int kEndUnits = 1;
+// A cut this many tiles or fewer from an end of a segment moves there: one tile more or less is
+// cheaper than a segment that two CTAs have to join (64 sequences of 1 to 250 tokens: 16.7 -> 13.9 us,
+// 8 of 1 to 512: 15.3 -> 13.3, but 64 of 1 to 500: 23.3 -> 25.2; two tiles make short caches of few
+// heads worse, 2000 tokens of 2 heads: 9.0 -> 10.7).
+constexpr int kSnap = 1;
 
 template <class T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   __shared__ float row_m[kRows], row_l[kRows];
   __shared__ long long sums[kDecodeWarps], tile_sums[kDecodeWarps];
   __shared__ int start_slot, start_part, start_t;
-  __shared__ long long tile_at[2];
+  __shared__ long long unit_at[2], tile_at[2];
   __shared__ unsigned ticket;
 
   pdl_wait();
@@ -294,15 +299,17 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
     total += sums[w];
     total_tiles += tile_sums[w];
   }
-  const long long useful = (total_tiles + kMinTiles - 1) / kMinTiles;
+  // a CTA for every kMinTiles tiles, or for every segment, if those are more (4 sequences of 1 to 128
+  // tokens, 8 heads: 8.9 us; 10.8 with two segments a CTA)
+  const long long useful = max((total_tiles + kMinTiles - 1) / kMinTiles, (total - total_tiles) / kEndUnits);
   const long long ctas = useful < (long long)gridDim.x ? useful : (long long)gridDim.x;
   const bool works = blockIdx.x < ctas;
-  const long long begin = works ? quotient(blockIdx.x * total, ctas) : 0, end = works ? quotient((blockIdx.x + 1) * total, ctas) : 0;
+  const long long even_begin = works ? quotient(blockIdx.x * total, ctas) : 0, even_end = works ? quotient((blockIdx.x + 1) * total, ctas) : 0;
   // where the run begins, and the numbers of its first tile and of the one behind it
   if (works) {
 #pragma unroll 1
     for (int x = 0; x < 2; ++x) {
-      const long long unit = x ? end : begin;
+      const long long unit = x ? even_end : even_begin;
       if (unit < before || unit >= before + own) continue;
       long long at = before, at_tile = before_tiles;
       int s = s0, count;
@@ -313,14 +320,19 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
         at_tile += (long long)count * parts;
       }
       const long long in = unit - at, seg = quotient(in, count + kEndUnits), t = in - seg * (count + kEndUnits);
-      tile_at[x] = at_tile + seg * count + min(t, (long long)count);
+      const int to = 2 * t < count ? (t <= kSnap ? 0 : (int)t) : (t >= count - kSnap ? count : (int)t);
+      unit_at[x] = unit - t + to;
+      tile_at[x] = at_tile + seg * count + to;
       if (x == 0) {
         start_slot = s;
         start_part = (int)seg;
-        start_t = (int)t;
+        start_t = to;
       }
     }
-    if (end == total && tid == 0) tile_at[1] = total_tiles;
+    if (even_end == total && tid == 0) {
+      unit_at[1] = total;
+      tile_at[1] = total_tiles;
+    }
   }
   // slots with nothing to see
   for (int s = blockIdx.x; s < p.slots; s += gridDim.x) {
@@ -335,8 +347,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   if (work.deep && tid == 0) work.spans[blockIdx.x] = make_int2(-1, -1);
   __syncthreads();
   if (!works) return;
+  const long long begin = unit_at[0], end = unit_at[1];
   const int steps = (int)(tile_at[1] - tile_at[0]);
-  if (steps == 0) return;  // a run of a segment's end alone
+  if (steps == 0) return;  // its cuts have moved together, or only a segment's end lies between
 
   Cursor load;
   load.slot = start_slot;
@@ -634,8 +647,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
         partial[tid * (DP + 4) + DP] = row_m[tid];
         partial[tid * (DP + 4) + DP + 1] = row_l[tid];
       }
-      // the CTAs whose runs hold the segment's first and last tile
-      const int first = (int)quotient((seg_begin + 1) * ctas - 1, total), last = (int)quotient(seg_end * ctas - 1, total);
+      // The CTAs whose runs hold the segment's first and last tile: as many run boundaries as there
+      // are up to its first kSnap tiles lie before it, those in its last kSnap behind it.
+      const int first = (int)quotient((seg_begin + kSnap + 1) * ctas - 1, total), last = (int)quotient((seg_end - kSnap) * ctas - 1, total);
       if (work.deep) {
         if (seg_begin >= begin && tid == 0) work.spans[blockIdx.x] = make_int2(use.slot * parts + use.part, last);
         __syncthreads();  // the sums have been read

@@ -336,6 +336,14 @@ def test_token_many_slots(dtype, cuda_device):
     decode(dtype, rng.integers(0, 300, 1100).tolist(), 16, 1, 1, 64, 40, 2, seed=5)
 
 
+@pytest.mark.parametrize("slots, most, d", [(1, 130, 64), (2, 64, 128), (150, 130, 64), (151, 128, 128), (297, 65, 128), (40, 1000, 96)])
+def test_token_many_short_caches(slots, most, d, cuda_device):
+    """Runs that begin and end at, just behind and just before the ends of segments of a few tiles."""
+    lens = [(i * 37) % (most + 1) for i in range(slots)]
+    decode("bf16", lens, 16, 6, 3, d, 0, 0, seed=slots)
+    decode("f16", [most] * slots, 16, 6, 3, d, 0, 0, seed=slots + 1)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_token_layouts_and_scores(dtype, cuda_device):
     decode(dtype, [100, 333], 16, 8, 2, 128, 0, 0, seed=6, order="nhd")
