@@ -769,73 +769,121 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
 }
 
 // Joins the segments that span CTAs: blockIdx.x counts them, blockIdx.y is a row; the
-// parts are dealt to eight warps.
+// parts are dealt to eight warps, each with a running maximum.  A chain of three reads: the
+// spans, the parts, all of a warp's first kAtOnce together, and the eight warps' sums.
 constexpr int kJoinWarps = 8;
+constexpr int kMostSpans = 4;  // of a thread: up to 1024 CTAs
 
 template <class T, int DP, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodeParams p, DecodeWork work) {
-  constexpr int kRows = 8 * NT, kCols = DP / 32;
+  constexpr int kRows = 8 * NT, kCols = DP / 32, kAtOnce = 8;
   __shared__ float scratch[kJoinWarps * (DP + 2)];
-  __shared__ int found;
+  __shared__ int counts[kMostSpans * kJoinWarps];
+  __shared__ int2 found;  // the first and the last CTA's span
+  __shared__ int found_at;
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) found = -1;
+  int2 mine[kMostSpans];
+#pragma unroll
+  for (int x = 0; x < kMostSpans; ++x) {
+    const int c = x * kJoinWarps * 32 + tid;
+    mine[x] = c < work.ctas ? work.spans[c] : make_int2(-1, -1);
+  }
+#pragma unroll
+  for (int x = 0; x < kMostSpans; ++x) {
+    const unsigned some = __ballot_sync(0xffffffffu, mine[x].x >= 0);
+    if (lane == 0) counts[x * kJoinWarps + warp] = __popc(some);
+    if (mine[x].x >= 0) mine[x].y |= __popc(some & ((1u << lane) - 1)) << 16;  // its rank in the warp beside the CTA
+  }
+  if (tid == 0) found_at = -1;
   __syncthreads();
-  if (warp == 0) {
-    int left = blockIdx.x;
-    for (int base = 0; base < work.ctas; base += 32) {
-      const unsigned some = __ballot_sync(0xffffffffu, base + lane < work.ctas && work.spans[base + lane].x >= 0);
-      const int here = __popc(some);
-      if (left < here) {
-        if ((some >> lane & 1) && __popc(some & ((1u << lane) - 1)) == left) found = base + lane;
-        break;
-      }
-      left -= here;
+  const int upto = counts[lane];  // kMostSpans * kJoinWarps is a warp's lanes
+  int before = upto;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += up;
+  }
+  before -= upto;
+#pragma unroll
+  for (int x = 0; x < kMostSpans; ++x) {
+    const int rank = __shfl_sync(0xffffffffu, before, x * kJoinWarps + warp) + (mine[x].y >> 16);
+    if (mine[x].x >= 0 && rank == (int)blockIdx.x) {
+      found_at = x * kJoinWarps * 32 + tid;
+      found = make_int2(mine[x].x, mine[x].y & 0xffff);
     }
   }
   __syncthreads();
-  const int first = found, row = blockIdx.y;
+  const int first = found_at, row = blockIdx.y;
   if (first < 0) return;
-  const int2 span = work.spans[first];
+  const int2 span = found;
   const int group = p.q_heads / p.kv_heads, chunks = (group + kRows - 1) / kRows, parts = p.kv_heads * chunks;
   const int slot = span.x / parts, part = span.x % parts, head = part / chunks, h = head * group + part % chunks * kRows + row;
   if (h >= (head + 1) * group) return;
   // CTA c's share of the row: the segment began in CTA `first` and before every other
   auto share = [&](int c) { return work.partials + ((int64_t)c * 2 + (c == first)) * kRows * (DP + 4) + row * (DP + 4); };
-  float top = -INFINITY;
-  for (int c = first + tid; c <= span.y; c += kJoinWarps * 32) top = fmaxf(top, __ldcg(share(c) + DP));
-  top = block_max(top, scratch);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, o[kCols];
+  float top = -INFINITY, sum = 0.f, o[kCols];
 #pragma unroll
   for (int x = 0; x < kCols; ++x) o[x] = 0.f;
-#pragma unroll 8
-  for (int c = first + warp; c <= span.y; c += kJoinWarps) {
-    const float *from = share(c);
-    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from + DP));
-    const float weight = softmax::ex2(ml.x - base);
-    sum = fmaf(ml.y, weight, sum);
+#pragma unroll 1
+  for (int c0 = first + warp; c0 <= span.y; c0 += kAtOnce * kJoinWarps) {
+    float2 ml[kAtOnce], two[kAtOnce][kCols / 2];
 #pragma unroll
-    for (int x = 0; x < kCols; x += 2) {
-      const float2 two = __ldcg(reinterpret_cast<const float2 *>(from + lane * kCols + x));
-      o[x] = fmaf(two.x, weight, o[x]);
-      o[x + 1] = fmaf(two.y, weight, o[x + 1]);
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int c = c0 + u * kJoinWarps;
+      ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int x = 0; x < kCols / 2; ++x) two[u][x] = make_float2(0.f, 0.f);
+      if (c <= span.y) {
+        const float *from = share(c);
+        ml[u] = __ldcg(reinterpret_cast<const float2 *>(from + DP));
+#pragma unroll
+        for (int x = 0; x < kCols / 2; ++x) two[u][x] = __ldcg(reinterpret_cast<const float2 *>(from + lane * kCols + x * 2));
+      }
+    }
+    float top_new = top;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) top_new = fmaxf(top_new, ml[u].x);
+    const float base = top_new == -INFINITY ? 0.f : top_new, alpha = softmax::ex2(top - base);
+    top = top_new;
+    sum *= alpha;
+#pragma unroll
+    for (int x = 0; x < kCols; ++x) o[x] *= alpha;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float weight = softmax::ex2(ml[u].x - base);
+      sum = fmaf(ml[u].y, weight, sum);
+#pragma unroll
+      for (int x = 0; x < kCols / 2; ++x) {
+        o[x * 2] = fmaf(two[u][x].x, weight, o[x * 2]);
+        o[x * 2 + 1] = fmaf(two[u][x].y, weight, o[x * 2 + 1]);
+      }
     }
   }
-  __syncthreads();  // block_max's scratch has been read
 #pragma unroll
   for (int x = 0; x < kCols; ++x) scratch[warp * (DP + 2) + lane * kCols + x] = o[x];
-  if (lane == 0) scratch[warp * (DP + 2) + DP] = sum;
+  if (lane == 0) {
+    scratch[warp * (DP + 2) + DP] = sum;
+    scratch[warp * (DP + 2) + DP + 1] = top;
+  }
   __syncthreads();
+  float weights[kJoinWarps];
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, scratch[w * (DP + 2) + DP + 1]);
   sum = 0.f;
-  for (int w = 0; w < kJoinWarps; ++w) sum += scratch[w * (DP + 2) + DP];
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    weights[w] = softmax::ex2(scratch[w * (DP + 2) + DP + 1] - (top == -INFINITY ? 0.f : top));
+    sum = fmaf(scratch[w * (DP + 2) + DP], weights[w], sum);
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T *out = static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1];
   bool odd = false;
   if (tid < p.d) {
     float v = 0.f;
-    for (int w = 0; w < kJoinWarps; ++w) v += scratch[w * (DP + 2) + tid];
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) v = fmaf(scratch[w * (DP + 2) + tid], weights[w], v);
     v *= inv;
     odd = !isfinite(v);
     out[tid] = Elem<T>::from_float(v);
@@ -860,7 +908,7 @@ int launch_decode(const DecodeParams &p, cudaStream_t s) {
       return rc;
     if (dev >= 0 && dev < 64) configured[dev] = 1;
   }
-  const int ctas = sm_count() * CTAS;
+  const int ctas = std::min(sm_count(), kMostSpans * kJoinWarps * 32 / CTAS) * CTAS;
   const int group = p.q_heads / p.kv_heads;
   const int64_t parts = (int64_t)p.kv_heads * ((group + L::kRows - 1) / L::kRows);
   DecodeWork w = {};
