@@ -89,9 +89,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // sequence both fill the GPU.  A segment that spans CTAs leaves an unnormalised
 // (O, m, l) per CTA in the workspace; the CTA that arrives last joins them in CTA
 // order (the run boundaries depend on the lengths alone, so results repeat), or,
-// where a segment may span kDeepParts of them or more, a second kernel with a CTA per row
-// (one sequence of 131072 with one key-value head, 444 parts: 29 us; 167 us with the last
-// CTA, which reads 1.9 MB alone).
+// where a segment may span kDeepParts of them or more, a second kernel with a CTA per row (one
+// sequence of 131072 with one key-value head, 444 parts: 28 us, 167 with the last CTA, which
+// reads 1.9 MB alone; 4 of 1 to 8192 tokens, 8 heads: 20.3 us, 24.7 with it from 16 parts on; one
+// of 512: 9.2, 11.1).
 //
 // In a CTA each warp takes 16 keys of every tile and is on its own until the
 // segment ends: it copies its keys' rows (cp.async, 16 bytes per lane, zeros where
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // groups of 16: 127, 161 with two of six).
 constexpr int kDecodeWarps = 4;
 constexpr int kTileKeys = 16;
-constexpr int kDeepParts = 16;
+constexpr int kDeepParts = 5;
 constexpr int kMinTiles = 2;  // CTA tiles below which a segment is not cut further
 // Runs are cut into equal numbers of units, a tile's time each: a segment's end (the warps' sums
 // joined and written) counts as one too, or a CTA of nine segments of a tile each is done long after
@@ -267,7 +268,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   __shared__ unsigned ticket;
 
   pdl_wait();
-  pdl_trigger();
+  // Before a join the next kernel is not let in early: the join's CTAs, and the next call's behind
+  // them, on SMs that are still reading cost more than their launch (5 x 32687 tokens, heads of 64,
+  // call after call: 60 us, 82 let in).
+  if (!work.deep) pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.q_heads / p.kv_heads;
   const int chunks = (group + kRows - 1) / kRows;
