@@ -625,7 +625,10 @@ int lc_jit_rowprog(const void *image, size_t image_size, const lc_pw_program *pr
  * 256; the innermost axis is contiguous, `strides` are host arrays of element
  * (attention) or byte (page operations) strides.  lse may be null; it is f32
  * and contiguous.  Outputs overlap no input.  What masked or absent tokens hold does not matter (infinities
- * and NaN included). */
+ * and NaN included).
+ * Workspaces belong to a stream and grow with its calls, which must not happen during a capture.  A CUDA graph
+ * keeps those of the stream it was captured on: it may not run beside a call on that stream or beside another
+ * graph captured on it. */
 
 /* o[b, i, h, :] = sum_j softmax_j(scale q[b, i, h] . k[b, j, h / g]) v[b, j, h / g, :].
  * Sequence b has q_lens[b] queries (null: s_q) and kv_lens[b] keys (null: s_kv),

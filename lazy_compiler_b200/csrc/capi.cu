@@ -1,5 +1,6 @@
 // Library plumbing: version, per-thread error messages, device facts and the
 // library-owned reduction workspace.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -19,6 +20,7 @@ std::map<std::pair<int, cudaStream_t>, lc::ReduceWorkspace> g_workspaces;
 struct Scratch {
   void *ptr = nullptr;
   size_t bytes = 0;
+  bool held = false;  // handed out during a stream capture: a CUDA graph has its address
 };
 std::map<std::tuple<int, cudaStream_t, int>, Scratch> g_scratch;
 int *g_error_words[64] = {nullptr};
@@ -91,7 +93,12 @@ static int scratch_of(cudaStream_t stream, int slot, size_t bytes, bool zeroed, 
   std::lock_guard<std::mutex> lock(g_mutex);
   Scratch &sc = g_scratch[std::make_tuple(dev, stream, slot)];
   if (sc.bytes < bytes) {
-    if (sc.ptr) {
+    size_t size = bytes;
+    if (sc.held) {
+      // A graph may run with the old buffer at any later time, so it stays until the process ends.
+      // Doubling keeps all that stay below the one in use.
+      size = std::max(bytes, 2 * sc.bytes);
+    } else if (sc.ptr) {
       // the stream may still read the old buffer
       if (int rc = check_cuda(cudaStreamSynchronize(stream), "scratch: stream")) return rc;
       cudaFree(sc.ptr);
@@ -99,19 +106,29 @@ static int scratch_of(cudaStream_t stream, int slot, size_t bytes, bool zeroed, 
       sc.bytes = 0;
     }
     void *mem = nullptr;
-    if (cudaMalloc(&mem, bytes) != cudaSuccess) {
+    if (cudaMalloc(&mem, size) != cudaSuccess) {
       cudaGetLastError();
-      return fail(LC_ERR_NOMEM, "scratch: cudaMalloc(%zu) failed", bytes);
+      size = bytes;
+      if (cudaMalloc(&mem, size) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(LC_ERR_NOMEM, "scratch: cudaMalloc(%zu) failed", bytes);
+      }
     }
     // a synchronous memset: the zeros are there before any kernel of any stream reads them
     if (zeroed) {
-      if (int rc = check_cuda(cudaMemset(mem, 0, bytes), "scratch: memset")) {
+      if (int rc = check_cuda(cudaMemset(mem, 0, size), "scratch: memset")) {
         cudaFree(mem);
         return rc;
       }
     }
     sc.ptr = mem;
-    sc.bytes = bytes;
+    sc.bytes = size;
+    sc.held = false;
+  }
+  if (!sc.held) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) cudaGetLastError();  // the launch will say what is wrong
+    sc.held = capture != cudaStreamCaptureStatusNone;
   }
   *out = sc.ptr;
   return LC_OK;

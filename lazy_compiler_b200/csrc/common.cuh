@@ -60,7 +60,8 @@ int gemm_mixed(int mma_type, int a_type, int b_type, int c_type, int b_layout, i
 
 // Library-owned scratch of at least `bytes`, one per (device, stream, slot),
 // grown (never shrunk) on demand with cudaMalloc.  Growing synchronises the
-// device, so it must not happen inside stream capture.
+// device, so it must not happen inside stream capture.  A buffer that was handed
+// out during a capture is never freed: the graph goes on using it.
 int scratch_buffer(cudaStream_t stream, int slot, size_t bytes, void **out);
 // The same, all zero when it is created or grown (for counters that each kernel
 // leaves at zero).

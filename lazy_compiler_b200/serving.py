@@ -16,7 +16,8 @@ given ones, which may be the same (not for :func:`cache_fork`).  :class:`PagedCa
 
 A tensor used on another stream than the one it was made on needs ``record_stream`` or an event, as any torch tensor.
 The library's workspaces belong to a stream and grow on its first calls: before a capture, run the step once on the
-stream that will capture it.
+stream that will capture it.  A graph keeps the workspaces of the stream it was captured on, also when later calls make
+them grow; so graphs captured on one stream, and calls on that stream, may not run at the same time.
 """
 from __future__ import annotations
 
