@@ -57,6 +57,18 @@ int sm_count() {
   return g_sms[dev];
 }
 
+// Zeros that are in `mem` when this returns, whatever stream its kernels run on.  cudaMemset alone
+// would not do: it returns before they are, and writes them in the order of the default stream,
+// which other streams need not wait for.
+static int zero_now(void *mem, size_t bytes, const char *what) {
+  cudaStream_t own = nullptr;
+  int rc = check_cuda(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking), what);
+  if (!rc) rc = check_cuda(cudaMemsetAsync(mem, 0, bytes, own), what);
+  if (!rc) rc = check_cuda(cudaStreamSynchronize(own), what);
+  if (own) cudaStreamDestroy(own);
+  return rc;
+}
+
 int reduce_workspace(cudaStream_t stream, ReduceWorkspace *out) {
   int dev = 0;
   if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
@@ -73,8 +85,8 @@ int reduce_workspace(cudaStream_t stream, ReduceWorkspace *out) {
     cudaGetLastError();
     return fail(LC_ERR_NOMEM, "reduction workspace: cudaMalloc(%zu) failed", bytes);
   }
-  // synchronous memset: the counter must read zero before any kernel uses it
-  if (int rc = check_cuda(cudaMemset(mem, 0, bytes), "workspace memset")) {
+  // the counter must read zero before any kernel uses it
+  if (int rc = zero_now(mem, bytes, "workspace memset")) {
     cudaFree(mem);
     return rc;
   }
@@ -114,9 +126,8 @@ static int scratch_of(cudaStream_t stream, int slot, size_t bytes, bool zeroed, 
         return fail(LC_ERR_NOMEM, "scratch: cudaMalloc(%zu) failed", bytes);
       }
     }
-    // a synchronous memset: the zeros are there before any kernel of any stream reads them
     if (zeroed) {
-      if (int rc = check_cuda(cudaMemset(mem, 0, size), "scratch: memset")) {
+      if (int rc = zero_now(mem, size, "scratch: memset")) {
         cudaFree(mem);
         return rc;
       }
@@ -153,7 +164,7 @@ int device_error_word(int **out) {
       cudaGetLastError();
       return fail(LC_ERR_NOMEM, "device error word: cudaMalloc failed");
     }
-    if (int rc = check_cuda(cudaMemset(mem, 0, 256), "error word memset")) {
+    if (int rc = zero_now(mem, 256, "error word memset")) {
       cudaFree(mem);
       return rc;
     }

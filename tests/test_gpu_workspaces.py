@@ -84,3 +84,48 @@ def test_a_captured_step_keeps_its_workspaces(cuda_device):
     assert caches[0].check() == caches[1].check()
     assert torch.equal(outs[0], outs[1])
     assert torch.equal(caches[0].maps.lens, caches[1].maps.lens) and torch.equal(caches[0].maps.refs, caches[1].maps.refs)
+
+
+def test_counters_are_zero_on_a_stream_beside_a_busy_default_stream(cuda_device):
+    """A stream's first call, while the default stream has work queued: nothing of it waits for that work, and its
+    counters read zero although the memory they lie in held something before."""
+    import torch
+    from cuda.bindings import runtime as cudart
+    from lazy_compiler_b200 import runtime
+    from lazy_compiler_b200 import serving as S
+    # 30 slots of one long and 29 short caches: the long one's parts are counted and joined by the last of its CTAs
+    slots, page, h, d, n = 30, 16, 8, 128, 6000
+    width = n // page
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(2 * width, h, page, d, generator=g, device="cuda").half() for _ in range(2))
+    q = torch.randn(slots, 32, d, generator=g, device="cuda").half()
+    table = torch.randint(0, 2 * width, (slots, width), generator=g, device="cuda", dtype=torch.int32)
+    lens = ints([n] + [100] * (slots - 1))
+    x = torch.randn(1 << 22, generator=g, device="cuda")
+    want = S.paged_decode(q, k, v, table, lens, return_lse=True)
+    want_sum = torch.empty(1, device="cuda")
+    runtime.call("lc_sum_f32", ctypes.c_void_p(x.data_ptr()), ctypes.c_void_p(want_sum.data_ptr()), x.numel(), None)
+    # memory as the workspaces will find it, not zero
+    dirty = [cudart.cudaMalloc(size)[1] for size in (slots * h * 4, 1 << 14, 1 << 16) for _ in range(4)]
+    for at, size in zip(dirty, [slots * h * 4] * 4 + [1 << 14] * 4 + [1 << 16] * 4):
+        cudart.cudaMemset(at, 0xFF, size)
+    torch.cuda.synchronize()
+    for at in dirty:
+        cudart.cudaFree(at)
+    got = [torch.full_like(w, float("nan")) for w in want] + [torch.full_like(want_sum, float("nan"))]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    busy = torch.cuda.Event()
+    torch.cuda._sleep(2_000_000_000)
+    busy.record()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            o, lse = S.paged_decode(q, k, v, table, lens, out=got[0], return_lse=True)
+        handle = ctypes.c_void_p(side.cuda_stream)
+        for _ in range(3):
+            runtime.call("lc_sum_f32", ctypes.c_void_p(x.data_ptr()), ctypes.c_void_p(got[2].data_ptr()), x.numel(), handle)
+    side.synchronize()
+    waited = busy.query()
+    torch.cuda.synchronize()
+    assert not waited
+    assert torch.equal(o, want[0]) and torch.equal(lse, want[1]) and torch.equal(got[2], want_sum)
