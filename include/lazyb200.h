@@ -676,6 +676,13 @@ int lc_cache_write(const void *k, const void *v, void *k_pages, void *v_pages, c
                    const int32_t *lens, const int32_t *add, int64_t slots, int64_t most, int64_t width,
                    int64_t pages, int64_t page_size, int64_t kv_heads, int64_t row_bytes,
                    const int64_t *strides, void *stream);
+/* The same, but nothing is written where the device word *refused is not 0 (null: as above): with the status
+ * of the lc_cache_extend before it, the tokens that found no room do not overwrite the newest ones there are. */
+int lc_cache_write_unless(const void *k, const void *v, void *k_pages, void *v_pages, const int32_t *table,
+                          const int32_t *lens, const int32_t *add, int64_t slots, int64_t most,
+                          int64_t width, int64_t pages, int64_t page_size, int64_t kv_heads,
+                          int64_t row_bytes, const int64_t *strides, const int32_t *refused,
+                          void *stream);
 
 /* Slot i continues as slot parent[i] was (-1: it is dropped).  Full pages are
  * shared; a last page that is not full stays with the lowest slot of its parent,

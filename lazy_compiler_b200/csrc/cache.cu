@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(256) copy_kernel(CopyParams p) {
 struct WriteParams {
   const char *k, *v;
   char *k_pages, *v_pages;
-  const int *table, *lens, *add;
+  const int *table, *lens, *add, *refused;  // refused: null, or a word; nothing is written where it is not 0
   int slots, most, width, pages, page_size, heads;
   int64_t row_bytes;              // head_dim elements
   int64_t ks[3], vs[3];           // byte strides of the new tokens: slot, token, head
@@ -549,9 +549,10 @@ __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
   pdl_wait();
   pdl_trigger();
   const int slot = blockIdx.y;
+  const int refused = p.refused ? *p.refused : 0;
   const int add = min(max(p.add[slot], 0), p.most);
   const int first = blockIdx.x * kWriteTokens;
-  if (first >= add) return;
+  if (first >= add || refused) return;
   const int64_t start = (int64_t)p.lens[slot] - p.add[slot];
   if (start < 0) return;
   constexpr int V = sizeof(Vec);
@@ -652,10 +653,10 @@ extern "C" int lc_cache_extend(const int32_t *table_in, int32_t *table_out, cons
   return launch_maps(me, extend_kernel, slots * width + pages, s, p);
 }
 
-extern "C" int lc_cache_write(const void *k, const void *v, void *k_pages, void *v_pages, const int32_t *table,
-                              const int32_t *lens, const int32_t *add, int64_t slots, int64_t most, int64_t width,
-                              int64_t pages, int64_t page_size, int64_t kv_heads, int64_t row_bytes,
-                              const int64_t *strides, void *stream) {
+extern "C" int lc_cache_write_unless(const void *k, const void *v, void *k_pages, void *v_pages, const int32_t *table,
+                                     const int32_t *lens, const int32_t *add, int64_t slots, int64_t most, int64_t width,
+                                     int64_t pages, int64_t page_size, int64_t kv_heads, int64_t row_bytes,
+                                     const int64_t *strides, const int32_t *refused, void *stream) {
   using namespace lc;
   const char *me = "lc_cache_write";
   if (int rc = check_maps(me, slots, width, pages, page_size)) return rc;
@@ -666,13 +667,21 @@ extern "C" int lc_cache_write(const void *k, const void *v, void *k_pages, void 
   if (slots == 0 || most == 0 || width == 0 || pages == 0) return LC_OK;
   if (!k || !v || !k_pages || !v_pages || !table || !lens || !add) return fail(LC_ERR_INVALID, "%s: null buffer", me);
   WriteParams p = {static_cast<const char *>(k), static_cast<const char *>(v), static_cast<char *>(k_pages), static_cast<char *>(v_pages),
-                   table, lens, add, (int)slots, (int)most, (int)width, (int)pages, (int)page_size, (int)kv_heads, row_bytes, {}, {}, {}, {}};
+                   table, lens, add, refused, (int)slots, (int)most, (int)width, (int)pages, (int)page_size, (int)kv_heads, row_bytes, {}, {}, {}, {}};
   for (int i = 0; i < 3; ++i) p.ks[i] = strides[i], p.vs[i] = strides[3 + i], p.kp[i] = strides[6 + i], p.vp[i] = strides[9 + i];
   const bool wide = aligned(k, 16) && aligned(v, 16) && aligned(k_pages, 16) && aligned(v_pages, 16) &&
                     row_bytes % 16 == 0 && all_multiple(strides, 12, 16);
   const dim3 grid((unsigned)((most + kWriteTokens - 1) / kWriteTokens), (unsigned)slots);
   cudaStream_t s = as_stream(stream);
   return check_cuda(wide ? launch_pdl(write_kernel<uint4>, grid, dim3(256), 0, s, p) : launch_pdl(write_kernel<uint8_t>, grid, dim3(256), 0, s, p), me);
+}
+
+extern "C" int lc_cache_write(const void *k, const void *v, void *k_pages, void *v_pages, const int32_t *table,
+                              const int32_t *lens, const int32_t *add, int64_t slots, int64_t most, int64_t width,
+                              int64_t pages, int64_t page_size, int64_t kv_heads, int64_t row_bytes,
+                              const int64_t *strides, void *stream) {
+  return lc_cache_write_unless(k, v, k_pages, v_pages, table, lens, add, slots, most, width, pages, page_size, kv_heads, row_bytes,
+                               strides, nullptr, stream);
 }
 
 extern "C" int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes, const int64_t *strides,

@@ -24,7 +24,7 @@ struct Entries {
   decltype(&lc_window_attention) window_attention;
   decltype(&lc_paged_decode) paged_decode;
   decltype(&lc_cache_extend) cache_extend;
-  decltype(&lc_cache_write) cache_write;
+  decltype(&lc_cache_write_unless) cache_write;
   decltype(&lc_cache_fork) cache_fork;
   decltype(&lc_cache_release) cache_release;
   decltype(&lc_cache_compact) cache_compact;
@@ -324,7 +324,8 @@ PyObject *cache_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
   }
   const c10::cuda::CUDAGuard guard(m.table.device());
   return PyLong_FromLong(lib.cache_write(ptr(k), ptr(v), ptr(kp), ptr(vp), ptr<int32_t>(m.table), ptr<int32_t>(m.lens), ptr<int32_t>(add),
-                                         m.slots, most, m.width, m.pages, page_size, heads, d * size, strides, stream_of(a[9], m.table)));
+                                         m.slots, most, m.width, m.pages, page_size, heads, d * size, strides,
+                                         m.status.defined() ? ptr<int32_t>(m.status) : nullptr, stream_of(a[9], m.table)));
   END_HANDLE_TH_ERRORS
 }
 

@@ -29,8 +29,8 @@ import torch
 from . import runtime
 
 # the order in which csrc/serving_ext.cpp takes the entry points
-_ENTRIES = ("lc_window_attention", "lc_paged_decode", "lc_cache_extend", "lc_cache_write", "lc_cache_fork", "lc_cache_release",
-            "lc_cache_compact", "lc_cache_copy")
+_ENTRIES = ("lc_window_attention", "lc_paged_decode", "lc_cache_extend", "lc_cache_write_unless", "lc_cache_fork",
+            "lc_cache_release", "lc_cache_compact", "lc_cache_copy")
 
 
 def _extension():
@@ -113,7 +113,8 @@ def cache_extend(maps: CacheMaps, add, *, page_size: int, into: CacheMaps | None
 def cache_write(k, v, k_pages, v_pages, maps: CacheMaps, add, *, stream: int | None = None) -> None:
     """Writes the newest ``add[i]`` tokens of every slot, ``k, v[slots, most, kv_heads, d]``, to the positions
     ``lens[i] - add[i]`` and on (``maps`` as :func:`cache_extend` left them).  ``k_pages, v_pages[pages, kv_heads,
-    page_size, d]`` are planes of the pool; any element type."""
+    page_size, d]`` are planes of the pool; any element type.  Where ``maps.status[0]`` is not 0 (room was refused, and
+    ``lens`` did not grow) nothing is written: the positions are those of tokens that are there."""
     status = _ext.cache_write(k, v, k_pages, v_pages, *maps, add, stream)
     if status:
         raise _failed("lc_cache_write", status)

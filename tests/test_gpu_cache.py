@@ -320,3 +320,29 @@ def test_refusals_of_maps(cuda_device):
     for call, kind, text in refused:
         with pytest.raises(kind, match=text):
             call()
+
+
+def test_nothing_is_written_after_a_refused_extend(cuda_device):
+    """Where room was refused the newest positions are those of older tokens, some of them in pages that samples share."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    cache = S.PagedCache(1, 6, 4, 1, 16, 3, 8, dtype=torch.float16)
+    cache.extend(ints([8, 0, 12]))
+    old, new = (torch.full((3, 12, 1, 16), x, dtype=torch.float16, device="cuda") for x in (1.0, 2.0))
+    cache.write(0, old, old, ints([8, 0, 12]))
+    cache.fork(ints([0, 0, 2]))  # 5 pages of 6 in use, 2 of them by two slots
+    assert cache.check() == 1
+    before = cache.pool.clone()
+    one = ints([1, 1, 1])
+    refused = S.cache_extend(cache.maps, one, page_size=4)  # 3 pages wanted
+    assert refused.status.tolist() == [2, 1]
+    S.cache_write(new, new, cache.pool[0], cache.pool[1], refused, one)
+    cache.extend(one)
+    cache.write(0, new[:, :1], new[:, :1], one)
+    assert torch.equal(cache.pool, before)
+    with pytest.raises(RuntimeError, match="2 pages are missing"):
+        cache.check()
+    one = ints([0, 1, 0])
+    cache.extend(one)
+    cache.write(0, new[:, :1], new[:, :1], one)
+    assert cache.check() == 0 and int((cache.pool != before).sum()) == 2 * 16
