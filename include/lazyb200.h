@@ -667,6 +667,12 @@ int lc_cache_extend(const int32_t *table_in, int32_t *table_out, const int32_t *
                     int32_t *lens_out, const int32_t *refs_in, int32_t *refs_out, const int32_t *add,
                     int32_t *status, int64_t slots, int64_t width, int64_t pages, int64_t page_size,
                     void *stream);
+/* The same, for a loop that does not look at each status: a status[0] that is not 0 also goes to refusals[0]
+ * (device, two words; null: as above) where that is still 0, and every call's to refusals[1]. */
+int lc_cache_extend_recorded(const int32_t *table_in, int32_t *table_out, const int32_t *lens_in,
+                             int32_t *lens_out, const int32_t *refs_in, int32_t *refs_out,
+                             const int32_t *add, int32_t *status, int32_t *refusals, int64_t slots,
+                             int64_t width, int64_t pages, int64_t page_size, void *stream);
 
 /* Writes the keys and values of the newest add[i] <= most tokens of each slot
  * (k, v [slots, most, kv_heads, row_bytes]) to positions lens[i] - add[i] and on.
@@ -677,7 +683,7 @@ int lc_cache_write(const void *k, const void *v, void *k_pages, void *v_pages, c
                    int64_t pages, int64_t page_size, int64_t kv_heads, int64_t row_bytes,
                    const int64_t *strides, void *stream);
 /* The same, but nothing is written where the device word *refused is not 0 (null: as above): with the status
- * of the lc_cache_extend before it, the tokens that found no room do not overwrite the newest ones there are. */
+ * of the lc_cache_extend before it, or its refusals[1], the tokens that found no room do not overwrite the newest ones there are. */
 int lc_cache_write_unless(const void *k, const void *v, void *k_pages, void *v_pages, const int32_t *table,
                           const int32_t *lens, const int32_t *add, int64_t slots, int64_t most,
                           int64_t width, int64_t pages, int64_t page_size, int64_t kv_heads,
@@ -694,6 +700,13 @@ int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64_t token_by
                   const int32_t *lens_in, int32_t *lens_out, const int32_t *refs_in, int32_t *refs_out,
                   const int32_t *parent, int32_t *status, int64_t slots, int64_t width, int64_t pages,
                   int64_t page_size, void *stream);
+/* The same; a status[0] that is not 0 also goes to refusals[0] (device; null: as above) where that is still 0. */
+int lc_cache_fork_recorded(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes,
+                           const int64_t *strides, const int32_t *table_in, int32_t *table_out,
+                           const int32_t *lens_in, int32_t *lens_out, const int32_t *refs_in,
+                           int32_t *refs_out, const int32_t *parent, int32_t *status,
+                           int32_t *refusals, int64_t slots, int64_t width, int64_t pages,
+                           int64_t page_size, void *stream);
 
 /* Gives pages back, in place: of every slot with gone[i] != 0, which is empty
  * afterwards; or, gone null, the pages that no position from lens[i] on sees

@@ -118,6 +118,7 @@ __device__ __forceinline__ void before_and_total(cg::cluster_group &cluster, int
 struct ExtendParams {
   const int *table_in, *lens_in, *refs_in, *add;
   int *table_out, *lens_out, *refs_out, *status;
+  int *refusals;        // null, or the first refusal and the last call's
   int *offsets, *list;  // scratch: each slot's first new page in `list`, the pages taken
   int slots, width, pages, page_size;
 };
@@ -192,8 +193,13 @@ __global__ void __launch_bounds__(kMostThreads, 1) extend_kernel(ExtendParams p)
     if (lane == 0) p.lens_out[i] = fits ? len + more : p.lens_in[i];
   }
   if (rank == 0 && tid == 0) {
-    p.status[0] = wide ? -1 : fits ? 0 : need - total_free;
+    const int code = wide ? -1 : fits ? 0 : need - total_free;
+    p.status[0] = code;
     p.status[1] = total_free - take;
+    if (p.refusals) {
+      if (code != 0 && p.refusals[0] == 0) p.refusals[0] = code;
+      p.refusals[1] = code;
+    }
   }
 }
 
@@ -209,7 +215,8 @@ constexpr int kMostForkSlots = 8192;
 struct ForkParams {
   const int *table_in, *lens_in, *refs_in, *parent;
   int *table_out, *lens_out, *refs_out, *status;
-  int *list;  // scratch: the pages taken
+  int *refusals;  // null, or the first refusal
+  int *list;      // scratch: the pages taken
   CopyList copies;
   int slots, width, pages, page_size;
 };
@@ -322,8 +329,10 @@ __global__ void __launch_bounds__(kMostThreads, 1) fork_kernel(ForkParams p) {
     before_and_total(cluster, &free_here, before, total_free);
   }
   if (rank == 0 && tid == 0) {
-    p.status[0] = bad ? -1 : fits ? 0 : short_by;
+    const int code = bad ? -1 : fits ? 0 : short_by;
+    p.status[0] = code;
     p.status[1] = fits ? total_free - need : total_free;
+    if (p.refusals && code != 0 && p.refusals[0] == 0) p.refusals[0] = code;
     *p.copies.count = fits ? need : 0;
   }
   cluster.sync();  // no CTA leaves while its shared memory is read
@@ -635,9 +644,10 @@ int launch_copy(const char *me, const CopyParams &p, int64_t most_pairs, cudaStr
 }  // namespace
 }  // namespace lc
 
-extern "C" int lc_cache_extend(const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
-                               const int32_t *refs_in, int32_t *refs_out, const int32_t *add, int32_t *status,
-                               int64_t slots, int64_t width, int64_t pages, int64_t page_size, void *stream) {
+extern "C" int lc_cache_extend_recorded(const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
+                                        const int32_t *refs_in, int32_t *refs_out, const int32_t *add, int32_t *status,
+                                        int32_t *refusals, int64_t slots, int64_t width, int64_t pages, int64_t page_size,
+                                        void *stream) {
   using namespace lc;
   const char *me = "lc_cache_extend";
   if (int rc = check_maps(me, slots, width, pages, page_size)) return rc;
@@ -648,9 +658,16 @@ extern "C" int lc_cache_extend(const int32_t *table_in, int32_t *table_out, cons
   void *scratch = nullptr;
   if (int rc = scratch_buffer(s, kScratchSlot, (size_t)(slots + pages + 1) * 4, &scratch)) return rc;
   int *ints = static_cast<int *>(scratch);
-  const ExtendParams p = {table_in, lens_in, refs_in, add, table_out, lens_out, refs_out, status, ints, ints + slots,
+  const ExtendParams p = {table_in, lens_in, refs_in, add, table_out, lens_out, refs_out, status, refusals, ints, ints + slots,
                           (int)slots, (int)width, (int)pages, (int)page_size};
   return launch_maps(me, extend_kernel, slots * width + pages, s, p);
+}
+
+extern "C" int lc_cache_extend(const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
+                               const int32_t *refs_in, int32_t *refs_out, const int32_t *add, int32_t *status,
+                               int64_t slots, int64_t width, int64_t pages, int64_t page_size, void *stream) {
+  return lc_cache_extend_recorded(table_in, table_out, lens_in, lens_out, refs_in, refs_out, add, status, nullptr, slots, width, pages,
+                                  page_size, stream);
 }
 
 extern "C" int lc_cache_write_unless(const void *k, const void *v, void *k_pages, void *v_pages, const int32_t *table,
@@ -684,10 +701,11 @@ extern "C" int lc_cache_write(const void *k, const void *v, void *k_pages, void 
                                strides, nullptr, stream);
 }
 
-extern "C" int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes, const int64_t *strides,
-                             const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
-                             const int32_t *refs_in, int32_t *refs_out, const int32_t *parent, int32_t *status,
-                             int64_t slots, int64_t width, int64_t pages, int64_t page_size, void *stream) {
+extern "C" int lc_cache_fork_recorded(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes, const int64_t *strides,
+                                      const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
+                                      const int32_t *refs_in, int32_t *refs_out, const int32_t *parent, int32_t *status,
+                                      int32_t *refusals, int64_t slots, int64_t width, int64_t pages, int64_t page_size,
+                                      void *stream) {
   using namespace lc;
   const char *me = "lc_cache_fork";
   if (int rc = check_maps(me, slots, width, pages, page_size)) return rc;
@@ -703,13 +721,21 @@ extern "C" int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64
   void *scratch = nullptr;
   if (int rc = scratch_buffer(s, kScratchSlot, (size_t)(4 * slots + 1) * 4, &scratch)) return rc;
   int *ints = static_cast<int *>(scratch);
-  ForkParams p = {table_in, lens_in, refs_in, parent, table_out, lens_out, refs_out, status, ints + 1,
+  ForkParams p = {table_in, lens_in, refs_in, parent, table_out, lens_out, refs_out, status, refusals, ints + 1,
                   {ints, ints + 1 + slots, ints + 1 + 2 * slots, ints + 1 + 3 * slots},
                   (int)slots, (int)width, (int)pages, (int)page_size};
   if (int rc = launch_maps(me, fork_kernel, slots * width + pages, s, p)) return rc;
   if (planes == 0 || pages == 0 || slots == 0) return LC_OK;
   c.src = p.copies.src, c.dst = p.copies.dst, c.tokens = p.copies.tokens, c.count = p.copies.count;
   return launch_copy(me, c, slots, s);
+}
+
+extern "C" int lc_cache_fork(void *pool, int64_t planes, int64_t kv_heads, int64_t token_bytes, const int64_t *strides,
+                             const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
+                             const int32_t *refs_in, int32_t *refs_out, const int32_t *parent, int32_t *status,
+                             int64_t slots, int64_t width, int64_t pages, int64_t page_size, void *stream) {
+  return lc_cache_fork_recorded(pool, planes, kv_heads, token_bytes, strides, table_in, table_out, lens_in, lens_out, refs_in, refs_out,
+                                parent, status, nullptr, slots, width, pages, page_size, stream);
 }
 
 extern "C" int lc_cache_release(int32_t *table, int32_t *lens, int32_t *refs, const int32_t *gone, int64_t window,

@@ -23,9 +23,9 @@ namespace {
 struct Entries {
   decltype(&lc_window_attention) window_attention;
   decltype(&lc_paged_decode) paged_decode;
-  decltype(&lc_cache_extend) cache_extend;
+  decltype(&lc_cache_extend_recorded) cache_extend;
   decltype(&lc_cache_write_unless) cache_write;
-  decltype(&lc_cache_fork) cache_fork;
+  decltype(&lc_cache_fork_recorded) cache_fork;
   decltype(&lc_cache_release) cache_release;
   decltype(&lc_cache_compact) cache_compact;
   decltype(&lc_cache_copy) cache_copy;
@@ -261,6 +261,12 @@ Maps into_of(const Maps &m, PyObject *const *a) {
   if (!to.status.defined()) to.status = fresh({2}, at::kInt, m.table);
   return to;
 }
+// The words of a refusal (null where there are none).
+int32_t *refusals_of(PyObject *o, const Maps &m) {
+  const at::Tensor *t = maybe(o, "refusals");
+  if (t) check_ints(*t, "refusals", m.table, {2});
+  return ptr<int32_t>(t);
+}
 PyObject *wrapped(const Maps &m) {
   PyObject *parts[4] = {THPVariable_Wrap(m.table), THPVariable_Wrap(m.lens), THPVariable_Wrap(m.refs), THPVariable_Wrap(m.status)};
   PyObject *all = PyTuple_Pack(4, parts[0], parts[1], parts[2], parts[3]);
@@ -282,26 +288,26 @@ Pool pool_of(const at::Tensor &t, const at::Tensor &like, int64_t pages) {
   return {ptr(t), t.size(0), t.size(2), t.size(3), t.size(4) * size, {t.stride(0) * size, t.stride(1) * size, t.stride(2) * size}};
 }
 
-// maps (4), add, page_size, into (4), stream
+// maps (4), add, page_size, into (4), refusals, stream
 PyObject *cache_extend(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 11);
+  arguments(n, 12);
   const Maps m = maps_of(a, "maps");
   const at::Tensor &add = tensor(a[4], "add");
   check_ints(add, "add", m.table, {m.slots});
   const c10::cuda::CUDAGuard guard(m.table.device());
   const Maps to = into_of(m, a + 6);
   const int status = lib.cache_extend(ptr<int32_t>(m.table), ptr<int32_t>(to.table), ptr<int32_t>(m.lens), ptr<int32_t>(to.lens),
-                                      ptr<int32_t>(m.refs), ptr<int32_t>(to.refs), ptr<int32_t>(add), ptr<int32_t>(to.status), m.slots,
-                                      m.width, m.pages, integer(a[5]), stream_of(a[10], m.table));
+                                      ptr<int32_t>(m.refs), ptr<int32_t>(to.refs), ptr<int32_t>(add), ptr<int32_t>(to.status),
+                                      refusals_of(a[10], m), m.slots, m.width, m.pages, integer(a[5]), stream_of(a[11], m.table));
   return status ? PyLong_FromLong(status) : wrapped(to);
   END_HANDLE_TH_ERRORS
 }
 
-// k, v, k_pages, v_pages, maps (4), add, stream
+// k, v, k_pages, v_pages, maps (4), add, refusals, stream
 PyObject *cache_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 10);
+  arguments(n, 11);
   const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &kp = tensor(a[2], "k_pages"), &vp = tensor(a[3], "v_pages");
   const Maps m = maps_of(a + 4, "maps");
   const at::Tensor &add = tensor(a[8], "add");
@@ -322,17 +328,20 @@ PyObject *cache_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
     check_inner(*views[x], names[x]);
     for (int i = 0; i < 3; ++i) strides[x * 3 + i] = views[x]->stride(i) * size;
   }
+  // whether room was refused: the last extend's word, else the maps' own status
+  const int32_t *refused = refusals_of(a[9], m);
+  refused = refused ? refused + 1 : m.status.defined() ? ptr<int32_t>(m.status) : nullptr;
   const c10::cuda::CUDAGuard guard(m.table.device());
   return PyLong_FromLong(lib.cache_write(ptr(k), ptr(v), ptr(kp), ptr(vp), ptr<int32_t>(m.table), ptr<int32_t>(m.lens), ptr<int32_t>(add),
                                          m.slots, most, m.width, m.pages, page_size, heads, d * size, strides,
-                                         m.status.defined() ? ptr<int32_t>(m.status) : nullptr, stream_of(a[9], m.table)));
+                                         refused, stream_of(a[10], m.table)));
   END_HANDLE_TH_ERRORS
 }
 
-// pool, maps (4), parent, into (4), stream
+// pool, maps (4), parent, into (4), refusals, stream
 PyObject *cache_fork(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 11);
+  arguments(n, 12);
   const Maps m = maps_of(a + 1, "maps");
   const Pool pool = pool_of(tensor(a[0], "pool"), m.table, m.pages);
   const at::Tensor &parent = tensor(a[5], "parent");
@@ -341,8 +350,8 @@ PyObject *cache_fork(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Maps to = into_of(m, a + 6);
   const int status = lib.cache_fork(pool.data, pool.planes, pool.heads, pool.token_bytes, pool.strides, ptr<int32_t>(m.table),
                                     ptr<int32_t>(to.table), ptr<int32_t>(m.lens), ptr<int32_t>(to.lens), ptr<int32_t>(m.refs),
-                                    ptr<int32_t>(to.refs), ptr<int32_t>(parent), ptr<int32_t>(to.status), m.slots, m.width, m.pages,
-                                    pool.page_size, stream_of(a[10], m.table));
+                                    ptr<int32_t>(to.refs), ptr<int32_t>(parent), ptr<int32_t>(to.status), refusals_of(a[10], m),
+                                    m.slots, m.width, m.pages, pool.page_size, stream_of(a[11], m.table));
   return status ? PyLong_FromLong(status) : wrapped(to);
   END_HANDLE_TH_ERRORS
 }

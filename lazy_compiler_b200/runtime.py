@@ -75,9 +75,11 @@ SIGNATURES = {
     "lc_window_attention": [_INT] + [_P] * 7 + [_I64] * 6 + [_P, _I64, _I64, ctypes.c_float, _P],
     "lc_paged_decode": [_INT] + [_P] * 7 + [_I64] * 7 + [_P, _I64, _I64, ctypes.c_float, _P],
     "lc_cache_extend": [_P] * 8 + [_I64] * 4 + [_P],
+    "lc_cache_extend_recorded": [_P] * 9 + [_I64] * 4 + [_P],
     "lc_cache_write": [_P] * 7 + [_I64] * 7 + [_P, _P],
     "lc_cache_write_unless": [_P] * 7 + [_I64] * 7 + [_P, _P, _P],
     "lc_cache_fork": [_P, _I64, _I64, _I64, _P] + [_P] * 8 + [_I64] * 4 + [_P],
+    "lc_cache_fork_recorded": [_P, _I64, _I64, _I64, _P] + [_P] * 9 + [_I64] * 4 + [_P],
     "lc_cache_release": [_P] * 4 + [_I64, _I64, _P] + [_I64] * 4 + [_P],
     "lc_cache_compact": [_P, _I64, _I64, _I64, _P] + [_P] * 7 + [_I64] * 4 + [_P],
     "lc_cache_copy": [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P],

@@ -29,8 +29,8 @@ import torch
 from . import runtime
 
 # the order in which csrc/serving_ext.cpp takes the entry points
-_ENTRIES = ("lc_window_attention", "lc_paged_decode", "lc_cache_extend", "lc_cache_write_unless", "lc_cache_fork",
-            "lc_cache_release", "lc_cache_compact", "lc_cache_copy")
+_ENTRIES = ("lc_window_attention", "lc_paged_decode", "lc_cache_extend_recorded", "lc_cache_write_unless",
+            "lc_cache_fork_recorded", "lc_cache_release", "lc_cache_compact", "lc_cache_copy")
 
 
 def _extension():
@@ -99,35 +99,39 @@ def paged_decode(q, k_pages, v_pages, table, lens, *, window: int = 0, sinks: in
 _NONE = (None, None, None, None)
 
 
-def cache_extend(maps: CacheMaps, add, *, page_size: int, into: CacheMaps | None = None, stream: int | None = None) -> CacheMaps:
+def cache_extend(maps: CacheMaps, add, *, page_size: int, into: CacheMaps | None = None, refusals=None,
+                 stream: int | None = None) -> CacheMaps:
     """Room for ``add[slots]`` more tokens: pages are taken (the lowest free ones, in slot order) and ``lens`` grow.
 
-    All or nothing: where pages or table columns are missing, the maps stay as they are and ``status`` says so.
+    All or nothing: where pages or table columns are missing, the maps stay as they are and ``status`` says so.  The
+    next operation writes another status; ``refusals[2]`` (int32 on the device) keeps the first one that was not 0 in
+    ``refusals[0]`` until the caller clears it, and that of the last extension in ``refusals[1]``.
     """
-    r = _ext.cache_extend(*maps, add, page_size, *(into or _NONE), stream)
+    r = _ext.cache_extend(*maps, add, page_size, *(into or _NONE), refusals, stream)
     if type(r) is int:
         raise _failed("lc_cache_extend", r)
     return CacheMaps(*r)
 
 
-def cache_write(k, v, k_pages, v_pages, maps: CacheMaps, add, *, stream: int | None = None) -> None:
+def cache_write(k, v, k_pages, v_pages, maps: CacheMaps, add, *, refusals=None, stream: int | None = None) -> None:
     """Writes the newest ``add[i]`` tokens of every slot, ``k, v[slots, most, kv_heads, d]``, to the positions
     ``lens[i] - add[i]`` and on (``maps`` as :func:`cache_extend` left them).  ``k_pages, v_pages[pages, kv_heads,
-    page_size, d]`` are planes of the pool; any element type.  Where ``maps.status[0]`` is not 0 (room was refused, and
-    ``lens`` did not grow) nothing is written: the positions are those of tokens that are there."""
-    status = _ext.cache_write(k, v, k_pages, v_pages, *maps, add, stream)
+    page_size, d]`` are planes of the pool; any element type.  Where ``refusals[1]``, or without them ``maps.status[0]``, is
+    not 0 (room was refused, and ``lens`` did not grow) nothing is written: the positions are those of tokens that are
+    there."""
+    status = _ext.cache_write(k, v, k_pages, v_pages, *maps, add, refusals, stream)
     if status:
         raise _failed("lc_cache_write", status)
 
 
-def cache_fork(pool, maps: CacheMaps, parent, *, into: CacheMaps | None = None, stream: int | None = None) -> CacheMaps:
+def cache_fork(pool, maps: CacheMaps, parent, *, into: CacheMaps | None = None, refusals=None, stream: int | None = None) -> CacheMaps:
     """Slot ``i`` goes on as slot ``parent[i]`` was (-1: it is dropped): samples of one prompt, or beams that reorder.
 
     Full pages are shared.  A last page that is not full stays with the lowest slot of its parent; the others get a
     page of their own (the lowest free ones, in slot order) with its tokens.  All or nothing, as :func:`cache_extend`;
-    the new maps may not be the old ones.
+    the new maps may not be the old ones.  ``refusals[0]`` is kept as there.
     """
-    r = _ext.cache_fork(pool, *maps, parent, *(into or _NONE), stream)
+    r = _ext.cache_fork(pool, *maps, parent, *(into or _NONE), refusals, stream)
     if type(r) is int:
         raise _failed("lc_cache_fork", r)
     return CacheMaps(*r)
@@ -171,7 +175,7 @@ class PagedCache:
 
     ``pool[2 * layers, pages, kv_heads, page_size, head_dim]`` holds layer ``l``'s keys in plane ``2 l`` and its values
     in plane ``2 l + 1``; ``maps`` are its :class:`CacheMaps`.  Every method works on the device, in stream order;
-    :meth:`check` waits for it and raises where an operation could not be done.
+    :meth:`check` waits for it and raises where one could not be done since the check before.
     """
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, slots: int, width: int,
@@ -184,14 +188,16 @@ class PagedCache:
         self.maps, self._spare = (CacheMaps(torch.full((slots, width), -1, **ints), torch.zeros(slots, **ints),
                                             torch.zeros(pages, **ints), torch.zeros(2, **ints)) for _ in range(2))
         self.maps.status[1] = pages
+        self._refusals = torch.zeros(2, **ints)
 
     def extend(self, add, stream=None) -> None:
         """Room for ``add[slots]`` more tokens (:func:`cache_extend`)."""
-        cache_extend(self.maps, add, page_size=self.page_size, into=self.maps, stream=stream)
+        cache_extend(self.maps, add, page_size=self.page_size, into=self.maps, refusals=self._refusals, stream=stream)
 
     def write(self, layer: int, k, v, add, stream=None) -> None:
-        """The newest tokens' keys and values of one layer (:func:`cache_write`)."""
-        cache_write(k, v, self.pool[2 * layer], self.pool[2 * layer + 1], self.maps, add, stream=stream)
+        """The newest tokens' keys and values of one layer (:func:`cache_write`); nothing where the last
+        :meth:`extend` was refused."""
+        cache_write(k, v, self.pool[2 * layer], self.pool[2 * layer + 1], self.maps, add, refusals=self._refusals, stream=stream)
 
     def decode(self, layer: int, q, **options):
         """Attention of one new token per slot in one layer (:func:`paged_decode`)."""
@@ -199,7 +205,7 @@ class PagedCache:
 
     def fork(self, parent, stream=None) -> None:
         """Slots continue others (:func:`cache_fork`).  The maps are other tensors afterwards."""
-        cache_fork(self.pool, self.maps, parent, into=self._spare, stream=stream)
+        cache_fork(self.pool, self.maps, parent, into=self._spare, refusals=self._refusals, stream=stream)
         self.maps, self._spare = self._spare, self.maps
 
     def release(self, gone, stream=None) -> None:
@@ -215,9 +221,12 @@ class PagedCache:
         cache_compact(self.pool, self.maps, into=self.maps, stream=stream)
 
     def check(self) -> int:
-        """Waits for the last operation on the maps; the pages free after it, or an error where it was refused."""
-        code, free = self.maps.status.tolist()
+        """Waits for the last operation on the maps; the pages free after it.  Raises where an operation could not be
+        done, the first of them since the last check, whatever came after it."""
+        code, free, refused, _ = torch.cat((self.maps.status, self._refusals)).tolist()
+        code = refused or code
         if code:
+            self._refusals[0] = 0
             what = "an argument is out of range" if code < 0 else f"{code} pages are missing"
-            raise RuntimeError(f"the cache is unchanged: {what} ({free} pages are free)")
+            raise RuntimeError(f"an operation was refused and changed nothing: {what} ({free} pages are free)")
         return free

@@ -346,3 +346,69 @@ def test_nothing_is_written_after_a_refused_extend(cuda_device):
     cache.extend(one)
     cache.write(0, new[:, :1], new[:, :1], one)
     assert cache.check() == 0 and int((cache.pool != before).sum()) == 2 * 16
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_refusal_is_told_whatever_came_after_it(captured, cuda_device):
+    """A loop that looks at its steps' end only: the refused step's tokens are written nowhere, and check() says so."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    cache = S.PagedCache(1, 7, 4, 1, 16, 3, 8, dtype=torch.float16)
+    side = torch.cuda.Stream()
+    start = ints([8, 0, 12])
+    old, new = (torch.full((3, 12, 1, 16), x, dtype=torch.float16, device="cuda") for x in (1.0, 2.0))
+    add, gone = ints([0, 0, 0]), ints([0, 0, 1])
+
+    def step():
+        cache.extend(add)
+        cache.trim(100)
+        cache.write(0, new[:, :1], new[:, :1], add)
+        cache.release(gone)
+        cache.compact()
+
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.extend(start)
+        cache.write(0, old, old, start)
+        cache.fork(ints([0, 0, 2]))
+        gone.zero_()
+        step()
+        run = step
+        if captured:
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                step()
+            run = graph.replay
+        assert cache.check() == 2
+        before, table = cache.pool.clone(), cache.maps.table.clone()
+        add.copy_(ints([1, 1, 1]))  # a page each, and 2 are free
+        run()
+        assert torch.equal(cache.pool, before) and torch.equal(cache.maps.table, table) and cache.maps.status.tolist() == [0, 2]
+        add.copy_(ints([0, 1, 0]))  # this one fits
+        gone.copy_(ints([0, 0, 1]))
+        run()
+        assert cache.maps.lens.tolist() == [8, 9, 0]
+        with pytest.raises(RuntimeError, match="1 pages are missing"):
+            cache.check()
+        assert cache.check() == 4
+
+
+def test_a_refused_fork_is_told_too(cuda_device):
+    import torch
+    from lazy_compiler_b200 import serving as S
+    cache = S.PagedCache(1, 2, 4, 1, 16, 4, 2, dtype=torch.float16)
+    cache.extend(ints([3, 0, 0, 0]))
+    cache.fork(ints([0, 0, 0, 0]))
+    cache.fork(ints([0, -1, -1, 7]))
+    cache.trim(1)
+    with pytest.raises(RuntimeError, match="2 pages are missing"):
+        cache.check()
+    assert cache.check() == 1 and cache.maps.lens.tolist() == [3, 0, 0, 0]
+    refusals = ints([0, 0])
+    first = S.cache_extend(cache.maps, ints([9, 0, 0, 0]), page_size=4, refusals=refusals)
+    S.cache_extend(cache.maps, ints([1, 8, 0, 0]), page_size=4, refusals=refusals)
+    S.cache_fork(cache.pool, cache.maps, ints([0, 0, 0, 0]), refusals=refusals)
+    assert first.status.tolist() == [-1, 1] and refusals.tolist() == [-1, 1]
+    with pytest.raises(ValueError, match="refusals: shape"):
+        S.cache_extend(cache.maps, ints([0, 0, 0, 0]), page_size=4, refusals=refusals[:1])
