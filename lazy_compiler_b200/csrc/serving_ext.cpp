@@ -112,10 +112,18 @@ int attention_dtype(const at::Tensor &q) {
   return q.scalar_type() == at::kHalf ? LC_F16 : LC_BF16;
 }
 
-void *stream_of(PyObject *o, const at::Tensor &t) {
-  if (o == Py_None) return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
-  return reinterpret_cast<void *>(static_cast<intptr_t>(integer(o)));
-}
+// Makes the stream of a call current (None: the device's current one), so that what the call
+// allocates is memory of the stream that it runs on: of another one, work queued there could
+// still use the block, or be given it before this call has run.
+struct On {
+  c10::cuda::CUDAGuard device;
+  c10::cuda::OptionalCUDAStreamGuard given;
+  void *stream;
+  On(PyObject *o, const at::Tensor &t) : device(t.device()) {
+    if (o != Py_None) given.reset_stream(c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(static_cast<intptr_t>(integer(o))), t.get_device()));
+    stream = c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+  }
+};
 // An uninitialised tensor on the device of `like`, without the dispatcher's way there.
 at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Tensor &like) {
   return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
@@ -168,7 +176,7 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (q_lens) check_ints(*q_lens, "q_lens", q, {batch});
   if (kv_lens) check_ints(*kv_lens, "kv_lens", q, {batch});
   if (given) check(*given, "out", q, q.scalar_type(), {batch, s_q, heads, d}), check_out(*given, "out");
-  const c10::cuda::CUDAGuard guard(q.device());
+  const On on(a[10], q);
   const at::Tensor out = given ? *given : fresh({batch, s_q, heads, d}, q.scalar_type(), q);
   const at::Tensor lse = truth(a[9]) ? fresh({batch, heads, s_q}, at::kFloat, q) : at::Tensor();
   const at::Tensor *views[4] = {&q, &k, &v, &out};
@@ -180,7 +188,7 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   }
   const int status = lib.window_attention(dtype, ptr(q), ptr(k), ptr(v), ptr(out), lse.defined() ? ptr<float>(lse) : nullptr,
                                           ptr<int32_t>(q_lens), ptr<int32_t>(kv_lens), batch, s_q, s_kv, heads, kv_heads, d, strides,
-                                          integer(a[3]), integer(a[4]), scale_of(a[5], d), stream_of(a[10], q));
+                                          integer(a[3]), integer(a[4]), scale_of(a[5], d), on.stream);
   if (status) return PyLong_FromLong(status);
   return outputs(out, a[8], lse);
   END_HANDLE_TH_ERRORS
@@ -204,7 +212,7 @@ PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
   check_ints(lens, "lens", q, {slots});
   const at::Tensor *given = maybe(a[8], "out");
   if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d}), check_out(*given, "out");
-  const c10::cuda::CUDAGuard guard(q.device());
+  const On on(a[10], q);
   const at::Tensor out = given ? *given : fresh({slots, heads, d}, q.scalar_type(), q);
   const at::Tensor lse = truth(a[9]) ? fresh({slots, heads}, at::kFloat, q) : at::Tensor();
   check_inner(q, "q");
@@ -216,7 +224,7 @@ PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
                                v.stride(1), v.stride(2), out.stride(0), out.stride(1), table.stride(0)};
   const int status = lib.paged_decode(dtype, ptr(q), ptr(k), ptr(v), ptr(out), lse.defined() ? ptr<float>(lse) : nullptr,
                                       ptr<int32_t>(table), ptr<int32_t>(lens), slots, width, pages, page_size, heads, kv_heads, d,
-                                      strides, integer(a[5]), integer(a[6]), scale_of(a[7], d), stream_of(a[10], q));
+                                      strides, integer(a[5]), integer(a[6]), scale_of(a[7], d), on.stream);
   if (status) return PyLong_FromLong(status);
   return outputs(out, a[8], lse);
   END_HANDLE_TH_ERRORS
@@ -295,11 +303,11 @@ PyObject *cache_extend(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Maps m = maps_of(a, "maps");
   const at::Tensor &add = tensor(a[4], "add");
   check_ints(add, "add", m.table, {m.slots});
-  const c10::cuda::CUDAGuard guard(m.table.device());
+  const On on(a[11], m.table);
   const Maps to = into_of(m, a + 6);
   const int status = lib.cache_extend(ptr<int32_t>(m.table), ptr<int32_t>(to.table), ptr<int32_t>(m.lens), ptr<int32_t>(to.lens),
                                       ptr<int32_t>(m.refs), ptr<int32_t>(to.refs), ptr<int32_t>(add), ptr<int32_t>(to.status),
-                                      refusals_of(a[10], m), m.slots, m.width, m.pages, integer(a[5]), stream_of(a[11], m.table));
+                                      refusals_of(a[10], m), m.slots, m.width, m.pages, integer(a[5]), on.stream);
   return status ? PyLong_FromLong(status) : wrapped(to);
   END_HANDLE_TH_ERRORS
 }
@@ -331,10 +339,10 @@ PyObject *cache_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
   // whether room was refused: the last extend's word, else the maps' own status
   const int32_t *refused = refusals_of(a[9], m);
   refused = refused ? refused + 1 : m.status.defined() ? ptr<int32_t>(m.status) : nullptr;
-  const c10::cuda::CUDAGuard guard(m.table.device());
+  const On on(a[10], m.table);
   return PyLong_FromLong(lib.cache_write(ptr(k), ptr(v), ptr(kp), ptr(vp), ptr<int32_t>(m.table), ptr<int32_t>(m.lens), ptr<int32_t>(add),
                                          m.slots, most, m.width, m.pages, page_size, heads, d * size, strides,
-                                         refused, stream_of(a[10], m.table)));
+                                         refused, on.stream));
   END_HANDLE_TH_ERRORS
 }
 
@@ -346,12 +354,12 @@ PyObject *cache_fork(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Pool pool = pool_of(tensor(a[0], "pool"), m.table, m.pages);
   const at::Tensor &parent = tensor(a[5], "parent");
   check_ints(parent, "parent", m.table, {m.slots});
-  const c10::cuda::CUDAGuard guard(m.table.device());
+  const On on(a[11], m.table);
   const Maps to = into_of(m, a + 6);
   const int status = lib.cache_fork(pool.data, pool.planes, pool.heads, pool.token_bytes, pool.strides, ptr<int32_t>(m.table),
                                     ptr<int32_t>(to.table), ptr<int32_t>(m.lens), ptr<int32_t>(to.lens), ptr<int32_t>(m.refs),
                                     ptr<int32_t>(to.refs), ptr<int32_t>(parent), ptr<int32_t>(to.status), refusals_of(a[10], m),
-                                    m.slots, m.width, m.pages, pool.page_size, stream_of(a[11], m.table));
+                                    m.slots, m.width, m.pages, pool.page_size, on.stream);
   return status ? PyLong_FromLong(status) : wrapped(to);
   END_HANDLE_TH_ERRORS
 }
@@ -363,10 +371,10 @@ PyObject *cache_release(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Maps m = maps_of(a, "maps");
   const at::Tensor *gone = maybe(a[4], "gone");
   if (gone) check_ints(*gone, "gone", m.table, {m.slots});
-  const c10::cuda::CUDAGuard guard(m.table.device());
+  const On on(a[8], m.table);
   const Maps to = into_of(m, a);
   const int status = lib.cache_release(ptr<int32_t>(m.table), ptr<int32_t>(m.lens), ptr<int32_t>(m.refs), ptr<int32_t>(gone), integer(a[5]),
-                                       integer(a[6]), ptr<int32_t>(to.status), m.slots, m.width, m.pages, integer(a[7]), stream_of(a[8], m.table));
+                                       integer(a[6]), ptr<int32_t>(to.status), m.slots, m.width, m.pages, integer(a[7]), on.stream);
   return status ? PyLong_FromLong(status) : wrapped(to);
   END_HANDLE_TH_ERRORS
 }
@@ -377,12 +385,12 @@ PyObject *cache_compact(PyObject *, PyObject *const *a, Py_ssize_t n) {
   arguments(n, 10);
   const Maps m = maps_of(a + 1, "maps");
   const Pool pool = pool_of(tensor(a[0], "pool"), m.table, m.pages);
-  const c10::cuda::CUDAGuard guard(m.table.device());
+  const On on(a[9], m.table);
   const Maps to = into_of(m, a + 5);
   const int status = lib.cache_compact(pool.data, pool.planes, pool.heads, pool.token_bytes, pool.strides, ptr<int32_t>(m.table),
                                        ptr<int32_t>(to.table), ptr<int32_t>(m.lens), ptr<int32_t>(to.lens), ptr<int32_t>(m.refs),
                                        ptr<int32_t>(to.refs), ptr<int32_t>(to.status), m.slots, m.width, m.pages, pool.page_size,
-                                       stream_of(a[9], m.table));
+                                       on.stream);
   return status ? PyLong_FromLong(status) : wrapped(to);
   END_HANDLE_TH_ERRORS
 }
@@ -397,9 +405,9 @@ PyObject *cache_copy(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Pool pool = pool_of(t, t, t.size(1));
   check_ints(src, "src", t, {src.numel()});
   check_ints(dst, "dst", t, {src.numel()});
-  const c10::cuda::CUDAGuard guard(t.device());
+  const On on(a[3], t);
   return PyLong_FromLong(lib.cache_copy(pool.data, pool.planes, pool.heads, pool.token_bytes, pool.strides, ptr<int32_t>(src),
-                                        ptr<int32_t>(dst), src.numel(), t.size(1), pool.page_size, stream_of(a[3], t)));
+                                        ptr<int32_t>(dst), src.numel(), t.size(1), pool.page_size, on.stream));
   END_HANDLE_TH_ERRORS
 }
 

@@ -14,7 +14,8 @@ and its :class:`CacheMaps`, int32 tensors on the device.  What is free is read f
 needs the host: a decode step can be captured in a CUDA graph.  Operations on maps return new ones, or write ``into``
 given ones, which may be the same (not for :func:`cache_fork`).  :class:`PagedCache` keeps a pool with its maps.
 
-A tensor used on another stream than the one it was made on needs ``record_stream`` or an event, as any torch tensor.
+A tensor used on another stream than the one it was made on needs ``record_stream`` or an event, as any torch tensor;
+what a call with ``stream`` returns was made on that one.
 The library's workspaces belong to a stream and grow on its first calls: before a capture, run the step once on the
 stream that will capture it.  A graph keeps the workspaces of the stream it was captured on, also when later calls make
 them grow; so graphs captured on one stream, and calls on that stream, may not run at the same time.
@@ -221,8 +222,9 @@ class PagedCache:
         cache_compact(self.pool, self.maps, into=self.maps, stream=stream)
 
     def check(self) -> int:
-        """Waits for the last operation on the maps; the pages free after it.  Raises where an operation could not be
-        done, the first of them since the last check, whatever came after it."""
+        """Waits for the last operation on the maps (on the current stream, or one that it waits for); the pages free
+        after it.  Raises where an operation could not be done, the first of them since the last check, whatever came
+        after it."""
         code, free, refused, _ = torch.cat((self.maps.status, self._refusals)).tolist()
         code = refused or code
         if code:

@@ -1,0 +1,62 @@
+"""Serving calls with ``stream=``: what they allocate is that stream's memory, and their results are those of the current stream."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def ints(values):
+    import torch
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def streams_of(tensors):
+    """The stream whose memory each tensor lies in."""
+    import torch
+    segments = [(s["address"], s["address"] + s["total_size"], s["stream"]) for s in torch.cuda.memory_snapshot()]
+    found = []
+    for t in tensors:
+        (stream,) = [x for lo, hi, x in segments if lo <= t.data_ptr() < hi]
+        found.append(stream)
+    return found
+
+
+def test_results_are_memory_of_the_stream_they_are_written_on(cuda_device):
+    import torch
+    from lazy_compiler_b200 import serving as S
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda").half()  # noqa: E731
+    q, k, v = rand(2, 150, 4, 64), rand(2, 150, 2, 64), rand(2, 150, 2, 64)
+    pool, maps = rand(2, 40, 2, 8, 64), S.CacheMaps(ints([[3, 9, 1, -1], [7, -1, -1, -1]]), ints([20, 5]), ints([0] * 40))
+    maps.refs[ints([3, 9, 1, 7]).long()] = 1
+    add, parent = ints([3, 4]), ints([1, 1])
+
+    def calls(stream):
+        """Every operation that returns new tensors; all of them work on copies of the same inputs."""
+        kept = pool.clone(), pool.clone()
+        old = S.CacheMaps(*(t.clone() for t in maps[:3]))
+        if stream:
+            torch.cuda.synchronize()  # the copies above
+        new = S.cache_extend(maps, add, page_size=8, stream=stream)
+        forked = S.cache_fork(kept[0], maps, parent, stream=stream)
+        packed = S.cache_compact(kept[1], maps, stream=stream)
+        trimmed = S.cache_trim(old, window=4, page_size=8, stream=stream)
+        found = [*S.window_attention(q, k, v, window=40, sinks=2, return_lse=True, stream=stream),
+                 *S.paged_decode(q[:, 0], pool[0], pool[1], maps.table, maps.lens, return_lse=True, stream=stream), *new, *forked,
+                 *packed, trimmed.status]
+        return found, [*trimmed[:3], *kept]
+
+    side, current = torch.cuda.Stream(), torch.cuda.current_stream()
+    made, given = calls(None)
+    torch.cuda.synchronize()
+    made2, given2 = calls(side.cuda_stream)
+    assert torch.cuda.current_stream() == current
+    assert set(streams_of(made)) == {current.cuda_stream}
+    assert set(streams_of(made2)) == {side.cuda_stream}
+    side.synchronize()
+    for x, y in zip([*made, *given], [*made2, *given2]):
+        assert torch.equal(x, y)
+    S.window_attention(q, k, v, stream=0)
+    with torch.cuda.stream(side):
+        o = S.window_attention(q, k, v, stream=current.cuda_stream)
+        assert torch.cuda.current_stream() == side
+    assert streams_of([o]) == [current.cuda_stream]
