@@ -175,8 +175,8 @@ class PagedCache:
     """The keys and values of ``layers`` attention layers of up to ``slots`` sequences, in pages.
 
     ``pool[2 * layers, pages, kv_heads, page_size, head_dim]`` holds layer ``l``'s keys in plane ``2 l`` and its values
-    in plane ``2 l + 1``; ``maps`` are its :class:`CacheMaps`.  Every method works on the device, in stream order;
-    :meth:`check` waits for it and raises where one could not be done since the check before.
+    in plane ``2 l + 1``; ``maps`` are its :class:`CacheMaps`, the same tensors always.  Every method works on the
+    device, in stream order; :meth:`check` waits for it and raises where one could not be done since the check before.
     """
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, slots: int, width: int,
@@ -186,8 +186,11 @@ class PagedCache:
         self.pool = torch.zeros((2 * layers, pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
         ints = dict(dtype=torch.int32, device=self.pool.device)
         self.page_size = page_size
-        self.maps, self._spare = (CacheMaps(torch.full((slots, width), -1, **ints), torch.zeros(slots, **ints),
-                                            torch.zeros(pages, **ints), torch.zeros(2, **ints)) for _ in range(2))
+        # the maps, and those that a fork writes; each set is one block of memory
+        self._blocks = [torch.zeros(slots * width + slots + pages + 2, **ints) for _ in range(2)]
+        self.maps, self._spare = (CacheMaps(t.view(slots, width), n, r, s) for t, n, r, s in
+                                  (b.split([slots * width, slots, pages, 2]) for b in self._blocks))
+        self.maps.table.fill_(-1)
         self.maps.status[1] = pages
         self._refusals = torch.zeros(2, **ints)
 
@@ -205,9 +208,11 @@ class PagedCache:
         return paged_decode(q, self.pool[2 * layer], self.pool[2 * layer + 1], self.maps.table, self.maps.lens, **options)
 
     def fork(self, parent, stream=None) -> None:
-        """Slots continue others (:func:`cache_fork`).  The maps are other tensors afterwards."""
+        """Slots continue others (:func:`cache_fork`).  The new maps are copied back into the same tensors, so that a
+        step captured before goes on with them."""
         cache_fork(self.pool, self.maps, parent, into=self._spare, refusals=self._refusals, stream=stream)
-        self.maps, self._spare = self._spare, self.maps
+        with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream, self.pool.device)):
+            self._blocks[0].copy_(self._blocks[1])
 
     def release(self, gone, stream=None) -> None:
         """Empties slots (:func:`cache_release`)."""

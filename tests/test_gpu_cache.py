@@ -412,3 +412,63 @@ def test_a_refused_fork_is_told_too(cuda_device):
     assert first.status.tolist() == [-1, 1] and refusals.tolist() == [-1, 1]
     with pytest.raises(ValueError, match="refusals: shape"):
         S.cache_extend(cache.maps, ints([0, 0, 0, 0]), page_size=4, refusals=refusals[:1])
+
+
+@pytest.mark.parametrize("fork_captured", [False, True])
+def test_a_captured_step_goes_on_after_a_fork(fork_captured, cuda_device):
+    """Beams: a fork between the replays of one captured step, or inside it, as if every step were made anew."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    rng = np.random.default_rng(0)
+    slots, h, d, page, width, pages = 4, 2, 64, 4, 12, 40
+    model = R.Pages([[-1] * width for _ in range(slots)], [0] * slots, [0] * pages, page, np.zeros((2, pages, h, page, d), np.float32))
+    cache = S.PagedCache(1, pages, page, h, d, slots, width, dtype=torch.float16)
+    k, v = (torch.zeros((slots, 9, h, d), dtype=torch.float16, device="cuda") for _ in range(2))
+    q, out = torch.randn((slots, 4, d), device="cuda").half(), torch.empty((slots, 4, d), dtype=torch.float16, device="cuda")
+    parent, one = ints(list(range(slots))), ints([1] * slots)
+
+    def tokens(most):
+        new = [rng.integers(-9, 9, (slots, most, h, d)).astype(np.float32) for _ in range(2)]
+        for x, y in zip((k, v), new):
+            x[:, :most] = torch.from_numpy(y).cuda()
+        return new
+
+    def fork():
+        cache.fork(parent, stream=side.cuda_stream)
+
+    def step():
+        if fork_captured:
+            fork()
+        cache.extend(one)
+        cache.write(0, k[:, :1], v[:, :1], one)
+        cache.decode(0, q, out=out)
+
+    side, graph, maps = torch.cuda.Stream(), torch.cuda.CUDAGraph(), cache.maps
+    add = [9, 0, 6, 0]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        new = tokens(9)
+        cache.extend(ints(add))
+        cache.write(0, k, v, ints(add))
+        model.extend(add)
+        model.write(*new, add)
+        for t, parents in enumerate([[0, 2, 2, 0], [0, 1, 2, 3], [3, 3, 1, 0], [1, 1, 1, 1], [0, 0, 2, -1], [2, 2, 2, 2]]):
+            parent.copy_(ints(parents))
+            if not fork_captured:
+                fork()
+            new = tokens(1)
+            if t == 0:
+                step()
+                side.synchronize()
+                with torch.cuda.graph(graph, stream=side):
+                    step()
+            else:
+                graph.replay()
+            assert model.fork(parents)[0] == 0
+            status = model.extend([1] * slots)
+            model.write(*new, [1] * slots)
+            same(model, cache.maps, status, cache.pool)
+            assert cache.maps is maps and cache.check() == status[1]
+            pool = torch.from_numpy(model.pool).cuda().half()
+            want = S.paged_decode(q, pool[0], pool[1], ints(model.table), ints(model.lens))
+            assert torch.equal(out, want)
