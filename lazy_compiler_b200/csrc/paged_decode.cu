@@ -105,7 +105,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // tcgen05 has no use here: its 128-row tiles would be 1/16 full, and the tensor
 // pipe is idle most of the time as it is.
 // P is split into two 16-bit parts (value and remainder) and multiplied twice: the
-// extra products hide behind the loads and keep P to 16 bits or more.
+// extra products hide behind the loads and keep P to 16 bits or more.  An f16 part ends at
+// 2^-25, where a bf16 one has f32's range, so f16 weights are taken 2^kLift larger (the row's
+// reference is its maximum less kLift): a weight is off by 2^-39 of the row's largest one at most,
+// and a long tail below a sink that outweighs it is not lost.
 // Bound by HBM.  Measured, 32/8 heads of 128, bf16: 64 sequences of 1 to 8192 tokens
 // in pages of 16: 167 us, 6440 GB/s, the rate of a copy; 64/8, f16, 100003 and 131072
 // tokens: 149 us, 6360 GB/s.  Three CTAs per SM of two stages against two of three:
@@ -127,6 +130,12 @@ constexpr int kEndUnits = 1;
 // 8 of 1 to 512: 15.3 -> 13.3, but 64 of 1 to 500: 23.3 -> 25.2; two tiles make short caches of few
 // heads worse, 2000 tokens of 2 heads: 9.0 -> 10.7).
 constexpr int kSnap = 1;
+
+// The largest weight of a row is 2^kLift: far from f16's largest number, its sums in f32.
+template <class T>
+constexpr float kLift = 0.f;
+template <>
+constexpr float kLift<__half> = 14.f;
 
 template <class T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -498,7 +507,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
       for (int x = 0; x < 2; ++x) {
         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16)) - kLift<T>;
       }
       const bool grew = top[0] > m[nt][0] || top[1] > m[nt][1];
       if (__any_sync(0xffffffffu, grew)) {

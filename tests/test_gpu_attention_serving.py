@@ -500,3 +500,44 @@ def test_refusals_of_tensors(cuda_device):
             call()
     o, lse = S.window_attention(q, k, k, return_lse=1)
     assert o.shape == q.shape and lse.shape == (2, 4, 5)
+
+
+# ---------------------------------------------------------------- a sink that outweighs a long tail
+
+def sink_rows(dtype, shape, axis, d, gap, seed):
+    """Keys and values: key 0 along `axis` scores `gap` over all others for a query of ones, and its value is zero."""
+    import torch
+    k = torch.zeros(shape, dtype=torch_dtype(dtype), device="cuda")
+    k.select(axis, 0).fill_(gap / d ** 0.5)
+    v = normal(shape, dtype, seed).abs() + 0.5
+    v.select(axis, 0).zero_()
+    return k, v
+
+
+def check_tail(o, lse, ref, dtype, keys, weight):
+    """As check_attention, and what a weight may be off by beside its relative error: `weight` of the row's largest
+    one for each key (f16 only; the values are below 8)."""
+    extra = keys * weight * 8 if dtype == "f16" else 0.0
+    far = np.abs(o - ref[0]) - extra
+    R.check_attention(np.where(far <= 0, ref[0], ref[0] + np.sign(o - ref[0]) * far), lse, ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [8.0, 12.0, 18.0])
+@pytest.mark.parametrize("lens,heads", [([700] * 64, 8), ([6000] + [100] * 29, 8), ([100003], 2)])
+def test_token_tail_under_a_sink(lens, heads, gap, dtype, cuda_device):
+    """Whole segments, segments joined by a CTA, and by the second kernel.  Two 16-bit parts end at 2^-25, the largest
+    weight is 2^14: 2^-39 of it a key."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    d, page = 64, 16
+    width = -(-max(lens) // page)
+    k, v = sink_rows(dtype, (heads, width * page, d), 1, d, gap, 40)
+    k_pages, v_pages = (x.view(heads, width, page, d).transpose(0, 1).contiguous() for x in (k, v))
+    q = torch.ones((len(lens), 2 * heads, d), dtype=k.dtype, device="cuda")
+    table = torch.arange(width, dtype=torch.int32, device="cuda").repeat(len(lens), 1)
+    o, lse = S.paged_decode(q, k_pages, v_pages, table, ints(lens), return_lse=True)
+    for x in {0, len(lens) - 1}:
+        n = lens[x]
+        ref = [np.array(a) for a in zip(*(R.attend(f64(q[x, y]), f64(k[y // 2, :n]), f64(v[y // 2, :n]), d ** -0.5) for y in range(2 * heads)))]
+        check_tail(f64(o[x]), f64(lse[x]), ref, dtype, n, 2.0 ** -39)
