@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) window_row_kernel(WindowParams
 //           in shared memory, and a row whose sums come out infinite or NaN is
 //           computed again key by key (it may hold a value that its mask hides).
 // P is rounded to the storage type for the second product: an error of the size of the
-// output's own rounding.
+// output's own rounding (and kLift's, where a row's weights are many and small).
 // Bound by a tile's chain of softmax and products (3500 cycles a block of 128 keys, of
 // which the tensor pipe needs 2080 for both tiles), in long runs by the power cap.
 // Measured, f16, 32/8 heads of 128: 32768 tokens, window 4096: 1.75 ms, 1180 TFLOP/s;
@@ -134,6 +134,13 @@ constexpr uint32_t kTmemCols = 512;
 // run at once.)
 constexpr uint32_t kOCol = 256;
 constexpr float kRescale = 8.0f;            // log2 units a row's maximum may lag behind
+// A row's reference is its maximum less kLift, so that with the lag f16 weights reach 2^15 (its
+// largest number is just under 2^16).  They end at 2^-25, and a row's largest weight is 2^7 or more:
+// what is lost is 2^-32 of it a key, 2^-25 without the lift.  bf16 has f32's range.
+template <class T>
+constexpr float kLift = 0.f;
+template <>
+constexpr float kLift<__half> = 7.f;
 constexpr int kChunkBytes = 128 * 64 * 2;   // 128 rows x 64 columns, one swizzle span
 
 template <int DP>
@@ -756,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_async_shared();
         }
         const float mx = max3(max3(mx8[0], mx8[1], mx8[2]), max3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])) * p.scale_log2;
-        const float m_new = fmaxf(m, mx);
+        const float m_new = fmaxf(m, mx - kLift<T>);
         const bool need = m_new > m + kRescale;
         if (__any_sync(0xffffffffu, need)) {
           const float alpha = need ? ex2(m - m_new) : 1.0f;

@@ -541,3 +541,22 @@ def test_token_tail_under_a_sink(lens, heads, gap, dtype, cuda_device):
         n = lens[x]
         ref = [np.array(a) for a in zip(*(R.attend(f64(q[x, y]), f64(k[y // 2, :n]), f64(v[y // 2, :n]), d ** -0.5) for y in range(2 * heads)))]
         check_tail(f64(o[x]), f64(lse[x]), ref, dtype, n, 2.0 ** -39)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [8.0, 12.0, 18.0])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("s_q,s_kv,heads,window", [(3000, 3000, 16, 0), (3000, 3000, 16, 2000), (9, 40000, 2, 0), (260, 30000, 2, 0)])
+def test_prompt_tail_under_a_sink(s_q, s_kv, heads, window, d, gap, dtype, cuda_device):
+    """Whole items, and runs of them joined with and without the deep form.  One 16-bit part ends at 2^-25, the largest
+    weight is 2^7 or more: 2^-32 of it a key."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    k, v = sink_rows(dtype, (1, s_kv, heads, d), 1, d, gap, 41)
+    q = torch.ones((1, s_q, 2 * heads, d), dtype=k.dtype, device="cuda")
+    o, lse = S.window_attention(q, k, v, window=window, sinks=1, return_lse=True)
+    for i in (s_q - 1, s_q // 2, 0):
+        js = torch.from_numpy(R.seen(s_kv - s_q + i, s_kv, window, 1)).cuda()
+        ys = (0, heads, 2 * heads - 1)
+        ref = [np.array(a) for a in zip(*(R.attend(f64(q[0, i, y]), f64(k[0, js, y // 2]), f64(v[0, js, y // 2]), d ** -0.5) for y in ys))]
+        check_tail(f64(o[0, i, list(ys)]), f64(lse[0, list(ys), i]), ref, dtype, len(js), 2.0 ** -32)
