@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -106,6 +107,15 @@ void check_cuda(const at::Tensor &t, const char *what) {
 void check_axes(const at::Tensor &t, const char *what, int64_t axes) {
   if (t.dim() != axes) refuse(what, ": ", t.dim(), " axes, expected ", axes);
 }
+// Nothing here has a gradient: a tensor that asks for one is refused, not cut off without a word.
+void check_no_gradient(const at::Tensor &t, const char *what) {
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    refuse(what, ": requires a gradient, which the serving operators do not compute; call them under torch.no_grad() or detach it");
+}
+// A tensor that a call writes: what autograd has saved of it is out of date afterwards.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 int attention_dtype(const at::Tensor &q) {
   if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) refuse("q: ", name_of(q.scalar_type()), " is not float16 or bfloat16");
   check_cuda(q, "q");
@@ -166,6 +176,9 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments(n, 11);
   const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
+  check_no_gradient(q, "q");
+  check_no_gradient(k, "k");
+  check_no_gradient(v, "v");
   const int dtype = attention_dtype(q);
   check_axes(q, "q", 4);
   check_axes(k, "k", 4);
@@ -175,7 +188,7 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const at::Tensor *q_lens = maybe(a[6], "q_lens"), *kv_lens = maybe(a[7], "kv_lens"), *given = maybe(a[8], "out");
   if (q_lens) check_ints(*q_lens, "q_lens", q, {batch});
   if (kv_lens) check_ints(*kv_lens, "kv_lens", q, {batch});
-  if (given) check(*given, "out", q, q.scalar_type(), {batch, s_q, heads, d}), check_out(*given, "out");
+  if (given) check(*given, "out", q, q.scalar_type(), {batch, s_q, heads, d}), check_out(*given, "out"), check_no_gradient(*given, "out");
   const On on(a[10], q);
   const at::Tensor out = given ? *given : fresh({batch, s_q, heads, d}, q.scalar_type(), q);
   const at::Tensor lse = truth(a[9]) ? fresh({batch, heads, s_q}, at::kFloat, q) : at::Tensor();
@@ -190,6 +203,7 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
                                           ptr<int32_t>(q_lens), ptr<int32_t>(kv_lens), batch, s_q, s_kv, heads, kv_heads, d, strides,
                                           integer(a[3]), integer(a[4]), scale_of(a[5], d), on.stream);
   if (status) return PyLong_FromLong(status);
+  if (given) written(out);
   return outputs(out, a[8], lse);
   END_HANDLE_TH_ERRORS
 }
@@ -200,6 +214,9 @@ PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
   arguments(n, 11);
   const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k_pages"), &v = tensor(a[2], "v_pages");
   const at::Tensor &table = tensor(a[3], "table"), &lens = tensor(a[4], "lens");
+  check_no_gradient(q, "q");
+  check_no_gradient(k, "k_pages");
+  check_no_gradient(v, "v_pages");
   const int dtype = attention_dtype(q);
   check_axes(q, "q", 3);
   check_axes(k, "k_pages", 4);
@@ -211,7 +228,7 @@ PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
   check(table, "table", q, at::kInt, {slots, width});
   check_ints(lens, "lens", q, {slots});
   const at::Tensor *given = maybe(a[8], "out");
-  if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d}), check_out(*given, "out");
+  if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d}), check_out(*given, "out"), check_no_gradient(*given, "out");
   const On on(a[10], q);
   const at::Tensor out = given ? *given : fresh({slots, heads, d}, q.scalar_type(), q);
   const at::Tensor lse = truth(a[9]) ? fresh({slots, heads}, at::kFloat, q) : at::Tensor();
@@ -226,6 +243,7 @@ PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
                                       ptr<int32_t>(table), ptr<int32_t>(lens), slots, width, pages, page_size, heads, kv_heads, d,
                                       strides, integer(a[5]), integer(a[6]), scale_of(a[7], d), on.stream);
   if (status) return PyLong_FromLong(status);
+  if (given) written(out);
   return outputs(out, a[8], lse);
   END_HANDLE_TH_ERRORS
 }
@@ -265,6 +283,8 @@ Maps into_of(const Maps &m, PyObject *const *a) {
     to = maps_of(a, "into");
     if (to.slots != m.slots || to.width != m.width || to.pages != m.pages || to.table.device() != m.table.device())
       refuse("into: other sizes or another device than the maps");
+    for (const at::Tensor &t : {to.table, to.lens, to.refs, to.status})
+      if (t.defined()) written(t);
   }
   if (!to.status.defined()) to.status = fresh({2}, at::kInt, m.table);
   return to;
@@ -289,6 +309,7 @@ struct Pool {
 Pool pool_of(const at::Tensor &t, const at::Tensor &like, int64_t pages) {
   if (t.dim() != 5 || t.device() != like.device() || t.size(1) != pages)
     refuse("pool: ", shape_text(t.sizes()), " on ", t.device(), ", expected [planes, ", pages, ", kv_heads, page_size, d] on ", like.device());
+  check_no_gradient(t, "pool");
   check_inner(t, "pool");
   check_out(t, "pool");
   if (t.size(3) > 1 && t.stride(3) != t.size(4)) refuse("pool: the tokens of a head must be contiguous");
@@ -320,6 +341,10 @@ PyObject *cache_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const Maps m = maps_of(a + 4, "maps");
   const at::Tensor &add = tensor(a[8], "add");
   check_ints(add, "add", m.table, {m.slots});
+  check_no_gradient(k, "k");
+  check_no_gradient(v, "v");
+  check_no_gradient(kp, "k_pages");
+  check_no_gradient(vp, "v_pages");
   check_axes(k, "k", 4);
   check_axes(kp, "k_pages", 4);
   const int64_t most = k.size(1), heads = k.size(2), d = k.size(3), page_size = kp.size(2), size = k.element_size();
@@ -340,9 +365,11 @@ PyObject *cache_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const int32_t *refused = refusals_of(a[9], m);
   refused = refused ? refused + 1 : m.status.defined() ? ptr<int32_t>(m.status) : nullptr;
   const On on(a[10], m.table);
-  return PyLong_FromLong(lib.cache_write(ptr(k), ptr(v), ptr(kp), ptr(vp), ptr<int32_t>(m.table), ptr<int32_t>(m.lens), ptr<int32_t>(add),
-                                         m.slots, most, m.width, m.pages, page_size, heads, d * size, strides,
-                                         refused, on.stream));
+  const int status = lib.cache_write(ptr(k), ptr(v), ptr(kp), ptr(vp), ptr<int32_t>(m.table), ptr<int32_t>(m.lens), ptr<int32_t>(add),
+                                     m.slots, most, m.width, m.pages, page_size, heads, d * size, strides, refused, on.stream);
+  written(kp);
+  written(vp);
+  return PyLong_FromLong(status);
   END_HANDLE_TH_ERRORS
 }
 
@@ -360,6 +387,7 @@ PyObject *cache_fork(PyObject *, PyObject *const *a, Py_ssize_t n) {
                                     ptr<int32_t>(to.table), ptr<int32_t>(m.lens), ptr<int32_t>(to.lens), ptr<int32_t>(m.refs),
                                     ptr<int32_t>(to.refs), ptr<int32_t>(parent), ptr<int32_t>(to.status), refusals_of(a[10], m),
                                     m.slots, m.width, m.pages, pool.page_size, on.stream);
+  written(tensor(a[0], "pool"));
   return status ? PyLong_FromLong(status) : wrapped(to);
   END_HANDLE_TH_ERRORS
 }
@@ -391,6 +419,7 @@ PyObject *cache_compact(PyObject *, PyObject *const *a, Py_ssize_t n) {
                                        ptr<int32_t>(to.table), ptr<int32_t>(m.lens), ptr<int32_t>(to.lens), ptr<int32_t>(m.refs),
                                        ptr<int32_t>(to.refs), ptr<int32_t>(to.status), m.slots, m.width, m.pages, pool.page_size,
                                        on.stream);
+  written(tensor(a[0], "pool"));
   return status ? PyLong_FromLong(status) : wrapped(to);
   END_HANDLE_TH_ERRORS
 }
@@ -406,8 +435,10 @@ PyObject *cache_copy(PyObject *, PyObject *const *a, Py_ssize_t n) {
   check_ints(src, "src", t, {src.numel()});
   check_ints(dst, "dst", t, {src.numel()});
   const On on(a[3], t);
-  return PyLong_FromLong(lib.cache_copy(pool.data, pool.planes, pool.heads, pool.token_bytes, pool.strides, ptr<int32_t>(src),
-                                        ptr<int32_t>(dst), src.numel(), t.size(1), pool.page_size, on.stream));
+  const int status = lib.cache_copy(pool.data, pool.planes, pool.heads, pool.token_bytes, pool.strides, ptr<int32_t>(src),
+                                    ptr<int32_t>(dst), src.numel(), t.size(1), pool.page_size, on.stream);
+  written(t);
+  return PyLong_FromLong(status);
   END_HANDLE_TH_ERRORS
 }
 

@@ -16,6 +16,8 @@ given ones, which may be the same (not for :func:`cache_fork`).  :class:`PagedCa
 
 A tensor used on another stream than the one it was made on needs ``record_stream`` or an event, as any torch tensor;
 what a call with ``stream`` returns was made on that one.
+No operation has a gradient: with grad mode on, an input that requires one is refused.
+
 The library's workspaces belong to a stream and grow on its first calls: before a capture, run the step once on the
 stream that will capture it.  A graph keeps the workspaces of the stream it was captured on, also when later calls make
 them grow; so graphs captured on one stream, and calls on that stream, may not run at the same time.

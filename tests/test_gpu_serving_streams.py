@@ -60,3 +60,39 @@ def test_results_are_memory_of_the_stream_they_are_written_on(cuda_device):
         o = S.window_attention(q, k, v, stream=current.cuda_stream)
         assert torch.cuda.current_stream() == side
     assert streams_of([o]) == [current.cuda_stream]
+
+
+def test_gradients_are_refused_and_writes_are_counted(cuda_device):
+    """Inputs that require a gradient, and tensors that autograd has saved before a call wrote them."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    half = lambda *s: torch.ones(s, dtype=torch.float16, device="cuda")  # noqa: E731
+    q, k, pool = half(2, 6, 4, 64), half(2, 6, 2, 64), half(2, 9, 2, 4, 64)
+    maps, one = S.CacheMaps(ints([[0, 1], [2, 3]]), ints([6, 5]), ints([1] * 4 + [0] * 5), ints([0, 5])), ints([1, 1])
+    g, gp = k.clone().requires_grad_(), pool.clone().requires_grad_()
+    for call, name in [
+        (lambda: S.window_attention(q, k, k, out=torch.empty_like(q, requires_grad=True)), "out"),
+        (lambda: S.cache_write(g[:, :1], k[:, :1], pool[0], pool[1], maps, one), "k"),
+        (lambda: S.cache_write(k[:, :1], k[:, :1], pool[0], gp[1], maps, one), "v_pages"),
+        (lambda: S.cache_fork(gp, maps, one), "pool"), (lambda: S.cache_compact(gp, maps), "pool"), (lambda: S.cache_copy(gp, one, one), "pool"),
+    ]:
+        with pytest.raises(ValueError, match=name + ": requires a gradient"):
+            call()
+    with torch.no_grad():
+        S.window_attention(q, g, g)
+        S.cache_copy(gp, ints([0]), ints([7]))
+    w = torch.ones((), device="cuda", dtype=torch.float16, requires_grad=True)
+    out = torch.empty_like(q)
+    for saved, call in [
+        (out, lambda: S.window_attention(q, k, k, out=out)), (pool, lambda: S.cache_write(k[:, :1], k[:, :1], pool[0], pool[1], maps, one)),
+        (pool, lambda: S.cache_fork(pool, maps, one)), (pool, lambda: S.cache_compact(pool, maps)), (pool, lambda: S.cache_copy(pool, one, ints([8, 7]))),
+    ]:
+        loss = (w * saved).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    before = maps.lens._version
+    S.cache_extend(maps, one, page_size=4, into=maps)
+    assert maps.lens._version > before
+    with torch.inference_mode():
+        S.window_attention(q, k, k, out=torch.empty_like(q))

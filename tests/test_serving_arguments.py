@@ -124,3 +124,20 @@ def test_numbers_in_the_refusals():
         _serving.window_attention(1)
     with pytest.raises(TypeError):
         _serving.bind(*[1.5] * 8)
+
+
+def test_what_requires_a_gradient():
+    """Nothing has a gradient, and no one that is asked for is dropped without a word."""
+    q, k = torch.zeros(1, 4, 2, 64, dtype=torch.half), torch.zeros(1, 4, 2, 64, dtype=torch.half)
+    table, lens, refs = (torch.zeros(n, dtype=torch.int32) for n in ((1, 2), 1, 4))
+    g, pages = (torch.zeros(s, dtype=torch.half, requires_grad=True) for s in ((1, 4, 2, 64), (4, 2, 16, 64)))
+    for call, name in [
+        (lambda: S.window_attention(g, k, k), "q"), (lambda: S.window_attention(q, g, k), "k"), (lambda: S.window_attention(q, k, g), "v"),
+        (lambda: S.paged_decode(g[0], pages.detach(), pages.detach(), table, lens), "q"),
+        (lambda: S.paged_decode(q[0], pages, pages.detach(), table, lens), "k_pages"),
+        (lambda: S.paged_decode(q[0], pages.detach(), pages, table, lens), "v_pages"),
+    ]:
+        with pytest.raises(ValueError, match=name + ": requires a gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA devices only"):
+            call()
