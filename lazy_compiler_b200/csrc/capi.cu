@@ -179,14 +179,16 @@ int device_error_word(int **out) {
 extern "C" int lc_device_status(void *stream) {
   int *word = nullptr;
   if (int rc = lc::device_error_word(&word)) return rc;
+  // on `stream` alone: the default stream's copies would wait for work that is not asked about
   cudaStream_t s = lc::as_stream(stream);
-  if (int rc = lc::check_cuda(cudaStreamSynchronize(s), "lc_device_status: stream")) return rc;
   int value = 0;
-  if (int rc = lc::check_cuda(cudaMemcpy(&value, word, sizeof(int), cudaMemcpyDeviceToHost),
+  if (int rc = lc::check_cuda(cudaMemcpyAsync(&value, word, sizeof(int), cudaMemcpyDeviceToHost, s),
                               "lc_device_status: read"))
     return rc;
+  if (int rc = lc::check_cuda(cudaStreamSynchronize(s), "lc_device_status: stream")) return rc;
   if (value == 0) return LC_OK;
-  cudaMemset(word, 0, sizeof(int));
+  cudaMemsetAsync(word, 0, sizeof(int), s);
+  cudaStreamSynchronize(s);
   return lc::fail(LC_ERR_TIMEOUT,
                   "a bounded device wait gave up (code %d: 1 producer, 2 mma, 3 epilogue, "
                   "4 softmax, 5 correction)",

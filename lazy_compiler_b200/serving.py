@@ -16,6 +16,9 @@ given ones, which may be the same (not for :func:`cache_fork`).  :class:`PagedCa
 
 A tensor used on another stream than the one it was made on needs ``record_stream`` or an event, as any torch tensor;
 what a call with ``stream`` returns was made on that one.
+The waits inside the prompt form's kernel are bounded.  One that runs out (a fault of the machine) leaves outputs
+unwritten; ``runtime.call("lc_device_status", stream)`` tells of it, as :meth:`PagedCache.check` does.
+
 No operation has a gradient: with grad mode on, an input that requires one is refused.
 
 The library's workspaces belong to a stream and grow on its first calls: before a capture, run the step once on the
@@ -231,11 +234,13 @@ class PagedCache:
     def check(self) -> int:
         """Waits for the last operation on the maps (on the current stream, or one that it waits for); the pages free
         after it.  Raises where an operation could not be done, the first of them since the last check, whatever came
-        after it."""
+        after it, and where a kernel gave up a wait inside it (``lc_device_status``)."""
         code, free, refused, _ = torch.cat((self.maps.status, self._refusals)).tolist()
         code = refused or code
         if code:
             self._refusals[0] = 0
             what = "an argument is out of range" if code < 0 else f"{code} pages are missing"
             raise RuntimeError(f"an operation was refused and changed nothing: {what} ({free} pages are free)")
+        with torch.cuda.device(self.pool.device):
+            runtime.call("lc_device_status", torch.cuda.current_stream().cuda_stream)
         return free

@@ -96,3 +96,27 @@ def test_gradients_are_refused_and_writes_are_counted(cuda_device):
     assert maps.lens._version > before
     with torch.inference_mode():
         S.window_attention(q, k, k, out=torch.empty_like(q))
+
+
+def test_check_tells_of_a_wait_that_ran_out(cuda_device):
+    """A kernel that gave up a bounded wait (the self-test's, which nothing ever ends) is reported by check(), once,
+    which waits for its own stream alone."""
+    import torch
+    from lazy_compiler_b200 import runtime
+    from lazy_compiler_b200 import serving as S
+    cache = S.PagedCache(1, 4, 4, 1, 64, 1, 2)
+    assert cache.check() == 4
+    runtime.call("lc_selftest_bounded_wait", 1_000_000, torch.cuda.current_stream().cuda_stream)
+    with pytest.raises(runtime.LcError, match="gave up"):
+        cache.check()
+    assert cache.check() == 4
+    side, busy = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(1_000_000_000)
+    busy.record()
+    with torch.cuda.stream(side):
+        runtime.call("lc_selftest_bounded_wait", 1_000_000, side.cuda_stream)
+        with pytest.raises(runtime.LcError, match="gave up"):
+            cache.check()
+        assert cache.check() == 4
+        assert not busy.query()
