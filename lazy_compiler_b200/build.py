@@ -5,7 +5,8 @@ parallel, skipped when the object is newer than its sources) and linked into
 ``lazy_compiler_b200/liblazyb200.so`` with the CUDA runtime linked
 statically, so the library only needs the driver at run time.  The Python
 side of the serving operators, ``csrc/serving_ext.cpp``, becomes the extension
-module ``_serving`` beside it (against the installed torch's headers).
+module ``_serving`` beside it (against the installed torch's headers, and
+again when another torch is installed).
 ``python -m lazy_compiler_b200.build`` runs it from the command line.
 """
 from __future__ import annotations
@@ -15,6 +16,7 @@ import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -57,10 +59,18 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _built_for() -> str:
+    """The interpreter and the torch that the extension module is built against: its ABI is theirs."""
+    try:
+        return f"{sys.implementation.cache_tag} torch {metadata.version('torch')}"
+    except metadata.PackageNotFoundError as e:
+        raise RuntimeError("the serving operators' extension module needs torch, which is not installed") from e
+
+
 def _build_extension(force: bool) -> None:
-    src = CSRC / "serving_ext.cpp"
+    src, stamp, built_for = CSRC / "serving_ext.cpp", BUILD / "_serving.stamp", _built_for()
     newest = max(p.stat().st_mtime for p in (src, Path(__file__), *INCLUDE.glob("*.h")))
-    if EXTENSION.exists() and EXTENSION.stat().st_mtime >= newest and not force:
+    if EXTENSION.exists() and EXTENSION.stat().st_mtime >= newest and not force and stamp.exists() and stamp.read_text() == built_for:
         return
     import sysconfig
 
@@ -77,10 +87,14 @@ def _build_extension(force: bool) -> None:
     if result.returncode:
         raise RuntimeError(f"{cmd[0]} failed on {src.name}:\n{result.stderr}")
     os.replace(tmp, EXTENSION)
+    stamp.write_text(built_for)
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
-    """Compile every kernel source, link the shared library and the extension module; returns the library's path."""
+    """Compile every kernel source, link the shared library and the extension module; returns the library's path.
+
+    The library needs nvcc alone: where the extension module cannot be built, it is linked before that is raised.
+    """
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     if force:
@@ -89,7 +103,6 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
         extension = pool.submit(_build_extension, force)
         objects = list(pool.map(lambda s: _compile(s, verbose), sources))
-        extension.result()
     newest = max(o.stat().st_mtime for o in objects)
     if not LIBRARY.exists() or LIBRARY.stat().st_mtime < newest or force:
         tmp = LIBRARY.with_suffix(".so.tmp")
@@ -98,6 +111,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         if result.returncode:
             raise RuntimeError(f"link failed:\n{result.stderr}")
         os.replace(tmp, LIBRARY)
+    extension.result()
     return LIBRARY
 
 
