@@ -6,7 +6,9 @@
 // A query at position p sees key j when j <= p and (window == 0, or
 // j > p - window, or j < sinks): two intervals, [0, sink_end) and [lo, p].
 // Scores are kept in units of log2 (s * scale * log2 e), so a weight is
-// 2^(s - m); m, l and the output sums are f32.
+// 2^(s - m); m, l and the output sums are f32.  The plain row form keeps the weighted mean
+// of the values so far in place of their sum: bf16 values reach f32's largest number, which
+// a sum of two of them would pass.
 #pragma once
 
 #include "common.cuh"
@@ -42,16 +44,18 @@ __host__ __device__ __forceinline__ Visible visible(int p, int window, int sinks
 }
 
 // Running softmax of one query row of up to 32 NC columns spread over the lanes of a
-// warp: lane c holds output elements c, c + 32, ...
+// warp: lane c holds the mean of columns c, c + 32, ...
 template <int NC>
 struct RowState {
   float m = -INFINITY, l = 0.f;
-  float acc[NC];
+  float mean[NC];
   __device__ __forceinline__ RowState() {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) acc[i] = 0.f;
+    for (int i = 0; i < NC; ++i) mean[i] = 0.f;
   }
 };
+// 1 / l; 0 for a row that saw nothing, or only scores of -inf.
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 template <class T, int NC>
 __device__ __forceinline__ void load_row(float (&q)[NC], const T *src, int d, int lane, float factor) {
@@ -108,44 +112,48 @@ __device__ __forceinline__ void attend_keys(RowState<NC> &st, const float (&q)[N
     for (int u = 0; u < U; ++u)
       if (real[u]) m_new = fmaxf(m_new, s[u]);
     const float base = m_new == -INFINITY ? 0.f : m_new;  // a row of -inf scores so far
-    const float alpha = exp2f(st.m - base);
+    const float kept = st.l * exp2f(st.m - base);
     st.m = m_new;
-    st.l *= alpha;
+    st.l = kept;
+    float w[U];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) st.acc[i] *= alpha;
+    for (int u = 0; u < U; ++u) {
+      w[u] = real[u] ? exp2f(s[u] - base) : 0.f;
+      st.l += w[u];
+    }
+    const float inv = inverse(st.l), old = kept * inv;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) st.mean[i] *= old;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!real[u]) continue;
-      const float w = exp2f(s[u] - base);
-      st.l += w;
 #pragma unroll
-      for (int i = 0; i < NC; ++i) st.acc[i] = fmaf(w, v[u][i], st.acc[i]);
+      for (int i = 0; i < NC; ++i) st.mean[i] = fmaf(w[u] * inv, v[u][i], st.mean[i]);
     }
   }
 }
 
-// Writes a row whose sums are complete: O / l, and the log-sum-exp.  A row
-// that saw nothing (or only scores of -inf) is 0 and -inf.
+// Writes a row that has seen all its keys, and the log-sum-exp.  A row that
+// saw nothing (or only scores of -inf) is 0 and -inf.
 template <class T, int NC>
 __device__ __forceinline__ void store_row(const RowState<NC> &st, T *o, float *lse, int d, int lane) {
-  const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = lane + 32 * i;
-    if (c < d) o[c] = Elem<T>::from_float(st.acc[i] * inv);
+    if (c < d) o[c] = Elem<T>::from_float(st.l == 0.f ? 0.f : st.mean[i]);
   }
   if (lse && lane == 0) *lse = st.l == 0.f ? -INFINITY : (st.m + log2f(st.l)) * kLn2;
 }
 
 // The same row for a kernel whose own sums came out infinite or NaN in some
-// columns: those alone are written, the others keep their bits.
+// columns, by a hidden value that is, or past f32's range: those alone are
+// written, the others keep their bits.
 template <class T, int NC>
 __device__ __forceinline__ void mend_row(const RowState<NC> &st, T *o, int d, int lane) {
-  const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = lane + 32 * i;
-    if (c < d && !isfinite(Elem<T>::to_float(o[c]))) o[c] = Elem<T>::from_float(st.acc[i] * inv);
+    if (c < d && !isfinite(Elem<T>::to_float(o[c]))) o[c] = Elem<T>::from_float(st.l == 0.f ? 0.f : st.mean[i]);
   }
 }
 
@@ -157,7 +165,7 @@ __device__ __forceinline__ void join_warps(RowState<NC> &st, float *scratch /* W
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float *mine = scratch + warp * (kWide + 2);
 #pragma unroll
-  for (int i = 0; i < NC; ++i) mine[lane + 32 * i] = st.acc[i];
+  for (int i = 0; i < NC; ++i) mine[lane + 32 * i] = st.mean[i];
   if (lane == 0) {
     mine[kWide] = st.m;
     mine[kWide + 1] = st.l;
@@ -166,17 +174,24 @@ __device__ __forceinline__ void join_warps(RowState<NC> &st, float *scratch /* W
   if (warp != 0) return;
   float m = -INFINITY;
   for (int w = 0; w < WARPS; ++w) m = fmaxf(m, scratch[w * (kWide + 2) + kWide]);
-  RowState<NC> sum;
-  sum.m = m;
+  RowState<NC> all;
+  all.m = m;
+  const float base = m == -INFINITY ? 0.f : m;
+  float share[WARPS];
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    share[w] = scratch[w * (kWide + 2) + kWide + 1] * exp2f(scratch[w * (kWide + 2) + kWide] - base);
+    all.l += share[w];
+  }
+  const float inv = inverse(all.l);
+#pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     const float *s = scratch + w * (kWide + 2);
-    if (s[kWide + 1] == 0.f) continue;  // no keys: its sums are zero
-    const float a = exp2f(s[kWide] - (m == -INFINITY ? 0.f : m));
-    sum.l = fmaf(s[kWide + 1], a, sum.l);
+    if (s[kWide + 1] == 0.f) continue;  // no keys: its mean is zero
 #pragma unroll
-    for (int i = 0; i < NC; ++i) sum.acc[i] = fmaf(s[lane + 32 * i], a, sum.acc[i]);
+    for (int i = 0; i < NC; ++i) all.mean[i] = fmaf(s[lane + 32 * i], share[w] * inv, all.mean[i]);
   }
-  st = sum;
+  st = all;
 }
 
 }  // namespace attend

@@ -560,3 +560,33 @@ def test_prompt_tail_under_a_sink(s_q, s_kv, heads, window, d, gap, dtype, cuda_
         ys = (0, heads, 2 * heads - 1)
         ref = [np.array(a) for a in zip(*(R.attend(f64(q[0, i, y]), f64(k[0, js, y // 2]), f64(v[0, js, y // 2]), d ** -0.5) for y in ys))]
         check_tail(f64(o[0, i, list(ys)]), f64(lse[0, list(ys), i]), ref, dtype, len(js), 2.0 ** -32)
+
+
+# ---------------------------------------------------------------- values near f32's largest number
+
+@pytest.mark.parametrize("case", [(1, 3, 20, 4, 2, 64, 0, 0), (1, 200, 200, 8, 2, 128, 60, 2), (1, 150, 420, 10, 2, 64, 0, 0), (1, 9, 5000, 4, 2, 128, 0, 0),
+                                  (1, 20, 50, 2, 1, 256, 24, 2), (1, 130, 2000, 3, 1, 96, 1100, 200)])
+def test_prompt_values_whose_sums_leave_f32(case, cuda_device):
+    """A mean of bf16 values is in their range, whatever their sum is; beside them, ordinary columns."""
+    from lazy_compiler_b200 import serving as S
+    b, s_q, s_kv, hq, h, d, window, sinks = case
+    q, k, v = normal((b, s_q, hq, d), "bf16", 50), normal((b, s_kv, h, d), "bf16", 51), normal((b, s_kv, h, d), "bf16", 52)
+    v[..., :d // 2] = v[..., :d // 2].sign() * 3e38
+    v[..., 1] = 3.3e38
+    ref = R.window_attention(f64(q), f64(k), f64(v), d ** -0.5, window, sinks, [s_q] * b, [s_kv] * b)
+    o, lse = S.window_attention(q, k, v, window=window, sinks=sinks, return_lse=True)
+    R.check_attention(f64(o), f64(lse), ref, "bf16")
+
+
+@pytest.mark.parametrize("case", [([30, 7], 16, 4, 2, 64), ([700] * 64, 16, 8, 2, 128), ([9000], 16, 4, 2, 64), ([3000] + [40] * 59, 16, 32, 8, 128),
+                                  ([150, 40], 16, 4, 2, 256), ([90], 16, 2, 2, 17)])
+def test_token_values_whose_sums_leave_f32(case, cuda_device):
+    from lazy_compiler_b200 import serving as S
+    lens, page, hq, h, d = case
+    k, v, table = cache("bf16", lens, page, h, d, 2, 53)
+    q = normal((len(lens), hq, d), "bf16", 54)
+    v[..., :d // 2] = v[..., :d // 2].sign() * 3e38
+    v[..., 1] = 3.3e38
+    ref = R.paged_decode(f64(q), f64(k), f64(v), table, lens, d ** -0.5, 0, 0)
+    o, lse = S.paged_decode(q, k, v, ints(table), ints(lens), return_lse=True)
+    R.check_attention(f64(o), f64(lse), ref, "bf16")
