@@ -679,7 +679,8 @@ extern "C" int lc_cache_write_unless(const void *k, const void *v, void *k_pages
   if (int rc = check_maps(me, slots, width, pages, page_size)) return rc;
   if (most < 0 || kv_heads < 1 || row_bytes < 1) return fail(LC_ERR_INVALID, "%s: negative or zero size", me);
   if (!strides) return fail(LC_ERR_INVALID, "%s: null strides", me);
-  if (most > (1 << 30) || kv_heads > (1 << 16) || row_bytes > (1 << 12) || slots > 65535)
+  if (most > (1 << 30) || kv_heads > (1 << 16) || row_bytes > (1 << 12) || slots > 65535 ||
+      kWriteTokens * kv_heads * row_bytes > INT32_MAX - 256)  // a CTA counts its tokens' pieces in an int
     return fail(LC_ERR_UNSUPPORTED, "%s: shape too large", me);
   if (slots == 0 || most == 0 || width == 0 || pages == 0) return LC_OK;
   if (!k || !v || !k_pages || !v_pages || !table || !lens || !add) return fail(LC_ERR_INVALID, "%s: null buffer", me);

@@ -141,3 +141,15 @@ def test_what_requires_a_gradient():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA devices only"):
             call()
+
+
+@pytest.mark.parametrize("heads,row_bytes,status", [(1 << 16, 1 << 12, -5), ((1 << 16) - 1, 1 << 12, 0), (1 << 16, (1 << 12) - 1, 0)])
+def test_write_counts_that_leave_32_bits(heads, row_bytes, status):
+    """Eight tokens of 2^28 bytes: their pieces are counted in an int.  (No slots: what fits launches nothing.)"""
+    write = lambda slots: runtime.call("lc_cache_write", P, P, P, P, P, P, P, slots, 1, 1, 1, 16, heads, row_bytes, strides(12), NULL)  # noqa: E731
+    if not status:
+        write(0)
+        return
+    with pytest.raises(runtime.LcError) as err:
+        write(0)
+    assert err.value.status == status
