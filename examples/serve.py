@@ -73,6 +73,8 @@ def main(argv=None) -> float:
     for name, default in (("layers", 2), ("steps", 64), ("samples", 3), ("window", 128), ("sinks", 4)):
         ap.add_argument(f"--{name}", type=int, default=default)
     a = ap.parse_args(argv)
+    if a.layers < 1 or a.samples < 1 or a.steps < 1:
+        ap.error("--layers, --samples and --steps are at least 1")
     model = Model(a.layers)
     ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
     lengths, page = [37, 300, 5], 16
@@ -131,7 +133,7 @@ def main(argv=None) -> float:
         end.record()
     torch.cuda.synchronize()
     free = cache.check()
-    print(f"{slots} sequences, {a.steps - 1} steps: {begin.elapsed_time(end) / (a.steps - 1) * 1e3:.1f} us a step, "
+    print(f"{slots} sequences, {a.steps - 1} steps: {begin.elapsed_time(end) / max(1, a.steps - 1) * 1e3:.1f} us a step, "
           f"{cache.pool.shape[1] - free} pages in use")
 
     # the same sequences as prompts

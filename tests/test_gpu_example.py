@@ -17,3 +17,13 @@ def test_serving_example(options, cuda_device):
     serve = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(serve)
     assert serve.main(options) < 1e-2
+
+
+def test_serving_example_of_one_step(cuda_device):
+    """The first step runs outside the graph: with no other there is nothing to time."""
+    spec = importlib.util.spec_from_file_location("serve", ROOT / "examples" / "serve.py")
+    serve = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(serve)
+    assert serve.main(["--steps", "1"]) < 1e-2
+    with pytest.raises(SystemExit):
+        serve.main(["--steps", "0"])
