@@ -6,9 +6,8 @@
 // A query at position p sees key j when j <= p and (window == 0, or
 // j > p - window, or j < sinks): two intervals, [0, sink_end) and [lo, p].
 // Scores are kept in units of log2 (s * scale * log2 e), so a weight is
-// 2^(s - m); m, l and the output sums are f32.  The plain row form keeps the weighted mean
-// of the values so far in place of their sum: bf16 values reach f32's largest number, which
-// a sum of two of them would pass.
+// 2^(s - m); m, l and the output sums are f32.  m is the row's reference: its maximum so far
+// less a constant, which keeps the weights where the operand type and the sums hold them.
 #pragma once
 
 #include "common.cuh"
@@ -43,19 +42,35 @@ __host__ __device__ __forceinline__ Visible visible(int p, int window, int sinks
   return {sinks < lo ? sinks : lo, lo};
 }
 
+// bf16 values reach f32's largest number, which the sum of two of them passes: the weights
+// of bf16 rows are at most 2^-40 (2^-32 where the prompt form's maximum lags), so that the sum
+// of 2^30 does not.  They end at f32's smallest number, 2^-86 of the largest weight.
+constexpr float kLiftBf16 = -40.f;
+// What the weights of the plain row form, whose operands are f32, are lifted by.
+template <class T>
+constexpr float kRowLift = kLiftBf16;
+template <>
+constexpr float kRowLift<__half> = 0.f;
+
+// The log-sum-exp of a row with the reference m: its maximum again plus a small logarithm,
+// since log2 of a lifted l alone would be rounded like a number of the lift's size.
+template <int LIFT>
+__device__ __forceinline__ float lse_of(float m, float l) {
+  constexpr float kBack = LIFT < 0 ? (float)(1ll << (-LIFT & 63)) : 1.f / (float)(1ll << (LIFT & 63));
+  return ((m + LIFT) + log2f(l * kBack)) * kLn2;
+}
+
 // Running softmax of one query row of up to 32 NC columns spread over the lanes of a
-// warp: lane c holds the mean of columns c, c + 32, ...
+// warp: lane c holds output elements c, c + 32, ...
 template <int NC>
 struct RowState {
   float m = -INFINITY, l = 0.f;
-  float mean[NC];
+  float acc[NC];
   __device__ __forceinline__ RowState() {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) mean[i] = 0.f;
+    for (int i = 0; i < NC; ++i) acc[i] = 0.f;
   }
 };
-// 1 / l; 0 for a row that saw nothing, or only scores of -inf.
-__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 template <class T, int NC>
 __device__ __forceinline__ void load_row(float (&q)[NC], const T *src, int d, int lane, float factor) {
@@ -110,50 +125,46 @@ __device__ __forceinline__ void attend_keys(RowState<NC> &st, const float (&q)[N
     float m_new = st.m;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (real[u]) m_new = fmaxf(m_new, s[u]);
+      if (real[u]) m_new = fmaxf(m_new, s[u] - kRowLift<T>);
     const float base = m_new == -INFINITY ? 0.f : m_new;  // a row of -inf scores so far
-    const float kept = st.l * exp2f(st.m - base);
+    const float alpha = exp2f(st.m - base);
     st.m = m_new;
-    st.l = kept;
-    float w[U];
+    st.l *= alpha;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      w[u] = real[u] ? exp2f(s[u] - base) : 0.f;
-      st.l += w[u];
-    }
-    const float inv = inverse(st.l), old = kept * inv;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) st.mean[i] *= old;
+    for (int i = 0; i < NC; ++i) st.acc[i] *= alpha;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!real[u]) continue;
+      const float w = exp2f(s[u] - base);
+      st.l += w;
 #pragma unroll
-      for (int i = 0; i < NC; ++i) st.mean[i] = fmaf(w[u] * inv, v[u][i], st.mean[i]);
+      for (int i = 0; i < NC; ++i) st.acc[i] = fmaf(w, v[u][i], st.acc[i]);
     }
   }
 }
 
-// Writes a row that has seen all its keys, and the log-sum-exp.  A row that
-// saw nothing (or only scores of -inf) is 0 and -inf.
+// Writes a row whose sums are complete: O / l, and the log-sum-exp.  A row
+// that saw nothing (or only scores of -inf) is 0 and -inf.
 template <class T, int NC>
 __device__ __forceinline__ void store_row(const RowState<NC> &st, T *o, float *lse, int d, int lane) {
+  const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = lane + 32 * i;
-    if (c < d) o[c] = Elem<T>::from_float(st.l == 0.f ? 0.f : st.mean[i]);
+    if (c < d) o[c] = Elem<T>::from_float(st.acc[i] * inv);
   }
-  if (lse && lane == 0) *lse = st.l == 0.f ? -INFINITY : (st.m + log2f(st.l)) * kLn2;
+  if (lse && lane == 0) *lse = st.l == 0.f ? -INFINITY : lse_of<(int)kRowLift<T>>(st.m, st.l);
 }
 
 // The same row for a kernel whose own sums came out infinite or NaN in some
-// columns, by a hidden value that is, or past f32's range: those alone are
-// written, the others keep their bits.
+// columns: those alone are written, the others keep their bits.
 template <class T, int NC>
 __device__ __forceinline__ void mend_row(const RowState<NC> &st, T *o, int d, int lane) {
+  const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = lane + 32 * i;
-    if (c < d && !isfinite(Elem<T>::to_float(o[c]))) o[c] = Elem<T>::from_float(st.l == 0.f ? 0.f : st.mean[i]);
+    if (c < d && !isfinite(Elem<T>::to_float(o[c]))) o[c] = Elem<T>::from_float(st.acc[i] * inv);
   }
 }
 
@@ -165,7 +176,7 @@ __device__ __forceinline__ void join_warps(RowState<NC> &st, float *scratch /* W
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float *mine = scratch + warp * (kWide + 2);
 #pragma unroll
-  for (int i = 0; i < NC; ++i) mine[lane + 32 * i] = st.mean[i];
+  for (int i = 0; i < NC; ++i) mine[lane + 32 * i] = st.acc[i];
   if (lane == 0) {
     mine[kWide] = st.m;
     mine[kWide + 1] = st.l;
@@ -174,24 +185,17 @@ __device__ __forceinline__ void join_warps(RowState<NC> &st, float *scratch /* W
   if (warp != 0) return;
   float m = -INFINITY;
   for (int w = 0; w < WARPS; ++w) m = fmaxf(m, scratch[w * (kWide + 2) + kWide]);
-  RowState<NC> all;
-  all.m = m;
-  const float base = m == -INFINITY ? 0.f : m;
-  float share[WARPS];
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    share[w] = scratch[w * (kWide + 2) + kWide + 1] * exp2f(scratch[w * (kWide + 2) + kWide] - base);
-    all.l += share[w];
-  }
-  const float inv = inverse(all.l);
-#pragma unroll
+  RowState<NC> sum;
+  sum.m = m;
   for (int w = 0; w < WARPS; ++w) {
     const float *s = scratch + w * (kWide + 2);
-    if (s[kWide + 1] == 0.f) continue;  // no keys: its mean is zero
+    if (s[kWide + 1] == 0.f) continue;  // no keys: its sums are zero
+    const float a = exp2f(s[kWide] - (m == -INFINITY ? 0.f : m));
+    sum.l = fmaf(s[kWide + 1], a, sum.l);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) all.mean[i] = fmaf(s[lane + 32 * i], share[w] * inv, all.mean[i]);
+    for (int i = 0; i < NC; ++i) sum.acc[i] = fmaf(s[lane + 32 * i], a, sum.acc[i]);
   }
-  st = all;
+  st = sum;
 }
 
 }  // namespace attend

@@ -131,9 +131,9 @@ constexpr int kEndUnits = 1;
 // heads worse, 2000 tokens of 2 heads: 9.0 -> 10.7).
 constexpr int kSnap = 1;
 
-// The largest weight of a row is 2^kLift: far from f16's largest number, its sums in f32.
+// The largest weight of a row is 2^kLift: f16's far from its largest number, with sums in f32.
 template <class T>
-constexpr float kLift = 0.f;
+constexpr float kLift = kLiftBf16;
 template <>
 constexpr float kLift<__half> = 14.f;
 
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
       }
     }
     if (p.lse && tid < live)
-      p.lse[(int64_t)use.slot * p.q_heads + first + tid] = row_l[tid] == 0.f ? -INFINITY : (row_m[tid] + log2f(row_l[tid])) * kLn2;
+      p.lse[(int64_t)use.slot * p.q_heads + first + tid] = row_l[tid] == 0.f ? -INFINITY : lse_of<(int)kLift<T>>(row_m[tid], row_l[tid]);
     return odd;
   };
   // What came out infinite or NaN is computed again one key at a time: the
@@ -901,7 +901,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodePara
     odd = !isfinite(v);
     out[tid] = Elem<T>::from_float(v);
   }
-  if (p.lse && tid == 0) p.lse[(int64_t)slot * p.q_heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  if (p.lse && tid == 0) p.lse[(int64_t)slot * p.q_heads + h] = sum == 0.f ? -INFINITY : lse_of<(int)kLift<T>>(top, sum);
   if (__syncthreads_or(odd)) {  // as in decode_kernel
     RowState<DP / 32> st;
     plain_row<T, kJoinWarps>(p, slot, h, head, st, scratch);

@@ -136,9 +136,9 @@ constexpr uint32_t kOCol = 256;
 constexpr float kRescale = 8.0f;            // log2 units a row's maximum may lag behind
 // A row's reference is its maximum less kLift, so that with the lag f16 weights reach 2^15 (its
 // largest number is just under 2^16).  They end at 2^-25, and a row's largest weight is 2^7 or more:
-// what is lost is 2^-32 of it a key, 2^-25 without the lift.  bf16 has f32's range.
+// what is lost is 2^-32 of it a key, 2^-25 without the lift.  bf16 has f32's range, and is kept down.
 template <class T>
-constexpr float kLift = 0.f;
+constexpr float kLift = kLiftBf16;
 template <>
 constexpr float kLift<__half> = 7.f;
 constexpr int kChunkBytes = 128 * 64 * 2;   // 128 rows x 64 columns, one swizzle span
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t inv2 = pack2(inv, inv);
         T *out = static_cast<T *>(p.o) + it.b * p.os[0] + i * p.os[1] + h * p.os[2];
         if (p.lse && stored && n == it.n)
-          p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
+          p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? lse_of<(int)kLift<T>>(m, l) : -INFINITY;
         if (!wait_all(&o_done[t], (g0 + n - 1) & 1, abort, tp, kErrTimeoutEpilogue)) {
           ok = false;
           break;
@@ -1077,7 +1077,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Windo
     }
   }
   if (p.lse && stored && (lane & 3) == 0 && (!DEEP || warp == 0))
-    p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
+    p.lse[((int64_t)it.b * p.q_heads + h) * p.s_q + i] = some ? lse_of<(int)kLift<T>>(m, l) : -INFINITY;
   if (DEEP) __syncthreads();  // the other warps' columns are there: mended once or more, but alike
   const unsigned odd_lanes = __ballot_sync(0xffffffffu, odd);
   if (odd_lanes) mend_rows<T, DP / 32>(p, (lane & 3) == 0 && (odd_lanes >> lane & 0xf) != 0, it.b, it.hk, pos, i, h);

@@ -590,3 +590,17 @@ def test_token_values_whose_sums_leave_f32(case, cuda_device):
     ref = R.paged_decode(f64(q), f64(k), f64(v), table, lens, d ** -0.5, 0, 0)
     o, lse = S.paged_decode(q, k, v, ints(table), ints(lens), return_lse=True)
     R.check_attention(f64(o), f64(lse), ref, "bf16")
+
+
+def test_large_values_take_no_other_path(cuda_device):
+    """Rows of values near f32's largest number are those of the same values 2^60 smaller, bit by bit."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    q, k = normal((2, 300, 8, 128), "bf16", 55), normal((2, 300, 2, 128), "bf16", 56)
+    v = normal((2, 300, 2, 128), "bf16", 57).clamp(-3.9, 3.9)
+    small = S.window_attention(q, k, v * 2.0 ** 66, window=90, sinks=3)
+    assert torch.equal(S.window_attention(q, k, v * 2.0 ** 126, window=90, sinks=3), small * 2.0 ** 60)
+    pages = [x[:, :288].reshape(2 * 18, 16, 2, 128).transpose(1, 2).contiguous() for x in (k, v)]
+    table, lens = torch.arange(36, dtype=torch.int32, device="cuda").view(2, 18), ints([288, 203])
+    small = S.paged_decode(q[:, 0], pages[0], pages[1] * 2.0 ** 66, table, lens)
+    assert torch.equal(S.paged_decode(q[:, 0], pages[0], pages[1] * 2.0 ** 126, table, lens), small * 2.0 ** 60)
