@@ -90,9 +90,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // (O, m, l) per CTA in the workspace; the CTA that arrives last joins them in CTA
 // order (the run boundaries depend on the lengths alone, so results repeat), or,
 // where a segment may span kDeepParts of them or more, a second kernel with a CTA per row (one
-// sequence of 131072 with one key-value head, 444 parts: 28 us, 167 with the last CTA, which
+// sequence of 131072 with one key-value head, 444 parts: 21 us, 167 with the last CTA, which
 // reads 1.9 MB alone; 4 of 1 to 8192 tokens, 8 heads: 20.3 us, 24.7 with it from 16 parts on; one
-// of 512: 9.2, 11.1).
+// of 512: 9.2, 11.1).  The host chooses, by the table's width and an even share of the CTAs: it does
+// not know the lengths.  So one long sequence among many short ones is joined by the last CTAs (64
+// slots, 8 heads, one of 131072 tokens, the others 100: 97 us where its bytes take 87; of 32768: 40, 25).
 //
 // In a CTA each warp takes 16 keys of every tile and is on its own until the
 // segment ends: it copies its keys' rows (cp.async, 16 bytes per lane, zeros where
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(DecodeParams
 // and a long tail below a sink that outweighs it is not lost.
 // Bound by HBM.  Measured, 32/8 heads of 128, bf16: 64 sequences of 1 to 8192 tokens
 // in pages of 16: 167 us, 6440 GB/s, the rate of a copy; 64/8, f16, 100003 and 131072
-// tokens: 149 us, 6360 GB/s.  Three CTAs per SM of two stages against two of three:
+// tokens: 147 us, 6430 GB/s.  Three CTAs per SM of two stages against two of three:
 // the warps' own latency (a tile is a chain of some 500 instructions) needs 12 of them
 // (177 us with 8).  Heads of 64, half the bytes a tile and nearly its instructions: four CTAs of
 // three stages (1 to 8192 tokens, before kEndUnits: 98 us; 105 with three of four, 98 with five of two, 111 with six of two;
