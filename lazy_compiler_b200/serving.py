@@ -193,8 +193,9 @@ class PagedCache:
         self.page_size = page_size
         # the maps, and those that a fork writes; each set is one block of memory
         self._blocks = [torch.zeros(slots * width + slots + pages + 2, **ints) for _ in range(2)]
-        self.maps, self._spare = (CacheMaps(t.view(slots, width), n, r, s) for t, n, r, s in
+        self._own, self._spare = (CacheMaps(t.view(slots, width), n, r, s) for t, n, r, s in
                                   (b.split([slots * width, slots, pages, 2]) for b in self._blocks))
+        self.maps = self._own
         self.maps.table.fill_(-1)
         self.maps.status[1] = pages
         self._refusals = torch.zeros(2, **ints)
@@ -218,6 +219,7 @@ class PagedCache:
         cache_fork(self.pool, self.maps, parent, into=self._spare, refusals=self._refusals, stream=stream)
         with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream, self.pool.device)):
             self._blocks[0].copy_(self._blocks[1])
+        self.maps = self._own  # where the caller had put others in their place
 
     def release(self, gone, stream=None) -> None:
         """Empties slots (:func:`cache_release`)."""

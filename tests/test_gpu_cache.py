@@ -472,3 +472,15 @@ def test_a_captured_step_goes_on_after_a_fork(fork_captured, cuda_device):
             pool = torch.from_numpy(model.pool).cuda().half()
             want = S.paged_decode(q, pool[0], pool[1], ints(model.table), ints(model.lens))
             assert torch.equal(out, want)
+
+
+def test_fork_of_maps_that_the_caller_put_in(cuda_device):
+    """Maps made by the functions and assigned to a cache are what its fork goes on from."""
+    import torch
+    from lazy_compiler_b200 import serving as S
+    cache = S.PagedCache(1, 8, 4, 1, 16, 2, 4, dtype=torch.float16)
+    first = cache.maps
+    cache.maps = S.cache_extend(cache.maps, ints([5, 0]), page_size=4)
+    cache.fork(ints([0, 0]))
+    assert cache.maps is first and cache.maps.lens.tolist() == [5, 5] and cache.maps.table.tolist() == [[0, 1, -1, -1], [0, 2, -1, -1]]
+    assert cache.check() == 5
