@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) window_row_kernel(WindowParams
 // output's own rounding (and kLift's, where a row's weights are many and small).
 // Bound by a tile's chain of softmax and products (3500 cycles a block of 128 keys, of
 // which the tensor pipe needs 2080 for both tiles), in long runs by the power cap.
-// Measured, f16, 32/8 heads of 128: 32768 tokens, window 4096: 1.75 ms, 1180 TFLOP/s;
+// Measured, f16, 32/8 heads of 128: 32768 tokens, window 4096: 1.77 ms, 1170 TFLOP/s;
 // bf16, 4 ragged chunks of up to 777 over 4001 keys, window 1024: 51 us, 685 TFLOP/s.
 using namespace sm100;
 using namespace softmax;
