@@ -257,7 +257,7 @@ def _logits(case, gen, cuda):
     """Logits with a head of some likely tokens over a bulk of unlikely ones, rows of different sharpness, and what each
     request asks for."""
     rows, vocab = case["rows"], case["vocab"]
-    x = torch.randn(rows, vocab, generator=cuda, device=DEVICE) * 1.5
+    x = torch.randn(rows, vocab, generator=cuda, device=DEVICE) * 1.5 - 2
     likely = min(vocab, 200)
     first = torch.randint(0, vocab, (rows, 1), generator=gen).to(DEVICE)
     at = torch.randperm(vocab, generator=gen).to(DEVICE)[(first + torch.arange(likely, device=DEVICE)) % vocab]
