@@ -731,6 +731,48 @@ int lc_cache_copy(void *pool, int64_t planes, int64_t kv_heads, int64_t token_by
                   const int64_t *strides, const int32_t *src, const int32_t *dst, int64_t n,
                   int64_t pages, int64_t page_size, void *stream);
 
+/* Positions as rotations. Of every head's d elements the first `rot` are pairs, (i, i + rot / 2) or, interleaved,
+ * (2 i, 2 i + 1); pair (a, b) at position p becomes (a cos - b sin, a sin + b cos) * magnitude with the angle of
+ * p * turns[i] / 2^64 turns (turns: device, rot / 2 of them; a product is taken modulo 2^64, so the angle is exact at
+ * any position). The other elements pass. dtype is LC_F32, LC_F16 or LC_BF16, the arithmetic f32, rounded once; heads
+ * of up to 1024 elements. x[batch, tokens, heads, d], positions[batch, tokens]; out may be x itself (with its strides).
+ * strides, in elements: batch, token, head of x and of out; batch, token of positions (8 values). */
+int lc_rotate(int dtype, const void *x, void *out, const int32_t *positions, const int64_t *turns,
+              int64_t batch, int64_t tokens, int64_t heads, int64_t d, int64_t rot, int interleaved,
+              float magnitude, const int64_t *strides, void *stream);
+
+/* lc_cache_write with the rotation on the way: of the newest add[i] <= most tokens of each slot the keys, turned to
+ * positions lens[i] - add[i] and on, and the values go to their pages, and the queries, turned alike, to out (q_heads
+ * may be 0, then q and out are not read). Rows of out behind add[i] are left as they were, or zeroed with zero_rest.
+ * Where the device word *refused (null: none) is not 0 no token counts as new. out may be q itself. strides, in
+ * elements: slot, token, head of q, k, v and out; page, head, token of k_pages and of v_pages (18 values). */
+int lc_cache_append(int dtype, const void *q, const void *k, const void *v, void *out, void *k_pages,
+                    void *v_pages, const int32_t *table, const int32_t *lens, const int32_t *add,
+                    const int32_t *refused, const int64_t *turns, int64_t slots, int64_t most,
+                    int64_t width, int64_t pages, int64_t page_size, int64_t q_heads, int64_t kv_heads,
+                    int64_t d, int64_t rot, int interleaved, float magnitude, int zero_rest,
+                    const int64_t *strides, void *stream);
+
+/* Which slots begin with the same pages: leader[i] is the lowest slot whose first page is that of slot i and full in
+ * both (i itself where there is none, or i has no full page); shared[i] the tokens of the full pages that all slots of
+ * that leader have in common (0 for a slot alone); order lists the slots by leader, each group in slot order. At most
+ * 8192 slots. Changes no map. */
+int lc_cache_prefixes(const int32_t *table, const int32_t *lens, int32_t *leader, int32_t *shared,
+                      int32_t *order, int64_t slots, int64_t width, int64_t pages, int64_t page_size,
+                      void *stream);
+
+/* One token of each row of logits[rows, vocab] (LC_F32, LC_F16 or LC_BF16; `stride` elements from row to row):
+ * with weights w_i = exp((x_i - max) / temperature), the top_k largest; of these the shortest run from the largest on
+ * that holds top_p of their sum; of these those with w_i >= min_p; and of what is left the first index at which the
+ * sum in index order passes uniform[row] times its total. Equal logits are taken in index order. temperature <= 0:
+ * the largest. top_k <= 0 or >= vocab, top_p >= 1, min_p <= 0: all. NaN logits and -infinity are never taken; where
+ * there is nothing else, the token is -1 and logprob -infinity. Each of the four is one value a row, or null and the
+ * value *_all for all rows. logprob (may be null): the logarithm of the token's share of what was left. */
+int lc_sample(int dtype, const void *logits, const float *uniform, const float *temperature,
+              const int32_t *top_k, const float *top_p, const float *min_p, float temperature_all,
+              int64_t top_k_all, float top_p_all, float min_p_all, int32_t *token, float *logprob,
+              int64_t rows, int64_t vocab, int64_t stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,7 @@
 //   release  drops whole sequences, or the pages a sliding window has left behind
 //   compact  moves the pages in use onto the lowest numbers
 //   copy     copies listed pages
+//   prefixes tells which slots begin with the same pages, and how far (it changes nothing)
 //
 // A map kernel is one cluster, whose barrier separates the phases where a grid would
 // need another launch.  It is a chain of some six dependent reads, each as long as an
@@ -587,6 +588,89 @@ __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
   }
 }
 
+// ---------------------------------------------------------------- prefixes
+
+struct PrefixParams {
+  const int *table, *lens;
+  int *leader, *shared, *order;
+  int *least;  // scratch: of each leader, the pages that its group has in common so far
+  int slots, width, pages, page_size;
+};
+constexpr int kCompare = 16;  // table entries of a lane at a time
+
+// A group is the slots whose first page, a full one, is the same; its lowest slot leads. What they share is the
+// least number of full pages at which every slot's row is the leader's. Rows are compared in pieces of 512
+// entries, dealt to all warps, none behind a difference that is known. Ranks by counting: slots^2 / 8192 steps a
+// thread at most, and slots are few.
+__global__ void __launch_bounds__(kMostThreads, 1) prefixes_kernel(PrefixParams p) {
+  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ int keys[kMostForkSlots];  // first pages, then leaders
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warps = cluster.num_blocks() * (blockDim.x >> 5);
+  const int warp = cluster.block_rank() * (blockDim.x >> 5) + (tid >> 5);
+  auto full_pages = [&](int s) {
+    const int64_t most = (int64_t)p.width * p.page_size;
+    return (int)min((int64_t)max(p.lens[s], 0), most) / p.page_size;
+  };
+  for (int s = tid; s < p.slots; s += blockDim.x) {
+    const int page = full_pages(s) > 0 ? p.table[(int64_t)s * p.width] : -1;
+    keys[s] = (unsigned)page < (unsigned)p.pages ? page : -1;
+  }
+  __syncthreads();
+  for (int s = warp; s < p.slots; s += warps) {
+    int lowest = s;
+    if (keys[s] >= 0)
+      for (int j = lane; j < s; j += 32)
+        if (keys[j] == keys[s]) {
+          lowest = j;
+          break;
+        }
+    lowest = __reduce_min_sync(0xffffffffu, lowest);
+    if (lane == 0) {
+      p.leader[s] = lowest;
+      p.least[s] = full_pages(s);
+    }
+  }
+  cluster.sync();
+  constexpr int kPiece = 32 * kCompare;
+  const int pieces = (p.width + kPiece - 1) / kPiece;
+  for (int64_t x = warp; x < (int64_t)p.slots * pieces; x += warps) {
+    const int s = (int)(x / pieces), begin = (int)(x - (int64_t)s * pieces) * kPiece;
+    const int leader = __ldcg(p.leader + s);
+    if (leader == s) continue;
+    const int end = min(min(full_pages(s), full_pages(leader)), begin + kPiece);
+    if (begin == 0 && lane == 0) atomicMin(p.least + leader, full_pages(s));
+    if (begin >= end || begin >= __ldcg(p.least + leader)) continue;
+    const int *a = p.table + (int64_t)s * p.width + begin, *b = p.table + (int64_t)leader * p.width + begin;
+    int other = end;
+#pragma unroll
+    for (int i = kCompare - 1; i >= 0; --i) {
+      const int j = lane + 32 * i;
+      if (begin + j < end && a[j] != b[j]) other = begin + j;
+    }
+    other = __reduce_min_sync(0xffffffffu, other);
+    if (other < end && lane == 0) atomicMin(p.least + leader, other);
+  }
+  cluster.sync();
+  for (int s = tid; s < p.slots; s += blockDim.x) keys[s] = __ldcg(p.leader + s);
+  __syncthreads();
+  for (int s = warp; s < p.slots; s += warps) {
+    int before = 0, members = 0;
+    for (int j = lane; j < p.slots; j += 32) {
+      const int same = keys[j] == keys[s];
+      before += keys[j] < keys[s] || (same && j < s);
+      members += same;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    members = __reduce_add_sync(0xffffffffu, members);
+    if (lane == 0) {
+      p.shared[s] = members > 1 ? __ldcg(p.least + keys[s]) * p.page_size : 0;
+      p.order[before] = s;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- host side
 
 template <class Params>
@@ -796,4 +880,19 @@ extern "C" int lc_cache_copy(void *pool, int64_t planes, int64_t kv_heads, int64
   if (!src || !dst) return fail(LC_ERR_INVALID, "%s: null buffer", me);
   c.src = src, c.dst = dst, c.n = (int)n;
   return launch_copy(me, c, n, as_stream(stream));
+}
+
+extern "C" int lc_cache_prefixes(const int32_t *table, const int32_t *lens, int32_t *leader, int32_t *shared, int32_t *order,
+                                 int64_t slots, int64_t width, int64_t pages, int64_t page_size, void *stream) {
+  using namespace lc;
+  const char *me = "lc_cache_prefixes";
+  if (int rc = check_maps(me, slots, width, pages, page_size)) return rc;
+  if (slots > kMostForkSlots) return fail(LC_ERR_UNSUPPORTED, "%s: %lld slots, at most %d", me, (long long)slots, kMostForkSlots);
+  if (slots == 0) return LC_OK;
+  if (!lens || !leader || !shared || !order || (width > 0 && !table)) return fail(LC_ERR_INVALID, "%s: null buffer", me);
+  cudaStream_t s = as_stream(stream);
+  void *scratch = nullptr;
+  if (int rc = scratch_buffer(s, kScratchSlot, (size_t)slots * 4, &scratch)) return rc;
+  const PrefixParams p = {table, lens, leader, shared, order, static_cast<int *>(scratch), (int)slots, (int)width, (int)pages, (int)page_size};
+  return launch_maps(me, prefixes_kernel, slots * width, s, p);
 }

@@ -15,6 +15,7 @@
 
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "lazyb200.h"
 
@@ -32,6 +33,14 @@ struct Entries {
   decltype(&lc_cache_copy) cache_copy;
 } lib;
 constexpr int kEntries = sizeof(Entries) / sizeof(void *);
+// Those of the operators around the attention (bind_steps).
+struct StepEntries {
+  decltype(&lc_rotate) rotate;
+  decltype(&lc_cache_append) cache_append;
+  decltype(&lc_cache_prefixes) cache_prefixes;
+  decltype(&lc_sample) sample;
+} steps;
+constexpr int kStepEntries = sizeof(StepEntries) / sizeof(void *);
 
 std::string piece(const std::string &s) { return s; }
 std::string piece(const char *s) { return s; }
@@ -157,6 +166,15 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   arguments(n, kEntries);
   void **to = reinterpret_cast<void **>(&lib);
   for (int i = 0; i < kEntries; ++i) to[i] = reinterpret_cast<void *>(static_cast<intptr_t>(integer(a[i])));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject *bind_steps(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, kStepEntries);
+  void **to = reinterpret_cast<void **>(&steps);
+  for (int i = 0; i < kStepEntries; ++i) to[i] = reinterpret_cast<void *>(static_cast<intptr_t>(integer(a[i])));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -373,6 +391,153 @@ PyObject *cache_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- positions
+
+int element_dtype(const at::Tensor &t, const char *what) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return LC_F32;
+    case at::kHalf: return LC_F16;
+    case at::kBFloat16: return LC_BF16;
+    default: refuse(what, ": ", name_of(t.scalar_type()), " is not float32, float16 or bfloat16");
+  }
+}
+// frequencies, interleaved, magnitude of a Rotary
+struct Rotary {
+  const int64_t *turns;
+  int64_t rot;
+  int interleaved;
+  float magnitude;
+};
+Rotary rotary_of(PyObject *const *a, const at::Tensor &like, int64_t d) {
+  const at::Tensor &t = tensor(a[0], "rotary");
+  check(t, "rotary", like, at::kLong, {t.numel()});
+  if (!t.is_contiguous()) refuse("rotary: must be contiguous");
+  if (2 * t.numel() > d) refuse("rotary: ", 2 * t.numel(), " elements of a head turn, it has ", d);
+  const double magnitude = PyFloat_AsDouble(a[2]);
+  if (magnitude == -1.0 && PyErr_Occurred()) throw python_error();
+  return {static_cast<const int64_t *>(t.data_ptr()), 2 * t.numel(), truth(a[1]), (float)magnitude};
+}
+
+// x, positions, rotary (3), out, stream
+PyObject *rotate(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 7);
+  const at::Tensor &x = tensor(a[0], "x"), &positions = tensor(a[1], "positions");
+  check_no_gradient(x, "x");
+  const int dtype = element_dtype(x, "x");
+  check_cuda(x, "x");
+  check_axes(x, "x", 4);
+  check_inner(x, "x");
+  check(positions, "positions", x, at::kInt, {x.size(0), x.size(1)});
+  const Rotary r = rotary_of(a + 2, x, x.size(3));
+  const at::Tensor *given = maybe(a[5], "out");
+  if (given) {
+    check(*given, "out", x, x.scalar_type(), x.sizes());
+    check_out(*given, "out");
+    check_no_gradient(*given, "out");
+    check_inner(*given, "out");
+  }
+  const On on(a[6], x);
+  const at::Tensor out = given ? *given : fresh(x.sizes(), x.scalar_type(), x);
+  const int64_t strides[8] = {x.stride(0),   x.stride(1),   x.stride(2),         out.stride(0),
+                              out.stride(1), out.stride(2), positions.stride(0), positions.stride(1)};
+  const int status = steps.rotate(dtype, ptr(x), ptr(out), ptr<int32_t>(positions), r.turns, x.size(0), x.size(1), x.size(2), x.size(3),
+                                  r.rot, r.interleaved, r.magnitude, strides, on.stream);
+  if (status) return PyLong_FromLong(status);
+  if (given) written(out);
+  return given ? Py_NewRef(a[5]) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// q (or None), k, v, k_pages, v_pages, maps (4), add, rotary (3), out, refusals, stream
+PyObject *cache_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 16);
+  const at::Tensor *q = maybe(a[0], "q");
+  const at::Tensor &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &kp = tensor(a[3], "k_pages"), &vp = tensor(a[4], "v_pages");
+  const Maps m = maps_of(a + 5, "maps");
+  const at::Tensor &add = tensor(a[9], "add");
+  check_ints(add, "add", m.table, {m.slots});
+  if (q) check_no_gradient(*q, "q");
+  check_no_gradient(k, "k");
+  check_no_gradient(v, "v");
+  check_no_gradient(kp, "k_pages");
+  check_no_gradient(vp, "v_pages");
+  const int dtype = element_dtype(k, "k");
+  check_axes(k, "k", 4);
+  check_axes(kp, "k_pages", 4);
+  const int64_t most = k.size(1), heads = k.size(2), d = k.size(3), page_size = kp.size(2);
+  check(k, "k", m.table, k.scalar_type(), {m.slots, most, heads, d});
+  check(v, "v", m.table, k.scalar_type(), {m.slots, most, heads, d});
+  check(kp, "k_pages", m.table, k.scalar_type(), {m.pages, heads, page_size, d});
+  check(vp, "v_pages", m.table, k.scalar_type(), {m.pages, heads, page_size, d});
+  check_out(kp, "k_pages");
+  check_out(vp, "v_pages");
+  const Rotary r = rotary_of(a + 10, m.table, d);
+  const at::Tensor *given = maybe(a[13], "out");
+  int64_t q_heads = 0;
+  if (q) {
+    check_axes(*q, "q", 4);
+    q_heads = q->size(2);
+    check(*q, "q", m.table, k.scalar_type(), {m.slots, most, q_heads, d});
+    if (given) {
+      check(*given, "out", m.table, k.scalar_type(), q->sizes());
+      check_out(*given, "out");
+      check_no_gradient(*given, "out");
+    }
+  } else if (given) {
+    refuse("out: there are no queries");
+  }
+  const int32_t *refused = refusals_of(a[14], m);
+  refused = refused ? refused + 1 : m.status.defined() ? ptr<int32_t>(m.status) : nullptr;
+  const On on(a[15], m.table);
+  const at::Tensor out = given ? *given : q ? fresh(q->sizes(), k.scalar_type(), k) : at::Tensor();
+  const at::Tensor *views[6] = {q, &k, &v, q ? &out : nullptr, &kp, &vp};
+  const char *names[6] = {"q", "k", "v", "out", "k_pages", "v_pages"};
+  int64_t strides[18] = {0};
+  for (int x = 0; x < 6; ++x) {
+    if (!views[x]) continue;
+    check_inner(*views[x], names[x]);
+    for (int i = 0; i < 3; ++i) strides[x * 3 + i] = views[x]->stride(i);
+  }
+  const int status = steps.cache_append(dtype, ptr(q), ptr(k), ptr(v), ptr(views[3]), ptr(kp), ptr(vp), ptr<int32_t>(m.table),
+                                        ptr<int32_t>(m.lens), ptr<int32_t>(add), refused, r.turns, m.slots, most, m.width, m.pages,
+                                        page_size, q_heads, heads, d, r.rot, r.interleaved, r.magnitude, !given, strides, on.stream);
+  if (status) return PyLong_FromLong(status);
+  written(kp);
+  written(vp);
+  if (given) written(out);
+  if (!q) Py_RETURN_NONE;
+  return given ? Py_NewRef(a[13]) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// maps (4), page_size, into (3 or None), stream
+PyObject *cache_prefixes(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 9);
+  const Maps m = maps_of(a, "maps");
+  const On on(a[8], m.table);
+  at::Tensor to[3];
+  for (int i = 0; i < 3; ++i) {
+    if (a[5 + i] == Py_None) {
+      to[i] = fresh({m.slots}, at::kInt, m.table);
+    } else {
+      to[i] = tensor(a[5 + i], "into");
+      check_ints(to[i], "into", m.table, {m.slots});
+      written(to[i]);
+    }
+  }
+  const int status = steps.cache_prefixes(ptr<int32_t>(m.table), ptr<int32_t>(m.lens), ptr<int32_t>(to[0]), ptr<int32_t>(to[1]),
+                                          ptr<int32_t>(to[2]), m.slots, m.width, m.pages, integer(a[4]), on.stream);
+  if (status) return PyLong_FromLong(status);
+  PyObject *parts[3] = {THPVariable_Wrap(to[0]), THPVariable_Wrap(to[1]), THPVariable_Wrap(to[2])};
+  PyObject *all = PyTuple_Pack(3, parts[0], parts[1], parts[2]);
+  for (PyObject *p : parts) Py_DECREF(p);
+  return all;
+  END_HANDLE_TH_ERRORS
+}
+
 // pool, maps (4), parent, into (4), refusals, stream
 PyObject *cache_fork(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -442,9 +607,63 @@ PyObject *cache_copy(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- tokens
+
+// One value for all rows, or a tensor of one a row.
+template <class Value, class Number>
+struct Asked {
+  const Value *each = nullptr;
+  Number all = 0;
+  Asked(PyObject *o, const char *what, const at::Tensor &like, at::ScalarType type) {
+    if (THPVariable_Check(o)) {
+      const at::Tensor &t = THPVariable_Unpack(o);
+      check(t, what, like, type, {like.size(0)});
+      if (!t.is_contiguous()) refuse(what, ": must be contiguous");
+      each = static_cast<const Value *>(t.data_ptr());
+    } else if constexpr (std::is_integral_v<Number>) {
+      all = integer(o);
+    } else {
+      all = PyFloat_AsDouble(o);
+      if (all == -1.0 && PyErr_Occurred()) throw python_error();
+    }
+  }
+};
+
+// logits, uniform, temperature, top_k, top_p, min_p, out, return_logprob, stream
+PyObject *sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 9);
+  const at::Tensor &logits = tensor(a[0], "logits"), &uniform = tensor(a[1], "uniform");
+  check_no_gradient(logits, "logits");
+  const int dtype = element_dtype(logits, "logits");
+  check_cuda(logits, "logits");
+  check_axes(logits, "logits", 2);
+  check_inner(logits, "logits");
+  const int64_t rows = logits.size(0);
+  check(uniform, "uniform", logits, at::kFloat, {rows});
+  if (!uniform.is_contiguous()) refuse("uniform: must be contiguous");
+  const Asked<float, double> temperature(a[2], "temperature", logits, at::kFloat), top_p(a[4], "top_p", logits, at::kFloat),
+      min_p(a[5], "min_p", logits, at::kFloat);
+  const Asked<int32_t, int64_t> top_k(a[3], "top_k", logits, at::kInt);
+  const at::Tensor *given = maybe(a[6], "out");
+  if (given) check_ints(*given, "out", logits, {rows});
+  const On on(a[8], logits);
+  const at::Tensor out = given ? *given : fresh({rows}, at::kInt, logits);
+  const at::Tensor logprob = truth(a[7]) ? fresh({rows}, at::kFloat, logits) : at::Tensor();
+  const int status = steps.sample(dtype, ptr(logits), ptr<float>(uniform), temperature.each, top_k.each, top_p.each, min_p.each,
+                                  (float)temperature.all, top_k.all, (float)top_p.all, (float)min_p.all, ptr<int32_t>(out),
+                                  logprob.defined() ? ptr<float>(logprob) : nullptr, rows, logits.size(1), logits.stride(0), on.stream);
+  if (status) return PyLong_FromLong(status);
+  if (given) written(out);
+  return outputs(out, a[6], logprob);
+  END_HANDLE_TH_ERRORS
+}
+
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind),         METHOD(window_attention), METHOD(paged_decode),  METHOD(cache_extend), METHOD(cache_write),
-                         METHOD(cache_fork),   METHOD(cache_release),    METHOD(cache_compact), METHOD(cache_copy),   {nullptr, nullptr, 0, nullptr}};
+                         METHOD(cache_fork),   METHOD(cache_release),    METHOD(cache_compact), METHOD(cache_copy),
+                         METHOD(bind_steps),   METHOD(rotate),           METHOD(cache_append),  METHOD(cache_prefixes),
+                         METHOD(sample),       {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving", "Calls of lazy_compiler_b200.serving.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -83,6 +83,10 @@ SIGNATURES = {
     "lc_cache_release": [_P] * 4 + [_I64, _I64, _P] + [_I64] * 4 + [_P],
     "lc_cache_compact": [_P, _I64, _I64, _I64, _P] + [_P] * 7 + [_I64] * 4 + [_P],
     "lc_cache_copy": [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P],
+    "lc_rotate": [_INT] + [_P] * 4 + [_I64] * 5 + [_INT, ctypes.c_float, _P, _P],
+    "lc_cache_append": [_INT] + [_P] * 11 + [_I64] * 9 + [_INT, ctypes.c_float, _INT, _P, _P],
+    "lc_cache_prefixes": [_P] * 5 + [_I64] * 4 + [_P],
+    "lc_sample": [_INT] + [_P] * 6 + [ctypes.c_float, _I64, ctypes.c_float, ctypes.c_float] + [_P] * 2 + [_I64] * 3 + [_P],
 }
 
 # pointwise programs (include/lazyb200.h lc_pw_program)

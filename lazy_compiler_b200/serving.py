@@ -28,6 +28,8 @@ them grow; so graphs captured on one stream, and calls on that stream, may not r
 from __future__ import annotations
 
 import ctypes
+import math
+from fractions import Fraction
 from typing import NamedTuple
 
 import torch
@@ -37,6 +39,7 @@ from . import runtime
 # the order in which csrc/serving_ext.cpp takes the entry points
 _ENTRIES = ("lc_window_attention", "lc_paged_decode", "lc_cache_extend_recorded", "lc_cache_write_unless",
             "lc_cache_fork_recorded", "lc_cache_release", "lc_cache_compact", "lc_cache_copy")
+_STEP_ENTRIES = ("lc_rotate", "lc_cache_append", "lc_cache_prefixes", "lc_sample")
 
 
 def _extension():
@@ -46,7 +49,8 @@ def _extension():
         from . import _serving
     except ImportError as e:
         raise RuntimeError("the extension module _serving is not built; run `python -m lazy_compiler_b200.build`") from e
-    _serving.bind(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in _ENTRIES))
+    for bind, names in ((_serving.bind, _ENTRIES), (_serving.bind_steps, _STEP_ENTRIES)):
+        bind(*(ctypes.cast(getattr(library, name), ctypes.c_void_p).value for name in names))
     return _serving
 
 
@@ -100,6 +104,104 @@ def paged_decode(q, k_pages, v_pages, table, lens, *, window: int = 0, sinks: in
     return r
 
 
+# ---------------------------------------------------------------- positions
+
+class Rotary:
+    """How positions enter queries and keys: the first ``dim`` elements of a head are pairs, ``(i, i + dim / 2)`` or
+    ``interleaved`` ``(2 i, 2 i + 1)``, and pair ``i`` at position ``p`` turns by the angle ``p f[i]``.
+
+    ``f[i]`` is ``base ** (-2 i / dim)``, for contexts longer than trained by ``factor`` with one of the ``scaling``:
+
+    * ``"linear"`` — ``f / factor``, every position interpolated;
+    * ``"base"`` — ``base * factor ** (dim / (dim - 2))``: the slowest pair is interpolated, the fastest stays;
+    * ``"bands"`` — pairs that turn ``fast`` times or more over the ``trained`` context stay, those that turn ``slow``
+      times or fewer are interpolated, a linear ramp in the turns between them; and the turned elements are multiplied
+      by ``magnitude``, here ``1 + 0.1 ln factor`` by default (1 elsewhere);
+
+    or ``frequencies`` (radians a position, float64 ``[dim / 2]``) are given.  ``turns[dim / 2]``, int64 on the device,
+    holds them as fractions of a turn, in units of 2^-64: angles are exact at any position.
+    """
+
+    def __init__(self, dim: int, base: float = 10000.0, *, interleaved: bool = False, scaling: str = "none", factor: float = 1.0,
+                 trained: int = 0, slow: float = 1.0, fast: float = 32.0, magnitude: float | None = None, frequencies=None, device="cuda"):
+        if dim < 0 or dim % 2:
+            raise ValueError(f"dim: {dim} elements are not pairs")
+        if scaling not in ("none", "linear", "base", "bands"):
+            raise ValueError(f"scaling: {scaling!r} is not none, linear, base or bands")
+        if not 0 < base < math.inf or not 0 < factor < math.inf:
+            raise ValueError("base and factor are positive")
+        if scaling == "none" and factor != 1.0:
+            raise ValueError("factor: there is no scaling")
+        if scaling == "base" and dim <= 2:
+            raise ValueError("scaling: a single pair turns by one radian whatever the base")
+        if scaling == "bands" and not (trained > 0 and 0 <= slow < fast):
+            raise ValueError("scaling: bands need the trained context, and slow < fast")
+        if frequencies is not None:
+            f = torch.as_tensor(frequencies, dtype=torch.float64).cpu()
+            if scaling != "none" or f.shape != (dim // 2,):
+                raise ValueError(f"frequencies: shape {tuple(f.shape)}, expected ({dim // 2},), and no scaling beside them")
+        else:
+            stretched = base * factor ** (dim / (dim - 2)) if scaling == "base" else base
+            f = stretched ** (-torch.arange(0, dim, 2, dtype=torch.float64) / max(1, dim))
+        if scaling == "linear":
+            f = f / factor
+        if scaling == "bands":
+            stays = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+            f = f * (stays + (1 - stays) / factor)
+        if not bool((f.abs() < 2.0 ** 31).all()):
+            raise ValueError("frequencies: not finite, or a position turns by more than 2^31 radians")
+        self.dim, self.interleaved, self.frequencies = dim, bool(interleaved), f
+        self.magnitude = float(magnitude) if magnitude is not None else 1 + 0.1 * math.log(factor) if scaling == "bands" else 1.0
+        if not 0 < self.magnitude < 3e38:
+            raise ValueError("magnitude: must be positive and finite")
+        # whole turns change nothing; the fraction to 64 bits, half a turn and more as its negative
+        turns = [round(Fraction(x) / _TURN * 2 ** 64) % 2 ** 64 for x in f.tolist()]
+        self.turns = torch.tensor([t - 2 ** 64 if t >> 63 else t for t in turns], dtype=torch.int64).to(device)
+
+
+# a turn in radians, to 100 bits or so: pi by Machin's formula
+def _arctan_inverse(n: int) -> Fraction:
+    return sum(Fraction((-1) ** k, (2 * k + 1) * n ** (2 * k + 1)) for k in range(30))
+
+
+_TURN = 8 * (4 * _arctan_inverse(5) - _arctan_inverse(239))
+
+
+def rotate(x, positions, rotary: Rotary, *, out=None, stream: int | None = None):
+    """``x[batch, tokens, heads, d]`` (f32, f16 or bf16; any strides with a contiguous last axis) with every head turned to
+    its token's place, ``positions[batch, tokens]`` (int32 on the device; negative ones turn back).
+
+    Elements behind ``rotary.dim`` pass.  The arithmetic is f32, rounded once.  ``out`` may be ``x`` itself, and overlaps
+    it in no other way.
+    """
+    r = _ext.rotate(x, positions, rotary.turns, rotary.interleaved, rotary.magnitude, out, stream)
+    if type(r) is int:
+        raise _failed("lc_rotate", r)
+    return r
+
+
+# ---------------------------------------------------------------- tokens
+
+def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, return_logprob: bool = False,
+           stream: int | None = None):
+    """A token of each row of ``logits[rows, vocab]`` (f32, f16 or bf16; any stride between rows), int32 ``[rows]``.
+
+    With the weights ``w = exp((x - max) / temperature)``, what is kept is the ``top_k`` largest, of these the shortest run
+    from the largest on that holds ``top_p`` of their sum, of these those with ``w >= min_p``; the token is the first index
+    at which the running sum of what is kept passes ``uniform[row]`` (f32, in [0, 1)) times its total.  Equal logits are
+    taken in index order.  ``temperature`` 0 takes the largest; ``top_k`` 0 (or ``vocab`` and more), ``top_p`` 1 and
+    ``min_p`` 0 leave all.  Each is a number, or a tensor of one a row (f32, ``top_k`` int32).  NaN and -infinity are never
+    taken: a row of nothing else gives -1.
+
+    With ``return_logprob`` also the logarithm of the token's share of what was kept, f32 ``[rows]``.  Sums are exact (whole
+    numbers), so a row's token depends on nothing but the row.
+    """
+    r = _ext.sample(logits, uniform, temperature, top_k, top_p, min_p, out, return_logprob, stream)
+    if type(r) is int:
+        raise _failed("lc_sample", r)
+    return r
+
+
 # ---------------------------------------------------------------- pages
 
 _NONE = (None, None, None, None)
@@ -128,6 +230,21 @@ def cache_write(k, v, k_pages, v_pages, maps: CacheMaps, add, *, refusals=None, 
     status = _ext.cache_write(k, v, k_pages, v_pages, *maps, add, refusals, stream)
     if status:
         raise _failed("lc_cache_write", status)
+
+
+def cache_append(q, k, v, k_pages, v_pages, maps: CacheMaps, add, rotary: Rotary, *, out=None, refusals=None,
+                 stream: int | None = None):
+    """:func:`cache_write` with the positions on the way: the newest ``add[i]`` tokens' keys, turned to the positions
+    ``lens[i] - add[i]`` and on (:func:`rotate`), and values go to their pages, and ``q[slots, most, q_heads, d]`` comes back
+    turned alike (``None`` where ``q`` is).
+
+    f32, f16 or bf16, the pages of the same type.  Queries behind ``add[i]`` come back as 0; in a given ``out``, which may
+    be ``q`` itself, they are left as they were.  After a refused extension (as in :func:`cache_write`) no token is new.
+    """
+    r = _ext.cache_append(q, k, v, k_pages, v_pages, *maps, add, rotary.turns, rotary.interleaved, rotary.magnitude, out, refusals, stream)
+    if type(r) is int:
+        raise _failed("lc_cache_append", r)
+    return r
 
 
 def cache_fork(pool, maps: CacheMaps, parent, *, into: CacheMaps | None = None, refusals=None, stream: int | None = None) -> CacheMaps:
@@ -176,6 +293,25 @@ def cache_copy(pool, src, dst, *, stream: int | None = None) -> None:
         raise _failed("lc_cache_copy", status)
 
 
+class CachePrefixes(NamedTuple):
+    """Which slots begin with the same pages: ``leader[slots]`` (the lowest slot with the same full first page),
+    ``shared[slots]`` (the tokens of the full pages that all slots of that leader have in common; 0 for a slot alone) and
+    ``order[slots]`` (the slots by leader, each group in slot order)."""
+    leader: torch.Tensor
+    shared: torch.Tensor
+    order: torch.Tensor
+
+
+def cache_prefixes(maps: CacheMaps, *, page_size: int, into: CachePrefixes | None = None, stream: int | None = None) -> CachePrefixes:
+    """Which slots begin with the same pages, and how far: what :func:`cache_fork` leaves of one prompt.  At most 8192
+    slots.  It holds until a slot is forked, released or trimmed: what is extended, written or compacted keeps its
+    prefix."""
+    r = _ext.cache_prefixes(*maps, page_size, *(into or (None, None, None)), stream)
+    if type(r) is int:
+        raise _failed("lc_cache_prefixes", r)
+    return CachePrefixes(*r)
+
+
 class PagedCache:
     """The keys and values of ``layers`` attention layers of up to ``slots`` sequences, in pages.
 
@@ -209,6 +345,11 @@ class PagedCache:
         :meth:`extend` was refused."""
         cache_write(k, v, self.pool[2 * layer], self.pool[2 * layer + 1], self.maps, add, refusals=self._refusals, stream=stream)
 
+    def append(self, layer: int, q, k, v, add, rotary: Rotary, out=None, stream=None):
+        """The same with the keys turned to their positions; returns the queries turned to theirs (:func:`cache_append`)."""
+        return cache_append(q, k, v, self.pool[2 * layer], self.pool[2 * layer + 1], self.maps, add, rotary, out=out,
+                            refusals=self._refusals, stream=stream)
+
     def decode(self, layer: int, q, **options):
         """Attention of one new token per slot in one layer (:func:`paged_decode`)."""
         return paged_decode(q, self.pool[2 * layer], self.pool[2 * layer + 1], self.maps.table, self.maps.lens, **options)
@@ -220,6 +361,10 @@ class PagedCache:
         with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream, self.pool.device)):
             self._blocks[0].copy_(self._blocks[1])
         self.maps = self._own  # where the caller had put others in their place
+
+    def prefixes(self, into: CachePrefixes | None = None, stream=None) -> CachePrefixes:
+        """Which slots begin with the same pages (:func:`cache_prefixes`)."""
+        return cache_prefixes(self.maps, page_size=self.page_size, into=into, stream=stream)
 
     def release(self, gone, stream=None) -> None:
         """Empties slots (:func:`cache_release`)."""
