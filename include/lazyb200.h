@@ -761,6 +761,16 @@ int lc_cache_prefixes(const int32_t *table, const int32_t *lens, int32_t *leader
                       int32_t *order, int64_t slots, int64_t width, int64_t pages, int64_t page_size,
                       void *stream);
 
+/* lc_paged_decode for slots that begin alike: leader, shared and order as lc_cache_prefixes left them, or any that say
+ * the same (slots with one leader lie together in order, the leader first, and hold the leader's pages over the first
+ * shared[leader] tokens, of which slots with fewer tokens count theirs alone). A prefix is read once for all slots that
+ * share it. At most 8192 slots; the rest is as there. */
+int lc_shared_decode(int dtype, const void *q, const void *k, const void *v, void *o, float *lse,
+                     const int32_t *table, const int32_t *lens, const int32_t *leader,
+                     const int32_t *shared, const int32_t *order, int64_t slots, int64_t width,
+                     int64_t pages, int64_t page_size, int64_t q_heads, int64_t kv_heads, int64_t d,
+                     const int64_t *strides, int64_t window, int64_t sinks, float scale, void *stream);
+
 /* One token of each row of logits[rows, vocab] (LC_F32, LC_F16 or LC_BF16; `stride` elements from row to row):
  * with weights w_i = exp((x_i - max) / temperature), the top_k largest; of these the shortest run from the largest on
  * that holds top_p of their sum; of these those with w_i >= min_p; and of what is left the first index at which the

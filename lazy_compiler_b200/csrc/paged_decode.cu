@@ -1,67 +1,23 @@
 // Attention of one new token of every sequence over its paged key-value cache
 // (the single-token form of window_attention.cu): slot s has lens[s] cached
 // tokens, its query is the last of them, and token j is row j % page_size of
-// page table[s][j / page_size].
+// page table[s][j / page_size].  The same kernels, instantiated with a Suffix, take
+// the tokens behind the prefixes that slots share, for shared_decode.cu, and leave the
+// rows unnormalised.
 #include <algorithm>
 
-#include "attend.cuh"
+#include "paged.cuh"
 #include "softmax.cuh"
 
 namespace lc {
-namespace {
 
 using namespace attend;
 
-struct DecodeParams {
-  const void *q, *k, *v;
-  void *o;
-  float *lse;
-  const int *table, *lens;
-  int slots, width, pages, page_size, q_heads, kv_heads, d;
-  int64_t qs[2], ks[3], vs[3], os[2], ts;  // element strides: q, o slot and head; k, v page, head, token; table slot
-  int window, sinks;
-  float scale_log2;
-  int page_shift;  // page_size is 1 << page_shift, or -1
-  int dense;       // a head's tokens follow each other in k and v, without padding
-};
-
-__device__ __forceinline__ int page_index(const DecodeParams &p, int key) {
-  return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-}
-
-__device__ __forceinline__ int cached_tokens(const DecodeParams &p, int slot) {
-  const int64_t most = (int64_t)p.width * p.page_size;
-  const int n = max(p.lens[slot], 0);
-  return n < most ? n : (int)most;
-}
+namespace {
 
 constexpr int kPartialsSlot = 41, kArrivedSlot = 42, kSpansSlot = 46;  // scratch_buffer slots
 
 // ---------------------------------------------------------------- plain form
-// One row key by key, by the WARPS warps of a CTA; warp 0 receives it.
-template <class T, int WARPS, int NC>
-__device__ __forceinline__ void plain_row(const DecodeParams &p, int slot, int h, int head, RowState<NC> &st, float *scratch) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = cached_tokens(p, slot);
-  float q[NC];
-  load_row(q, static_cast<const T *>(p.q) + slot * p.qs[0] + h * p.qs[1], p.d, lane, p.scale_log2);
-  const int *row = p.table + slot * p.ts;
-  auto at = [&](int j, const T *&k, const T *&v) {
-    const int entry = row[page_index(p, j)], r = j - page_index(p, j) * p.page_size;
-    const bool held = (unsigned)entry < (unsigned)p.pages;
-    const int64_t page = held ? entry : 0;
-    k = static_cast<const T *>(p.k) + page * p.ks[0] + head * p.ks[1] + r * p.ks[2];
-    v = static_cast<const T *>(p.v) + page * p.vs[0] + head * p.vs[1] + r * p.vs[2];
-    return held;
-  };
-  if (n > 0 && p.pages > 0) {
-    const Visible see = visible(n - 1, p.window, p.sinks);
-    attend_keys<T>(st, q, p.d, lane, warp, see.sink_end, WARPS, at);
-    attend_keys<T>(st, q, p.d, lane, see.lo + warp, n, WARPS, at);
-  }
-  join_warps<WARPS>(st, scratch);
-}
-
 // One CTA of eight warps per (slot, query head): few keys, and what the tensor-core form
 // below does not take (odd head sizes and alignments).
 constexpr int kRowWarps = 8;
@@ -206,6 +162,7 @@ __device__ __forceinline__ float round_to(float v) {
 struct SlotTiles {
   int n, sink_end, lo;       // keys, and the visible ones: j < sink_end or j >= lo
   int sink_tiles, first, tiles;  // tile x is keys 16 (x < sink_tiles ? x : x - sink_tiles + first)
+  int from = 0, sink_first = 0;  // with a Suffix: its first key; the first of the sinks' tiles
 };
 __device__ __forceinline__ SlotTiles slot_tiles(const DecodeParams &p, int slot) {
   SlotTiles t;
@@ -218,6 +175,20 @@ __device__ __forceinline__ SlotTiles slot_tiles(const DecodeParams &p, int slot)
   t.tiles = t.n <= 0 ? 0 : t.sink_tiles + (t.n + kTileKeys - 1) / kTileKeys - t.first;
   return t;
 }
+// The tiles that hold a key of the suffix.
+__device__ __forceinline__ SlotTiles slot_tiles(const DecodeParams &p, int slot, const Suffix &suffix) {
+  SlotTiles t;
+  t.n = cached_tokens(p, slot);
+  const Visible see = visible(t.n - 1, p.window, p.sinks);
+  t.from = min(group_prefix(p, suffix.sharing, slot), t.n);
+  t.lo = max(see.lo, t.from);
+  t.sink_end = see.sink_end > t.from ? see.sink_end : 0;
+  t.sink_first = t.sink_end ? t.from / kTileKeys : 0;
+  t.sink_tiles = (t.sink_end + kTileKeys - 1) / kTileKeys - t.sink_first;
+  t.first = max(t.lo / kTileKeys, t.sink_first + t.sink_tiles);
+  t.tiles = t.n <= t.from ? 0 : t.sink_tiles + max(0, (t.n + kTileKeys - 1) / kTileKeys - t.first);
+  return t;
+}
 __device__ __forceinline__ int cta_tiles(const SlotTiles &t) { return (t.tiles + kDecodeWarps - 1) / kDecodeWarps; }
 
 // A place in the sequence of all tiles.
@@ -225,14 +196,15 @@ struct Cursor {
   SlotTiles tiles;
   int slot, part, t, count;  // part: (head, group) of the slot; t of count CTA tiles
 };
-__device__ __forceinline__ void advance(Cursor &c, const DecodeParams &p, int parts) {
+template <class... WithSuffix>
+__device__ __forceinline__ void advance(Cursor &c, const DecodeParams &p, int parts, const WithSuffix &...suffix) {
   if (++c.t < c.count) return;
   c.t = 0;
   if (++c.part < parts) return;
   c.part = 0;
   do {
     if (++c.slot >= p.slots) return;
-    c.tiles = slot_tiles(p, c.slot);
+    c.tiles = slot_tiles(p, c.slot, suffix...);
     c.count = cta_tiles(c.tiles);
   } while (c.count == 0);
 }
@@ -260,9 +232,25 @@ struct DecodeLayout {
   static_assert(kRows * DP * 4 <= kStageBytes, "a warp's sums are joined in its last stage");
 };
 
+// What a kernel that takes a Suffix writes of its rows.
+template <class... WithSuffix>
+struct SuffixRows {};
+template <>
+struct SuffixRows<Suffix> {
+  const Suffix &suffix;
+  template <int DP>
+  __device__ __forceinline__ float *sums(int64_t row) const {
+    return suffix.sums + row * DP;
+  }
+  __device__ __forceinline__ void stats(int64_t row, float m, float l) const { suffix.stats[row] = make_float2(m, l); }
+};
+
 // PAGED16: a tile of 16 keys lies in one page (page_size is a multiple of 16).
-template <class T, int DP, int NT, int STAGES, int CTAS, bool PAGED16>
-__global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeParams p, DecodeWork work) {
+// WithSuffix: Suffix, or nothing.
+template <class T, int DP, int NT, int STAGES, int CTAS, bool PAGED16, class... WithSuffix>
+__device__ __forceinline__ void decode_run(const DecodeParams &p, const DecodeWork &work, const WithSuffix &...suffix) {
+  constexpr bool kSuffix = sizeof...(WithSuffix) > 0;
+  const SuffixRows<WithSuffix...> rows_to{suffix...};
   using L = DecodeLayout<T, DP, NT, STAGES>;
   constexpr int kRows = L::kRows;
   constexpr int kChunks = DP / 8;                   // 16-byte pieces of a row
@@ -278,7 +266,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   __shared__ long long unit_at[2], tile_at[2];
   __shared__ unsigned ticket;
 
-  pdl_wait();
   // Before a join the next kernel is not let in early: the join's CTAs, and the next call's behind
   // them, on SMs that are still reading cost more than their launch (5 x 32687 tokens, heads of 64,
   // call after call: 60 us, 82 let in).
@@ -295,7 +282,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   long long own = 0, own_tiles = 0;
   auto units_of = [&](int count) { return (long long)(count ? count + kEndUnits : 0) * parts; };
   for (int s = s0; s < s1; ++s) {
-    const int count = cta_tiles(slot_tiles(p, s));
+    const int count = cta_tiles(slot_tiles(p, s, suffix...));
     own += units_of(count);
     own_tiles += (long long)count * parts;
   }
@@ -329,7 +316,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
       long long at = before, at_tile = before_tiles;
       int s = s0, count;
       for (;; ++s) {
-        count = cta_tiles(slot_tiles(p, s));
+        count = cta_tiles(slot_tiles(p, s, suffix...));
         if (unit < at + units_of(count)) break;
         at += units_of(count);
         at_tile += (long long)count * parts;
@@ -351,13 +338,17 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   }
   // slots with nothing to see
   for (int s = blockIdx.x; s < p.slots; s += gridDim.x) {
-    if (slot_tiles(p, s).tiles != 0) continue;
-    for (int i = tid; i < p.q_heads * p.d; i += blockDim.x) {
-      const int h = i / p.d;
-      static_cast<T *>(p.o)[s * p.os[0] + h * p.os[1] + (i - h * p.d)] = Elem<T>::from_float(0.f);
+    if (slot_tiles(p, s, suffix...).tiles != 0) continue;
+    if constexpr (kSuffix) {
+      for (int h = tid; h < p.q_heads; h += blockDim.x) rows_to.stats((int64_t)s * p.q_heads + h, -INFINITY, 0.f);
+    } else {
+      for (int i = tid; i < p.q_heads * p.d; i += blockDim.x) {
+        const int h = i / p.d;
+        static_cast<T *>(p.o)[s * p.os[0] + h * p.os[1] + (i - h * p.d)] = Elem<T>::from_float(0.f);
+      }
+      if (p.lse)
+        for (int h = tid; h < p.q_heads; h += blockDim.x) p.lse[(int64_t)s * p.q_heads + h] = -INFINITY;
     }
-    if (p.lse)
-      for (int h = tid; h < p.q_heads; h += blockDim.x) p.lse[(int64_t)s * p.q_heads + h] = -INFINITY;
   }
   if (work.deep && tid == 0) work.spans[blockIdx.x] = make_int2(-1, -1);
   __syncthreads();
@@ -368,7 +359,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
 
   Cursor load;
   load.slot = start_slot;
-  load.tiles = slot_tiles(p, load.slot);
+  load.tiles = slot_tiles(p, load.slot, suffix...);
   load.count = cta_tiles(load.tiles);
   load.part = start_part;
   load.t = start_t;
@@ -376,7 +367,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   if (load.t >= load.count) {          // behind a segment's last tile: the next one
     seg_begin += load.count + kEndUnits;
     load.t = load.count - 1;
-    advance(load, p, parts);
+    advance(load, p, parts, suffix...);
   }
   Cursor use = load;
 
@@ -387,7 +378,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   int page = -1;  // of the tile the load cursor is at (PAGED16), or of its key `lane`
   auto key_of_tile = [&](const Cursor &c) {
     const int x = c.t * kDecodeWarps + warp;
-    return x < c.tiles.tiles ? kTileKeys * (x < c.tiles.sink_tiles ? x : x - c.tiles.sink_tiles + c.tiles.first) : -1;
+    const int sink = kSuffix ? c.tiles.sink_first : 0;
+    return x < c.tiles.tiles ? kTileKeys * (x < c.tiles.sink_tiles ? x + sink : x - c.tiles.sink_tiles + c.tiles.first) : -1;
   };
   auto find_page = [&]() {
     const int key = key_of_tile(load);
@@ -404,7 +396,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
     const int key = key_of_tile(load);
     const int j = key + (lane & 15);
     const bool sees = key >= 0 && (unsigned)page < (unsigned)p.pages && j < load.tiles.n &&
-                      (j >= load.tiles.lo || j < load.tiles.sink_end);
+                      (j >= load.tiles.lo || (j < load.tiles.sink_end && (!kSuffix || j >= load.tiles.from)));
     const unsigned mask = __ballot_sync(0xffffffffu, sees) & 0xffffu;
     if (lane == 0) masks[warp][stage] = mask;
     // Piece x of row r lies at x ^ (r & 7).  A lane's rows are i * kRowsPerCopy + piece_row, whose
@@ -566,23 +558,35 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
     const int head = use.part / chunks, first = head * group + use.part % chunks * kRows;
     const int live = min(kRows, (head + 1) * group - first);
     bool odd = false;
+    if constexpr (kSuffix) {
 #pragma unroll
-    for (int x = 0; x < kRpt; ++x) {
-      const int row = first_row + kSplit * x;
-      if (row >= live) continue;
-      const float sum = row_l[row], inv = sum == 0.f ? 0.f : 1.f / sum;
-      T *out = static_cast<T *>(p.o) + use.slot * p.os[0] + (first + row) * p.os[1];
+      for (int x = 0; x < kRpt; ++x) {
+        const int row = first_row + kSplit * x;
+        if (row >= live) continue;
+        float *to = rows_to.template sums<DP>((int64_t)use.slot * p.q_heads + first + row);
 #pragma unroll
-      for (int y = 0; y < kCpt; ++y) {
-        const float v = values[x][y] * inv;
-        if (col + kCols * y < p.d) {
-          odd |= !isfinite(v);
-          out[col + kCols * y] = Elem<T>::from_float(v);
+        for (int y = 0; y < kCpt; ++y) to[col + kCols * y] = values[x][y];
+      }
+      if (tid < live) rows_to.stats((int64_t)use.slot * p.q_heads + first + tid, row_m[tid], row_l[tid]);
+    } else {
+#pragma unroll
+      for (int x = 0; x < kRpt; ++x) {
+        const int row = first_row + kSplit * x;
+        if (row >= live) continue;
+        const float sum = row_l[row], inv = sum == 0.f ? 0.f : 1.f / sum;
+        T *out = static_cast<T *>(p.o) + use.slot * p.os[0] + (first + row) * p.os[1];
+#pragma unroll
+        for (int y = 0; y < kCpt; ++y) {
+          const float v = values[x][y] * inv;
+          if (col + kCols * y < p.d) {
+            odd |= !isfinite(v);
+            out[col + kCols * y] = Elem<T>::from_float(v);
+          }
         }
       }
+      if (p.lse && tid < live)
+        p.lse[(int64_t)use.slot * p.q_heads + first + tid] = row_l[tid] == 0.f ? -INFINITY : lse_of<(int)kLift<T>>(row_m[tid], row_l[tid]);
     }
-    if (p.lse && tid < live)
-      p.lse[(int64_t)use.slot * p.q_heads + first + tid] = row_l[tid] == 0.f ? -INFINITY : lse_of<(int)kLift<T>>(row_m[tid], row_l[tid]);
     return odd;
   };
   // What came out infinite or NaN is computed again one key at a time: the
@@ -750,7 +754,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   for (int i = 0; i < STAGES - 1; ++i) {
     if (i < steps) {
       issue(i);
-      advance(load, p, parts);
+      advance(load, p, parts, suffix...);
       if (i + 1 < steps) find_page();
     }
     copy_commit();
@@ -763,7 +767,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
     __syncwarp();  // this stage has landed, and the one before has been read, in every lane
     if (i + STAGES - 1 < steps) {
       issue(stage == 0 ? STAGES - 1 : stage - 1);
-      advance(load, p, parts);
+      advance(load, p, parts, suffix...);
       if (i + STAGES < steps) find_page();
     }
     copy_commit();
@@ -773,7 +777,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
       seg_begin += use.count + kEndUnits;
       if (i + 1 < steps) {
         use.t = use.count - 1;
-        advance(use, p, parts);
+        advance(use, p, parts, suffix...);
         start_segment();
       }
     } else {
@@ -783,14 +787,28 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeP
   }
 }
 
+template <class T, int DP, int NT, int STAGES, int CTAS, bool PAGED16>
+__global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) decode_kernel(DecodeParams p, DecodeWork work) {
+  pdl_wait();
+  decode_run<T, DP, NT, STAGES, CTAS, PAGED16>(p, work);
+}
+// The kernel before it, which takes the prefixes, let this one in when all before that was done, and neither
+// reads what the other writes: so it waits at its end, for what comes after both.
+template <class T, int DP, int NT, int STAGES, int CTAS, bool PAGED16>
+__global__ void __launch_bounds__(kDecodeWarps * 32, CTAS) suffix_kernel(DecodeParams p, DecodeWork work, Suffix suffix) {
+  decode_run<T, DP, NT, STAGES, CTAS, PAGED16>(p, work, suffix);
+  pdl_wait();
+}
+
 // Joins the segments that span CTAs: blockIdx.x counts them, blockIdx.y is a row; the
 // parts are dealt to eight warps, each with a running maximum.  A chain of three reads: the
 // spans, the parts, all of a warp's first kAtOnce together, and the eight warps' sums.
 constexpr int kJoinWarps = 8;
 constexpr int kMostSpans = 4;  // of a thread: up to 1024 CTAs
 
-template <class T, int DP, int NT>
-__global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodeParams p, DecodeWork work) {
+template <class T, int DP, int NT, class... WithSuffix>
+__global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodeParams p, DecodeWork work, WithSuffix... suffix) {
+  constexpr bool kSuffix = sizeof...(WithSuffix) > 0;
   constexpr int kRows = 8 * NT, kCols = DP / 32, kAtOnce = 8;
   __shared__ float scratch[kJoinWarps * (DP + 2)];
   __shared__ int counts[kMostSpans * kJoinWarps];
@@ -892,6 +910,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodePara
     weights[w] = softmax::ex2(scratch[w * (DP + 2) + DP + 1] - (top == -INFINITY ? 0.f : top));
     sum = fmaf(scratch[w * (DP + 2) + DP], weights[w], sum);
   }
+  if constexpr (kSuffix) {
+    const SuffixRows<WithSuffix...> rows_to{suffix...};
+    const int64_t row_at = (int64_t)slot * p.q_heads + h;
+    if (tid < DP) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) v = fmaf(scratch[w * (DP + 2) + tid], weights[w], v);
+      rows_to.template sums<DP>(row_at)[tid] = v;
+    }
+    if (tid == 0) rows_to.stats(row_at, top, sum);
+    return;
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T *out = static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1];
   bool odd = false;
@@ -911,10 +941,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(DecodePara
   }
 }
 
-template <class T, int DP, int NT, int STAGES, int CTAS, bool PAGED16>
-int launch_decode(const DecodeParams &p, cudaStream_t s) {
+template <class T, int DP, int NT, int STAGES, int CTAS, bool PAGED16, class... WithSuffix>
+int launch_decode(const DecodeParams &p, cudaStream_t s, const WithSuffix &...suffix) {
   using L = DecodeLayout<T, DP, NT, STAGES>;
-  auto *kernel = decode_kernel<T, DP, NT, STAGES, CTAS, PAGED16>;
+  auto *kernel = [] {
+    if constexpr (sizeof...(WithSuffix) > 0)
+      return suffix_kernel<T, DP, NT, STAGES, CTAS, PAGED16>;
+    else
+      return decode_kernel<T, DP, NT, STAGES, CTAS, PAGED16>;
+  }();
   static int configured[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -941,36 +976,24 @@ int launch_decode(const DecodeParams &p, cudaStream_t s) {
     if (int rc = scratch_buffer(s, kSpansSlot, ctas * sizeof(int2), &mem)) return rc;
     w.spans = static_cast<int2 *>(mem);
   }
-  if (int rc = check_cuda(launch_pdl(kernel, dim3(ctas), dim3(kDecodeWarps * 32), L::kBytes, s, p, w), "lc_paged_decode")) return rc;
+  if (int rc = check_cuda(launch_pdl(kernel, dim3(ctas), dim3(kDecodeWarps * 32), L::kBytes, s, p, w, suffix...), "lc_paged_decode")) return rc;
   if (!w.deep) return LC_OK;
-  return check_cuda(launch_pdl(decode_join_kernel<T, DP, NT>, dim3((unsigned)(p.slots * parts), L::kRows), dim3(kJoinWarps * 32), 0, s, p, w),
+  return check_cuda(launch_pdl(decode_join_kernel<T, DP, NT, WithSuffix...>, dim3((unsigned)(p.slots * parts), L::kRows), dim3(kJoinWarps * 32), 0, s,
+                               p, w, suffix...),
                     "lc_paged_decode (join)");
 }
 
-template <class T, bool PAGED16>
-int launch_sized(const DecodeParams &p, cudaStream_t s) {
+template <class T, bool PAGED16, class... WithSuffix>
+int launch_sized(const DecodeParams &p, cudaStream_t s, const WithSuffix &...suffix) {
   // NT: 8 or 16 query heads of a group in one pass over its keys (a group of 9 to 16
   // read twice, 8 heads at a time, would take the loads twice; larger groups are cut in sixteens)
   const bool wide = p.q_heads / p.kv_heads > 8;
-  if (p.d <= 64) return wide ? launch_decode<T, 64, 2, 3, 4, PAGED16>(p, s) : launch_decode<T, 64, 1, 3, 4, PAGED16>(p, s);
-  if (p.d <= 128) return wide ? launch_decode<T, 128, 2, 3, 2, PAGED16>(p, s) : launch_decode<T, 128, 1, 2, 3, PAGED16>(p, s);
-  return wide ? launch_decode<T, 256, 2, 3, 1, PAGED16>(p, s) : launch_decode<T, 256, 1, 3, 1, PAGED16>(p, s);
-}
-
-// The tensor-core form takes 16-byte pieces of keys and values and pairs of the query.
-bool decode_tensor(const DecodeParams &p) {
-  bool ok = p.d % 8 == 0 && aligned(p.k, 16) && aligned(p.v, 16) && aligned(p.q, 4) && p.pages > 0 && p.width > 0;
-  for (int i = 0; i < 3; ++i) ok = ok && p.ks[i] % 8 == 0 && p.vs[i] % 8 == 0;
-  for (int i = 0; i < 2; ++i) ok = ok && p.qs[i] % 2 == 0;
-  return ok;
-}
-
-// Few rows of few keys, by what any slot can see: as in window_attention.cu (1 x 8 rows
-// of 68 keys: 4.7 against 5.5 us, 16 x 8: 5.1 against 6.4; 64 x 8 of 68: 9.4 against 6.6, 1 x 8 of 128: 6.2 against 5.5).
-bool few_keys(const DecodeParams &p) {
-  const int64_t most = (int64_t)p.width * p.page_size;
-  const int64_t reach = p.window ? std::min<int64_t>((int64_t)p.window + p.sinks, most) : most;
-  return reach <= 96 && (int64_t)p.slots * p.q_heads * reach <= 16384;
+  if (p.d <= 64) return wide ? launch_decode<T, 64, 2, 3, 4, PAGED16>(p, s, suffix...) : launch_decode<T, 64, 1, 3, 4, PAGED16>(p, s, suffix...);
+  if (p.d <= 128) return wide ? launch_decode<T, 128, 2, 3, 2, PAGED16>(p, s, suffix...) : launch_decode<T, 128, 1, 2, 3, PAGED16>(p, s, suffix...);
+  if constexpr (sizeof...(WithSuffix) == 0)
+    return wide ? launch_decode<T, 256, 2, 3, 1, PAGED16>(p, s) : launch_decode<T, 256, 1, 3, 1, PAGED16>(p, s);
+  else
+    return fail(LC_ERR_UNSUPPORTED, "lc_paged_decode: head size %d behind a prefix", p.d);
 }
 
 template <class T>
@@ -983,14 +1006,26 @@ int launch_rows(const DecodeParams &p, cudaStream_t s) {
 }
 
 }  // namespace
-}  // namespace lc
 
-extern "C" int lc_paged_decode(int dtype, const void *q, const void *k, const void *v, void *o, float *lse,
-                               const int32_t *table, const int32_t *lens, int64_t slots, int64_t width, int64_t pages,
-                               int64_t page_size, int64_t q_heads, int64_t kv_heads, int64_t d, const int64_t *strides,
-                               int64_t window, int64_t sinks, float scale, void *stream) {
-  using namespace lc;
-  const char *me = "lc_paged_decode";
+// The tensor-core form takes 16-byte pieces of keys and values and pairs of the query.
+bool decode_tensor(const DecodeParams &p) {
+  bool ok = p.d % 8 == 0 && aligned(p.k, 16) && aligned(p.v, 16) && aligned(p.q, 4) && p.pages > 0 && p.width > 0;
+  for (int i = 0; i < 3; ++i) ok = ok && p.ks[i] % 8 == 0 && p.vs[i] % 8 == 0;
+  for (int i = 0; i < 2; ++i) ok = ok && p.qs[i] % 2 == 0;
+  return ok;
+}
+
+// Few rows of few keys, by what any slot can see: as in window_attention.cu (1 x 8 rows
+// of 68 keys: 4.7 against 5.5 us, 16 x 8: 5.1 against 6.4; 64 x 8 of 68: 9.4 against 6.6, 1 x 8 of 128: 6.2 against 5.5).
+bool decode_few_keys(const DecodeParams &p) {
+  const int64_t most = (int64_t)p.width * p.page_size;
+  const int64_t reach = p.window ? std::min<int64_t>((int64_t)p.window + p.sinks, most) : most;
+  return reach <= 96 && (int64_t)p.slots * p.q_heads * reach <= 16384;
+}
+
+int decode_params(const char *me, DecodeParams &p, int dtype, const void *q, const void *k, const void *v, void *o, float *lse,
+                  const int32_t *table, const int32_t *lens, int64_t slots, int64_t width, int64_t pages, int64_t page_size,
+                  int64_t q_heads, int64_t kv_heads, int64_t d, const int64_t *strides, int64_t window, int64_t sinks, float scale) {
   if (dtype != LC_F16 && dtype != LC_BF16) return fail(LC_ERR_INVALID, "%s: dtype %d is not f16 or bf16", me, dtype);
   if (slots < 0 || width < 0 || pages < 0 || page_size < 1 || q_heads < 1 || kv_heads < 1 || d < 1 || window < 0 || sinks < 0)
     return fail(LC_ERR_INVALID, "%s: negative or zero size", me);
@@ -1003,7 +1038,6 @@ extern "C" int lc_paged_decode(int dtype, const void *q, const void *k, const vo
   if (slots == 0) return LC_OK;
   if (!q || !o || !lens || (width > 0 && !table) || (pages > 0 && (!k || !v))) return fail(LC_ERR_INVALID, "%s: null buffer", me);
   if (!aligned(q, 2) || !aligned(k, 2) || !aligned(v, 2) || !aligned(o, 2)) return fail(LC_ERR_ALIGN, "%s: elements are two bytes", me);
-  DecodeParams p;
   p.q = q, p.k = k, p.v = v, p.o = o, p.lse = lse, p.table = table, p.lens = lens;
   p.slots = (int)slots, p.width = (int)width, p.pages = (int)pages, p.page_size = (int)page_size;
   p.q_heads = (int)q_heads, p.kv_heads = (int)kv_heads, p.d = (int)d;
@@ -1017,12 +1051,34 @@ extern "C" int lc_paged_decode(int dtype, const void *q, const void *k, const vo
   p.page_shift = -1;
   for (int x = 0; x < 21; ++x)
     if (page_size == 1ll << x) p.page_shift = x;
-  cudaStream_t s = as_stream(stream);
-  if (!few_keys(p) && decode_tensor(p)) {
-    const int padded = d <= 64 ? 64 : d <= 128 ? 128 : 256;
-    p.dense = d == padded && p.ks[2] == d && p.vs[2] == d;
-    if (dtype == LC_F16) return page_size % 16 == 0 ? launch_sized<__half, true>(p, s) : launch_sized<__half, false>(p, s);
-    return page_size % 16 == 0 ? launch_sized<__nv_bfloat16, true>(p, s) : launch_sized<__nv_bfloat16, false>(p, s);
+  const int padded = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  p.dense = d == padded && p.ks[2] == d && p.vs[2] == d;
+  return LC_OK;
+}
+
+int decode_all(int dtype, const DecodeParams &p, cudaStream_t s) {
+  if (!decode_few_keys(p) && decode_tensor(p)) {
+    if (dtype == LC_F16) return p.page_size % 16 == 0 ? launch_sized<__half, true>(p, s) : launch_sized<__half, false>(p, s);
+    return p.page_size % 16 == 0 ? launch_sized<__nv_bfloat16, true>(p, s) : launch_sized<__nv_bfloat16, false>(p, s);
   }
   return dtype == LC_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s);
+}
+
+int decode_suffix(int dtype, const DecodeParams &p, const Suffix &suffix, cudaStream_t s) {
+  if (dtype == LC_F16) return p.page_size % 16 == 0 ? launch_sized<__half, true>(p, s, suffix) : launch_sized<__half, false>(p, s, suffix);
+  return p.page_size % 16 == 0 ? launch_sized<__nv_bfloat16, true>(p, s, suffix) : launch_sized<__nv_bfloat16, false>(p, s, suffix);
+}
+
+}  // namespace lc
+
+extern "C" int lc_paged_decode(int dtype, const void *q, const void *k, const void *v, void *o, float *lse,
+                               const int32_t *table, const int32_t *lens, int64_t slots, int64_t width, int64_t pages,
+                               int64_t page_size, int64_t q_heads, int64_t kv_heads, int64_t d, const int64_t *strides,
+                               int64_t window, int64_t sinks, float scale, void *stream) {
+  using namespace lc;
+  attend::DecodeParams p;
+  if (int rc = decode_params("lc_paged_decode", p, dtype, q, k, v, o, lse, table, lens, slots, width, pages, page_size, q_heads, kv_heads,
+                             d, strides, window, sinks, scale))
+    return rc;
+  return slots == 0 ? LC_OK : decode_all(dtype, p, as_stream(stream));
 }

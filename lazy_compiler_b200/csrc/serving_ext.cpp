@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <type_traits>
@@ -39,6 +40,7 @@ struct StepEntries {
   decltype(&lc_cache_append) cache_append;
   decltype(&lc_cache_prefixes) cache_prefixes;
   decltype(&lc_sample) sample;
+  decltype(&lc_shared_decode) shared_decode;
 } steps;
 constexpr int kStepEntries = sizeof(StepEntries) / sizeof(void *);
 
@@ -226,43 +228,83 @@ PyObject *window_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// What both single-token forms take: the tensors, checked, and the outputs.
+struct Decode {
+  const at::Tensor &q, &k, &v, &table, &lens;
+  int dtype;
+  int64_t slots, heads, d, width, pages, kv_heads, page_size;
+  Decode(PyObject *const *a, PyObject *out_given)
+      : q(tensor(a[0], "q")), k(tensor(a[1], "k_pages")), v(tensor(a[2], "v_pages")), table(tensor(a[3], "table")), lens(tensor(a[4], "lens")) {
+    check_no_gradient(q, "q");
+    check_no_gradient(k, "k_pages");
+    check_no_gradient(v, "v_pages");
+    dtype = attention_dtype(q);
+    check_axes(q, "q", 3);
+    check_axes(k, "k_pages", 4);
+    check_axes(table, "table", 2);
+    slots = q.size(0), heads = q.size(1), d = q.size(2), width = table.size(1);
+    pages = k.size(0), kv_heads = k.size(1), page_size = k.size(2);
+    check(k, "k_pages", q, q.scalar_type(), {pages, kv_heads, page_size, d});
+    check(v, "v_pages", q, q.scalar_type(), {pages, kv_heads, page_size, d});
+    check(table, "table", q, at::kInt, {slots, width});
+    check_ints(lens, "lens", q, {slots});
+    const at::Tensor *given = maybe(out_given, "out");
+    if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d}), check_out(*given, "out"), check_no_gradient(*given, "out");
+  }
+  at::Tensor out, lse;
+  int64_t strides[11];
+  void outputs(PyObject *out_given, bool with_lse) {
+    const at::Tensor *given = maybe(out_given, "out");
+    out = given ? *given : fresh({slots, heads, d}, q.scalar_type(), q);
+    if (with_lse) lse = fresh({slots, heads}, at::kFloat, q);
+    check_inner(q, "q");
+    check_inner(k, "k_pages");
+    check_inner(v, "v_pages");
+    check_inner(out, "out");
+    check_inner(table, "table");
+    const int64_t all[11] = {q.stride(0), q.stride(1), k.stride(0),   k.stride(1),   k.stride(2),    v.stride(0),
+                             v.stride(1), v.stride(2), out.stride(0), out.stride(1), table.stride(0)};
+    std::copy(all, all + 11, strides);
+  }
+};
+
 // q, k_pages, v_pages, table, lens, window, sinks, scale, out, return_lse, stream
 PyObject *paged_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments(n, 11);
-  const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k_pages"), &v = tensor(a[2], "v_pages");
-  const at::Tensor &table = tensor(a[3], "table"), &lens = tensor(a[4], "lens");
-  check_no_gradient(q, "q");
-  check_no_gradient(k, "k_pages");
-  check_no_gradient(v, "v_pages");
-  const int dtype = attention_dtype(q);
-  check_axes(q, "q", 3);
-  check_axes(k, "k_pages", 4);
-  check_axes(table, "table", 2);
-  const int64_t slots = q.size(0), heads = q.size(1), d = q.size(2), width = table.size(1);
-  const int64_t pages = k.size(0), kv_heads = k.size(1), page_size = k.size(2);
-  check(k, "k_pages", q, q.scalar_type(), {pages, kv_heads, page_size, d});
-  check(v, "v_pages", q, q.scalar_type(), {pages, kv_heads, page_size, d});
-  check(table, "table", q, at::kInt, {slots, width});
-  check_ints(lens, "lens", q, {slots});
-  const at::Tensor *given = maybe(a[8], "out");
-  if (given) check(*given, "out", q, q.scalar_type(), {slots, heads, d}), check_out(*given, "out"), check_no_gradient(*given, "out");
-  const On on(a[10], q);
-  const at::Tensor out = given ? *given : fresh({slots, heads, d}, q.scalar_type(), q);
-  const at::Tensor lse = truth(a[9]) ? fresh({slots, heads}, at::kFloat, q) : at::Tensor();
-  check_inner(q, "q");
-  check_inner(k, "k_pages");
-  check_inner(v, "v_pages");
-  check_inner(out, "out");
-  check_inner(table, "table");
-  const int64_t strides[11] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), k.stride(2), v.stride(0),
-                               v.stride(1), v.stride(2), out.stride(0), out.stride(1), table.stride(0)};
-  const int status = lib.paged_decode(dtype, ptr(q), ptr(k), ptr(v), ptr(out), lse.defined() ? ptr<float>(lse) : nullptr,
-                                      ptr<int32_t>(table), ptr<int32_t>(lens), slots, width, pages, page_size, heads, kv_heads, d,
-                                      strides, integer(a[5]), integer(a[6]), scale_of(a[7], d), on.stream);
+  Decode x(a, a[8]);
+  const On on(a[10], x.q);
+  x.outputs(a[8], truth(a[9]));
+  const int status = lib.paged_decode(x.dtype, ptr(x.q), ptr(x.k), ptr(x.v), ptr(x.out), x.lse.defined() ? ptr<float>(x.lse) : nullptr,
+                                      ptr<int32_t>(x.table), ptr<int32_t>(x.lens), x.slots, x.width, x.pages, x.page_size, x.heads,
+                                      x.kv_heads, x.d, x.strides, integer(a[5]), integer(a[6]), scale_of(a[7], x.d), on.stream);
   if (status) return PyLong_FromLong(status);
-  if (given) written(out);
-  return outputs(out, a[8], lse);
+  if (a[8] != Py_None) written(x.out);
+  return outputs(x.out, a[8], x.lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// q, k_pages, v_pages, table, lens, prefixes (3), window, sinks, scale, out, return_lse, stream
+PyObject *shared_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 14);
+  Decode x(a, a[11]);
+  const char *names[3] = {"prefixes.leader", "prefixes.shared", "prefixes.order"};
+  const int32_t *prefixes[3];
+  for (int i = 0; i < 3; ++i) {
+    const at::Tensor &t = tensor(a[5 + i], names[i]);
+    check_ints(t, names[i], x.q, {x.slots});
+    prefixes[i] = ptr<int32_t>(t);
+  }
+  const On on(a[13], x.q);
+  x.outputs(a[11], truth(a[12]));
+  const int status = steps.shared_decode(x.dtype, ptr(x.q), ptr(x.k), ptr(x.v), ptr(x.out), x.lse.defined() ? ptr<float>(x.lse) : nullptr,
+                                         ptr<int32_t>(x.table), ptr<int32_t>(x.lens), prefixes[0], prefixes[1], prefixes[2], x.slots,
+                                         x.width, x.pages, x.page_size, x.heads, x.kv_heads, x.d, x.strides, integer(a[8]), integer(a[9]),
+                                         scale_of(a[10], x.d), on.stream);
+  if (status) return PyLong_FromLong(status);
+  if (a[11] != Py_None) written(x.out);
+  return outputs(x.out, a[11], x.lse);
   END_HANDLE_TH_ERRORS
 }
 
@@ -663,7 +705,7 @@ PyObject *sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
 PyMethodDef methods[] = {METHOD(bind),         METHOD(window_attention), METHOD(paged_decode),  METHOD(cache_extend), METHOD(cache_write),
                          METHOD(cache_fork),   METHOD(cache_release),    METHOD(cache_compact), METHOD(cache_copy),
                          METHOD(bind_steps),   METHOD(rotate),           METHOD(cache_append),  METHOD(cache_prefixes),
-                         METHOD(sample),       {nullptr, nullptr, 0, nullptr}};
+                         METHOD(sample),       METHOD(shared_decode),    {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving", "Calls of lazy_compiler_b200.serving.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -3,6 +3,8 @@
 // 32-byte row store.
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <stdint.h>
 
 namespace lc {
@@ -73,6 +75,26 @@ __device__ __forceinline__ uint64_t ex2_poly2(uint64_t x2) {
   const float2 qq = unpack2(q), tt = unpack2(t);
   return pack2(__int_as_float(__float_as_int(qq.x) + (__float_as_int(tt.x) << 23)),
                __int_as_float(__float_as_int(qq.y) + (__float_as_int(tt.y) << 23)));
+}
+
+// Bits [lo, hi) of a 32-bit word (either bound may lie outside it).
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+  const uint32_t below_hi = hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1;
+  const uint32_t below_lo = lo >= 32 ? 0xffffffffu : lo <= 0 ? 0u : (1u << lo) - 1;
+  return below_hi & ~below_lo;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack16(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 }  // namespace softmax

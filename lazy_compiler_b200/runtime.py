@@ -86,6 +86,7 @@ SIGNATURES = {
     "lc_rotate": [_INT] + [_P] * 4 + [_I64] * 5 + [_INT, ctypes.c_float, _P, _P],
     "lc_cache_append": [_INT] + [_P] * 11 + [_I64] * 9 + [_INT, ctypes.c_float, _INT, _P, _P],
     "lc_cache_prefixes": [_P] * 5 + [_I64] * 4 + [_P],
+    "lc_shared_decode": [_INT] + [_P] * 10 + [_I64] * 7 + [_P, _I64, _I64, ctypes.c_float, _P],
     "lc_sample": [_INT] + [_P] * 6 + [ctypes.c_float, _I64, ctypes.c_float, ctypes.c_float] + [_P] * 2 + [_I64] * 3 + [_P],
 }
 

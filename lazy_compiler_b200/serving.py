@@ -39,7 +39,7 @@ from . import runtime
 # the order in which csrc/serving_ext.cpp takes the entry points
 _ENTRIES = ("lc_window_attention", "lc_paged_decode", "lc_cache_extend_recorded", "lc_cache_write_unless",
             "lc_cache_fork_recorded", "lc_cache_release", "lc_cache_compact", "lc_cache_copy")
-_STEP_ENTRIES = ("lc_rotate", "lc_cache_append", "lc_cache_prefixes", "lc_sample")
+_STEP_ENTRIES = ("lc_rotate", "lc_cache_append", "lc_cache_prefixes", "lc_sample", "lc_shared_decode")
 
 
 def _extension():
@@ -312,6 +312,20 @@ def cache_prefixes(maps: CacheMaps, *, page_size: int, into: CachePrefixes | Non
     return CachePrefixes(*r)
 
 
+def shared_decode(q, k_pages, v_pages, table, lens, prefixes: CachePrefixes, *, window: int = 0, sinks: int = 0,
+                  scale: float | None = None, out=None, return_lse: bool = False, stream: int | None = None):
+    """:func:`paged_decode` for slots that begin alike: samples of one prompt, questions to one document.
+
+    ``prefixes`` is what :func:`cache_prefixes` found, or the same in other tensors: slots with one leader lie together in
+    ``order``, the leader first, and hold its pages over the first ``shared[leader]`` tokens.  Such a prefix is read once
+    for all of them.  At most 8192 slots; the rest is as there.
+    """
+    r = _ext.shared_decode(q, k_pages, v_pages, table, lens, *prefixes, window, sinks, scale, out, return_lse, stream)
+    if type(r) is int:
+        raise _failed("lc_shared_decode", r)
+    return r
+
+
 class PagedCache:
     """The keys and values of ``layers`` attention layers of up to ``slots`` sequences, in pages.
 
@@ -353,6 +367,10 @@ class PagedCache:
     def decode(self, layer: int, q, **options):
         """Attention of one new token per slot in one layer (:func:`paged_decode`)."""
         return paged_decode(q, self.pool[2 * layer], self.pool[2 * layer + 1], self.maps.table, self.maps.lens, **options)
+
+    def shared_decode(self, layer: int, q, prefixes: CachePrefixes, **options):
+        """The same where slots begin alike (:func:`shared_decode`)."""
+        return shared_decode(q, self.pool[2 * layer], self.pool[2 * layer + 1], self.maps.table, self.maps.lens, prefixes, **options)
 
     def fork(self, parent, stream=None) -> None:
         """Slots continue others (:func:`cache_fork`).  The new maps are copied back into the same tensors, so that a
