@@ -4,22 +4,26 @@
 // times its total (u is given).
 //
 // Weights are whole numbers: W = round(2^s 2^((x - max) log2(e) / T)), s = 62 - log2(vocab)
-// rounded up, 50 at most, from an exponential in f64 (2^-42 or so off).  So every sum is exact
+// rounded up, 50 at most, from an exponential in f64 (1e-12 or so off).  So every sum is exact
 // and the same in any order, for any split of the row and whatever atomics do; and since a cut
 // is off by the weights' rounding alone, some 1e-11 of the total, the token is that of the
 // definition in 64 bits but for one draw in a million even where the whole vocabulary is kept.
 //
 // A row is a cluster's: up to eight CTAs of 16 warps, a run of consecutive elements each.
-//   1  the largest element (the pass that reads HBM; the others find the row in L2)
-//   2  a threshold that at least J elements reach: the J-th largest of the threads' own maxima;
-//      what reaches it goes to a list, and where top-p needs it the total is added up
-//   3  where the list holds all that can be kept (the rule), one CTA has its entries in
-//      registers and finds the k-th, the end of the run and the token by bisection, each a
-//      sum over the CTA: of the keys' bits, of the indices' bits
-//   or, where it does not: histograms over the range of keys that the cut may be in, 2048
-//      bins of counts and weights each, until a bin is one key; then the sums of the warps'
-//      runs, and the run that holds the token again, element by element
-// Equal logits are taken in index order throughout.
+//   1  the largest element, from HBM (the passes after it find the row in L2), and a threshold
+//      that some hundred elements reach, from the lanes' own largest
+//   2  what reaches the threshold goes to a list; where top-p asks for it, the total
+//   3  one CTA has the list in registers and finds the k-th, the end of the run and the token
+//      by bisection of (logit, index) and of the index, each step a sum over the CTA
+// Where the list does not hold what may be kept, the cut is looked for first: a histogram of
+// counts over 4096 equal steps of the logits, the steps that the cut may lie in (a step's weights
+// are nearly one), and the list is of those, with the exact sums of what lies above them; where even
+// they hold too many (equal logits), histograms of counts and weights over the keys, down to one.
+// Then, and where nothing is cut: the sums of the warps' runs, and the run that holds the token
+// again, element by element.  Equal logits are taken in index order throughout.
+//
+// Bound by the f64 pipe where top-p wants the total (10 operations an element, 60 a clock and SM:
+// 6 elements), by latencies for few rows.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -34,8 +38,12 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMostCtas = 8;
 constexpr int kListed = 4, kList = kListed * kThreads;  // entries of a thread, of the list
-constexpr int kBinBits = 11, kBins = 1 << kBinBits;
-constexpr uint32_t kNone = 0x007fffffu;  // the key of -infinity
+constexpr int kWanted = 256;                             // entries of a list for top-p alone, at least
+constexpr int kFew = 128;                                // threads that a short list is dealt to
+constexpr int kBinBits = 11, kBins = 1 << kBinBits;     // of keys
+constexpr int kSteps = 4096;                             // of logits
+constexpr uint32_t kNone = 0x007fffffu;                  // the key of -infinity
+constexpr double kLn2 = 0.6931471805599453, kLog2e = 1.4426950408889634;
 
 struct SampleParams {
   const void *logits;
@@ -63,100 +71,88 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-// 2^(y / 256) for y <= 0 as a whole number of 2^-s: a table of 2^(i / 256), and 1 + r a1 + ... + r^3 a3 for
-// the rest, |r| <= 1/2 (off by 1.4e-13).
+// 2^(y / 32), y = (x - max) factor, as a whole number of 2^-s: 2^(i / 32) from lane i, times a polynomial of
+// degree 4 for the rest, |r| <= 1/2 (off by 1.2e-12 at the ends, and with r's sign).  By whole warps.
 struct Weights {
-  const double *table;
-  double max, factor;  // y = (x - max) factor, factor = 256 log2(e) / T
+  double factor;
+  float max, factor32;
+  double power;          // 2^(lane / 32)
   int scale;
-  __device__ __forceinline__ double place(float x) const { return x == (float)max ? 0.0 : ((double)x - max) * factor; }
-  __device__ __forceinline__ uint64_t at(double y) const {
-    if (!(y > -256.0 * (scale + 1))) return 0;  // rounds to nothing; NaN
-    constexpr double kMagic = 6755399441055744.0, kStep = 0.6931471805599453 / 256;  // 1.5 * 2^52
+  __device__ __forceinline__ uint64_t of(float x) const {
+    // what rounds to nothing, -infinity and NaN: the rest may compute anything
+    const bool some = (x - max) * factor32 > -32.f * ((float)scale + 1.5f);
+    constexpr double kMagic = 6755399441055744.0, kStep = kLn2 / 32;  // 1.5 * 2^52
+    const double y = ((double)x - (double)max) * factor;  // (x factor - max factor would cancel where T is small)
     const double z = y + kMagic, r = y - (z - kMagic);
     const int j = __double2loint(z);
-    double f = fma(r, kStep * kStep * kStep / 6, kStep * kStep / 2);
+    double f = fma(r, kStep * kStep * kStep * kStep / 24, kStep * kStep * kStep / 6);
+    f = fma(r, f, kStep * kStep / 2);
     f = fma(r, f, kStep);
-    f = fma(r, f, 1.0) * table[j & 255];
-    // times 2^(s + j / 256), then the whole number in the low bits
-    f = __hiloint2double(__double2hiint(f) + ((scale + (j >> 8)) << 20), __double2loint(f)) + 4503599627370496.0;
-    return (uint64_t)(__double_as_longlong(f) & 0xfffffffffffffll);
+    f = fma(r, f, 1.0);
+    const int lo = __shfl_sync(0xffffffffu, __double2loint(power), j & 31), hi = __shfl_sync(0xffffffffu, __double2hiint(power), j & 31);
+    f = fma(f, __hiloint2double(hi + (int)((unsigned)(scale + (j >> 5)) << 20), lo), 4503599627370496.0);  // 2^52: the whole number in the low bits
+    return some ? (uint64_t)__double_as_longlong(f) & 0xfffffffffffffull : 0;
   }
-  __device__ __forceinline__ uint64_t of(float x) const { return at(place(x)); }
 };
 
 struct SampleShared {
-  double table[256];
   union {
     struct {
       uint32_t key[kList];
       int index[kList];
+      uint32_t count[kSteps];
     } list;
     struct {
       uint32_t count[kBins], low[kBins], high[kBins];
     } bins;
-    struct {
-      uint64_t sum[kMostCtas * kWarps];
-      int ties[kMostCtas * kWarps];
-    } runs;
   };
-  uint64_t parts[2][kWarps];
+  struct Part {
+    uint64_t sum;
+    uint32_t count, pad;
+  } parts[2][kWarps];
+  double scan[3][kWarps];
   // what the cluster's other CTAs read
-  float max, threshold;
-  int listed;
-  uint64_t total, listed_sum;
+  float max, threshold, min;
+  int listed, first[kWarps];
+  uint64_t total, inside, count;
   uint64_t run_sum[kWarps];
-  int run_ties[kWarps];
+  // what the first CTA has found
+  uint32_t cut;
+  int cut_index, run;
+  uint64_t run_begin, kept;
+  uint64_t runs[kMostCtas * kWarps];
   // a histogram's crossing
-  uint32_t found;
-  uint64_t found_sum;
-  uint64_t found_count;
+  uint32_t found, found_end;
+  uint64_t found_sum, found_count;
 };
 
-__device__ __forceinline__ uint64_t warp_total(uint64_t v) {
-  // in pieces of 26 bits, whose sums over a warp fit 32
-  const uint64_t a = __reduce_add_sync(0xffffffffu, (uint32_t)(v & 0x3ffffff)), b = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 26 & 0x3ffffff));
-  const uint64_t c = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 52));
-  return a + (b << 26) + (c << 52);
+struct Sum {
+  uint64_t sum;
+  uint32_t count;
+};
+// Over a warp; the counts are below 2^16 in all.
+__device__ __forceinline__ Sum warp_total(uint64_t v, uint32_t count) {
+  // in pieces of 26 bits, whose sums over a warp fit 32; the counts with the last, which is short
+  const uint32_t a = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0x3ffffff), b = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 26) & 0x3ffffff);
+  const uint32_t c = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 52) | count << 16);
+  return {a + ((uint64_t)b << 26) + ((uint64_t)(c & 0xffff) << 52), c >> 16};
 }
 
-// Sum over the CTA, the same for every thread; one barrier a call, `turn` alternates.
-__device__ __forceinline__ uint64_t block_total(uint64_t v, SampleShared &s, int &turn) {
-  v = warp_total(v);
-  turn ^= 1;
-  if ((threadIdx.x & 31) == 0) s.parts[turn][threadIdx.x >> 5] = v;
-  __syncthreads();
-  uint64_t sum = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum += s.parts[turn][w];
-  return sum;
-}
-
-// The largest key in [lo, hi] whose sum over entries of at least it reaches `want` (lo does).
-template <class F>
-__device__ __forceinline__ uint32_t bisect_down(uint32_t lo, uint32_t hi, uint64_t want, SampleShared &s, int &turn, const F &sum_from) {
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo + 1) / 2;
-    if (block_total(sum_from(mid), s, turn) >= want)
-      lo = mid;
-    else
-      hi = mid - 1;
+// Sums over the first `threads` threads of the CTA, the same for each; one barrier a call, `turn` alternates.
+struct Totals {
+  SampleShared &s;
+  int threads, turn;
+  __device__ __forceinline__ Sum operator()(uint64_t v, uint32_t count = 0) {
+    const Sum w = warp_total(v, count);
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) s.parts[turn][threadIdx.x >> 5] = {w.sum, w.count, 0};
+    asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+    // a lane a part: sixteen warps reading sixteen parts each take a thousand cycles
+    const int lane = threadIdx.x & 31;
+    const bool part = lane < threads / 32;
+    return warp_total(part ? s.parts[turn][lane].sum : 0, part ? s.parts[turn][lane].count : 0);
   }
-  return lo;
-}
-// The smallest index in [0, hi] whose sum over entries up to it reaches `want` (hi does).
-template <class F>
-__device__ __forceinline__ int bisect_up(int hi, uint64_t want, SampleShared &s, int &turn, const F &sum_to) {
-  int lo = 0;
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (block_total(sum_to(mid), s, turn) >= want)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  return lo;
-}
+};
 
 // u times a total, as the whole number that a sum has to pass; p of a total, as the one it has to reach.
 __device__ __forceinline__ uint64_t passed(float u, uint64_t total) {
@@ -175,6 +171,7 @@ struct Row {
   const T *at;       // element 0
   int vocab, skew;   // of vector 0, the elements before element 0
   int begin, end;    // this warp's vectors
+  bool infinite;     // the largest is: its elements are 0, the others nothing
   __device__ __forceinline__ int index(int v, int e) const { return v * E + e - skew; }
   // A vector's elements; NaN where it reaches over the row's ends.
   __device__ __forceinline__ void load(int v, float (&x)[E]) const {
@@ -191,38 +188,52 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = first + e >= 0 && first + e < vocab ? widen(at[first + e]) : NAN;
     }
+    if (infinite) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
+    }
   }
-  // f(vector, elements) for the vectors of this lane, U in flight.
+  __device__ __forceinline__ void load_or_nothing(int v, float (&x)[E]) const {
+    if (v < end) {
+      load(v, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = NAN;
+    }
+  }
+  // f(vector, elements) by whole warps for all vectors of this lane, U in flight; behind the end they are NaN.
   template <int U, class F>
   __device__ __forceinline__ void each(const F &f) const {
-    for (int v = begin + (threadIdx.x & 31); v < end; v += 32 * U) {
+    const int lane = threadIdx.x & 31;
+    for (int base = begin; base < end; base += 32 * U) {
       float x[U][E];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (v + 32 * u < end) load(v + 32 * u, x[u]);
+      for (int u = 0; u < U; ++u) load_or_nothing(base + 32 * u + lane, x[u]);
+      __syncwarp();
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (v + 32 * u < end) f(v + 32 * u, x[u]);
+      for (int u = 0; u < U; ++u) f(base + 32 * u + lane, x[u]);
     }
   }
 };
 
 template <class T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleParams p) {
+  constexpr int E = Row<T>::E, U = 8 / E;
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ SampleShared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), r = blockIdx.x / ctas;
-  if (tid < 256) s.table[tid] = exp2(tid / 256.0);
-  if (tid == 0) s.listed = 0, s.total = s.listed_sum = 0;
+  auto other = [&](int c) -> SampleShared & { return *cluster.map_shared_rank(&s, c); };
+  if (tid == 0) s.listed = 0;
   pdl_wait();
   pdl_trigger();
   Row<T> row;
   row.at = static_cast<const T *>(p.logits) + r * p.stride;
   row.vocab = p.vocab;
   row.skew = (int)((reinterpret_cast<uintptr_t>(row.at) & 15) / sizeof(T));
-  const int vectors = (row.skew + p.vocab + Row<T>::E - 1) / Row<T>::E;
-  const int per = (vectors + ctas * kWarps - 1) / (ctas * kWarps);
+  row.infinite = false;
+  const int vectors = (row.skew + p.vocab + E - 1) / E;
+  const int per = (vectors + ctas * kWarps - 1) / (ctas * kWarps);  // of a warp's run
   row.begin = min(vectors, (rank * kWarps + warp) * per);
   row.end = min(vectors, row.begin + per);
 
@@ -231,406 +242,607 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
   const float top_p = p.top_p ? p.top_p[r] : p.top_p_all, min_p = p.min_p ? p.min_p[r] : p.min_p_all;
   if (top_k <= 0 || top_k >= p.vocab) top_k = 0;
-  const bool nucleus = top_p < 1.f;
+  const bool nucleus = top_p < 1.f, lists = !greedy && (top_k || nucleus);
   const float uniform = p.uniform[r];
 
-  // ---- 1: the largest, and a threshold
+  // ---- 1: the largest, where it is first, and a threshold
   float largest = -INFINITY;
-  row.template each<4>([&](int, const float (&x)[Row<T>::E]) {
+  int place = -1;  // its vector
+  row.template each<4>([&](int v, const float (&x)[E]) {
+    float most = x[0];
 #pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e) largest = fmaxf(largest, x[e]);
+    for (int e = 1; e < E; ++e) most = fmaxf(most, x[e]);
+    if (most > largest) largest = most, place = v;
   });
-  int turn = 0;
-  const bool lists = !greedy && (top_k || nucleus);
-  const uint32_t own = key_of(largest);
   {
-    const uint32_t top = __reduce_max_sync(0xffffffffu, own);
-    if (lane == 0) s.parts[0][warp] = top;
+    const uint32_t own = key_of(largest), most = __reduce_max_sync(0xffffffffu, own);
+    if (lane == 0) s.parts[0][warp].sum = most;
     __syncthreads();
-    uint32_t most = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) most = max(most, (uint32_t)s.parts[0][w]);
-    // at least `wanted` elements of the CTA reach it: the maxima of so many threads do
+    const uint32_t block_most = __reduce_max_sync(0xffffffffu, lane < kWarps ? (uint32_t)s.parts[0][lane].sum : 0);
+    // A key that the largest of `wanted` threads reach, and not many more: as many elements do.
     uint32_t reach = kNone;
-    const int wanted = top_k ? (top_k + ctas - 1) / ctas : 128;
+    const int wanted = top_k ? (top_k + ctas - 1) / ctas : kWanted / ctas;
     if (lists && p.vocab > kList && wanted <= kThreads / 2) {
-      uint32_t lo = kNone, hi = most;
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo + 1) / 2;
-        if (__syncthreads_count(own >= mid) >= wanted)
-          lo = mid;
+      uint32_t hi = block_most;
+      while (reach < hi) {
+        const uint32_t mid = reach + (hi - reach + 1) / 2;
+        const int n = __syncthreads_count(own >= mid);
+        if (n >= wanted)
+          reach = mid;
         else
           hi = mid - 1;
+        if (n >= wanted && n <= wanted + wanted / 4 + 2) break;
       }
-      reach = lo;
     }
-    if (tid == 0) {
-      s.max = value_of(most);
-      s.threshold = value_of(reach);
-    }
+    if (tid == 0) s.max = value_of(block_most), s.threshold = value_of(reach);
   }
   cluster.sync();
-  float threshold = INFINITY;
-  for (int c = 0; c < ctas; ++c) {
-    const SampleShared &other = *cluster.map_shared_rank(&s, c);
-    largest = fmaxf(c ? largest : -INFINITY, other.max);
-    threshold = fminf(threshold, other.threshold);
-  }
-  if (largest == -INFINITY) {  // nothing to take
-    if (rank == 0 && tid == 0) {
-      p.token[r] = -1;
-      if (p.logprob) p.logprob[r] = -INFINITY;
+  const float own_largest = largest;
+  // (what the cluster's CTAs have is read by a lane each)
+  const bool reads = lane < ctas;
+  largest = value_of(__reduce_max_sync(0xffffffffu, reads ? key_of(other(lane).max) : 0));
+  float threshold = value_of(__reduce_min_sync(0xffffffffu, reads ? key_of(other(lane).threshold) : UINT32_MAX));
+  if (greedy || largest == -INFINITY) {
+    int first = INT32_MAX;
+    if (own_largest == largest && place >= 0) {
+      float x[E];
+      row.load(place, x);
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (x[e] == largest) first = row.index(place, e);
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) s.first[warp] = first;
+    cluster.sync();
+    if (rank == 0 && warp == 0) {
+      for (int x = lane; x < ctas * kWarps; x += 32) first = min(first, other(x / kWarps).first[x % kWarps]);
+      first = __reduce_min_sync(0xffffffffu, first);
+      if (lane == 0) {
+        p.token[r] = largest == -INFINITY ? -1 : first;
+        if (p.logprob) p.logprob[r] = largest == -INFINITY ? -INFINITY : 0.f;
+      }
     }
     cluster.sync();  // no CTA leaves while its shared memory is read
     return;
   }
-
-  if (greedy) {
-    int first = INT32_MAX;
-    row.template each<4>([&](int v, const float (&x)[Row<T>::E]) {
-#pragma unroll
-      for (int e = Row<T>::E - 1; e >= 0; --e)
-        if (x[e] == largest) first = min(first, row.index(v, e));
-    });
-    first = __reduce_min_sync(0xffffffffu, first);
-    if (lane == 0) s.run_ties[warp] = first;
-    cluster.sync();
-    if (rank == 0 && warp == 0) {
-      for (int x = lane; x < ctas * kWarps; x += 32) first = min(first, cluster.map_shared_rank(&s, x / kWarps)->run_ties[x % kWarps]);
-      first = __reduce_min_sync(0xffffffffu, first);
-      if (lane == 0) {
-        p.token[r] = first;
-        if (p.logprob) p.logprob[r] = 0.f;
-      }
-    }
-    cluster.sync();
-    return;
+  if (largest == INFINITY) {
+    row.infinite = true;
+    largest = 0.f;
+    threshold = threshold == INFINITY ? 0.f : -INFINITY;
   }
-
-  const Weights weights = {s.table, largest, 256.0 * 1.4426950408889634 / (double)temperature, p.scale};
-  const double least = min_p > 0.f ? 256.0 * log2((double)fminf(min_p, 1.f)) : -INFINITY;  // of y
+  Weights weights;
+  weights.max = largest;
+  weights.scale = p.scale;
+  weights.factor = fmin(32.0 * kLog2e / (double)temperature, 3e38);  // (a temperature below 2e-37 counts as that)
+  weights.factor32 = (float)weights.factor;
+  weights.power = exp2(lane / 32.0);
+  // the least logit of weight min_p: the next f32 from the bound on
+  float least = -INFINITY;
+  if (min_p > 0.f) least = min_p < 1.f ? __double2float_ru((double)largest + (double)temperature * log((double)min_p)) : largest;
   // the token and the logarithm of its share
   auto answer = [&](int index, float x, uint64_t total) {
     p.token[r] = index;
-    if (p.logprob) p.logprob[r] = (float)(weights.place(x) * (0.6931471805599453 / 256) + (p.scale * 0.6931471805599453 - log((double)total)));
+    const double of_largest = x == largest ? 0.0 : ((double)x - (double)largest) / (double)temperature;
+    if (p.logprob) p.logprob[r] = (float)(of_largest + (p.scale * kLn2 - log((double)total)));
   };
-  // what is kept: keys over `cut`, and the first `ties` elements of that key
+  Totals totals = {s, kThreads, 0};
+  // What is kept: keys over `cut`, and of that key the indices up to `cut_index`.
   uint32_t cut = kNone;
-  int64_t ties = 0;
+  int cut_index = -1;
+  bool have_runs = false;
 
   if (lists) {
     // ---- 2: what reaches the threshold, and the total
     const bool sums = nucleus && !top_k;
-    uint64_t total = 0;
-    row.template each<2>([&](int v, const float (&x)[Row<T>::E]) {
+    auto list = [&](int v, const float (&x)[E], float from, float to) {  // logits from .. to
       bool some = false;
 #pragma unroll
-      for (int e = 0; e < Row<T>::E; ++e) some |= x[e] >= threshold;
+      for (int e = 0; e < E; ++e) some |= x[e] >= from && x[e] <= to;
       if (some && *(volatile int *)&s.listed <= kList) {  // (not all of a flat row)
 #pragma unroll
-        for (int e = 0; e < Row<T>::E; ++e)
-          if (x[e] >= threshold && x[e] > -INFINITY) {
+        for (int e = 0; e < E; ++e)
+          if (x[e] >= from && x[e] <= to && x[e] > -INFINITY) {
             const int at = atomicAdd(&s.listed, 1);
             if (at < kList) s.list.key[at] = key_of(x[e]), s.list.index[at] = row.index(v, e);
           }
       }
+      __syncwarp();
+    };
+    float list_lo = threshold, list_hi = largest;
+    uint64_t total = 0, inside = 0;  // of weights: of all (or above a list), in the list
+    uint64_t count = 0;              // above the list
+    float lowest = INFINITY;
+    int before = 0, all = 0;  // entries of the CTAs before, of all
+    // Sums up `total`, `count` and the list over the cluster.
+    auto exchange = [&] {
+      total = totals(total).sum;  // (its barrier: the list is complete)
+      count = totals(count).sum;
+      const int listed = s.listed;
+      inside = 0;
+      if (nucleus && listed <= kList)
+        for (int x = 0; x < listed; x += kThreads) inside += weights.of(x + tid < listed ? value_of(s.list.key[x + tid]) : NAN);
+      inside = totals(inside).sum;
+      if (tid == 0) s.total = total, s.inside = inside, s.count = count;
+      cluster.sync();
+      const int here = reads ? min(other(lane).listed, kList + 1) : 0;
+      total = reads ? other(lane).total : 0;
+      inside = reads ? other(lane).inside : 0;
+      count = reads ? other(lane).count : 0;
+      const Sum t = warp_total(total, here);
+      total = t.sum;
+      all = min((int)t.count, kList + 1);
+      const Sum b = warp_total(inside, lane < rank ? here : 0);
+      inside = b.sum;
+      before = (int)b.count;
+      count = warp_total(count, 0).sum;
+    };
+    row.template each<U>([&](int v, const float (&x)[E]) {
+      list(v, x, threshold, INFINITY);
+#pragma unroll
+      for (int e = 0; e < E; ++e) lowest = fminf(lowest, x[e] > -INFINITY ? x[e] : INFINITY);
       if (sums) {
 #pragma unroll
-        for (int e = 0; e < Row<T>::E; ++e) total += weights.of(x[e]);
+        for (int e = 0; e < E; ++e) total += weights.of(x[e]);
       }
     });
-    total = block_total(total, s, turn);  // (its barrier: the list is complete)
-    int listed = s.listed;
-    uint64_t inside = 0;
-    if (sums && listed <= kList)
-      for (int x = tid; x < listed; x += kThreads) inside += weights.of(value_of(s.list.key[x]));
-    inside = block_total(inside, s, turn);
-    if (tid == 0) s.total = total, s.listed_sum = inside;
-    cluster.sync();
-    total = inside = 0;
-    int before = 0, all = 0;
-    for (int c = 0; c < ctas; ++c) {
-      const SampleShared &other = *cluster.map_shared_rank(&s, c);
-      if (c == rank) before = all;
-      all = (int)min((int64_t)all + other.listed, (int64_t)kList + 1);
-      total += other.total;
-      inside += other.listed_sum;
+    {
+      const uint32_t key = __reduce_min_sync(0xffffffffu, key_of(lowest));
+      if (lane == 0) s.first[warp] = (int)(key ^ 0x80000000u);  // in the order of ints
     }
-    if (all <= kList && (!sums || inside >= reached(top_p, total))) {
-      // ---- 3: all entries to the first CTA
-      if (rank != 0) {
-        SampleShared &to = *cluster.map_shared_rank(&s, 0);
-        for (int x = tid; x < listed; x += kThreads) to.list.key[before + x] = s.list.key[x], to.list.index[before + x] = s.list.index[x];
-      }
+    exchange();
+    const uint64_t row_total = total, want_sum = sums ? reached(top_p, total) : 0;
+
+    // The list's entries into the registers of the first CTA's first threads, and what is done there.
+    uint32_t key[kListed];
+    int index[kListed];
+    uint64_t w[kListed];
+    bool kept[kListed];
+    int threads = 0;
+    auto gather = [&] {
+      if (rank != 0)
+        for (int x = tid; x < min(s.listed, kList); x += kThreads) other(0).list.key[before + x] = s.list.key[x], other(0).list.index[before + x] = s.list.index[x];
       cluster.sync();
-      if (rank != 0) return;
-      uint32_t key[kListed];
-      int index[kListed];
-      uint64_t w[kListed];
-      bool kept[kListed];
+      threads = all <= kListed * kFew ? kFew : kThreads;
+      totals.threads = threads;
+      if (rank != 0 || tid >= threads) return;
 #pragma unroll
       for (int x = 0; x < kListed; ++x) {
-        const int at = x * kThreads + tid;
+        const int at = x * threads + tid;
         kept[x] = at < all;
         key[x] = kept[x] ? s.list.key[at] : 0;
-        index[x] = kept[x] ? s.list.index[at] : INT32_MAX;
-        w[x] = kept[x] ? weights.of(value_of(key[x])) : 0;
+        index[x] = kept[x] ? s.list.index[at] : 0;
+        w[x] = weights.of(kept[x] ? value_of(key[x]) : NAN);
       }
-      const uint32_t lowest = key_of(threshold), highest = key_of(largest);
-      // cuts the kept entries behind the `want`-th unit of `amount`, in the order of keys, then of indices
-      auto cut_at = [&](uint64_t want, const uint64_t (&amount)[kListed]) {
-        const uint32_t last = bisect_down(lowest, highest, want, s, turn, [&](uint32_t from) {
-          uint64_t sum = 0;
+    };
+    // Keys, then indices from the lowest, as one number in the order of what is kept first.
+    auto order_of = [&](int x) { return (uint64_t)key[x] << 32 | ~(uint32_t)index[x]; };
+    // The entry that holds the `want`-th unit of `amount` of the kept entries: those up to it stay.
+    auto cut_list = [&](uint64_t want, auto amount) {
+      uint64_t lo = (uint64_t)key_of(list_lo) << 32, hi = (uint64_t)key_of(list_hi) << 32 | UINT32_MAX;
+      uint32_t n = 0;
 #pragma unroll
-          for (int x = 0; x < kListed; ++x) sum += kept[x] && key[x] >= from ? amount[x] : 0;
-          return sum;
-        });
-        uint64_t over = 0;
+      for (int x = 0; x < kListed; ++x) n += kept[x];
+      for (n = totals(0, n).count; n > 1;) {  // the entry is one of the n in lo .. hi
+        const uint64_t mid = lo + (hi - lo) / 2 + 1;
+        uint64_t sum = 0;
+        uint32_t upper = 0;
 #pragma unroll
-        for (int x = 0; x < kListed; ++x) over += kept[x] && key[x] > last ? amount[x] : 0;
-        over = block_total(over, s, turn);
-        const int end = bisect_up(p.vocab - 1, want - over, s, turn, [&](int to) {
-          uint64_t sum = 0;
-#pragma unroll
-          for (int x = 0; x < kListed; ++x) sum += kept[x] && key[x] == last && index[x] <= to ? amount[x] : 0;
-          return sum;
-        });
-#pragma unroll
-        for (int x = 0; x < kListed; ++x) kept[x] = kept[x] && (key[x] > last || (key[x] == last && index[x] <= end));
-      };
-      if (top_k && top_k < all) {
-        const uint64_t one[kListed] = {1, 1, 1, 1};
-        cut_at(top_k, one);
+        for (int x = 0; x < kListed; ++x)
+          if (kept[x] && order_of(x) >= mid) sum += amount(x), upper += order_of(x) <= hi;
+        const Sum t = totals(sum, upper);
+        if (t.sum >= want)
+          lo = mid, n = t.count;
+        else
+          hi = mid - 1, n -= t.count;
       }
+#pragma unroll
+      for (int x = 0; x < kListed; ++x) kept[x] = kept[x] && order_of(x) >= lo;
+    };
+    auto one = [](int) -> uint64_t { return 1; };
+    auto weight = [&](int x) -> uint64_t { return w[x]; };
+
+    if (all <= kList && (!sums || inside >= want_sum)) {
+      // ---- 3
+      gather();
+      if (rank != 0 || tid >= threads) return;
+      if (top_k && top_k < all) cut_list(top_k, one);
+      uint64_t sum = 0;
       if (nucleus) {
         if (top_k) {
-          total = 0;
 #pragma unroll
-          for (int x = 0; x < kListed; ++x) total += kept[x] ? w[x] : 0;
-          total = block_total(total, s, turn);
+          for (int x = 0; x < kListed; ++x) sum += kept[x] ? w[x] : 0;
+          sum = totals(sum).sum;
         }
-        cut_at(reached(top_p, total), w);
+        cut_list(reached(top_p, sums ? row_total : sum), weight);
       }
-      total = 0;
+      sum = 0;
+      uint32_t n = 0;
 #pragma unroll
       for (int x = 0; x < kListed; ++x) {
-        kept[x] = kept[x] && weights.place(value_of(key[x])) >= least;
-        total += kept[x] ? w[x] : 0;
+        kept[x] = kept[x] && value_of(key[x]) >= least;
+        sum += kept[x] ? w[x] : 0;
+        n += kept[x];
       }
-      total = block_total(total, s, turn);
-      const int token = bisect_up(p.vocab - 1, passed(uniform, total) + 1, s, turn, [&](int to) {
-        uint64_t sum = 0;
+      const Sum left = totals(sum, n);
+      const uint64_t target = passed(uniform, left.sum);
+      n = left.count;
+      int lo = 0, hi = p.vocab - 1;
+      while (n > 1) {  // the token is one of the n in lo .. hi
+        const int mid = lo + (hi - lo) / 2;
+        sum = 0;
+        uint32_t lower = 0;
 #pragma unroll
-        for (int x = 0; x < kListed; ++x) sum += kept[x] && index[x] <= to ? w[x] : 0;
-        return sum;
-      });
+        for (int x = 0; x < kListed; ++x)
+          if (kept[x] && index[x] <= mid) sum += w[x], lower += index[x] >= lo;
+        const Sum t = totals(sum, lower);
+        if (t.sum > target)
+          hi = mid, n = t.count;
+        else
+          lo = mid + 1, n -= t.count;
+      }
 #pragma unroll
       for (int x = 0; x < kListed; ++x)
-        if (kept[x] && index[x] == token) answer(token, value_of(key[x]), total);
+        if (kept[x] && index[x] >= lo && index[x] <= hi) answer(index[x], value_of(key[x]), left.sum);
       return;
     }
-    // ---- or histograms.  First the k-th key by counts, then the run's end by weights.
-    for (int by = top_k ? 0 : 1; by < (nucleus ? 2 : 1); ++by) {
-      const uint64_t want = by == 0 ? (uint64_t)top_k : reached(top_p, total);
-      uint32_t lo = kNone + 1, hi = key_of(largest);
-      uint64_t over = 0, over_count = 0;  // of keys over hi: weights, elements
-      for (;;) {
-        const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
-        cluster.sync();  // the histograms before, and the list, have been read
-        for (int b = tid; b < kBins; b += kThreads) s.bins.count[b] = s.bins.low[b] = s.bins.high[b] = 0;
-        if (tid == 0) s.found = UINT32_MAX;
+
+    bool found = false;
+    if (!(top_k && nucleus)) {
+      // ---- the steps of the logits that the cut may lie in: by weights below the list, if there is one, down to
+      // where weights are nothing
+      const bool below = sums && all <= kList;
+      for (int x = lane; x < ctas * kWarps; x += 32) lowest = fminf(lowest, value_of((uint32_t)other(x / kWarps).first[x % kWarps] ^ 0x80000000u));
+      lowest = value_of(__reduce_min_sync(0xffffffffu, key_of(lowest)));
+      const float range_hi = below ? threshold : largest;
+      const float range_lo = fmaxf(lowest, largest - (float)((p.scale + 2) * kLn2 * (double)temperature));
+      const float step = (range_hi - range_lo) / kSteps, per_step = kSteps / (range_hi - range_lo);
+      float lo = range_lo, hi = range_hi;
+      if (step > 0.f && step < 1e30f && per_step < 1e30f) {
+        cluster.sync();  // the list has been read
+        for (int b = tid; b < kSteps; b += kThreads) s.list.count[b] = 0;
+        if (tid == 0) s.found = s.found_end = UINT32_MAX, s.listed = 0;
         __syncthreads();
-        row.template each<2>([&](int, const float (&x)[Row<T>::E]) {
+        row.template each<U>([&](int, const float (&x)[E]) {
 #pragma unroll
-          for (int e = 0; e < Row<T>::E; ++e) {
-            const uint32_t key = key_of(x[e]);
-            if (!(x[e] > -INFINITY) || key < lo || key > hi) continue;
-            const uint32_t b = (hi - key) >> shift;
-            const uint64_t w = weights.of(x[e]);
-            atomicAdd(&s.bins.count[b], 1u);
-            if (w == 0) continue;
-            const uint32_t add = (uint32_t)w, old = atomicAdd(&s.bins.low[b], add);
-            const uint32_t up = (uint32_t)(w >> 32) + (old + add < old);
-            if (up) atomicAdd(&s.bins.high[b], up);
-          }
+          for (int e = 0; e < E; ++e)
+            if (x[e] >= range_lo && x[e] <= range_hi && !(below && x[e] == range_hi))
+              atomicAdd(&s.list.count[min(kSteps - 1, (int)((range_hi - x[e]) * per_step))], 1u);
         });
         cluster.sync();
-        // a thread's consecutive bins, of all CTAs
-        constexpr int kOwn = kBins / kThreads;
-        uint64_t count[kOwn] = {0}, sum[kOwn] = {0}, amount = 0;
-        for (int c = 0; c < ctas; ++c) {
-          const SampleShared &other = *cluster.map_shared_rank(&s, c);
+        // A thread's consecutive steps: their elements, and the least and the most that their weights (of the
+        // largest's) may come to: of the steps' edges, a little wider for the rounding of a step's number, of
+        // the exponential and of the weights.
+        constexpr int kOwn = kSteps / kThreads;
+        uint32_t n[kOwn] = {0};
+        for (int c = 0; c < ctas; ++c)
 #pragma unroll
-          for (int x = 0; x < kOwn; ++x) {
-            const int b = tid * kOwn + x;
-            count[x] += other.bins.count[b];
-            sum[x] += ((uint64_t)other.bins.high[b] << 32) + other.bins.low[b];
-          }
-        }
-        uint64_t counts = 0, sums_here = 0;
+          for (int x = 0; x < kOwn; ++x) n[x] += other(c).list.count[tid * kOwn + x];
+        const double unit = exp2(-(double)p.scale);
+        auto amount = [&](int x, int side) -> double {
+          if (n[x] == 0) return 0.0;
+          if (!sums) return n[x];
+          const float edge = range_hi - ((float)(tid * kOwn + x) + (side ? -0.01f : 1.01f)) * step;
+          const double weight = exp2f(fminf(0.f, (edge - largest) * (weights.factor32 / 32.f)));
+          return n[x] * fmax(0.0, side ? weight * (1 + 1e-4) + unit : weight * (1 - 1e-4) - unit);
+        };
+        double run[2];
 #pragma unroll
-        for (int x = 0; x < kOwn; ++x) counts += count[x], sums_here += sum[x];
-        // exclusive prefixes over the threads
-        uint64_t run[2] = {counts, sums_here};
+        for (int side = 0; side < 2; ++side) {
+          double mine = 0;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint64_t mine = run[q];
+          for (int x = 0; x < kOwn; ++x) mine += amount(x, side);
+          run[side] = mine;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t up = __shfl_up_sync(0xffffffffu, run[q], o);
-            if (lane >= o) run[q] += up;
+            const double up = __shfl_up_sync(0xffffffffu, run[side], o);
+            if (lane >= o) run[side] += up;
           }
-          __syncthreads();
-          if (lane == 31) s.parts[q][warp] = run[q];
-          run[q] -= mine;
+          if (lane == 31) s.scan[side][warp] = run[side];
+          run[side] -= mine;
         }
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w)
-          if (w < warp) run[0] += s.parts[0][w], run[1] += s.parts[1][w];
-        run[0] += over_count, run[1] += over;
-        amount = run[by];
+        for (int x = 0; x < warp; ++x) run[0] += s.scan[0][x], run[1] += s.scan[1][x];
+        const double need = sums ? (double)(below ? want_sum - inside : want_sum) * unit : (double)top_k;
+        // the first step that may hold the cut, and the first by which it is surely reached
 #pragma unroll
         for (int x = 0; x < kOwn; ++x) {
-          const uint64_t next = amount + (by ? sum[x] : count[x]);
-          if (amount < want && next >= want) {
-            s.found = tid * kOwn + x;
-            s.found_count = run[0];
-            s.found_sum = run[1];
-          }
-          amount = next;
-          run[0] += count[x], run[1] += sum[x];
+          run[0] += amount(x, 0);
+          run[1] += amount(x, 1);
+          if (n[x] && run[1] * (1 + 1e-9) >= need) atomicMin(&s.found, tid * kOwn + x);
+          if (n[x] && run[0] * (1 - 1e-9) >= need) atomicMin(&s.found_end, tid * kOwn + x);
         }
         __syncthreads();
-        if (s.found == UINT32_MAX) {  // fewer elements than k: all are kept
-          cut = kNone, ties = 0;
-          if (by == 0) {
-            total = over;
-            for (int w = 0; w < kWarps; ++w) total += s.parts[1][w];
+        const uint32_t from = s.found, to = s.found_end;
+        if (from == UINT32_MAX && !sums) {
+          found = true;  // fewer than k elements weigh anything: no cut
+        } else if (from != UINT32_MAX) {
+          if (from > 0) hi = range_hi - ((float)from - 0.01f) * step;
+          if (to < kSteps - 1) lo = range_hi - ((float)to + 1.01f) * step;
+          // the list of lo .. hi, and the sums of what lies above it
+          list_lo = lo, list_hi = hi;
+          uint64_t mine = 0;  // of this warp's run, of those that min_p leaves
+          total = count = 0;
+          row.template each<U>([&](int v, const float (&x)[E]) {
+            list(v, x, lo, hi);
+            bool some = false;
+#pragma unroll
+            for (int e = 0; e < E; ++e) some |= x[e] > hi, count += x[e] > hi;
+            if (__any_sync(0xffffffffu, some)) {
+#pragma unroll
+              for (int e = 0; e < E; ++e) {
+                const uint64_t weight = weights.of(x[e] > hi ? x[e] : NAN);
+                total += weight;
+                mine += x[e] >= least ? weight : 0;
+              }
+            }
+          });
+          mine = warp_total(mine, 0).sum;
+          if (lane == 0) s.run_sum[warp] = mine;
+          exchange();
+          if (all <= kList && (sums ? total < want_sum && total + inside >= want_sum : count < (uint64_t)top_k && count + all >= (uint64_t)top_k)) {
+            found = have_runs = true;
+            for (int x = tid; x < ctas * kWarps; x += kThreads) s.runs[x] = other(x / kWarps).run_sum[x % kWarps];
+            gather();
+            if (rank == 0 && tid < threads) {
+              if (sums)
+                cut_list(want_sum - total, weight);
+              else
+                cut_list(top_k - count, one);
+              // the kept entries join their runs
+#pragma unroll
+              for (int x = 0; x < kListed; ++x)
+                if (kept[x] && value_of(key[x]) >= least) atomicAdd((unsigned long long *)&s.runs[(index[x] + row.skew) / E / per], (unsigned long long)w[x]);
+              // the last of them is the cut
+              uint32_t last = UINT32_MAX;
+#pragma unroll
+              for (int x = 0; x < kListed; ++x)
+                if (kept[x]) last = min(last, key[x]);
+              if (tid == 0) s.found = UINT32_MAX, s.cut_index = -1;
+              totals(0);
+              last = __reduce_min_sync(0xffffffffu, last);
+              if (lane == 0) atomicMin(&s.found, last);
+              totals(0);
+#pragma unroll
+              for (int x = 0; x < kListed; ++x)
+                if (kept[x] && key[x] == s.found) atomicMax(&s.cut_index, index[x]);
+              totals(0);
+              if (tid == 0) s.cut = s.found;
+            }
+            totals.threads = kThreads;
+            totals.turn = 0;  // the others have not taken part
+            cluster.sync();
+            cut = other(0).cut;
+            cut_index = other(0).cut_index;
           }
-          break;
         }
-        over_count = s.found_count, over = s.found_sum;
-        hi -= s.found << shift;
-        if (shift == 0) {
-          const uint64_t w = weights.of(value_of(hi));
-          const int64_t last = by == 0 ? (int64_t)(want - over_count) : (int64_t)((want - over + w - 1) / w);
-          if (by == 0) total = over + last * w;
-          // a run that ends at the k-th key keeps no more of it than the k
-          ties = by == 1 && top_k && hi == cut ? min(ties, last) : last;
-          cut = hi;
-          break;
-        }
-        lo = max(lo, hi - ((1u << shift) - 1));
       }
     }
-    cluster.sync();  // the histograms have been read
+    if (!found) {
+      // ---- histograms of the keys.  First the k-th key by counts, then the run's end by weights.
+      total = row_total;
+      uint32_t k_cut = kNone;
+      int64_t ties = 0, all_ties = 0;  // of the cut's key: those kept, those there are
+      for (int by = top_k ? 0 : 1; by < (nucleus ? 2 : 1); ++by) {
+        const uint64_t want = by == 0 ? (uint64_t)top_k : reached(top_p, total);
+        uint32_t lo = kNone + 1, hi = key_of(largest);
+        uint64_t over = 0, over_count = 0;  // of keys over hi: weights, elements
+        for (;;) {
+          const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
+          cluster.sync();  // the histograms before, and the list, have been read
+          for (int b = tid; b < kBins; b += kThreads) s.bins.count[b] = s.bins.low[b] = s.bins.high[b] = 0;
+          if (tid == 0) s.found = UINT32_MAX;
+          __syncthreads();
+          row.template each<U>([&](int, const float (&x)[E]) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const uint32_t key = key_of(x[e]);
+              const bool in = x[e] > -INFINITY && key >= lo && key <= hi;
+              if (!__any_sync(0xffffffffu, in)) continue;
+              const uint64_t w = weights.of(x[e]);
+              if (!in) continue;
+              const uint32_t b = (hi - key) >> shift;
+              atomicAdd(&s.bins.count[b], 1u);
+              if (w != 0) {
+                const uint32_t add = (uint32_t)w, old = atomicAdd(&s.bins.low[b], add);
+                const uint32_t up = (uint32_t)(w >> 32) + (old + add < old);
+                if (up) atomicAdd(&s.bins.high[b], up);
+              }
+            }
+            __syncwarp();
+          });
+          cluster.sync();
+          // a thread's consecutive bins, of all CTAs
+          constexpr int kOwn = kBins / kThreads;
+          uint64_t counts[kOwn] = {0}, weighs[kOwn] = {0};
+          for (int c = 0; c < ctas; ++c)
+#pragma unroll
+            for (int x = 0; x < kOwn; ++x) {
+              const int b = tid * kOwn + x;
+              counts[x] += other(c).bins.count[b];
+              weighs[x] += ((uint64_t)other(c).bins.high[b] << 32) + other(c).bins.low[b];
+            }
+          uint64_t run[2] = {0, 0};
+#pragma unroll
+          for (int x = 0; x < kOwn; ++x) run[0] += counts[x], run[1] += weighs[x];
+          // exclusive prefixes over the threads
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint64_t mine = run[q];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const uint64_t up = __shfl_up_sync(0xffffffffu, run[q], o);
+              if (lane >= o) run[q] += up;
+            }
+            if (lane == 31) s.scan[q][warp] = __longlong_as_double((long long)run[q]);
+            run[q] -= mine;
+          }
+          __syncthreads();
+          uint64_t whole = over;
+          for (int x = 0; x < kWarps; ++x) {
+            const uint64_t a = __double_as_longlong(s.scan[0][x]), b = __double_as_longlong(s.scan[1][x]);
+            if (x < warp) run[0] += a, run[1] += b;
+            whole += b;
+          }
+          run[0] += over_count, run[1] += over;
+#pragma unroll
+          for (int x = 0; x < kOwn; ++x) {
+            const uint64_t next[2] = {run[0] + counts[x], run[1] + weighs[x]};
+            if (run[by] < want && next[by] >= want) {
+              s.found = tid * kOwn + x;
+              s.found_count = run[0];
+              s.found_sum = run[1];
+              s.count = counts[x];
+            }
+            run[0] = next[0], run[1] = next[1];
+          }
+          __syncthreads();
+          if (s.found == UINT32_MAX) {  // fewer elements than k: all are kept
+            total = whole;
+            break;
+          }
+          over_count = s.found_count, over = s.found_sum;
+          hi -= s.found << shift;
+          if (shift == 0) {
+            const uint64_t w = weights.of(value_of(hi));
+            int64_t last = by == 0 ? (int64_t)(want - over_count) : (int64_t)((want - over + w - 1) / w);
+            if (by == 0) total = over + last * w, k_cut = hi;
+            // a run that ends at the k-th key keeps no more of it than the k
+            if (by == 1 && top_k && hi == k_cut) last = min(ties, last);
+            ties = last;
+            all_ties = (int64_t)s.count;
+            cut = hi;
+            break;
+          }
+          lo = max(lo, hi - ((1u << shift) - 1));
+        }
+      }
+      cut_index = INT32_MAX;
+      if (ties < all_ties) {
+        // the index of the last of them: the warps' runs count theirs, and the one that has it looks again
+        int64_t mine = 0;
+        row.template each<U>([&](int, const float (&x)[E]) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) mine += x[e] > -INFINITY && key_of(x[e]) == cut;
+        });
+        mine = (int64_t)warp_total((uint64_t)mine, 0).sum;
+        if (lane == 0) s.run_sum[warp] = (uint64_t)mine;
+        cluster.sync();
+        int64_t before_me = 0;
+        for (int x = lane; x < rank * kWarps + warp; x += 32) before_me += (int64_t)other(x / kWarps).run_sum[x % kWarps];
+        before_me = (int64_t)warp_total((uint64_t)before_me, 0).sum;
+        if (before_me < ties && before_me + mine >= ties) {
+          int left = (int)(ties - before_me);
+          for (int base = row.begin; base < row.end && left > 0; base += 32) {
+            float x[E];
+            row.load_or_nothing(base + lane, x);
+            __syncwarp();
+            int here = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) here += x[e] > -INFINITY && key_of(x[e]) == cut;
+            int upto = here;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const int up = __shfl_up_sync(0xffffffffu, upto, o);
+              if (lane >= o) upto += up;
+            }
+            int at = upto - here;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (x[e] > -INFINITY && key_of(x[e]) == cut && ++at == left) other(0).cut_index = row.index(base + lane, e);
+            left -= __shfl_sync(0xffffffffu, upto, 31);
+          }
+        }
+        cluster.sync();
+        cut_index = other(0).cut_index;
+      }
+    }
   }
 
-  // ---- what is kept of every warp's run
-  uint64_t sum = 0;
-  int tied = 0;
-  row.template each<2>([&](int, const float (&x)[Row<T>::E]) {
+  auto keeps = [&](float x, int index) {
+    const uint32_t key = key_of(x);
+    return x >= least && x > -INFINITY && (key > cut || (key == cut && index <= cut_index));
+  };
+  if (!have_runs) {
+    // ---- what is kept of every warp's run
+    uint64_t sum = 0;
+    row.template each<U>([&](int v, const float (&x)[E]) {
 #pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e) {
-      const uint32_t key = key_of(x[e]);
-      if (!(x[e] > -INFINITY) || key < cut) continue;
-      const double y = weights.place(x[e]);
-      if (!(y >= least)) continue;
-      if (key == cut)
-        ++tied;
-      else
-        sum += weights.at(y);
+      for (int e = 0; e < E; ++e) sum += weights.of(keeps(x[e], row.index(v, e)) ? x[e] : NAN);
+    });
+    sum = warp_total(sum, 0).sum;
+    if (lane == 0) s.run_sum[warp] = sum;
+    cluster.sync();
+    if (rank == 0)
+      for (int x = tid; x < ctas * kWarps; x += kThreads) s.runs[x] = other(x / kWarps).run_sum[x % kWarps];
+  }
+  if (rank == 0) {
+    __syncthreads();
+    if (warp == 0) {  // the run with the token, and the sum of those before it
+      constexpr int kOwn = kMostCtas * kWarps / 32;
+      uint64_t sums[kOwn], upto = 0;
+#pragma unroll
+      for (int x = 0; x < kOwn; ++x) {
+        sums[x] = lane * kOwn + x < ctas * kWarps ? s.runs[lane * kOwn + x] : 0;
+        upto += sums[x];
+      }
+      uint64_t at = upto;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t up = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += up;
+      }
+      const uint64_t kept = __shfl_sync(0xffffffffu, at, 31), target = passed(uniform, kept);
+      at -= upto;
+#pragma unroll
+      for (int x = 0; x < kOwn; ++x) {
+        if (target >= at && target < at + sums[x]) s.run = lane * kOwn + x, s.run_begin = at;
+        at += sums[x];
+      }
+      if (lane == 0) s.kept = kept;
     }
-  });
-  sum = warp_total(sum);
-  tied = __reduce_add_sync(0xffffffffu, tied);
-  if (lane == 0) s.run_sum[warp] = sum, s.run_ties[warp] = tied;
-  cluster.sync();
-  const uint64_t tie = ties ? weights.of(value_of(cut)) : 0;
-  const int runs = ctas * kWarps;
-  for (int x = tid; x < runs; x += kThreads) {
-    const SampleShared &other = *cluster.map_shared_rank(&s, x / kWarps);
-    s.runs.sum[x] = other.run_sum[x % kWarps];
-    s.runs.ties[x] = other.run_ties[x % kWarps];
   }
   cluster.sync();
-  // every thread the same: the total, then this warp's share of it
-  uint64_t total = 0, begin = 0, end = 0;
-  int64_t left = ties, left_here = 0;
-  for (int x = 0; x < runs; ++x) {
-    const int64_t some = min(left, (int64_t)s.runs.ties[x]);
-    if (x == rank * kWarps + warp) begin = total, left_here = left;
-    total += s.runs.sum[x] + some * tie;
-    if (x == rank * kWarps + warp) end = total;
-    left -= some;
-  }
-  const uint64_t target = passed(uniform, total);
-  if (target < begin || target >= end) return;
-  // the warp with the token: its run again
-  uint64_t seen = begin;
+  const int run = other(0).run;
+  const uint64_t total = other(0).kept, target = passed(uniform, total);
+  uint64_t seen = other(0).run_begin;
+  cluster.sync();
+  if (run != rank * kWarps + warp) return;
+  // ---- that run again
   for (int base = row.begin; base < row.end; base += 32) {
-    float x[Row<T>::E];
+    float x[E];
     const int v = base + lane;
-    if (v < row.end) {
-      row.load(v, x);
-    } else {
+    row.load_or_nothing(v, x);
+    __syncwarp();
+    uint64_t w[E], here = 0;
 #pragma unroll
-      for (int e = 0; e < Row<T>::E; ++e) x[e] = NAN;
+    for (int e = 0; e < E; ++e) {
+      w[e] = weights.of(keeps(x[e], row.index(v, e)) ? x[e] : NAN);
+      here += w[e];
     }
-    int mine = 0;  // elements of the cut's key
-#pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e) mine += x[e] > -INFINITY && key_of(x[e]) == cut && weights.place(x[e]) >= least;
-    int upto = mine;
+    uint64_t upto = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      const uint64_t up = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += up;
     }
-    const int64_t mine_left = left_here - (upto - mine);
-    left_here -= __shfl_sync(0xffffffffu, upto, 31);
-    auto weight = [&](int e, int64_t &quota) -> uint64_t {
-      const uint32_t key = key_of(x[e]);
-      if (!(x[e] > -INFINITY) || key < cut) return 0;
-      const double y = weights.place(x[e]);
-      if (!(y >= least)) return 0;
-      return key != cut || quota-- > 0 ? weights.at(y) : 0;
-    };
-    uint64_t here = 0;
-    int64_t quota = mine_left;
+    uint64_t at = seen + upto - here;
+    seen += __shfl_sync(0xffffffffu, upto, 31);
+    if (seen <= target) continue;
 #pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e) here += weight(e, quota);
-    uint64_t run = here;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
+    for (int e = 0; e < E; ++e) {
+      if (target >= at && target < at + w[e]) answer(row.index(v, e), x[e], total);
+      at += w[e];
     }
-    const uint64_t stop = seen + run;  // behind this lane's elements
-    if (target >= stop - here && target < stop) {
-      uint64_t at = stop - here;
-      quota = mine_left;
-      bool done = false;
-#pragma unroll
-      for (int e = 0; e < Row<T>::E; ++e) {
-        at += weight(e, quota);
-        if (!done && at > target) {
-          answer(row.index(v, e), x[e], total);
-          done = true;
-        }
-      }
-    }
-    seen = __shfl_sync(0xffffffffu, stop, 31);
-    if (seen > target) return;
+    return;
   }
 }
 
 template <class T>
 int launch_sample(const SampleParams &p, int64_t rows, cudaStream_t s) {
-  // CTAs of a row: for few rows as many as have a vector or two a thread, for many what fills the GPU.
+  // CTAs of a row: for few rows as many as have a vector a thread, for many so that all rows are in work at once.
   const int64_t vectors = p.vocab / Row<T>::E;
   int ctas = 1;
-  while (ctas < kMostCtas && vectors / ctas > kThreads && rows * ctas < 8 * sm_count()) ctas *= 2;
+  while (ctas < kMostCtas && vectors / ctas > kThreads && rows * ctas * 2 <= 2 * sm_count()) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(kThreads);
