@@ -775,7 +775,7 @@ int lc_shared_decode(int dtype, const void *q, const void *k, const void *v, voi
  * with weights w_i = exp((x_i - max) / temperature), the top_k largest; of these the shortest run from the largest on
  * that holds top_p of their sum; of these those with w_i >= min_p; and of what is left the first index at which the
  * sum in index order passes uniform[row] times its total. Equal logits are taken in index order. temperature <= 0:
- * the largest. top_k <= 0 or >= vocab, top_p >= 1, min_p <= 0: all. NaN logits and -infinity are never taken; where
+ * the largest; over 1e29: as 1e29. top_k <= 0 or >= vocab, top_p >= 1, min_p <= 0: all. NaN logits and -infinity are never taken; where
  * there is nothing else, the token is -1 and logprob -infinity. Each of the four is one value a row, or null and the
  * value *_all for all rows. logprob (may be null): the logarithm of the token's share of what was left. */
 int lc_sample(int dtype, const void *logits, const float *uniform, const float *temperature,

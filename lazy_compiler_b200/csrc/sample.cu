@@ -27,6 +27,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "common.cuh"
 
@@ -43,6 +44,7 @@ constexpr int kFew = 128;                                // threads that a short
 constexpr int kBinBits = 11, kBins = 1 << kBinBits;     // of keys
 constexpr int kSteps = 4096;                             // of logits
 constexpr uint32_t kNone = 0x007fffffu;                  // the key of -infinity
+constexpr float kLowest = -3.402823466e38f;              // the lowest f32
 constexpr double kLn2 = 0.6931471805599453, kLog2e = 1.4426950408889634;
 
 struct SampleParams {
@@ -70,32 +72,67 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
+// The next f32 below.
+__device__ __forceinline__ float below(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __uint_as_float(x > 0.f ? b - 1 : x < 0.f ? b + 1 : 0x80000001u);
+}
 
 // 2^(y / 32), y = (x - max) factor, as a whole number of 2^-s: 2^(i / 32) from lane i, times a polynomial of
-// degree 4 for the rest, |r| <= 1/2 (off by 1.2e-12 at the ends, and with r's sign).  By whole warps.
+// degree 4 for the rest, |r| <= 1/2 (off by 1.2e-12 at the ends, and with r's sign).  By whole warps.  f32
+// only where it is exact: the larger of x and `floor`, which weighs nothing (so does NaN, then).
 struct Weights {
-  double factor;
-  float max, factor32;
-  double power;          // 2^(lane / 32)
-  int scale;
-  __device__ __forceinline__ uint64_t of(float x) const {
-    // what rounds to nothing, -infinity and NaN: the rest may compute anything
-    const bool some = (x - max) * factor32 > -32.f * ((float)scale + 1.5f);
+  double max, factor;
+  float floor;
+  double power;  // 2^(s + lane / 32)
+  // N at a time, step by step: one after the other, the chain of ten f64 operations would be waited for.
+  template <int N>
+  __device__ __forceinline__ void of(const float (&x)[N], uint64_t (&w)[N]) const {
     constexpr double kMagic = 6755399441055744.0, kStep = kLn2 / 32;  // 1.5 * 2^52
-    const double y = ((double)x - (double)max) * factor;  // (x factor - max factor would cancel where T is small)
-    const double z = y + kMagic, r = y - (z - kMagic);
-    const int j = __double2loint(z);
-    double f = fma(r, kStep * kStep * kStep * kStep / 24, kStep * kStep * kStep / 6);
-    f = fma(r, f, kStep * kStep / 2);
-    f = fma(r, f, kStep);
-    f = fma(r, f, 1.0);
-    const int lo = __shfl_sync(0xffffffffu, __double2loint(power), j & 31), hi = __shfl_sync(0xffffffffu, __double2hiint(power), j & 31);
-    f = fma(f, __hiloint2double(hi + (int)((unsigned)(scale + (j >> 5)) << 20), lo), 4503599627370496.0);  // 2^52: the whole number in the low bits
-    return some ? (uint64_t)__double_as_longlong(f) & 0xfffffffffffffull : 0;
+    double f[N], r[N];
+    int j[N], lo[N], hi[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = ((double)fmaxf(x[e], floor) - max) * factor;  // (x factor - max factor would cancel where T is small)
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = r[e] + kMagic;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      j[e] = __double2loint(f[e]);
+      lo[e] = __shfl_sync(0xffffffffu, __double2loint(power), j[e]);
+      hi[e] = __shfl_sync(0xffffffffu, __double2hiint(power), j[e]) + ((j[e] & ~31) << 15);
+      r[e] -= f[e] - kMagic;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = fma(r[e], kStep * kStep * kStep * kStep / 24, kStep * kStep * kStep / 6);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = fma(r[e], f[e], kStep * kStep / 2);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = fma(r[e], f[e], kStep);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = fma(r[e], f[e], 1.0);
+#pragma unroll
+    for (int e = 0; e < N; ++e)  // plus 2^52: the whole number in the low bits
+      w[e] = (uint64_t)__double_as_longlong(fma(f[e], __hiloint2double(hi[e], lo[e]), 4503599627370496.0)) - 0x4330000000000000ull;
+  }
+  __device__ __forceinline__ uint64_t of(float x) const {
+    const float one[1] = {x};
+    uint64_t w[1];
+    of(one, w);
+    return w[0];
+  }
+  // The largest is above the lowest f32.  Temperatures that f32's logits cannot tell from none, or from infinite, are
+  // brought to where the numbers above keep their range: one step of f32 below the largest weighs nothing
+  // already; 1e29.
+  __device__ __forceinline__ void set(float largest, float temperature, int scale) {
+    const float next = below(largest);
+    max = largest;
+    factor = fmin(32.0 * kLog2e / fmin((double)temperature, 1e29), 16384.0 / ((double)largest - (double)next));
+    floor = fmaxf(fminf(__double2float_rd((double)largest - 33.0 * (scale + 2) / factor), next), kLowest);
+    power = exp2(scale + (threadIdx.x & 31) / 32.0);
   }
 };
 
-struct SampleShared {
+struct alignas(16) SampleShared {
   union {
     struct {
       uint32_t key[kList];
@@ -165,53 +202,79 @@ __device__ __forceinline__ uint64_t reached(float p, uint64_t total) {
   return t < 1.0 ? 1 : t < (double)total ? (uint64_t)t : total;
 }
 
+// Adds a thread's N words of shared memory, maybe another CTA's, by 16 bytes: word by word, the lanes' strides make
+// many accesses of one (a histogram of eight CTAs: 57000 cycles).
+template <int N, class Word>
+__device__ __forceinline__ void add_words(Word (&to)[N], const uint32_t *from) {
+  static_assert(N % 4 == 0, "whole vectors");
+#pragma unroll
+  for (int x = 0; x < N; x += 4) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(from + x);
+    to[x] += v.x, to[x + 1] += v.y, to[x + 2] += v.z, to[x + 3] += v.w;
+  }
+}
+
 template <class T>
 struct Row {
   static constexpr int E = 16 / sizeof(T);  // elements of a vector
   const T *at;       // element 0
   int vocab, skew;   // of vector 0, the elements before element 0
   int begin, end;    // this warp's vectors
-  bool infinite;     // the largest is: its elements are 0, the others nothing
+  bool single;       // only elements that are `only` weigh anything: they are 0, the others nothing
+  float only;
   __device__ __forceinline__ int index(int v, int e) const { return v * E + e - skew; }
-  // A vector's elements; NaN where it reaches over the row's ends.
-  __device__ __forceinline__ void load(int v, float (&x)[E]) const {
+  // A vector as it lies there; NaN where it reaches over the ends of the row or of the run.
+  union Raw {
+    uint4 all;
+    T t[E];
+  };
+  __device__ __forceinline__ Raw fetch(int v) const {
+    Raw raw;
     const int first = index(v, 0);
-    if (first >= 0 && first + E <= vocab) {
-      union {
-        uint4 raw;
-        T t[E];
-      } u;
-      u.raw = __ldg(reinterpret_cast<const uint4 *>(at + first));
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = widen(u.t[e]);
+    if (v < end && first >= 0 && first + E <= vocab) {
+      raw.all = __ldg(reinterpret_cast<const uint4 *>(at + first));
     } else {
+      raw.all = make_uint4(UINT32_MAX, UINT32_MAX, UINT32_MAX, UINT32_MAX);  // NaN in any type
+      if (v < end) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = first + e >= 0 && first + e < vocab ? widen(at[first + e]) : NAN;
+        for (int e = 0; e < E; ++e)
+          if (first + e >= 0 && first + e < vocab) raw.t[e] = at[first + e];
+      }
     }
-    if (infinite) {
+    return raw;
+  }
+  __device__ __forceinline__ void open(const Raw &raw, float (&x)[E]) const {
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
+    for (int e = 0; e < E; ++e) x[e] = widen(raw.t[e]);
+    if (single) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = x[e] == only ? 0.f : -INFINITY;
     }
   }
-  __device__ __forceinline__ void load_or_nothing(int v, float (&x)[E]) const {
-    if (v < end) {
-      load(v, x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = NAN;
-    }
-  }
-  // f(vector, elements) by whole warps for all vectors of this lane, U in flight; behind the end they are NaN.
+  // A vector's elements, of a lane of this warp's.
+  __device__ __forceinline__ void load(int v, float (&x)[E]) const { open(fetch(v), x); }
+  // f(vector, elements) by whole warps for all vectors of this lane, U in flight while U are worked on; behind
+  // the end they are NaN.
   template <int U, class F>
   __device__ __forceinline__ void each(const F &f) const {
-    const int lane = threadIdx.x & 31;
-    for (int base = begin; base < end; base += 32 * U) {
-      float x[U][E];
+    const int first = begin + (threadIdx.x & 31);
+    Raw next[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) load_or_nothing(base + 32 * u + lane, x[u]);
+    for (int u = 0; u < U; ++u) next[u] = fetch(first + 32 * u);
+    for (int base = begin; base < end; base += 32 * U) {
+      Raw now[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) now[u] = next[u];
+      const int v = base + (threadIdx.x & 31);
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = fetch(v + 32 * (U + u));
       __syncwarp();
 #pragma unroll
-      for (int u = 0; u < U; ++u) f(base + 32 * u + lane, x[u]);
+      for (int u = 0; u < U; ++u) {
+        float x[E];
+        open(now[u], x);
+        f(v + 32 * u, x);
+      }
     }
   }
 };
@@ -231,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   row.at = static_cast<const T *>(p.logits) + r * p.stride;
   row.vocab = p.vocab;
   row.skew = (int)((reinterpret_cast<uintptr_t>(row.at) & 15) / sizeof(T));
-  row.infinite = false;
+  row.single = false;
   const int vectors = (row.skew + p.vocab + E - 1) / E;
   const int per = (vectors + ctas * kWarps - 1) / (ctas * kWarps);  // of a warp's run
   row.begin = min(vectors, (rank * kWarps + warp) * per);
@@ -246,12 +309,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const float uniform = p.uniform[r];
 
   // ---- 1: the largest, where it is first, and a threshold
-  float largest = -INFINITY;
+  float largest = -INFINITY, lowest = INFINITY;
   int place = -1;  // its vector
   row.template each<4>([&](int v, const float (&x)[E]) {
     float most = x[0];
 #pragma unroll
     for (int e = 1; e < E; ++e) most = fmaxf(most, x[e]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) lowest = fminf(lowest, x[e]);
     if (most > largest) largest = most, place = v;
   });
   {
@@ -305,20 +370,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     cluster.sync();  // no CTA leaves while its shared memory is read
     return;
   }
-  if (largest == INFINITY) {
-    row.infinite = true;
-    largest = 0.f;
-    threshold = threshold == INFINITY ? 0.f : -INFINITY;
+  if (largest == INFINITY || largest == kLowest) {
+    row.single = true;
+    row.only = largest;
+    threshold = threshold == largest ? 0.f : -INFINITY;
+    largest = lowest = 0.f;
   }
   Weights weights;
-  weights.max = largest;
-  weights.scale = p.scale;
-  weights.factor = fmin(32.0 * kLog2e / (double)temperature, 3e38);  // (a temperature below 2e-37 counts as that)
-  weights.factor32 = (float)weights.factor;
-  weights.power = exp2(lane / 32.0);
+  weights.set(largest, temperature, p.scale);
   // the least logit of weight min_p: the next f32 from the bound on
   float least = -INFINITY;
   if (min_p > 0.f) least = min_p < 1.f ? __double2float_ru((double)largest + (double)temperature * log((double)min_p)) : largest;
+  // the sum of a vector's weights
+  auto weigh = [&](const float (&x)[E]) {
+    uint64_t w[E], sum = 0;
+    weights.of(x, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += w[e];
+    return sum;
+  };
   // the token and the logarithm of its share
   auto answer = [&](int index, float x, uint64_t total) {
     p.token[r] = index;
@@ -335,10 +405,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     // ---- 2: what reaches the threshold, and the total
     const bool sums = nucleus && !top_k;
     auto list = [&](int v, const float (&x)[E], float from, float to) {  // logits from .. to
-      bool some = false;
+      float most = x[0];
 #pragma unroll
-      for (int e = 0; e < E; ++e) some |= x[e] >= from && x[e] <= to;
-      if (some && *(volatile int *)&s.listed <= kList) {  // (not all of a flat row)
+      for (int e = 1; e < E; ++e) most = fmaxf(most, x[e]);
+      if (most >= from && *(volatile int *)&s.listed <= kList) {  // (not all of a flat row)
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (x[e] >= from && x[e] <= to && x[e] > -INFINITY) {
@@ -351,7 +421,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     float list_lo = threshold, list_hi = largest;
     uint64_t total = 0, inside = 0;  // of weights: of all (or above a list), in the list
     uint64_t count = 0;              // above the list
-    float lowest = INFINITY;
     int before = 0, all = 0;  // entries of the CTAs before, of all
     // Sums up `total`, `count` and the list over the cluster.
     auto exchange = [&] {
@@ -376,14 +445,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       before = (int)b.count;
       count = warp_total(count, 0).sum;
     };
-    row.template each<U>([&](int v, const float (&x)[E]) {
+    row.template each<1>([&](int v, const float (&x)[E]) {
       list(v, x, threshold, INFINITY);
-#pragma unroll
-      for (int e = 0; e < E; ++e) lowest = fminf(lowest, x[e] > -INFINITY ? x[e] : INFINITY);
-      if (sums) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) total += weights.of(x[e]);
-      }
+      if (sums) total += weigh(x);
     });
     {
       const uint32_t key = __reduce_min_sync(0xffffffffu, key_of(lowest));
@@ -490,12 +554,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (!(top_k && nucleus)) {
       // ---- the steps of the logits that the cut may lie in: by weights below the list, if there is one, down to
       // where weights are nothing
-      const bool below = sums && all <= kList;
+      const bool under = sums && all <= kList;
       for (int x = lane; x < ctas * kWarps; x += 32) lowest = fminf(lowest, value_of((uint32_t)other(x / kWarps).first[x % kWarps] ^ 0x80000000u));
       lowest = value_of(__reduce_min_sync(0xffffffffu, key_of(lowest)));
-      const float range_hi = below ? threshold : largest;
+      const float range_hi = under ? threshold : largest;
       const float range_lo = fmaxf(lowest, largest - (float)((p.scale + 2) * kLn2 * (double)temperature));
       const float step = (range_hi - range_lo) / kSteps, per_step = kSteps / (range_hi - range_lo);
+      const float range_to = under ? range_hi : INFINITY;  // the largest is at range_hi, and counts
       float lo = range_lo, hi = range_hi;
       if (step > 0.f && step < 1e30f && per_step < 1e30f) {
         cluster.sync();  // the list has been read
@@ -504,9 +569,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         __syncthreads();
         row.template each<U>([&](int, const float (&x)[E]) {
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (x[e] >= range_lo && x[e] <= range_hi && !(below && x[e] == range_hi))
-              atomicAdd(&s.list.count[min(kSteps - 1, (int)((range_hi - x[e]) * per_step))], 1u);
+          for (int e = 0; e < E; ++e) {
+            const int b = min(kSteps - 1, (int)((range_hi - x[e]) * per_step));
+            if (x[e] >= range_lo && x[e] < range_to) atomicAdd(&s.list.count[b], 1u);
+          }
         });
         cluster.sync();
         // A thread's consecutive steps: their elements, and the least and the most that their weights (of the
@@ -514,15 +580,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         // the exponential and of the weights.
         constexpr int kOwn = kSteps / kThreads;
         uint32_t n[kOwn] = {0};
-        for (int c = 0; c < ctas; ++c)
-#pragma unroll
-          for (int x = 0; x < kOwn; ++x) n[x] += other(c).list.count[tid * kOwn + x];
+        for (int c = 0; c < ctas; ++c) add_words(n, other(c).list.count + tid * kOwn);
         const double unit = exp2(-(double)p.scale);
         auto amount = [&](int x, int side) -> double {
           if (n[x] == 0) return 0.0;
           if (!sums) return n[x];
           const float edge = range_hi - ((float)(tid * kOwn + x) + (side ? -0.01f : 1.01f)) * step;
-          const double weight = exp2f(fminf(0.f, (edge - largest) * (weights.factor32 / 32.f)));
+          const double weight = exp2f(fminf(0.f, (edge - largest) * (float)(weights.factor / 32)));
           return n[x] * fmax(0.0, side ? weight * (1 + 1e-4) + unit : weight * (1 - 1e-4) - unit);
         };
         double run[2];
@@ -542,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
         __syncthreads();
         for (int x = 0; x < warp; ++x) run[0] += s.scan[0][x], run[1] += s.scan[1][x];
-        const double need = sums ? (double)(below ? want_sum - inside : want_sum) * unit : (double)top_k;
+        const double need = sums ? (double)(under ? want_sum - inside : want_sum) * unit : (double)top_k;
         // the first step that may hold the cut, and the first by which it is surely reached
 #pragma unroll
         for (int x = 0; x < kOwn; ++x) {
@@ -562,20 +626,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           list_lo = lo, list_hi = hi;
           uint64_t mine = 0;  // of this warp's run, of those that min_p leaves
           total = count = 0;
-          row.template each<U>([&](int v, const float (&x)[E]) {
+          row.template each<1>([&](int v, const float (&x)[E]) {
             list(v, x, lo, hi);
+            float over[E];
             bool some = false;
 #pragma unroll
-            for (int e = 0; e < E; ++e) some |= x[e] > hi, count += x[e] > hi;
-            if (__any_sync(0xffffffffu, some)) {
+            for (int e = 0; e < E; ++e) {
+              const bool is = x[e] > hi;
+              some |= is;
+              count += is;
+              over[e] = is ? x[e] : -INFINITY;
+            }
+            if (!__any_sync(0xffffffffu, some)) return;
+            total += weigh(over);
+            if (least > hi) {
 #pragma unroll
-              for (int e = 0; e < E; ++e) {
-                const uint64_t weight = weights.of(x[e] > hi ? x[e] : NAN);
-                total += weight;
-                mine += x[e] >= least ? weight : 0;
-              }
+              for (int e = 0; e < E; ++e) over[e] = over[e] >= least ? over[e] : -INFINITY;
+              mine += weigh(over);
             }
           });
+          if (!(least > hi)) mine = total;
           mine = warp_total(mine, 0).sum;
           if (lane == 0) s.run_sum[warp] = mine;
           exchange();
@@ -654,13 +724,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           // a thread's consecutive bins, of all CTAs
           constexpr int kOwn = kBins / kThreads;
           uint64_t counts[kOwn] = {0}, weighs[kOwn] = {0};
-          for (int c = 0; c < ctas; ++c)
+          for (int c = 0; c < ctas; ++c) {
+            add_words(counts, other(c).bins.count + tid * kOwn);
+            add_words(weighs, other(c).bins.low + tid * kOwn);
+            uint64_t high[kOwn] = {0};
+            add_words(high, other(c).bins.high + tid * kOwn);
 #pragma unroll
-            for (int x = 0; x < kOwn; ++x) {
-              const int b = tid * kOwn + x;
-              counts[x] += other(c).bins.count[b];
-              weighs[x] += ((uint64_t)other(c).bins.high[b] << 32) + other(c).bins.low[b];
-            }
+            for (int x = 0; x < kOwn; ++x) weighs[x] += high[x] << 32;
+          }
           uint64_t run[2] = {0, 0};
 #pragma unroll
           for (int x = 0; x < kOwn; ++x) run[0] += counts[x], run[1] += weighs[x];
@@ -734,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           int left = (int)(ties - before_me);
           for (int base = row.begin; base < row.end && left > 0; base += 32) {
             float x[E];
-            row.load_or_nothing(base + lane, x);
+            row.load(base + lane, x);
             __syncwarp();
             int here = 0;
 #pragma unroll
@@ -758,16 +829,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
   }
 
-  auto keeps = [&](float x, int index) {
-    const uint32_t key = key_of(x);
-    return x >= least && x > -INFINITY && (key > cut || (key == cut && index <= cut_index));
-  };
+  // A logit that is kept, or nothing in its place: those over `bound`, and of it the indices up to `bound_index`.
+  float bound = value_of(cut);
+  int bound_index = cut_index;
+  if (least > bound) {
+    bound = below(least);
+    bound_index = -1;
+  }
+  auto kept_of = [&](float x, int index) { return x > bound || (bound_index >= 0 && x == bound && index <= bound_index) ? x : -INFINITY; };
   if (!have_runs) {
     // ---- what is kept of every warp's run
     uint64_t sum = 0;
-    row.template each<U>([&](int v, const float (&x)[E]) {
+    row.template each<1>([&](int v, const float (&x)[E]) {
+      float kept[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum += weights.of(keeps(x[e], row.index(v, e)) ? x[e] : NAN);
+      for (int e = 0; e < E; ++e) kept[e] = kept_of(x[e], row.index(v, e));
+      sum += weigh(kept);
     });
     sum = warp_total(sum, 0).sum;
     if (lane == 0) s.run_sum[warp] = sum;
@@ -806,19 +883,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const uint64_t total = other(0).kept, target = passed(uniform, total);
   uint64_t seen = other(0).run_begin;
   cluster.sync();
-  if (run != rank * kWarps + warp) return;
-  // ---- that run again
+  if (run / kWarps != rank) return;
+  // ---- that run again, a sixteenth a warp, and the sixteenth that holds the token once more
+  const int run_end = min(vectors, (run + 1) * per), share = (per + kWarps - 1) / kWarps;
+  row.begin = min(run_end, run * per + warp * share);
+  row.end = min(run_end, row.begin + share);
+  uint64_t mine = 0;
+  row.template each<1>([&](int v, const float (&x)[E]) {
+    float kept[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) kept[e] = kept_of(x[e], row.index(v, e));
+    mine += weigh(kept);
+  });
+  mine = warp_total(mine, 0).sum;
+  if (lane == 0) s.run_sum[warp] = mine;
+  __syncthreads();
+  for (int x = 0; x < warp; ++x) seen += s.run_sum[x];
+  if (target < seen || target >= seen + mine) return;
   for (int base = row.begin; base < row.end; base += 32) {
     float x[E];
     const int v = base + lane;
-    row.load_or_nothing(v, x);
+    row.load(v, x);
     __syncwarp();
     uint64_t w[E], here = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      w[e] = weights.of(keeps(x[e], row.index(v, e)) ? x[e] : NAN);
-      here += w[e];
-    }
+    for (int e = 0; e < E; ++e) x[e] = kept_of(x[e], row.index(v, e));
+    weights.of(x, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) here += w[e];
     uint64_t upto = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -842,7 +934,8 @@ int launch_sample(const SampleParams &p, int64_t rows, cudaStream_t s) {
   // CTAs of a row: for few rows as many as have a vector a thread, for many so that all rows are in work at once.
   const int64_t vectors = p.vocab / Row<T>::E;
   int ctas = 1;
-  while (ctas < kMostCtas && vectors / ctas > kThreads && rows * ctas * 2 <= 2 * sm_count()) ctas *= 2;
+  const int64_t kk = getenv("KC") ? atoi(getenv("KC")) : 2;
+  while (ctas < kMostCtas && vectors / ctas > kThreads && rows * ctas * 2 <= kk * sm_count()) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(kThreads);
