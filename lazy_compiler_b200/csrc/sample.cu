@@ -14,7 +14,7 @@
 //      that some hundred elements reach, from the lanes' own largest
 //   2  what reaches the threshold goes to a list; where top-p asks for it, the total
 //   3  one CTA has the list in registers and finds the k-th, the end of the run and the token
-//      by bisection of (logit, index) and of the index, each step a sum over the CTA
+//      by bisection of (logit, index) and of the index, each step a sum over the threads
 // Where the list does not hold what may be kept, the cut is looked for first: a histogram of
 // counts over 4096 equal steps of the logits, the steps that the cut may lie in (a step's weights
 // are nearly one), and the list is of those, with the exact sums of what lies above them; where even
@@ -27,7 +27,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "common.cuh"
 
@@ -72,6 +71,16 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
+// 2^(i / 32).
+__constant__ double kPowers[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484,
+    1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407,
+    1.5759808451078865, 1.6104903319492543, 1.645755478153965, 1.681792830507429, 1.718619298122478,
+    1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474,
+    1.9571441241754002};
+
 // The next f32 below.
 __device__ __forceinline__ float below(float x) {
   const uint32_t b = __float_as_uint(x);
@@ -120,15 +129,18 @@ struct Weights {
     of(one, w);
     return w[0];
   }
-  // The largest is above the lowest f32.  Temperatures that f32's logits cannot tell from none, or from infinite, are
-  // brought to where the numbers above keep their range: one step of f32 below the largest weighs nothing
-  // already; 1e29.
-  __device__ __forceinline__ void set(float largest, float temperature, int scale) {
+  // Temperatures that f32's logits cannot tell from none, or from infinite, are brought to where the numbers above
+  // keep their range: one step of f32 below the largest weighs nothing already; 1e29.
+  __device__ __forceinline__ void set(float temperature, int scale) {
+    factor = 32.0 * kLog2e / fmin((double)temperature, 1e29);
+    power = kPowers[threadIdx.x & 31];
+    power = __hiloint2double(__double2hiint(power) + (scale << 20), __double2loint(power));
+  }
+  __device__ __forceinline__ void set_largest(float largest, int scale) {  // above the lowest f32
     const float next = below(largest);
     max = largest;
-    factor = fmin(32.0 * kLog2e / fmin((double)temperature, 1e29), 16384.0 / ((double)largest - (double)next));
-    floor = fmaxf(fminf(__double2float_rd((double)largest - 33.0 * (scale + 2) / factor), next), kLowest);
-    power = exp2(scale + (threadIdx.x & 31) / 32.0);
+    factor = fmin(factor, (double)__fdiv_rd(16384.f, largest - next));
+    floor = fmaxf(fminf(__fsub_rd(largest, __fdiv_ru(33.f * (scale + 2), (float)factor)), next), kLowest);
   }
 };
 
@@ -137,7 +149,13 @@ struct alignas(16) SampleShared {
     struct {
       uint32_t key[kList];
       int index[kList];
-      uint32_t count[kSteps];
+      union {
+        uint32_t count[kSteps];
+        struct {  // in the first CTA: the lists, each in its part
+          uint32_t in_key[kList];
+          int in_index[kList];
+        };
+      };
     } list;
     struct {
       uint32_t count[kBins], low[kBins], high[kBins];
@@ -148,11 +166,16 @@ struct alignas(16) SampleShared {
     uint32_t count, pad;
   } parts[2][kWarps];
   double scan[3][kWarps];
-  // what the cluster's other CTAs read
-  float max, threshold, min;
-  int listed, first[kWarps];
-  uint64_t total, inside, count;
-  uint64_t run_sum[kWarps];
+  // what the cluster's CTAs have left here, each in its place
+  struct {
+    float max, threshold, min;
+    int listed;
+    uint64_t total, inside, count;
+  } from[2][kMostCtas];
+  int first[kMostCtas * kWarps];
+  uint64_t run_sum[kMostCtas * kWarps];
+  int listed;
+  uint64_t count;
   // what the first CTA has found
   uint32_t cut;
   int cut_index, run;
@@ -308,6 +331,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const bool nucleus = top_p < 1.f, lists = !greedy && (top_k || nucleus);
   const float uniform = p.uniform[r];
 
+  Weights weights;
+  weights.set(temperature, p.scale);
+
   // ---- 1: the largest, where it is first, and a threshold
   float largest = -INFINITY, lowest = INFINITY;
   int place = -1;  // its vector
@@ -339,14 +365,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (n >= wanted && n <= wanted + wanted / 4 + 2) break;
       }
     }
-    if (tid == 0) s.max = value_of(block_most), s.threshold = value_of(reach);
+    if (tid < ctas) {
+      auto &to = other(tid).from[0][rank];
+      to.max = value_of(block_most), to.threshold = value_of(reach);
+    }
   }
   cluster.sync();
   const float own_largest = largest;
-  // (what the cluster's CTAs have is read by a lane each)
-  const bool reads = lane < ctas;
-  largest = value_of(__reduce_max_sync(0xffffffffu, reads ? key_of(other(lane).max) : 0));
-  float threshold = value_of(__reduce_min_sync(0xffffffffu, reads ? key_of(other(lane).threshold) : UINT32_MAX));
+  const bool reads = lane < ctas;  // a lane a CTA
+  largest = value_of(__reduce_max_sync(0xffffffffu, reads ? key_of(s.from[0][lane].max) : 0));
+  float threshold = value_of(__reduce_min_sync(0xffffffffu, reads ? key_of(s.from[0][lane].threshold) : UINT32_MAX));
   if (greedy || largest == -INFINITY) {
     int first = INT32_MAX;
     if (own_largest == largest && place >= 0) {
@@ -357,17 +385,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (x[e] == largest) first = row.index(place, e);
     }
     first = __reduce_min_sync(0xffffffffu, first);
-    if (lane == 0) s.first[warp] = first;
+    if (lane == 0) other(0).first[rank * kWarps + warp] = first;
     cluster.sync();
     if (rank == 0 && warp == 0) {
-      for (int x = lane; x < ctas * kWarps; x += 32) first = min(first, other(x / kWarps).first[x % kWarps]);
+      for (int x = lane; x < ctas * kWarps; x += 32) first = min(first, s.first[x]);
       first = __reduce_min_sync(0xffffffffu, first);
       if (lane == 0) {
         p.token[r] = largest == -INFINITY ? -1 : first;
         if (p.logprob) p.logprob[r] = largest == -INFINITY ? -INFINITY : 0.f;
       }
     }
-    cluster.sync();  // no CTA leaves while its shared memory is read
     return;
   }
   if (largest == INFINITY || largest == kLowest) {
@@ -376,8 +403,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     threshold = threshold == largest ? 0.f : -INFINITY;
     largest = lowest = 0.f;
   }
-  Weights weights;
-  weights.set(largest, temperature, p.scale);
+  weights.set_largest(largest, p.scale);
   // the least logit of weight min_p: the next f32 from the bound on
   float least = -INFINITY;
   if (min_p > 0.f) least = min_p < 1.f ? __double2float_ru((double)largest + (double)temperature * log((double)min_p)) : largest;
@@ -421,62 +447,70 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     float list_lo = threshold, list_hi = largest;
     uint64_t total = 0, inside = 0;  // of weights: of all (or above a list), in the list
     uint64_t count = 0;              // above the list
-    int before = 0, all = 0;  // entries of the CTAs before, of all
-    // Sums up `total`, `count` and the list over the cluster.
-    auto exchange = [&] {
-      total = totals(total).sum;  // (its barrier: the list is complete)
-      count = totals(count).sum;
+    int all = 0;                     // entries of all
+    // Sums up `total`, `count` and the list over the cluster, and takes the lists to the first CTA, if each fits its part.
+    const int part = kList / ctas;
+    int exchanges = 0;
+    auto exchange = [&](bool weighs, bool counts) {
+      exchanges ^= 1;
+      if (weighs)
+        total = totals(total).sum;  // (its barrier: the list is complete)
+      else
+        __syncthreads();
+      if (counts) count = totals(count).sum;
       const int listed = s.listed;
       inside = 0;
-      if (nucleus && listed <= kList)
+      if (sums && listed <= part) {
         for (int x = 0; x < listed; x += kThreads) inside += weights.of(x + tid < listed ? value_of(s.list.key[x + tid]) : NAN);
-      inside = totals(inside).sum;
-      if (tid == 0) s.total = total, s.inside = inside, s.count = count;
+        inside = totals(inside).sum;
+      }
+      if (tid < ctas) {
+        auto &to = other(tid).from[exchanges][rank];
+        to.listed = listed <= part ? listed : kList + 1;
+        to.total = total, to.inside = inside, to.count = count;
+      }
+      if (listed <= part) {
+        SampleShared &to = other(0);
+        for (int x = tid; x < listed; x += kThreads) to.list.in_key[rank * part + x] = s.list.key[x], to.list.in_index[rank * part + x] = s.list.index[x];
+      }
       cluster.sync();
-      const int here = reads ? min(other(lane).listed, kList + 1) : 0;
-      total = reads ? other(lane).total : 0;
-      inside = reads ? other(lane).inside : 0;
-      count = reads ? other(lane).count : 0;
-      const Sum t = warp_total(total, here);
-      total = t.sum;
-      all = min((int)t.count, kList + 1);
-      const Sum b = warp_total(inside, lane < rank ? here : 0);
-      inside = b.sum;
-      before = (int)b.count;
-      count = warp_total(count, 0).sum;
+      const auto &have = s.from[exchanges][lane & (kMostCtas - 1)];
+      total = warp_total(reads ? have.total : 0, 0).sum;
+      if (sums) inside = warp_total(reads ? have.inside : 0, 0).sum;
+      if (counts) count = warp_total(reads ? have.count : 0, 0).sum;
+      all = min((int)__reduce_add_sync(0xffffffffu, reads ? have.listed : 0), kList + 1);
     };
     row.template each<1>([&](int v, const float (&x)[E]) {
       list(v, x, threshold, INFINITY);
       if (sums) total += weigh(x);
     });
-    {
-      const uint32_t key = __reduce_min_sync(0xffffffffu, key_of(lowest));
-      if (lane == 0) s.first[warp] = (int)(key ^ 0x80000000u);  // in the order of ints
-    }
-    exchange();
+    lowest = value_of(__reduce_min_sync(0xffffffffu, key_of(lowest)));
+    if (lane < ctas) other(lane).first[rank * kWarps + warp] = (int)(key_of(lowest) ^ 0x80000000u);  // in the order of ints
+    exchange(sums, false);
     const uint64_t row_total = total, want_sum = sums ? reached(top_p, total) : 0;
 
-    // The list's entries into the registers of the first CTA's first threads, and what is done there.
+    // In the first CTA: the lists' entries into the registers of its first threads.
     uint32_t key[kListed];
     int index[kListed];
     uint64_t w[kListed];
     bool kept[kListed];
     int threads = 0;
     auto gather = [&] {
-      if (rank != 0)
-        for (int x = tid; x < min(s.listed, kList); x += kThreads) other(0).list.key[before + x] = s.list.key[x], other(0).list.index[before + x] = s.list.index[x];
-      cluster.sync();
       threads = all <= kListed * kFew ? kFew : kThreads;
       totals.threads = threads;
-      if (rank != 0 || tid >= threads) return;
+      if (tid >= threads) return;
 #pragma unroll
       for (int x = 0; x < kListed; ++x) {
-        const int at = x * threads + tid;
+        int at = x * threads + tid, c = 0;
         kept[x] = at < all;
-        key[x] = kept[x] ? s.list.key[at] : 0;
-        index[x] = kept[x] ? s.list.index[at] : 0;
-        w[x] = weights.of(kept[x] ? value_of(key[x]) : NAN);
+        if (kept[x])
+          for (int n; at >= (n = s.from[exchanges][c].listed); ++c) at -= n;
+        key[x] = kept[x] ? s.list.in_key[c * part + at] : 0;
+        index[x] = kept[x] ? s.list.in_index[c * part + at] : 0;
       }
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < kListed; ++x) w[x] = weights.of(kept[x] ? value_of(key[x]) : NAN);
     };
     // Keys, then indices from the lowest, as one number in the order of what is kept first.
     auto order_of = [&](int x) { return (uint64_t)key[x] << 32 | ~(uint32_t)index[x]; };
@@ -507,8 +541,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
     if (all <= kList && (!sums || inside >= want_sum)) {
       // ---- 3
+      if (rank != 0) return;
       gather();
-      if (rank != 0 || tid >= threads) return;
+      if (tid >= threads) return;
       if (top_k && top_k < all) cut_list(top_k, one);
       uint64_t sum = 0;
       if (nucleus) {
@@ -555,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       // ---- the steps of the logits that the cut may lie in: by weights below the list, if there is one, down to
       // where weights are nothing
       const bool under = sums && all <= kList;
-      for (int x = lane; x < ctas * kWarps; x += 32) lowest = fminf(lowest, value_of((uint32_t)other(x / kWarps).first[x % kWarps] ^ 0x80000000u));
+      for (int x = lane; x < ctas * kWarps; x += 32) lowest = fminf(lowest, value_of((uint32_t)s.first[x] ^ 0x80000000u));
       lowest = value_of(__reduce_min_sync(0xffffffffu, key_of(lowest)));
       const float range_hi = under ? threshold : largest;
       const float range_lo = fmaxf(lowest, largest - (float)((p.scale + 2) * kLn2 * (double)temperature));
@@ -581,14 +616,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         constexpr int kOwn = kSteps / kThreads;
         uint32_t n[kOwn] = {0};
         for (int c = 0; c < ctas; ++c) add_words(n, other(c).list.count + tid * kOwn);
-        const double unit = exp2(-(double)p.scale);
-        auto amount = [&](int x, int side) -> double {
-          if (n[x] == 0) return 0.0;
-          if (!sums) return n[x];
-          const float edge = range_hi - ((float)(tid * kOwn + x) + (side ? -0.01f : 1.01f)) * step;
-          const double weight = exp2f(fminf(0.f, (edge - largest) * (float)(weights.factor / 32)));
-          return n[x] * fmax(0.0, side ? weight * (1 + 1e-4) + unit : weight * (1 - 1e-4) - unit);
-        };
+        const float unit = exp2f(-(float)p.scale), octaves = (float)(weights.factor / 32);
+        const float wider = exp2f(0.01f * step * octaves) * (1 + 1e-4f);
+        float amounts[2][kOwn];
+        float edge = exp2f(fminf(0.f, (range_hi - (float)(tid * kOwn) * step - largest) * octaves));
+#pragma unroll
+        for (int x = 0; x < kOwn; ++x) {
+          const float next = exp2f(fminf(0.f, (range_hi - (float)(tid * kOwn + x + 1) * step - largest) * octaves));
+          amounts[0][x] = sums ? n[x] * fmaxf(0.f, next / wider - unit) : n[x];
+          amounts[1][x] = sums ? n[x] * (edge * wider + unit) : n[x];
+          edge = next;
+        }
+        auto amount = [&](int x, int side) { return (double)amounts[side][x]; };
         double run[2];
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
@@ -606,24 +645,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
         __syncthreads();
         for (int x = 0; x < warp; ++x) run[0] += s.scan[0][x], run[1] += s.scan[1][x];
-        const double need = sums ? (double)(under ? want_sum - inside : want_sum) * unit : (double)top_k;
+        const double need = sums ? (double)(under ? want_sum - inside : want_sum) * (double)unit : (double)top_k;
         // the first step that may hold the cut, and the first by which it is surely reached
 #pragma unroll
         for (int x = 0; x < kOwn; ++x) {
           run[0] += amount(x, 0);
           run[1] += amount(x, 1);
-          if (n[x] && run[1] * (1 + 1e-9) >= need) atomicMin(&s.found, tid * kOwn + x);
-          if (n[x] && run[0] * (1 - 1e-9) >= need) atomicMin(&s.found_end, tid * kOwn + x);
+          if (n[x] && run[1] * (1 + 1e-6) >= need) atomicMin(&s.found, tid * kOwn + x);
+          if (n[x] && run[0] * (1 - 1e-6) >= need) atomicMin(&s.found_end, tid * kOwn + x);
         }
         __syncthreads();
-        const uint32_t from = s.found, to = s.found_end;
-        if (from == UINT32_MAX && !sums) {
+        const uint32_t step_from = s.found, step_to = s.found_end;
+        if (step_from == UINT32_MAX && !sums) {
           found = true;  // fewer than k elements weigh anything: no cut
-        } else if (from != UINT32_MAX) {
-          if (from > 0) hi = range_hi - ((float)from - 0.01f) * step;
-          if (to < kSteps - 1) lo = range_hi - ((float)to + 1.01f) * step;
+        } else if (step_from != UINT32_MAX) {
+          if (step_from > 0) hi = range_hi - ((float)step_from - 0.01f) * step;
+          if (step_to < kSteps - 1) lo = range_hi - ((float)step_to + 1.01f) * step;
           // the list of lo .. hi, and the sums of what lies above it
           list_lo = lo, list_hi = hi;
+          cluster.sync();  // the histogram has been read, in whose place lists may arrive
           uint64_t mine = 0;  // of this warp's run, of those that min_p leaves
           total = count = 0;
           row.template each<1>([&](int v, const float (&x)[E]) {
@@ -647,12 +687,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           });
           if (!(least > hi)) mine = total;
           mine = warp_total(mine, 0).sum;
-          if (lane == 0) s.run_sum[warp] = mine;
-          exchange();
+          if (lane == 0) other(0).run_sum[rank * kWarps + warp] = mine;
+          exchange(true, true);
           if (all <= kList && (sums ? total < want_sum && total + inside >= want_sum : count < (uint64_t)top_k && count + all >= (uint64_t)top_k)) {
             found = have_runs = true;
-            for (int x = tid; x < ctas * kWarps; x += kThreads) s.runs[x] = other(x / kWarps).run_sum[x % kWarps];
-            gather();
+            if (rank == 0) {
+              for (int x = tid; x < ctas * kWarps; x += kThreads) s.runs[x] = s.run_sum[x];
+              gather();
+            }
             if (rank == 0 && tid < threads) {
               if (sums)
                 cut_list(want_sum - total, weight);
@@ -796,10 +838,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           for (int e = 0; e < E; ++e) mine += x[e] > -INFINITY && key_of(x[e]) == cut;
         });
         mine = (int64_t)warp_total((uint64_t)mine, 0).sum;
-        if (lane == 0) s.run_sum[warp] = (uint64_t)mine;
+        if (lane < ctas) other(lane).run_sum[rank * kWarps + warp] = (uint64_t)mine;
         cluster.sync();
         int64_t before_me = 0;
-        for (int x = lane; x < rank * kWarps + warp; x += 32) before_me += (int64_t)other(x / kWarps).run_sum[x % kWarps];
+        for (int x = lane; x < rank * kWarps + warp; x += 32) before_me += (int64_t)s.run_sum[x];
         before_me = (int64_t)warp_total((uint64_t)before_me, 0).sum;
         if (before_me < ties && before_me + mine >= ties) {
           int left = (int)(ties - before_me);
@@ -847,10 +889,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       sum += weigh(kept);
     });
     sum = warp_total(sum, 0).sum;
-    if (lane == 0) s.run_sum[warp] = sum;
+    if (lane == 0) other(0).runs[rank * kWarps + warp] = sum;
     cluster.sync();
-    if (rank == 0)
-      for (int x = tid; x < ctas * kWarps; x += kThreads) s.runs[x] = other(x / kWarps).run_sum[x % kWarps];
   }
   if (rank == 0) {
     __syncthreads();
@@ -931,11 +971,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
 template <class T>
 int launch_sample(const SampleParams &p, int64_t rows, cudaStream_t s) {
-  // CTAs of a row: for few rows as many as have a vector a thread, for many so that all rows are in work at once.
+  // CTAs of a row: for few rows as many as have a vector a thread, for many so that all rows are in work at once;
+  // but two where there are vectors for them, since a row whose cut lies deep holds its CTAs twice as long (256
+  // rows of 151643, f32, every fourth of them: 169 us with two, 213 with one, 218 with four).
   const int64_t vectors = p.vocab / Row<T>::E;
   int ctas = 1;
-  const int64_t kk = getenv("KC") ? atoi(getenv("KC")) : 2;
-  while (ctas < kMostCtas && vectors / ctas > kThreads && rows * ctas * 2 <= kk * sm_count()) ctas *= 2;
+  while (ctas < kMostCtas && vectors / ctas > kThreads && (ctas == 1 || rows * ctas * 2 <= 2 * sm_count())) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(kThreads);
