@@ -37,12 +37,14 @@ struct Sharing {
 };
 // Prefixes below this many tokens are read by each slot alone.
 constexpr int kLeastPrefix = 128;
-__device__ __forceinline__ int group_prefix(const DecodeParams &p, const Sharing &g, int slot) {
-  const int leader = g.leader[slot];
-  if ((unsigned)leader >= (unsigned)p.slots) return 0;
+__device__ __forceinline__ int prefix_tokens(const DecodeParams &p, const Sharing &g, int leader) {
   const int64_t most = (int64_t)p.width * p.page_size;
   const int n = g.shared[leader];
   return n < kLeastPrefix ? 0 : n < most ? n : (int)most;
+}
+__device__ __forceinline__ int group_prefix(const DecodeParams &p, const Sharing &g, int slot) {
+  const int leader = g.leader[slot];
+  return (unsigned)leader < (unsigned)p.slots ? prefix_tokens(p, g, leader) : 0;
 }
 // The tokens of a slot that belong to the prefix.
 __device__ __forceinline__ int slot_prefix(const DecodeParams &p, const Sharing &g, int slot) {

@@ -76,6 +76,7 @@ struct SharedParams {
   int4 *where;  // of every row of a prefix: first and last CTA, row of its tiles, how (kSplitKeys, kWhole)
   int *err;
   int ctas;
+  int runs;  // 16 tokens of a head, from a multiple of 16 on, are one run of memory in k and in v
 };
 constexpr int kSplitKeys = 1, kWhole = 2;
 
@@ -105,7 +106,7 @@ __device__ __forceinline__ Group group_of(const SharedParams &sp, const uint16_t
       hi = mid;
   }
   g.count = lo - at;
-  g.keys = group_prefix(p, sp.sharing, g.slot);
+  g.keys = prefix_tokens(p, sp.sharing, g.slot);
   int first = 0, sinks = 0;
   if (p.window) {
     first = INT32_MAX;
@@ -133,54 +134,55 @@ struct Piece {
   int head, row0, rows, j0, j1;
   int first, last;  // the CTAs that the segment's blocks are in
 };
-// A CTA's run, and the segment that a reader of it is at.
+// a * b / c for units and CTAs: 32 bits where the product has no more, which is a fifth of the instructions.
+__device__ __forceinline__ int share_of(int a, int b, int c, bool below = false) {  // below: of one less
+  const unsigned long long product = (unsigned long long)(unsigned)a * (unsigned)b - below;
+  return (int)((product >> 32) == 0 ? (unsigned)product / (unsigned)c : product / (unsigned)c);
+}
+// A CTA's run, in units, and the segment that a reader of it is at.
 struct Run {
-  long long begin, end, total, seg_begin;
-  int ctas, at, seg;  // seg: (head, 256 rows) of the group
+  int begin, end, total, seg_begin;
+  int ctas, seg;  // seg: (head, 256 rows) of the group
+  Group g;        // at: the group's first place in the order, or behind the last
 };
+__device__ __forceinline__ int row_parts(int count, int group) { return (int)(((int64_t)count * group + kTiles * kRows - 1) / (kTiles * kRows)); }
 struct Pieces {
   Run run;
-  Group g;
-  bool known;
-  __device__ __forceinline__ explicit Pieces(const Run &r) : run(r), known(false) {}
+  __device__ __forceinline__ explicit Pieces(const Run &r) : run(r) {}
   // By a whole warp.
   __device__ __forceinline__ bool next(const SharedParams &sp, const uint16_t *leaders, Piece &out) {
     const DecodeParams &p = sp.p;
     const int lane = threadIdx.x & 31, group = p.q_heads / p.kv_heads;
-    while (run.seg_begin < run.end && run.at < p.slots) {
-      if (!known) {
-        g = group_of(sp, leaders, run.at);
-        known = true;
-      }
-      const int64_t all = (int64_t)g.count * group;
-      const int parts = (int)((all + kTiles * kRows - 1) / (kTiles * kRows));
-      const bool some = g.blocks > 0;
+    while (run.seg_begin < run.end && run.g.at < p.slots) {
+      const int parts = row_parts(run.g.count, group);
+      const bool some = run.g.blocks > 0;
       if (some) {
-        out.g = g;
+        out.g = run.g;
         out.head = run.seg / parts;
         out.row0 = (run.seg - out.head * parts) * (kTiles * kRows);
-        out.rows = (int)min((int64_t)kTiles * kRows, all - out.row0);
-        out.j0 = (int)max(0ll, run.begin - run.seg_begin);
-        out.j1 = (int)min((long long)g.blocks, run.end - run.seg_begin);
-        out.first = (int)(((run.seg_begin + 1) * run.ctas - 1) / run.total);
-        out.last = (int)(((run.seg_begin + g.blocks) * run.ctas - 1) / run.total);
-        run.seg_begin += g.blocks + kEndUnits;
+        out.rows = (int)min((int64_t)kTiles * kRows, (int64_t)run.g.count * group - out.row0);
+        out.j0 = max(0, run.begin - run.seg_begin);
+        out.j1 = min(run.g.blocks, run.end - run.seg_begin);
+        // the CTA of a unit x: the last whose run begins at x or before, ((x + 1) ctas - 1) / total
+        const bool begins = out.j0 == 0, ends = out.j1 == run.g.blocks;
+        out.first = begins ? (int)blockIdx.x : share_of(run.seg_begin + 1, run.ctas, run.total, true);
+        out.last = ends ? (int)blockIdx.x : share_of(run.seg_begin + run.g.blocks, run.ctas, run.total, true);
+        run.seg_begin += run.g.blocks + kEndUnits;
         if (++run.seg == parts * p.kv_heads) run.seg = 0;
       }
       if (!some || run.seg == 0) {  // the next group that begins
         run.seg = 0;
-        known = false;
-        int at = run.at + g.count;
-        for (;;) {
+        int at = run.g.at + run.g.count;
+        while (at < p.slots) {
           const unsigned begins = __ballot_sync(0xffffffffu, at + lane < p.slots && (leaders[at + lane] & kBegins) != 0);
           if (begins) {
             at += __ffs(begins) - 1;
             break;
           }
           at += 32;
-          if (at >= p.slots) break;
         }
-        run.at = at;
+        run.g.at = at;
+        if (at < p.slots && run.seg_begin < run.end) run.g = group_of(sp, leaders, at);
       }
       if (some && out.j1 > out.j0) return true;
     }
@@ -202,6 +204,9 @@ __device__ __forceinline__ bool wait_all(uint64_t *bar, uint32_t parity, volatil
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copies_done() {
   asm volatile("cp.async.commit_group;" ::: "memory");
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -222,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   __shared__ __align__(16) uint32_t key_bits[4][kKeys / 32];  // of a block, its number modulo 4: the keys that are there
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
-  __shared__ long long warp_units[kWarps];
+  __shared__ int warp_units[kWarps];
   __shared__ Run run_shared;
   volatile int *abort = &abort_flag;
   const DecodeParams &p = sp.p;
@@ -260,49 +265,50 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   // ---- this CTA's run
   for (int i = tid; i < p.slots; i += kThreads) {
     const int slot = sp.sharing.order[i];
-    const int leader = (unsigned)slot < (unsigned)p.slots ? sp.sharing.leader[slot] : -1;
     uint16_t mark = 0x7fff;  // no group
-    if ((unsigned)leader < (unsigned)p.slots) mark = (uint16_t)(leader | (leader == slot && group_prefix(p, sp.sharing, slot) > 0 ? kBegins : 0));
+    if ((unsigned)slot < (unsigned)p.slots) {
+      const int leader = sp.sharing.leader[slot], keys = prefix_tokens(p, sp.sharing, slot);
+      if ((unsigned)leader < (unsigned)p.slots) mark = (uint16_t)(leader | (leader == slot && keys > 0 ? kBegins : 0));
+    }
     leaders[i] = mark;
   }
+  if (tid == 0) run_shared = {};
+  if (tid == 0) run_shared.g.at = p.slots;
   __syncthreads();
-  long long *units = reinterpret_cast<long long *>(smem);  // of the group that begins at a position
+  int *units = reinterpret_cast<int *>(smem);  // of the group that begins at a position
   for (int i = warp; i < p.slots; i += kWarps) {
-    long long n = 0;
+    int n = 0;
     if (leaders[i] & kBegins) {
       const Group g = group_of(sp, leaders, i);
-      const long long parts = ((long long)g.count * group + kTiles * kRows - 1) / (kTiles * kRows);
-      if (g.blocks > 0) n = (g.blocks + kEndUnits) * parts * p.kv_heads;
+      if (g.blocks > 0) n = (g.blocks + kEndUnits) * row_parts(g.count, group) * p.kv_heads;
     }
     if (lane == 0) units[i] = n;
   }
-  if (tid == 0) run_shared = {0, 0, 0, 0, 0, p.slots, 0};
   __syncthreads();
   {
     const int per = (p.slots + kThreads - 1) / kThreads;
     const int i0 = min(p.slots, tid * per), i1 = min(p.slots, i0 + per);
-    long long own = 0;
+    int own = 0;
     for (int i = i0; i < i1; ++i) own += units[i];
-    long long inc = own;
+    int inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += up;
     }
     if (lane == 31) warp_units[warp] = inc;
     __syncthreads();
-    long long before = inc - own, total = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += warp_units[w];
-      total += warp_units[w];
-    }
-    const int ctas = (int)min((long long)sp.ctas, (total + kMinRun - 1) / kMinRun);
+    const int of_warp = lane < kWarps ? warp_units[lane] : 0;
+    const int total = __reduce_add_sync(0xffffffffu, of_warp);
+    int before = inc - own + __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0);
+    const int ctas = min(sp.ctas, (total + kMinRun - 1) / kMinRun);
     if ((int)blockIdx.x < ctas) {
-      const long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
+      const int begin = share_of(blockIdx.x, total, ctas), end = share_of(blockIdx.x + 1, total, ctas);
       if (begin >= before && begin < before + own) {
         for (int i = i0; i < i1; ++i) {
           if (begin < before + units[i]) {
-            run_shared = {begin, end, total, before, ctas, i, 0};
+            run_shared.begin = begin, run_shared.end = end, run_shared.total = total;
+            run_shared.seg_begin = before, run_shared.ctas = ctas, run_shared.g.at = i;
             break;
           }
           before += units[i];
@@ -314,10 +320,9 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   // (the units have been read: the buffers are free)
   Run run = run_shared;
   if (run.ctas > 0) {
-    const Group g = group_of(sp, leaders, run.at);
-    const long long in = run.begin - run.seg_begin;
-    run.seg = (int)(in / (g.blocks + kEndUnits));
-    run.seg_begin += (long long)run.seg * (g.blocks + kEndUnits);
+    run.g = group_of(sp, leaders, run.g.at);
+    run.seg = (run.begin - run.seg_begin) / (run.g.blocks + kEndUnits);
+    run.seg_begin += run.seg * (run.g.blocks + kEndUnits);
   }
 
   if (warp < 4) {
@@ -581,8 +586,22 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           break;
         }
         if (!values && lane == 0) *reinterpret_cast<uint4 *>(key_bits[g & 3]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+        // Where 16 keys lie in one page one behind the other, without padding, they are one run of memory: one
+        // place for 16 rows, and the addresses differ by constants (issuing a block: 4400 cycles without).
+        const bool whole = sp.runs && (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu && (key & 15) == 0;
+        if (whole) {
+          const uint32_t to = buffer + row_in * 128 + (((c & 7) ^ (row_in & 7)) << 4);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const T *from = base + __shfl_sync(0xffffffffu, off[x >> 1], (x & 1) * 16) + lane * 8;
+#pragma unroll
+            for (int i = 0; i < 16; i += kRowsPerCopy)  // row i + row_in: bits apart, as piece ^ row wants it
+              copy16((to ^ ((i & 7) << 4)) + (x * 16 + i) * 128, from + i * DP);
+          }
+        }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
+          if (whole) break;
 #pragma unroll 8
           for (int i = 0; i < 32; i += kRowsPerCopy) {
             const int r = x * 32 + i + row_in;
@@ -607,90 +626,106 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   }
 }
 
-// Adds up a row's parts, a warp a row: the prefix's in CTA order, then the suffix.
+// Adds up a row's parts, the prefix's in CTA order, then the suffix: a CTA a row, the parts dealt to its warps.
 constexpr int kMergeWarps = 4;
 
 template <class T, int DP>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ SharedParams sp, const float *own_sums, const float2 *own_stats) {
-  constexpr int kCols = DP / 32;
+  constexpr int kCols = DP / 32, kAtOnce = 8;
+  __shared__ float sums[kMergeWarps][DP];
+  __shared__ float warp_m[kMergeWarps], warp_l[kMergeWarps];
   pdl_wait();
   pdl_trigger();
   const DecodeParams &p = sp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kMergeWarps + warp;
-  if (row >= (int64_t)p.slots * p.q_heads) return;
+  const int64_t row = blockIdx.x;
   const int slot = (int)(row / p.q_heads), h = (int)(row - (int64_t)slot * p.q_heads);
+  const int4 w = __ldcg(sp.where + row);
+  const float2 own = __ldcg(own_stats + row);
   int parts = 0, first = 0, tile_row = 0;
   bool split = false, whole = false;
-  if (slot_prefix(p, sp.sharing, slot) > 0) {
-    const int4 w = __ldcg(sp.where + row);
-    if (w.x >= 0 && w.x <= w.y && w.y < sp.ctas && (unsigned)w.z < kTiles * kRows) {
-      first = w.x, tile_row = w.z, split = w.w & kSplitKeys, whole = w.w & kWhole;
-      parts = (split ? 2 : 1) * (whole ? 1 : w.y - w.x + 1);
-    }
+  if (slot_prefix(p, sp.sharing, slot) > 0 && w.x >= 0 && w.x <= w.y && w.y < sp.ctas && (unsigned)w.z < kTiles * kRows) {
+    first = w.x, tile_row = w.z, split = w.w & kSplitKeys, whole = w.w & kWhole;
+    parts = (split ? 2 : 1) * (whole ? 1 : w.y - w.x + 1);
   }
   auto part = [&](int x) -> int64_t {
     const int cta = first + (split ? x >> 1 : x), t = split ? x & 1 : tile_row / kRows;
     if (whole) return cut_rows(sp.ctas) + row * kTiles + (split ? x : 0);
     return (((int64_t)cta * 2 + (cta == first)) * kTiles + t) * kRows + tile_row % kRows;
   };
-  const float2 own = __ldcg(own_stats + row);
-  float m = own.x;
-  for (int x = lane; x < parts; x += 32) m = fmaxf(m, __ldcg(sp.stats + part(x)).x);
-  m = warp_max(m);
-  const float base = m == -INFINITY ? 0.f : m;
   auto counts = [](const float2 &st) { return st.x != -INFINITY || isnan(st.y); };  // else its sums hold anything
-  float l = 0.f, o[kCols];
+  // this warp's parts, of which the suffix is the last: a lane a part's statistics, then the sums, kAtOnce in flight
+  float m = -INFINITY, l = 0.f, o[kCols];
 #pragma unroll
   for (int y = 0; y < kCols; ++y) o[y] = 0.f;
-  auto take = [&](const float *from, float weight) {
-#pragma unroll
-    for (int y = 0; y < kCols; y += 2) {
-      const float2 two = __ldcg(reinterpret_cast<const float2 *>(from + lane * kCols + y));
-      o[y] = fmaf(two.x, weight, o[y]);
-      o[y + 1] = fmaf(two.y, weight, o[y + 1]);
-    }
-  };
-  for (int x0 = 0; x0 < parts; x0 += 32) {
+  for (int x0 = warp; x0 <= parts; x0 += 32 * kMergeWarps) {
+    const int x = x0 + lane * kMergeWarps;
     float2 st = make_float2(-INFINITY, 0.f);
-    int64_t at = 0;
-    if (x0 + lane < parts) {
-      at = part(x0 + lane);
+    const float *from = own_sums + row * DP;
+    if (x < parts) {
+      const int64_t at = part(x);
       st = __ldcg(sp.stats + at);
+      from = sp.sums + at * DP;
+    } else if (x == parts) {
+      st = own;
     }
     const unsigned some = __ballot_sync(0xffffffffu, counts(st));
+    const float top = fmaxf(m, warp_max(st.x)), base = top == -INFINITY ? 0.f : top, alpha = ex2(m - base);
     const float weight = ex2(st.x - base);
-    if (counts(st)) l = fmaf(st.y, weight, l);
-    const int here = min(32, parts - x0);
-#pragma unroll 4
-    for (int x = 0; x < here; ++x) {
-      const float w = __shfl_sync(0xffffffffu, weight, x);
-      const int64_t from = __shfl_sync(0xffffffffu, at, x);
-      if (some >> x & 1) take(sp.sums + from * DP, w);
-    }
-  }
-  l = warp_sum(l);
-  if (counts(own)) {
-    const float weight = ex2(own.x - base);
-    l = fmaf(own.y, weight, l);
-    take(own_sums + row * DP, weight);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *out = static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1];
-  bool odd = false;
+    m = top;
+    l = l * alpha + warp_sum(counts(st) ? st.y * weight : 0.f);
 #pragma unroll
-  for (int y = 0; y < kCols; ++y) {
-    const float v = o[y] * inv;
-    if (lane * kCols + y < p.d) {
-      odd |= !isfinite(v);
-      out[lane * kCols + y] = Elem<T>::from_float(v);
+    for (int y = 0; y < kCols; ++y) o[y] *= alpha;
+    for (unsigned left = some; left;) {
+      float2 two[kAtOnce][kCols / 2];
+      float ws[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = left ? __ffs(left) - 1 : 0;
+        const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)from, i));
+        ws[u] = __shfl_sync(0xffffffffu, weight, i);
+#pragma unroll
+        for (int y = 0; y < kCols / 2; ++y)
+          two[u][y] = left ? __ldcg(reinterpret_cast<const float2 *>(src + lane * kCols + 2 * y)) : make_float2(0.f, 0.f);
+        left &= left - 1;
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+        for (int y = 0; y < kCols / 2; ++y) {
+          o[2 * y] = fmaf(two[u][y].x, ws[u], o[2 * y]);
+          o[2 * y + 1] = fmaf(two[u][y].y, ws[u], o[2 * y + 1]);
+        }
     }
   }
-  if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : lse_of<(int)kLift<T>>(m, l);
-  if (__any_sync(0xffffffffu, odd)) {  // what came out infinite or NaN again, key by key
+#pragma unroll
+  for (int y = 0; y < kCols; ++y) sums[warp][lane * kCols + y] = o[y];
+  if (lane == 0) warp_m[warp] = m, warp_l[warp] = l;
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f, weights[kMergeWarps];
+#pragma unroll
+  for (int x = 0; x < kMergeWarps; ++x) top = fmaxf(top, warp_m[x]);
+#pragma unroll
+  for (int x = 0; x < kMergeWarps; ++x) {
+    weights[x] = ex2(warp_m[x] - (top == -INFINITY ? 0.f : top));
+    sum = fmaf(warp_l[x], weights[x], sum);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T *out = static_cast<T *>(p.o) + slot * p.os[0] + h * p.os[1];
+  const int col = threadIdx.x;
+  bool odd = false;
+  if (col < p.d) {
+    float v = 0.f;
+#pragma unroll
+    for (int x = 0; x < kMergeWarps; ++x) v = fmaf(sums[x][col], weights[x], v);
+    v *= inv;
+    odd = !isfinite(v);
+    out[col] = Elem<T>::from_float(v);
+  }
+  if (p.lse && threadIdx.x == 0) p.lse[row] = sum == 0.f ? -INFINITY : lse_of<(int)kLift<T>>(top, sum);
+  if (__syncthreads_or(odd) && warp == 0) {  // what came out infinite or NaN again, key by key
     RowState<kCols> st;
     plain_part<T>(p, slot, h, h / (p.q_heads / p.kv_heads), st, 0, 1);
-    __syncwarp();
     mend_row(st, out, p.d, lane);
   }
 }
@@ -709,6 +744,7 @@ int launch_shared(int dtype, SharedParams &sp, cudaStream_t s) {
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   sp.ctas = std::min(sm_count(), kMostCtas);
+  sp.runs = p.dense && p.page_size % 16 == 0;
   const int64_t rows = (int64_t)p.slots * p.q_heads, parts = cut_rows(sp.ctas) + rows * kTiles;
   void *mem = nullptr;
   Suffix suffix = {sp.sharing, nullptr, nullptr};
@@ -725,14 +761,19 @@ int launch_shared(int dtype, SharedParams &sp, cudaStream_t s) {
   suffix.stats = static_cast<float2 *>(mem);
   if (int rc = check_cuda(launch_pdl(kernel, dim3(sp.ctas), dim3(kThreads), L::bytes(p.slots), s, sp), "lc_shared_decode")) return rc;
   if (int rc = decode_suffix(dtype, p, suffix, s)) return rc;
-  return check_cuda(launch_pdl(merge_kernel<T, DP>, dim3((unsigned)((rows + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), 0, s, sp,
+  return check_cuda(launch_pdl(merge_kernel<T, DP>, dim3((unsigned)rows), dim3(kMergeWarps * 32), 0, s, sp,
                                suffix.sums, suffix.stats),
                     "lc_shared_decode (merge)");
 }
 
 // Whether reading the prefixes once can pay, by what all slots' keys and values may come to.
 constexpr int64_t kWorthBytes = 32 << 20;
-bool worth_sharing(const DecodeParams &p) { return (int64_t)p.slots * p.width * p.page_size * p.kv_heads * p.d * 4 >= kWorthBytes; }
+// (Its units, of all segments together, are counted in 32 bits.)
+bool worth_sharing(const DecodeParams &p) {
+  const int64_t rows = (int64_t)p.slots * p.q_heads, blocks = (int64_t)p.width * p.page_size / kKeys + 3;
+  if ((rows / (kTiles * kRows) + (int64_t)p.slots * p.kv_heads) * blocks >= INT32_MAX) return false;
+  return (int64_t)p.slots * p.width * p.page_size * p.kv_heads * p.d * 4 >= kWorthBytes;
+}
 
 }  // namespace
 }  // namespace lc
