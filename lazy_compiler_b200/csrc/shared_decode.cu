@@ -45,8 +45,11 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostCtas = 256;
 constexpr int kMostSlots = 8192;
+constexpr int kLensHeld = 1024;  // slots whose lengths are kept in shared memory
 constexpr int kEndUnits = 1;  // what a segment's end costs, in blocks
 constexpr int kMinRun = 4;    // units of a run
+constexpr int kRing = 4;      // pieces of work known ahead
+constexpr int kReaders = 1 + 8 + 4;  // of a piece: the warps of products, softmax and copies
 constexpr int kFewRegs = 72, kManyRegs = 184;  // of 128 at launch, as in window_attention.cu
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;  // S of tile t at t * 128, P over it, O of tile t at kOCol + t * DP
@@ -63,7 +66,8 @@ struct SharedLayout {
   static constexpr int kTileBytes = DP / 64 * kChunkBytes;
   static constexpr int kQBytes = kTiles * kTileBytes;
   static constexpr int kBuffers = kQBytes + kStages * 2 * kTileBytes;
-  static int bytes(int slots) { return kBuffers + 1024 + (slots * 2 + 15) / 16 * 16; }
+  // the buffers, and of every slot its leader, its place in the order, and its length if there are few
+  static int bytes(int slots) { return kBuffers + 1024 + slots * 4 + (slots <= kLensHeld ? slots * 4 : 0); }
 };
 
 struct SharedParams {
@@ -91,7 +95,7 @@ struct Group {
   int at, count, slot, keys, n_sink, start, blocks;
 };
 // By a whole warp.
-__device__ __forceinline__ Group group_of(const SharedParams &sp, const uint16_t *leaders, int at) {
+__device__ __forceinline__ Group group_of(const SharedParams &sp, const uint16_t *leaders, const uint16_t *order, int at) {
   const DecodeParams &p = sp.p;
   const int lane = threadIdx.x & 31;
   Group g;
@@ -111,8 +115,8 @@ __device__ __forceinline__ Group group_of(const SharedParams &sp, const uint16_t
   if (p.window) {
     first = INT32_MAX;
     for (int i = lane; i < g.count; i += 32) {
-      const int slot = sp.sharing.order[at + i];
-      const int n = (unsigned)slot < (unsigned)p.slots ? cached_tokens(p, slot) : 0;
+      const int slot = order[at + i];
+      const int n = slot < p.slots ? cached_tokens(p, slot) : 0;
       if (n <= 0) continue;
       const Visible see = visible(n - 1, p.window, p.sinks);
       first = min(first, see.lo);
@@ -150,7 +154,7 @@ struct Pieces {
   Run run;
   __device__ __forceinline__ explicit Pieces(const Run &r) : run(r) {}
   // By a whole warp.
-  __device__ __forceinline__ bool next(const SharedParams &sp, const uint16_t *leaders, Piece &out) {
+  __device__ __forceinline__ bool next(const SharedParams &sp, const uint16_t *leaders, const uint16_t *order, Piece &out) {
     const DecodeParams &p = sp.p;
     const int lane = threadIdx.x & 31, group = p.q_heads / p.kv_heads;
     while (run.seg_begin < run.end && run.g.at < p.slots) {
@@ -182,7 +186,7 @@ struct Pieces {
           at += 32;
         }
         run.g.at = at;
-        if (at < p.slots && run.seg_begin < run.end) run.g = group_of(sp, leaders, at);
+        if (at < p.slots && run.seg_begin < run.end) run.g = group_of(sp, leaders, order, at);
       }
       if (some && out.j1 > out.j0) return true;
     }
@@ -201,11 +205,31 @@ __device__ __forceinline__ bool wait_all(uint64_t *bar, uint32_t parity, volatil
   return ok != 0;
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// The pieces as the planning warp leaves them, for the others to take one after the other.
+struct Ring {
+  Piece piece[kRing];
+  uint64_t full[kRing], empty[kRing];
+};
+// The k-th; false: there is none (or the wait for it was given up).
+__device__ __forceinline__ bool take(Ring &ring, int k, Piece &out, volatile int *abort, const SharedParams &sp, int code) {
+  if (!wait_all(&ring.full[k % kRing], k / kRing & 1, abort, sp, code)) return false;
+  out = ring.piece[k % kRing];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[k % kRing]);
+  return out.j1 > 0;
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+
+// What is read once leaves L2 first, so that code, maps, queries and parts stay there.
+__device__ __forceinline__ uint64_t first_to_leave() {
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::128B [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
 __device__ __forceinline__ void copies_done() {
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -217,10 +241,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   using L = SharedLayout<DP>;
   constexpr int kTile = L::kTileBytes;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
+  const DecodeParams &p = sp.p;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t *q_s = smem, *kv_s = smem + L::kQBytes;
-  uint16_t *leaders = reinterpret_cast<uint16_t *>(smem + L::kBuffers);
+  uint16_t *leaders = reinterpret_cast<uint16_t *>(smem + L::kBuffers), *order = leaders + p.slots;
+  int *lens = reinterpret_cast<int *>(order + p.slots);  // by place in the order
   __shared__ __align__(8) uint64_t q_full, q_empty;
   __shared__ __align__(8) uint64_t k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
   __shared__ __align__(8) uint64_t s_full[kTiles], p_full[kTiles], o_done[kTiles];
@@ -229,12 +255,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   __shared__ int abort_flag;
   __shared__ int warp_units[kWarps];
   __shared__ Run run_shared;
+  __shared__ __align__(16) Ring ring;
   volatile int *abort = &abort_flag;
-  const DecodeParams &p = sp.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.q_heads / p.kv_heads;
 
   if (tid == 0) {
+    for (int x = 0; x < kRing; ++x) {
+      mbar_init(&ring.full[x], 1);
+      mbar_init(&ring.empty[x], kReaders);
+    }
     mbar_init(&q_full, 8);
     mbar_init(&q_empty, 1);
     for (int s = 0; s < kStages; ++s) {
@@ -269,18 +299,23 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     if ((unsigned)slot < (unsigned)p.slots) {
       const int leader = sp.sharing.leader[slot], keys = prefix_tokens(p, sp.sharing, slot);
       if ((unsigned)leader < (unsigned)p.slots) mark = (uint16_t)(leader | (leader == slot && keys > 0 ? kBegins : 0));
+      if (p.slots <= kLensHeld) lens[i] = cached_tokens(p, slot);
     }
     leaders[i] = mark;
+    order[i] = (unsigned)slot < (unsigned)p.slots ? (uint16_t)slot : 0xffff;
   }
   if (tid == 0) run_shared = {};
   if (tid == 0) run_shared.g.at = p.slots;
   __syncthreads();
   int *units = reinterpret_cast<int *>(smem);  // of the group that begins at a position
+  Group *groups = reinterpret_cast<Group *>(smem + kMostSlots * sizeof(int));  // and that group, if there are few slots
+  const bool held = p.slots * (int)sizeof(Group) <= L::kBuffers - kMostSlots * (int)sizeof(int);
   for (int i = warp; i < p.slots; i += kWarps) {
     int n = 0;
     if (leaders[i] & kBegins) {
-      const Group g = group_of(sp, leaders, i);
+      const Group g = group_of(sp, leaders, order, i);
       if (g.blocks > 0) n = (g.blocks + kEndUnits) * row_parts(g.count, group) * p.kv_heads;
+      if (held && lane == 0) groups[i] = g;
     }
     if (lane == 0) units[i] = n;
   }
@@ -309,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           if (begin < before + units[i]) {
             run_shared.begin = begin, run_shared.end = end, run_shared.total = total;
             run_shared.seg_begin = before, run_shared.ctas = ctas, run_shared.g.at = i;
+            if (held) run_shared.g = groups[i];
             break;
           }
           before += units[i];
@@ -318,16 +354,29 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   }
   __syncthreads();
   // (the units have been read: the buffers are free)
-  Run run = run_shared;
-  if (run.ctas > 0) {
-    run.g = group_of(sp, leaders, run.g.at);
-    run.seg = (run.begin - run.seg_begin) / (run.g.blocks + kEndUnits);
-    run.seg_begin += run.seg * (run.g.blocks + kEndUnits);
-  }
-
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
-    if (warp == 1) {
+    if (warp == 0) {
+      Run run = run_shared;
+      if (run.ctas > 0) {
+        if (!held) run.g = group_of(sp, leaders, order, run.g.at);
+        run.seg = (run.begin - run.seg_begin) / (run.g.blocks + kEndUnits);
+        run.seg_begin += run.seg * (run.g.blocks + kEndUnits);
+      }
+      Pieces pieces(run);
+      Piece piece = {};
+      for (int k = 0;; ++k) {
+        const bool more = pieces.next(sp, leaders, order, piece);
+        if (!more) piece.j1 = 0;
+        if (k >= kRing && !wait_all(&ring.empty[k % kRing], (k / kRing - 1) & 1, abort, sp, kErrTimeoutProducer)) break;
+        if (lane == 0) {
+          ring.piece[k % kRing] = piece;
+          mbar_arrive(&ring.full[k % kRing]);
+        }
+        __syncwarp();
+        if (!more) break;
+      }
+    } else if (warp == 1) {
       const uint32_t leader = elect_one();
       constexpr uint32_t idesc_s = idesc_f16(kBf16, false, false, kRows, kKeys);
       constexpr uint32_t idesc_o = idesc_f16(kBf16, false, true, kRows, DP);
@@ -335,11 +384,10 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
       const uint64_t k_desc = smem_desc_sw128(smem_u32(kv_s), 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(smem_u32(kv_s) + kTile, kChunkBytes, 1024);
       constexpr uint32_t kStageStep = 2 * kTile / 16;
-      Pieces pieces(run);
       Piece piece;
       int g0 = 0, local = 0, done[kTiles] = {0, 0};  // blocks and pieces so far, steps of a tile
       bool ok = true;
-      while (ok && pieces.next(sp, leaders, piece)) {
+      while (ok && take(ring, local, piece, abort, sp, kErrTimeoutMma)) {
         // Step x is tile x & 1; of both tiles' rows one block (more than 128), else of the same rows the next.
         const bool wide = piece.rows > kRows;
         const int blocks = piece.j1 - piece.j0, steps = wide ? 2 * blocks : blocks;
@@ -393,33 +441,50 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     const int t = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_at = tmem + lane_base + t * kKeys, o_at = tmem + lane_base + kOCol + t * DP;
-    Pieces pieces(run);
     Piece piece;
     int g0 = 0, local = 0, step = 0;
     bool ok = true;
-    while (ok && pieces.next(sp, leaders, piece)) {
+    while (ok && take(ring, local, piece, abort, sp, kErrTimeoutSoftmax)) {
       const bool wide = piece.rows > kRows;
       const int blocks = piece.j1 - piece.j0, steps = wide ? blocks : (blocks + 1 - t) / 2;
       // this thread's row: a slot of the group and one of its query heads
       const int tile_row = wide ? t * kRows + row : row;
       const bool real = tile_row < piece.rows;
       const int in_group = real ? piece.row0 + tile_row : 0, member = in_group / group;
-      int slot = real ? sp.sharing.order[piece.g.at + member] : piece.g.slot;
-      if ((unsigned)slot >= (unsigned)p.slots) slot = piece.g.slot;
+      const int place = piece.g.at + (real ? member : 0), listed = order[place];
+      const bool sound = listed < p.slots;  // (a place in the order may say anything)
+      const int slot = sound ? listed : piece.g.slot;
       const int h = piece.head * group + in_group - member * group;
-      const int n = cached_tokens(p, slot), upto = real ? min(n, piece.g.keys) : INT32_MAX;
+      const int n = p.slots <= kLensHeld && sound ? lens[place] : cached_tokens(p, slot);
+      const int upto = real ? min(n, piece.g.keys) : INT32_MAX;
       const Visible see = visible(n - 1, p.window, p.sinks);
       const int lo = real ? see.lo : 0, sink_end = see.sink_end;
       if (local > 0 && !wait_all(&q_empty, (local - 1) & 1, abort, sp, kErrTimeoutSoftmax)) break;
-      if (wide || t == 0) {  // the row of Q, piece c of 16 bytes at c ^ (row & 7) of its 128
-        const T *q = static_cast<const T *>(p.q) + slot * p.qs[0] + h * p.qs[1];
-        uint8_t *to = q_s + (wide ? t * kTile : 0) + row * 128;
+      if (wide || t == 0) {
+        // The warp's rows of Q, 128 bytes a copy, piece c of 16 bytes at c ^ (row & 7): (a thread a row took 7 us)
+        const int64_t at = slot * p.qs[0] + h * p.qs[1];
+        const unsigned reals = __ballot_sync(0xffffffffu, real);
+        uint8_t *to = q_s + (wide ? t * kTile : 0) + quarter * 32 * 128;
+        // (every address is readable, so the loads need no condition, and are on their way together)
+        constexpr int kHalves = DP / 64, kAtOnce = 16;
+        const T *column[kHalves];
 #pragma unroll
-        for (int c = 0; c < DP / 8; ++c) {
-          uint32_t v[4];
+        for (int x = 0; x < kHalves; ++x) column[x] = static_cast<const T *>(p.q) + (x * 64 + lane * 2 < p.d ? x * 64 + lane * 2 : 0);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] = real && c * 8 < p.d ? *reinterpret_cast<const uint32_t *>(q + c * 8 + 2 * x) : 0u;
-          *reinterpret_cast<uint4 *>(to + (c >> 3) * kChunkBytes + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
+          uint32_t v[kAtOnce][kHalves];
+#pragma unroll
+          for (int r = 0; r < kAtOnce; ++r) {
+            const int64_t from = __shfl_sync(0xffffffffu, at, r0 + r);
+#pragma unroll
+            for (int x = 0; x < kHalves; ++x) v[r][x] = __ldg(reinterpret_cast<const uint32_t *>(column[x] + from));
+          }
+#pragma unroll
+          for (int r = 0; r < kAtOnce; ++r)
+#pragma unroll
+            for (int x = 0; x < kHalves; ++x)
+              *reinterpret_cast<uint32_t *>(to + x * kChunkBytes + (r0 + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
+                  (reals >> (r0 + r) & 1) && x * 64 + lane * 2 < p.d ? v[r][x] : 0u;
         }
         fence_async_shared();
         if (real && piece.j0 == 0)
@@ -559,12 +624,14 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     const int64_t *strides = values ? p.vs : p.ks;
     uint64_t *full = values ? &v_full[stage] : &k_full[stage], *empty = values ? &v_empty[stage] : &k_empty[stage];
     const uint32_t buffer = smem_u32(kv_s) + stage * 2 * kTile + (values ? kTile : 0) + (c >> 3) * kChunkBytes;
-    Pieces pieces(run);
     Piece piece;
     int g = 0;
     bool ok = true;
-    while (ok && pieces.next(sp, leaders, piece)) {
+    for (int local = 0; ok && take(ring, local, piece, abort, sp, kErrTimeoutProducer); ++local) {
+      // The first queries come first: behind the copies of all CTAs they took 10 us.
+      if (local == 0 && !wait_all(&q_full, 0, abort, sp, kErrTimeoutProducer)) break;
       const int *table = p.table + piece.g.slot * p.ts;
+      const uint64_t policy = (int64_t)piece.g.count * group > kTiles * kRows ? l2_policy_evict_normal() : first_to_leave();
       for (int j = piece.j0; j < piece.j1; ++j, ++g) {
         if ((g & 1) != stage) continue;
         const int key = block_key(piece.g, j);
@@ -596,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
             const T *from = base + __shfl_sync(0xffffffffu, off[x >> 1], (x & 1) * 16) + lane * 8;
 #pragma unroll
             for (int i = 0; i < 16; i += kRowsPerCopy)  // row i + row_in: bits apart, as piece ^ row wants it
-              copy16((to ^ ((i & 7) << 4)) + (x * 16 + i) * 128, from + i * DP);
+              copy16((to ^ ((i & 7) << 4)) + (x * 16 + i) * 128, from + i * DP, policy);
           }
         }
 #pragma unroll
@@ -607,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
             const int r = x * 32 + i + row_in;
             const int64_t o = __shfl_sync(0xffffffffu, off[x], i + row_in);
             const bool copied = o >= 0 && c_real;
-            copy16(buffer + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (copied ? o + c * 8 : 0), copied ? 16 : 0);
+            copy16(buffer + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (copied ? o + c * 8 : 0), copied ? 16 : 0, policy);
           }
         }
         copies_done();
