@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "softmax.cuh"
 
 namespace lc {
 namespace {
@@ -24,6 +25,18 @@ constexpr int kThreads = 256;
 constexpr int kMostTokens = 32;    // of a CTA
 constexpr int kMostRotations = 2048;  // of a CTA's tokens, in shared memory
 constexpr int kMostHead = 1024;
+
+// A division by a number known at the launch: (x * multiplier) >> shift, exact for x below 2^26 (the products stay
+// below 2^64, the multiplier's rounding below x's last part).
+struct Divisor {
+  unsigned multiplier, shift;
+};
+inline Divisor divisor_of(unsigned n) {
+  unsigned shift = 26;
+  while ((1u << (shift - 26)) < n) ++shift;  // 2^shift / n is below 2^26 + 1, and off by less than 2^(shift - 26) / n <= 1 in 2^26
+  return {(unsigned)(((1ull << shift) + n - 1) / n), shift};
+}
+__device__ __forceinline__ unsigned by(int x, const Divisor &d) { return (unsigned)((unsigned long long)(unsigned)x * d.multiplier >> d.shift); }
 
 struct RotaryParams {
   const int64_t *turns;  // rot / 2 of them, in 2^-64 of a turn
@@ -44,6 +57,7 @@ struct RotateParams {
   int64_t kp[2][3];       // page, head, token
   const int *table, *lens, *add, *refused;
   int width, page_count, page_size, zero_rest;
+  Divisor per_token, per_row;  // units of a token, of a head
   int tokens, tiles, tile, heads[2], rows, d, units, turned;  // tile: tokens of a CTA; rows: of a token
 };
 
@@ -88,9 +102,29 @@ __device__ __forceinline__ float2 rotation(int64_t turns, int64_t position, floa
   return make_float2(c * magnitude, s * magnitude);
 }
 
+// Pairs (f, g) turned, two by two in Blackwell's paired f32 form.
+template <int V>
+__device__ __forceinline__ void turn_pairs(float (&f)[V], float (&g)[V], const float *cosines, const float *sines) {
+  using namespace softmax;
+  if constexpr (V == 1) {
+    const float c = cosines[0], s = sines[0], u = f[0], v = g[0];
+    f[0] = u * c - v * s;
+    g[0] = u * s + v * c;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const uint64_t u = pack2(f[e], f[e + 1]), v = pack2(g[e], g[e + 1]);
+      const uint64_t c = *reinterpret_cast<const uint64_t *>(cosines + e), s = *reinterpret_cast<const uint64_t *>(sines + e);
+      const float2 x = unpack2(fsub2(ffma2(u, c, 0ull), ffma2(v, s, 0ull))), y = unpack2(ffma2(u, s, ffma2(v, c, 0ull)));
+      f[e] = x.x, f[e + 1] = x.y;
+      g[e] = y.x, g[e + 1] = y.y;
+    }
+  }
+}
+
 template <class T, int V, bool APPEND>
 __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant__ RotateParams p) {
-  __shared__ float2 turns[kMostRotations];
+  __shared__ __align__(16) float cosines[kMostRotations], sines[kMostRotations];
   __shared__ int64_t to[2][kMostTokens];  // where a token's key and value go, -1: nowhere
   pdl_wait();
   pdl_trigger();
@@ -116,16 +150,20 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   for (int i = tid; i < real * half; i += kThreads) {
     const int t = i / half, pair = i - t * half;
     const int64_t pos = APPEND ? start + first + t : p.positions[b * p.ps[0] + (first + t) * p.ps[1]];
-    turns[i] = rotation(p.rotary.turns[pair], pos, p.rotary.magnitude);
+    const float2 cs = rotation(p.rotary.turns[pair], pos, p.rotary.magnitude);
+    cosines[i] = cs.x;
+    sines[i] = cs.y;
   }
   __syncthreads();
 
   using P = Piece<T, V>;
   const int per_token = p.rows * p.units, inner = p.rotary.interleaved ? V : half;  // from a unit's first piece to its second
-#pragma unroll 2
+  // (Two or four units a thread with their loads together: 134 and 198 us for 4 x 8191 tokens of 40 heads, since fewer
+  // CTAs fit an SM then, against 120 one by one.)
+#pragma unroll 1
   for (int i = tid; i < count * per_token; i += kThreads) {
-    const int t = i / per_token, in_token = i - t * per_token;
-    const int row = in_token / p.units, unit = in_token - row * p.units;
+    const int t = (int)by(i, p.per_token), in_token = i - t * per_token;
+    const int row = (int)by(in_token, p.per_row), unit = in_token - row * p.units;
     // whose row: queries, keys, values
     const int which = !APPEND || row < p.heads[0] ? 0 : row < p.heads[0] + p.heads[1] ? 1 : 2;
     const int head = which == 0 ? row : which == 1 ? row - p.heads[0] : row - p.heads[0] - p.heads[1];
@@ -150,25 +188,27 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
       x = *reinterpret_cast<const P *>(src + a);
       if (c < p.d) y = *reinterpret_cast<const P *>(src + c);
       if (turn) {
-        const float2 *cs = turns + t * half + V * unit;
-        if (p.rotary.interleaved) {
-          T both[2 * V];
+        float f[V], g[V];  // the pairs
 #pragma unroll
-          for (int e = 0; e < V; ++e) both[e] = x.v[e], both[V + e] = y.v[e];
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float u = widen<T>(both[2 * e]), v = widen<T>(both[2 * e + 1]);
-            both[2 * e] = narrow<T>(u * cs[e].x - v * cs[e].y);
-            both[2 * e + 1] = narrow<T>(u * cs[e].y + v * cs[e].x);
+        for (int e = 0; e < V; ++e) {
+          if (p.rotary.interleaved) {
+            f[e] = widen<T>(2 * e < V ? x.v[2 * e % V] : y.v[2 * e % V]);
+            g[e] = widen<T>(2 * e < V ? x.v[(2 * e + 1) % V] : y.v[(2 * e + 1) % V]);
+          } else {
+            f[e] = widen<T>(x.v[e]);
+            g[e] = widen<T>(y.v[e]);
           }
+        }
+        if (V == 1 && p.rotary.interleaved) f[0] = widen<T>(x.v[0]), g[0] = widen<T>(y.v[0]);
+        turn_pairs<V>(f, g, cosines + t * half + V * unit, sines + t * half + V * unit);
 #pragma unroll
-          for (int e = 0; e < V; ++e) x.v[e] = both[e], y.v[e] = both[V + e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float u = widen<T>(x.v[e]), v = widen<T>(y.v[e]);
-            x.v[e] = narrow<T>(u * cs[e].x - v * cs[e].y);
-            y.v[e] = narrow<T>(u * cs[e].y + v * cs[e].x);
+        for (int e = 0; e < V; ++e) {
+          if (p.rotary.interleaved && V > 1) {
+            (2 * e < V ? x : y).v[2 * e % V] = narrow<T>(f[e]);
+            (2 * e < V ? x : y).v[(2 * e + 1) % V] = narrow<T>(g[e]);
+          } else {
+            x.v[e] = narrow<T>(f[e]);
+            y.v[e] = narrow<T>(g[e]);
           }
         }
       }
@@ -210,9 +250,10 @@ int launch_rotate(const char *me, int dtype, RotateParams &p, int64_t batch, con
     if (x * size >= 8 && fits(x)) v = x;
   p.turned = rot / (2 * v);
   p.units = p.turned + (p.d - rot + 2 * v - 1) / (2 * v);
-  // Tokens of a CTA: four units a thread, but no fewer than two CTAs an SM for the sake of it.
+  p.per_token = divisor_of((unsigned)p.rows * p.units), p.per_row = divisor_of(p.units);
+  // Tokens of a CTA: eight units a thread (four: 124 us, 16: 120), but no fewer than two CTAs an SM for the sake of it.
   const int64_t all = batch * p.tokens, per_token = (int64_t)p.rows * p.units;
-  int64_t tile = std::min<int64_t>((4 * kThreads + per_token - 1) / per_token, kMostTokens);
+  int64_t tile = std::min<int64_t>(8 * kThreads / per_token, kMostTokens);
   tile = std::min<int64_t>(tile, kMostRotations / std::max(1, rot / 2));
   tile = std::max<int64_t>(1, std::min<int64_t>(tile, std::min<int64_t>(p.tokens, all / (2 * sm_count()))));
   p.tile = (int)tile;

@@ -80,6 +80,7 @@ struct SharedParams {
   int4 *where;  // of every row of a prefix: first and last CTA, row of its tiles, how (kSplitKeys, kWhole)
   int *err;
   int ctas;
+  int q_pieces;  // the queries are aligned to 16 bytes
   int runs;  // 16 tokens of a head, from a multiple of 16 on, are one run of memory in k and in v
 };
 constexpr int kSplitKeys = 1, kWhole = 2;
@@ -101,7 +102,9 @@ __device__ __forceinline__ Group group_of(const SharedParams &sp, const uint16_t
   Group g;
   g.at = at;
   g.slot = leaders[at] & ~kBegins;
-  int lo = at + 1, hi = p.slots;
+  // the group's end: among the next 32 places, or by bisection behind them
+  const unsigned others = __ballot_sync(0xffffffffu, at + 1 + lane >= p.slots || leaders[at + 1 + lane] != (uint16_t)g.slot);
+  int lo = at + 1 + (others ? __ffs(others) - 1 : 32), hi = others ? lo : p.slots;
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     if (leaders[mid] == (uint16_t)g.slot)
@@ -138,10 +141,9 @@ struct Piece {
   int head, row0, rows, j0, j1;
   int first, last;  // the CTAs that the segment's blocks are in
 };
-// a * b / c for units and CTAs: 32 bits where the product has no more, which is a fifth of the instructions.
+// a * b / c for units and CTAs; units times CTAs are below 2^32 (worth_sharing).
 __device__ __forceinline__ int share_of(int a, int b, int c, bool below = false) {  // below: of one less
-  const unsigned long long product = (unsigned long long)(unsigned)a * (unsigned)b - below;
-  return (int)((product >> 32) == 0 ? (unsigned)product / (unsigned)c : product / (unsigned)c);
+  return (int)(((unsigned)a * (unsigned)b - below) / (unsigned)c);
 }
 // A CTA's run, in units, and the segment that a reader of it is at.
 struct Run {
@@ -461,35 +463,47 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
       const int lo = real ? see.lo : 0, sink_end = see.sink_end;
       if (local > 0 && !wait_all(&q_empty, (local - 1) & 1, abort, sp, kErrTimeoutSoftmax)) break;
       if (wide || t == 0) {
-        // The warp's rows of Q, 128 bytes a copy, piece c of 16 bytes at c ^ (row & 7): (a thread a row took 7 us)
+        // The warp's rows of Q, piece c of 16 bytes at c ^ (row & 7).  A thread a row took 7 us; every address is
+        // readable, so the loads need no condition, and are on their way together.
         const int64_t at = slot * p.qs[0] + h * p.qs[1];
         const unsigned reals = __ballot_sync(0xffffffffu, real);
         uint8_t *to = q_s + (wide ? t * kTile : 0) + quarter * 32 * 128;
-        // (every address is readable, so the loads need no condition, and are on their way together)
-        constexpr int kHalves = DP / 64, kAtOnce = 16;
-        const T *column[kHalves];
+        if (sp.q_pieces) {
+          constexpr int kPieces = DP / 8, kLoads = kPieces;  // 16 bytes a lane: 32 / kPieces rows a load
+          const int c = lane % kPieces, row_in = lane / kPieces;
+          const T *from = static_cast<const T *>(p.q) + (c * 8 < p.d ? c * 8 : 0);
+          uint4 v[kLoads];
 #pragma unroll
-        for (int x = 0; x < kHalves; ++x) column[x] = static_cast<const T *>(p.q) + (x * 64 + lane * 2 < p.d ? x * 64 + lane * 2 : 0);
+          for (int i = 0; i < kLoads; ++i) v[i] = __ldg(reinterpret_cast<const uint4 *>(from + __shfl_sync(0xffffffffu, at, i * (32 / kPieces) + row_in)));
 #pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
-          uint32_t v[kAtOnce][kHalves];
-#pragma unroll
-          for (int r = 0; r < kAtOnce; ++r) {
-            const int64_t from = __shfl_sync(0xffffffffu, at, r0 + r);
-#pragma unroll
-            for (int x = 0; x < kHalves; ++x) v[r][x] = __ldg(reinterpret_cast<const uint32_t *>(column[x] + from));
+          for (int i = 0; i < kLoads; ++i) {
+            const int r = i * (32 / kPieces) + row_in;
+            *reinterpret_cast<uint4 *>(to + (c >> 3) * kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                (reals >> r & 1) && c * 8 < p.d ? v[i] : make_uint4(0, 0, 0, 0);
           }
+        } else {
+          constexpr int kHalves = DP / 64, kAtOnce = 8;
+          const T *column[kHalves];
 #pragma unroll
-          for (int r = 0; r < kAtOnce; ++r)
+          for (int x = 0; x < kHalves; ++x) column[x] = static_cast<const T *>(p.q) + (x * 64 + lane * 2 < p.d ? x * 64 + lane * 2 : 0);
+#pragma unroll 1
+          for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
+            uint32_t v[kAtOnce][kHalves];
 #pragma unroll
-            for (int x = 0; x < kHalves; ++x)
-              *reinterpret_cast<uint32_t *>(to + x * kChunkBytes + (r0 + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
-                  (reals >> (r0 + r) & 1) && x * 64 + lane * 2 < p.d ? v[r][x] : 0u;
+            for (int r = 0; r < kAtOnce; ++r) {
+              const int64_t from = __shfl_sync(0xffffffffu, at, r0 + r);
+#pragma unroll
+              for (int x = 0; x < kHalves; ++x) v[r][x] = __ldg(reinterpret_cast<const uint32_t *>(column[x] + from));
+            }
+#pragma unroll
+            for (int r = 0; r < kAtOnce; ++r)
+#pragma unroll
+              for (int x = 0; x < kHalves; ++x)
+                *reinterpret_cast<uint32_t *>(to + x * kChunkBytes + (r0 + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
+                    (reals >> (r0 + r) & 1) && x * 64 + lane * 2 < p.d ? v[r][x] : 0u;
+          }
         }
         fence_async_shared();
-        if (real && piece.j0 == 0)
-          sp.where[(int64_t)slot * p.q_heads + h] =
-              make_int4(piece.first, piece.last, tile_row, (wide ? 0 : kSplitKeys) | (piece.first == piece.last ? kWhole : 0));
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
@@ -594,6 +608,9 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
       const bool whole_segment = piece.first == piece.last;
       const int64_t at = whole_segment ? cut_rows(sp.ctas) + ((int64_t)slot * p.q_heads + h) * kTiles + (wide ? 0 : t)
                                        : (((int64_t)blockIdx.x * 2 + (piece.j0 == 0)) * kTiles + t) * kRows + row;
+      // (`where` not before: an arrival on a barrier waits for the stores ahead of it, 6 us at the first)
+      if (real && piece.j0 == 0 && (wide || t == 0))
+        sp.where[(int64_t)slot * p.q_heads + h] = make_int4(piece.first, piece.last, tile_row, (wide ? 0 : kSplitKeys) | (whole_segment ? kWhole : 0));
       if (real) sp.stats[at] = make_float2(m, l);
       if (steps > 0) {
         if (!wait_all(&o_done[t], (step - 1) & 1, abort, sp, kErrTimeoutEpilogue)) break;
@@ -812,6 +829,7 @@ int launch_shared(int dtype, SharedParams &sp, cudaStream_t s) {
   }
   sp.ctas = std::min(sm_count(), kMostCtas);
   sp.runs = p.dense && p.page_size % 16 == 0;
+  sp.q_pieces = aligned(p.q, 16) && p.qs[0] % 8 == 0 && p.qs[1] % 8 == 0;
   const int64_t rows = (int64_t)p.slots * p.q_heads, parts = cut_rows(sp.ctas) + rows * kTiles;
   void *mem = nullptr;
   Suffix suffix = {sp.sharing, nullptr, nullptr};
@@ -833,12 +851,14 @@ int launch_shared(int dtype, SharedParams &sp, cudaStream_t s) {
                     "lc_shared_decode (merge)");
 }
 
-// Whether reading the prefixes once can pay, by what all slots' keys and values may come to.
-constexpr int64_t kWorthBytes = 32 << 20;
-// (Its units, of all segments together, are counted in 32 bits.)
+// Whether reading the prefixes once can pay, by what all slots' keys and values may come to: below, lc_paged_decode,
+// which finds what another slot has read in L2, is done before three kernels are (64 samples of 300 tokens, 8 heads of
+// 128, 100 MB: 25 us against 37; 8 prompts of 8 samples, 2.1 GB: 174 against 75; 4 of 16, heads of 64, 1 GB: 110, 42).
+constexpr int64_t kWorthBytes = 192 << 20;
+// (The units of all segments together, times the CTAs, are counted in 32 bits.)
 bool worth_sharing(const DecodeParams &p) {
   const int64_t rows = (int64_t)p.slots * p.q_heads, blocks = (int64_t)p.width * p.page_size / kKeys + 3;
-  if ((rows / (kTiles * kRows) + (int64_t)p.slots * p.kv_heads) * blocks >= INT32_MAX) return false;
+  if ((rows / (kTiles * kRows) + (int64_t)p.slots * p.kv_heads) * blocks >= INT32_MAX / kMostCtas) return false;
   return (int64_t)p.slots * p.width * p.page_size * p.kv_heads * p.d * 4 >= kWorthBytes;
 }
 
