@@ -1,11 +1,12 @@
 """Answers a few prompts with a small random-weight transformer, on the library's serving operators.
 
-    python examples/serve.py [--layers 2 --steps 64 --samples 3 --window 128 --sinks 4]
+    python examples/serve.py [--layers 2 --steps 64 --samples 3 --window 128 --sinks 4 --temperature 0.8 --top-p 0.95]
 
-The prompts, of different lengths, run through windowed prompt attention while their keys and values enter a paged
-cache; every prompt is forked into samples that share its pages; each step of all samples is one replayed CUDA graph
-(projections with ``lc_gemm``, norms with ``lc_rmsnorm_f32``, pages taken, keys and values written, paged attention of
-the one new token, pages behind the window given back); at the end some requests leave and the cache is compacted.
+The prompts, of different lengths, turned to their positions, run through windowed prompt attention while their keys and
+values enter a paged cache; every prompt is forked into samples that share its pages; each step of all samples is one
+replayed CUDA graph (projections with ``lc_gemm``, norms with ``lc_rmsnorm_f32``, pages taken, keys turned and written
+with their values, attention of the one new token with the samples' common prefixes, pages behind the window given back,
+the next token drawn); at the end some requests leave and the cache is compacted.
 The last step's logits are then compared with those of the whole sequences run as prompts again.
 """
 from __future__ import annotations
@@ -72,6 +73,8 @@ def main(argv=None) -> float:
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
     for name, default in (("layers", 2), ("steps", 64), ("samples", 3), ("window", 128), ("sinks", 4)):
         ap.add_argument(f"--{name}", type=int, default=default)
+    for name, default in (("temperature", 0.8), ("top-p", 0.95)):
+        ap.add_argument(f"--{name}", type=float, default=default)
     a = ap.parse_args(argv)
     if a.layers < 1 or a.samples < 1 or a.steps < 1:
         ap.error("--layers, --samples and --steps are at least 1")
@@ -85,11 +88,19 @@ def main(argv=None) -> float:
     tokens = torch.zeros((slots, most + a.steps + 1), dtype=torch.long, device="cuda")
     tokens[:len(lengths), :most] = torch.randint(0, model.vocab, (len(lengths), most), generator=g, device="cuda")
 
+    rotary = S.Rotary(model.dim)
+    uniform = torch.rand((slots, most + a.steps + 1), generator=g, device="cuda")
+    positions = torch.arange(most + a.steps + 1, dtype=torch.int32, device="cuda").expand(slots, -1)
+
     # the prompts, padded to one batch; slots without a prompt have length 0
     lens = ints(lengths + [0] * (slots - len(lengths)))
     cache.extend(lens)
 
+    def turned(x):
+        return S.rotate(x, positions[:, :x.shape[1]], rotary)
+
     def prompt_attention(layer, q, k, v):
+        q, k = turned(q), turned(k)
         cache.write(layer, k, v, lens)
         return S.window_attention(q, k, v, window=a.window, sinks=a.sinks, q_lens=lens, kv_lens=lens)
 
@@ -99,23 +110,27 @@ def main(argv=None) -> float:
     parent = torch.arange(slots, device="cuda") % len(lengths)
     tokens, at = tokens[parent], lens[parent].long()
     first = logits[parent].gather(1, (at - 1).view(-1, 1, 1).expand(-1, 1, model.vocab)).squeeze(1)
-    # each sample begins with another of the likeliest tokens, and goes on greedily
+    # each sample begins with another of the likeliest tokens
     rank = torch.arange(slots, device="cuda") // len(lengths)
     now = first.topk(a.samples).indices.gather(1, rank.view(-1, 1)).squeeze(1)
     one = ints([1] * slots)
     step_logits = torch.empty((slots, model.vocab), dtype=torch.float16, device="cuda")
+    prefixes = cache.prefixes()
 
     def token_attention(layer, q, k, v):
-        cache.write(layer, k[:, None], v[:, None], one)
-        return cache.decode(layer, q, window=a.window, sinks=a.sinks)
+        q = cache.append(layer, q[:, None], k[:, None], v[:, None], one, rotary)[:, 0]
+        return cache.shared_decode(layer, q, prefixes, window=a.window, sinks=a.sinks)
 
     def step():
         tokens.scatter_(1, at.view(-1, 1), now.view(-1, 1))
         cache.extend(one)
+        if a.window:
+            cache.prefixes(into=prefixes)  # trimming takes pages from them
         step_logits.copy_(model.run(now, token_attention))
         if a.window:
             cache.trim(a.window, a.sinks)
-        now.copy_(step_logits.argmax(-1))
+        u = uniform.gather(1, at.view(-1, 1)).view(-1)
+        now.copy_(S.sample(step_logits, u, temperature=a.temperature, top_p=a.top_p))
         at.add_(1)
 
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
@@ -139,7 +154,7 @@ def main(argv=None) -> float:
     # the same sequences as prompts
     whole = at.int()
     full = model.run(tokens[:, :int(at.max())], lambda layer, q, k, v: S.window_attention(
-        q, k, v, window=a.window, sinks=a.sinks, q_lens=whole, kv_lens=whole))
+        turned(q), turned(k), v, window=a.window, sinks=a.sinks, q_lens=whole, kv_lens=whole))
     ref = full.gather(1, (at - 1).view(-1, 1, 1).expand(-1, 1, model.vocab)).squeeze(1).float()
     off = float((step_logits.float() - ref).norm() / ref.norm())
     print(f"last logits against the whole sequences run as prompts: {off:.1e} relative")

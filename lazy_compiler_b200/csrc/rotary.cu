@@ -12,7 +12,9 @@
 //
 // Bound by HBM, each element read and written once.  An angle belongs to all heads of a
 // token, so a CTA works out the rotations of its tokens once, in shared memory, and a
-// thread then takes units of V pairs (16 bytes of each half) of any head.
+// thread then takes units of V pairs (16 bytes of each half) of any head.  Measured, bf16,
+// 40 heads of 128: 4 x 8191 tokens in 108 us, 6.2 TB/s; f32: 203 us, 6.6 TB/s; into the cache,
+// f16, 32/8 heads, 16 prompts of 1023 to 4095 tokens: 206 us, 5.9 TB/s; 64 x 1 token: 3.1 and 4.2 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -82,6 +84,16 @@ template <class T, int V>
 struct alignas(sizeof(T) * V) Piece {
   T v[V];
 };
+
+// Whole pieces by streaming stores: what is written here leaves L2 before what is read (4 x 8191 tokens of 40 heads:
+// 114 -> 108 us).
+template <class T, int V>
+__device__ __forceinline__ void put(T *to, const Piece<T, V> &x) {
+  if constexpr (sizeof(x) == 16)
+    st_stream_u4(to, *reinterpret_cast<const uint4 *>(&x));
+  else
+    *reinterpret_cast<Piece<T, V> *>(to) = x;
+}
 
 // (cos, sin) of position * frequency, times the magnitude.
 __device__ __forceinline__ float2 rotation(int64_t turns, int64_t position, float magnitude) {
@@ -159,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   using P = Piece<T, V>;
   const int per_token = p.rows * p.units, inner = p.rotary.interleaved ? V : half;  // from a unit's first piece to its second
   // (Two or four units a thread with their loads together: 134 and 198 us for 4 x 8191 tokens of 40 heads, since fewer
-  // CTAs fit an SM then, against 120 one by one.)
+  // CTAs fit an SM then, against 120 one by one, all before the streaming stores.)
 #pragma unroll 1
   for (int i = tid; i < count * per_token; i += kThreads) {
     const int t = (int)by(i, p.per_token), in_token = i - t * per_token;
@@ -213,8 +225,8 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
         }
       }
     }
-    *reinterpret_cast<P *>(dst + a) = x;
-    if (c < p.d) *reinterpret_cast<P *>(dst + c) = y;
+    put(dst + a, x);
+    if (c < p.d) put(dst + c, y);
   }
 }
 
