@@ -155,16 +155,23 @@ class Rotary:
         if not 0 < self.magnitude < 3e38:
             raise ValueError("magnitude: must be positive and finite")
         # whole turns change nothing; the fraction to 64 bits, half a turn and more as its negative
-        turns = [round(Fraction(x) / _TURN * 2 ** 64) % 2 ** 64 for x in f.tolist()]
+        turns = [_turns(x) % 2 ** 64 for x in f.tolist()]
         self.turns = torch.tensor([t - 2 ** 64 if t >> 63 else t for t in turns], dtype=torch.int64).to(device)
 
 
-# a turn in radians, to 100 bits or so: pi by Machin's formula
+# a turn in radians, to 130 bits or so: pi by Machin's formula
 def _arctan_inverse(n: int) -> Fraction:
     return sum(Fraction((-1) ** k, (2 * k + 1) * n ** (2 * k + 1)) for k in range(30))
 
 
 _TURN = 8 * (4 * _arctan_inverse(5) - _arctan_inverse(239))
+_TURNS = round(2 ** 192 / _TURN)  # of a radian, in units of 2^-192
+
+
+def _turns(radians: float) -> int:
+    """Of an angle, in units of 2^-64."""
+    top, bottom = radians.as_integer_ratio()  # bottom is a power of two
+    return (2 * top * _TURNS // (bottom << 128) + 1) // 2
 
 
 def rotate(x, positions, rotary: Rotary, *, out=None, stream: int | None = None):

@@ -146,6 +146,34 @@ def test_rows_off_their_alignment(dtype, shift, stride):
     check(view, uniforms(rows, 13), t, k, p, m)
 
 
+def test_a_vocabulary_of_a_million():
+    t, k, p, m = (list(x) for x in zip(*ASKS))
+    check(peaked(len(t), 1000003, 18, "bf16"), uniforms(len(t), 19), t, k, p, m)
+
+
+def test_refusals():
+    x, u = torch.zeros(3, 10, device="cuda"), torch.zeros(3, device="cuda")
+    for name, wrong in (("temperature", u[:2]), ("temperature", u.double()), ("top_k", u), ("top_p", u.half()), ("min_p", u.cpu()),
+                        ("top_p", torch.zeros(6, device="cuda")[::2]), ("out", torch.zeros(3, dtype=torch.int64, device="cuda"))):
+        with pytest.raises(ValueError, match=name):
+            S.sample(x, u, **{name: wrong})
+    for call in (lambda: S.sample(x, u[:2]), lambda: S.sample(x[0], u), lambda: S.sample(x.T, u[:1].expand(10)), lambda: S.sample(x.double(), u)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        S.sample(x, u, top_k=1.5)
+
+
+def test_streams_at_once():
+    x, u = peaked(40, 30011, 20, "bf16"), torch.tensor(uniforms(40, 21), device="cuda")
+    want = S.sample(x, u, top_p=0.95)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = [S.sample(x, u, top_p=0.95, stream=s.cuda_stream) for s in streams * 5]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+
+
 def test_a_row_depends_on_itself_alone():
     """The same rows alone, in a batch of others and in another order: other splits of the rows over CTAs."""
     rows, vocab = 300, 20011

@@ -102,6 +102,24 @@ def test_scaled(scaling):
     check(S.rotate(x, positions, rotary), *rotated(x, positions, rotary), "f32")
 
 
+def test_refusals():
+    x, positions, rotary = torch.zeros(2, 3, 4, 16, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda"), S.Rotary(16)
+    for call in (lambda: S.rotate(x, positions.long(), rotary), lambda: S.rotate(x, positions[:, :2], rotary), lambda: S.rotate(x, positions, S.Rotary(18)),
+                 lambda: S.rotate(x, positions, S.Rotary(16, device="cpu")), lambda: S.rotate(x[0], positions, rotary),
+                 lambda: S.rotate(x.transpose(2, 3), positions, S.Rotary(4)), lambda: S.rotate(x, positions, rotary, out=x.half()),
+                 lambda: S.rotate(x, positions, rotary, out=x[:, :1].expand(-1, 3, -1, -1))):
+        with pytest.raises(ValueError):
+            call()
+    maps = S.CacheMaps(ints([[0], [1]]), ints([1, 1]), ints([1, 1]))
+    pages, add = torch.zeros(2, 4, 16, 16, device="cuda"), ints([1, 1])
+    k = x[:, :1].contiguous()
+    for call in (lambda: S.cache_append(k.half(), k, k, pages, pages, maps, add, rotary), lambda: S.cache_append(None, k, k, pages, pages, maps, add, rotary, out=k),
+                 lambda: S.cache_append(None, k, k[..., :8], pages, pages, maps, add, rotary), lambda: S.cache_append(None, k, k, pages, pages[:1].expand(2, -1, -1, -1), maps, add, rotary),
+                 lambda: S.cache_append(None, k, k, pages, pages, maps, add.long(), rotary)):
+        with pytest.raises(ValueError):
+            call()
+
+
 # ---------------------------------------------------------------- into the cache
 
 def ints(v):

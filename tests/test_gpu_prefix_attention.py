@@ -206,8 +206,9 @@ def test_repeats_bit_for_bit():
         assert torch.equal(first, S.shared_decode(q, k, v, maps.table, maps.lens, prefixes))
 
 
-def test_most_slots():
-    slots, d = 8192, 64
+@pytest.mark.parametrize("d", [64, 128])
+def test_most_slots(d):
+    slots = 8192
     table = torch.zeros((slots, 17), dtype=torch.int32)
     table[:, :9] = torch.arange(9)
     table[:, 9] = 9 + torch.arange(slots)
@@ -241,6 +242,35 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     runtime.call("lc_device_status", None)
+
+
+def test_two_streams_at_once():
+    """Calls that run beside each other keep to workspaces of their own."""
+    k, v, maps, prefixes = cache([(2000, [5, 30, 77] * 6), (700, [1, 1])], 16, 2, 64, "f16")
+    q = [queries(20, 8, 64, "f16", seed) for seed in range(4)]
+    want = [S.shared_decode(x, k, v, maps.table, maps.lens, prefixes) for x in q]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [S.shared_decode(x, k, v, maps.table, maps.lens, prefixes, stream=s.cuda_stream) for x, s in zip(q, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_refusals():
+    k, v, maps, prefixes = cache([(300, [5, 30])], 16, 2, 64, "f16")
+    q = queries(2, 8, 64, "f16")
+    call = lambda q=q, p=prefixes, **o: S.shared_decode(q, k, v, maps.table, maps.lens, p, **o)  # noqa: E731
+    for wrong in (prefixes._replace(leader=prefixes.leader.long()), prefixes._replace(shared=prefixes.shared[:1]),
+                  prefixes._replace(order=prefixes.order.cpu()), prefixes._replace(order=ints([0, 0, 1, 1])[::2])):
+        with pytest.raises(ValueError, match="prefixes"):
+            call(p=wrong)
+    with pytest.raises(ValueError, match="out"):
+        call(out=torch.zeros(2, 8, 63, dtype=torch.float16, device="cuda"))
+    with pytest.raises(ValueError, match="expanded"):
+        call(out=torch.zeros(2, 1, 64, dtype=torch.float16, device="cuda").expand(2, 8, 64))
+    with pytest.raises(runtime.LcError, match="scale"):
+        call(scale=0.0)
 
 
 def test_a_loop_of_samples():

@@ -34,7 +34,16 @@ def sample(dtype=0, logits=P, uniform=P, token=P, rows=2, vocab=10):
     runtime.call("lc_sample", dtype, logits, uniform, NULL, NULL, NULL, NULL, 1.0, 0, 1.0, 0.0, token, NULL, rows, vocab, 16, NULL)
 
 
+def shared(dtype=1, q=P, o=P, table=P, lens=P, leader=P, prefix=P, order=P, slots=1, width=2, pages=4, page=16, hq=2, h=1, d=64, st=None, win=0,
+           sinks=0, scale=1.0):
+    runtime.call("lc_shared_decode", dtype, q, P, P, o, NULL, table, lens, leader, prefix, order, slots, width, pages, page, hq, h, d,
+                 strides(11) if st is None else st, win, sinks, scale, NULL)
+
+
 INVALID = [
+    lambda: shared(dtype=0), lambda: shared(q=NULL), lambda: shared(o=NULL), lambda: shared(table=NULL), lambda: shared(lens=NULL),
+    lambda: shared(leader=NULL), lambda: shared(prefix=NULL), lambda: shared(order=NULL), lambda: shared(slots=-1), lambda: shared(page=0),
+    lambda: shared(hq=3, h=2), lambda: shared(st=NULL), lambda: shared(win=-1), lambda: shared(sinks=-1), lambda: shared(scale=math.nan),
     lambda: rotate(dtype=3), lambda: rotate(d=0), lambda: rotate(rot=3), lambda: rotate(rot=66), lambda: rotate(rot=-2), lambda: rotate(turns=NULL),
     lambda: rotate(magnitude=0.0), lambda: rotate(magnitude=math.nan), lambda: rotate(magnitude=math.inf), lambda: rotate(batch=-1),
     lambda: rotate(tokens=-1), lambda: rotate(heads=-1), lambda: rotate(st=NULL), lambda: rotate(x=NULL), lambda: rotate(out=NULL),
@@ -61,7 +70,7 @@ UNSUPPORTED = [
     lambda: rotate(d=1026, rot=2), lambda: rotate(heads=1 << 20), lambda: rotate(batch=1 << 31), lambda: rotate(tokens=1 << 30),
     lambda: append(slots=1 << 21), lambda: append(most=1 << 31), lambda: append(width=1 << 25), lambda: append(hq=1 << 20),
     lambda: append(page=1 << 21), lambda: prefixes(slots=8193), lambda: prefixes(width=1 << 30), lambda: sample(rows=1 << 25),
-    lambda: sample(vocab=(1 << 24) + 1),
+    lambda: sample(vocab=(1 << 24) + 1), lambda: shared(slots=8193), lambda: shared(d=257), lambda: shared(width=1 << 30),
 ]
 
 
@@ -88,6 +97,7 @@ def test_nothing_to_do_is_no_error():
     append(most=0, k=NULL)
     prefixes(slots=0, lens=NULL)
     sample(rows=0, logits=NULL)
+    shared(slots=0, q=NULL)
 
 
 def test_rotary():
@@ -137,6 +147,9 @@ def test_tensors_off_the_device_or_of_another_type():
         S.sample(x[0, 0], torch.zeros(3))
     with pytest.raises(ValueError, match="int32 is not"):
         S.sample(positions, torch.zeros(1))
+    q, ints = x[0].half(), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA devices only"):
+        S.shared_decode(q, pages.half(), pages.half(), maps.table, maps.lens, S.CachePrefixes(ints, ints, ints))
     with pytest.raises(ValueError, match="expected 9 arguments, got 1"):
         _serving.sample(1)
 
