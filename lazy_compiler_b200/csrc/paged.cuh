@@ -84,8 +84,8 @@ __device__ __forceinline__ void plain_row(const DecodeParams &p, int slot, int h
 }  // namespace attend
 
 // Attention over the tokens behind every slot's prefix, unnormalised: sums[slots * q_heads][padded head size]
-// and (reference, sum of weights) of every row.  `sharing` null: lc_paged_decode.  The caller has checked the
-// arguments and that decode_tensor() holds.
+// and (reference, sum of weights) of every row.  The caller has checked the arguments and that
+// decode_tensor() holds.
 struct Suffix {
   attend::Sharing sharing;
   float *sums;

@@ -21,6 +21,15 @@
 // Pages come by cp.async, 16 bytes a lane, so any page size, stride and page that is not
 // there (zero-filled, masked) is alike; four warps of copies: keys and values of even and
 // of odd blocks, each the only writer of its buffer.
+//
+// P is rounded to the storage type before the second product, as in window_attention.cu (1.35 times the
+// error of an output rounded once); all else is f32.
+//
+// Measured, 32/8 heads of 128, with the suffixes and the join: 8 prompts of 8000 tokens with 8 samples of
+// 600 more 77 us where the bytes take 42 (the prefixes by themselves 52 us: 20 blocks a CTA, then ends and
+// beginnings of segments, two or three a CTA); 64 questions to 100003 tokens 137 us in a graph, bytes 70, products
+// 64 (two tiles' block takes 3660 cycles, 2080 of them products: as in window_attention.cu a tile's scores, softmax
+// and products are a chain).
 #include <algorithm>
 #include <type_traits>
 
@@ -46,8 +55,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMostCtas = 256;
 constexpr int kMostSlots = 8192;
 constexpr int kLensHeld = 1024;  // slots whose lengths are kept in shared memory
-constexpr int kEndUnits = 1;  // what a segment's end costs, in blocks
-constexpr int kMinRun = 4;    // units of a run
+constexpr int kEndUnits = 1;  // what a segment's end costs, in blocks: its sums' way to memory
+constexpr int kMinRun = 4;    // units of a run: a run's beginning and its parts' join cost about as many
 constexpr int kRing = 4;      // pieces of work known ahead
 constexpr int kReaders = 1 + 8 + 4;  // of a piece: the warps of products, softmax and copies
 constexpr int kFewRegs = 72, kManyRegs = 184;  // of 128 at launch, as in window_attention.cu

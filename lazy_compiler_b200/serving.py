@@ -1,4 +1,5 @@
-"""Serving operators: attention of prompts and of single new tokens, and the paged key-value cache between them.
+"""Serving operators: attention of prompts and of single new tokens, the paged key-value cache between them, and what a
+step has around them: positions as rotations, and the drawing of the next token.
 
 The functions take torch tensors on one CUDA device and launch the library's kernels (``include/lazyb200.h``,
 "serving") on the tensors' device, on its current stream or on ``stream``:
@@ -6,6 +7,11 @@ The functions take torch tensors on one CUDA device and launch the library's ker
 * :func:`window_attention` — a prompt, or the next chunk of one, over its keys: causal, optionally with a sliding
   window and a few first tokens ("sinks") that stay visible;
 * :func:`paged_decode` — one new token per sequence over the pages of its keys and values;
+* :func:`shared_decode` — the same where sequences begin with the same pages: samples of a prompt, questions to a
+  document.  What they share, as :func:`cache_prefixes` finds it, is read once;
+* :func:`rotate` — positions as rotations of queries and keys, by a :class:`Rotary`'s frequencies;
+* :func:`cache_append` — a layer's new tokens on their way: queries and keys turned, keys and values into their pages;
+* :func:`sample` — a token of every row of logits, by temperature, top-k, top-p and min-p, from given uniform numbers;
 * :func:`cache_extend`, :func:`cache_write`, :func:`cache_fork`, :func:`cache_release`, :func:`cache_trim`,
   :func:`cache_compact`, :func:`cache_copy` — the pages themselves.
 
@@ -16,7 +22,7 @@ given ones, which may be the same (not for :func:`cache_fork`).  :class:`PagedCa
 
 A tensor used on another stream than the one it was made on needs ``record_stream`` or an event, as any torch tensor;
 what a call with ``stream`` returns was made on that one.
-The waits inside the prompt form's kernel are bounded.  One that runs out (a fault of the machine) leaves outputs
+The waits inside the kernels of the prompt form and of shared prefixes are bounded.  One that runs out (a fault of the machine) leaves outputs
 unwritten; ``runtime.call("lc_device_status", stream)`` tells of it, as :meth:`PagedCache.check` does.
 
 No operation has a gradient: with grad mode on, an input that requires one is refused.
