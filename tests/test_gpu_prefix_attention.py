@@ -257,6 +257,17 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_leaders_that_are_none():
+    """A plan whose leaders are no slots shares nothing."""
+    k, v, maps, prefixes = cache([(2000, [5, 30, 77] * 6)], 16, 2, 64, "f16")
+    q = queries(18, 8, 64, "f16")
+    want = S.paged_decode(q, k, v, maps.table, maps.lens).float()
+    for no in (-1, 18, 1 << 30):
+        plan = S.CachePrefixes(torch.full_like(prefixes.leader, no), torch.full_like(prefixes.shared, 1 << 30), torch.full_like(prefixes.order, no))
+        got = S.shared_decode(q, k, v, maps.table, maps.lens, plan).float()
+        assert (got - want).abs().max() <= 2.0 ** -10 * want.abs().max()  # each is off by a rounding, its sums by less
+
+
 def test_refusals():
     k, v, maps, prefixes = cache([(300, [5, 30])], 16, 2, 64, "f16")
     q = queries(2, 8, 64, "f16")
