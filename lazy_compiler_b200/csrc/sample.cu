@@ -25,8 +25,8 @@
 // Bound by instructions: the pass for the total takes some 10 operations in f64 and 20 others an
 // element (measured by itself, 4 elements a clock and SM, 34 us of 256 rows of 151643), the list
 // chains of sums over the CTA; by latencies for few rows. Measured: one row of 32000, f16, top-k and
-// top-p 10 us a call; in a graph, 64 rows of 50257, bf16: top-k 25, top-p 33; 256 rows of 151643,
-// f32: largest only 31 (5 TB/s), top-k 73, top-p of 0.9 107, of 0.99 252, nothing cut 99.
+// top-p 9 us a call; in a graph, 64 rows of 50257, bf16: top-k 17, top-p 24; 256 rows of 151643,
+// f32: largest only 31 (5 TB/s), top-k 73, top-p of 0.9 107, of 0.99 249, nothing cut 99.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -440,10 +440,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     // ---- 2: what reaches the threshold, and the total
     const bool sums = nucleus && !top_k;
     auto list = [&](int v, const float (&x)[E], float from, float to) {  // logits from .. to
-      float most = x[0];
+      bool some = false;
 #pragma unroll
-      for (int e = 1; e < E; ++e) most = fmaxf(most, x[e]);
-      if (most >= from && *(volatile int *)&s.listed <= kList) {  // (not all of a flat row)
+      for (int e = 0; e < E; ++e) some |= x[e] >= from && x[e] <= to;
+      if (some && *(volatile int *)&s.listed <= kList) {  // (not all of a flat row)
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (x[e] >= from && x[e] <= to && x[e] > -INFINITY) {
@@ -678,13 +678,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         // the first step that may hold the cut, and the first by which it is surely reached: f32's sums of weights are
         // off by 4e-6 or less (40 additions one after the other, and a difference), its counts are exact
         const float need = sums ? (float)((double)(under ? want_sum - inside : want_sum) * (double)unit) : (float)top_k, off = sums ? 1e-5f : 0.f;
+        uint32_t from = UINT32_MAX, to = UINT32_MAX;
 #pragma unroll
         for (int x = 0; x < kOwn; ++x) {
           run[0] += amounts[0][x];
           run[1] += amounts[1][x];
-          if (n[x] && run[1] * (1 + off) >= need) atomicMin(&s.found, tid * kOwn + x);
-          if (n[x] && run[0] * (1 - off) >= need) atomicMin(&s.found_end, tid * kOwn + x);
+          if (n[x] && run[1] * (1 + off) >= need) from = min(from, tid * kOwn + x);
+          if (n[x] && run[0] * (1 - off) >= need) to = min(to, tid * kOwn + x);
         }
+        from = __reduce_min_sync(0xffffffffu, from);
+        to = __reduce_min_sync(0xffffffffu, to);
+        if (lane == 0 && from != UINT32_MAX) atomicMin(&s.found, from);
+        if (lane == 0 && to != UINT32_MAX) atomicMin(&s.found_end, to);
         __syncthreads();
         const uint32_t step_from = s.found, step_to = s.found_end;
         if (step_from == UINT32_MAX && !sums) {
