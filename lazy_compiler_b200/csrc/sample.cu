@@ -18,7 +18,8 @@
 // Where the list does not hold what may be kept, the cut is looked for first: a histogram of
 // counts over 4096 equal steps of the logits, the steps that the cut may lie in (a step's weights
 // are nearly one), and the list is of those, with the exact sums of what lies above them; where even
-// they hold too many (equal logits), histograms of counts and weights over the keys, down to one.
+// they hold too many (equal logits), histograms of counts and weights over the keys, down to one. (Top-k with
+// top-p lists the k and the rest of the last of their steps, and takes 3: 256 rows of 151643, 591 -> 195 us.)
 // Then, and where nothing is cut: the sums of the warps' runs, and the run that holds the token
 // again, element by element.  Equal logits are taken in index order throughout.
 //
@@ -162,7 +163,7 @@ struct alignas(16) SampleShared {
       };
     } list;
     struct {
-      uint32_t count[kBins], low[kBins], high[kBins];
+      uint32_t count[kBins], low[kBins], high[kBins];  // (high follows low: add_word)
     } bins;
   };
   struct Part {
@@ -240,6 +241,14 @@ __device__ __forceinline__ void add_words(Word (&to)[N], const uint32_t *from) {
     const uint4 v = *reinterpret_cast<const uint4 *>(from + x);
     to[x] += v.x, to[x + 1] += v.y, to[x + 2] += v.z, to[x + 3] += v.w;
   }
+}
+
+// Adds to 64 bits in shared memory, the upper half `high` words behind the lower: by halves, since a 64-bit addition
+// there is a loop that tries until no other thread comes between.
+__device__ __forceinline__ void add_word(uint32_t *low, int high, uint64_t w) {
+  const uint32_t add = (uint32_t)w, old = atomicAdd(low, add);
+  const uint32_t up = (uint32_t)(w >> 32) + (old + add < old);
+  if (up) atomicAdd(low + high, up);
 }
 
 template <class T>
@@ -367,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           reach = mid;
         else
           hi = mid - 1;
-        if (n >= wanted && n <= wanted + wanted / 4 + 2) break;
+        if (n >= wanted && n <= wanted + wanted / 16 + 2) break;  // (of half the threads: some 1600 elements, of 2048 there is room for)
       }
     }
     if (tid < ctas) {
@@ -552,218 +561,229 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     auto one = [](int) -> uint64_t { return 1; };
     auto weight = [&](int x) -> uint64_t { return w[x]; };
 
-    if (all <= kList && (!sums || inside >= want_sum)) {
-      // ---- 3
-      if (rank != 0) return;
-      gather();
-      if (tid >= threads) return;
-      if (top_k && top_k < all) cut_list(top_k, one);
-      uint64_t sum = 0;
-      if (nucleus) {
-        if (top_k) {
+    bool found = false;
+    for (bool again = false;;) {  // once, or once more with another list
+      if (all <= kList && (!sums || inside >= want_sum) && (!again || all >= top_k)) {
+        // ---- 3
+        if (rank != 0) return;
+        gather();
+        if (tid >= threads) return;
+        if (top_k && top_k < all) cut_list(top_k, one);
+        uint64_t sum = 0;
+        if (nucleus) {
+          if (top_k) {
 #pragma unroll
-          for (int x = 0; x < kListed; ++x) sum += kept[x] ? w[x] : 0;
-          sum = totals(sum).sum;
+            for (int x = 0; x < kListed; ++x) sum += kept[x] ? w[x] : 0;
+            sum = totals(sum).sum;
+          }
+          cut_list(reached(top_p, sums ? row_total : sum), weight);
         }
-        cut_list(reached(top_p, sums ? row_total : sum), weight);
-      }
-      sum = 0;
-      uint32_t n = 0;
-#pragma unroll
-      for (int x = 0; x < kListed; ++x) {
-        kept[x] = kept[x] && value_of(key[x]) >= least;
-        sum += kept[x] ? w[x] : 0;
-        n += kept[x];
-      }
-      const Sum left = totals(sum, n);
-      const uint64_t target = passed(uniform, left.sum);
-      n = left.count;
-      int lo = 0, hi = p.vocab - 1;
-      while (n > 1) {  // the token is one of the n in lo .. hi
-        const int mid = lo + (hi - lo) / 2;
         sum = 0;
-        uint32_t lower = 0;
+        uint32_t n = 0;
+#pragma unroll
+        for (int x = 0; x < kListed; ++x) {
+          kept[x] = kept[x] && value_of(key[x]) >= least;
+          sum += kept[x] ? w[x] : 0;
+          n += kept[x];
+        }
+        const Sum left = totals(sum, n);
+        const uint64_t target = passed(uniform, left.sum);
+        n = left.count;
+        int lo = 0, hi = p.vocab - 1;
+        while (n > 1) {  // the token is one of the n in lo .. hi
+          const int mid = lo + (hi - lo) / 2;
+          sum = 0;
+          uint32_t lower = 0;
+#pragma unroll
+          for (int x = 0; x < kListed; ++x)
+            if (kept[x] && index[x] <= mid) sum += w[x], lower += index[x] >= lo;
+          const Sum t = totals(sum, lower);
+          if (t.sum > target)
+            hi = mid, n = t.count;
+          else
+            lo = mid + 1, n -= t.count;
+        }
 #pragma unroll
         for (int x = 0; x < kListed; ++x)
-          if (kept[x] && index[x] <= mid) sum += w[x], lower += index[x] >= lo;
-        const Sum t = totals(sum, lower);
-        if (t.sum > target)
-          hi = mid, n = t.count;
-        else
-          lo = mid + 1, n -= t.count;
+          if (kept[x] && index[x] >= lo && index[x] <= hi) answer(index[x], value_of(key[x]), left.sum);
+        return;
       }
-#pragma unroll
-      for (int x = 0; x < kListed; ++x)
-        if (kept[x] && index[x] >= lo && index[x] <= hi) answer(index[x], value_of(key[x]), left.sum);
-      return;
-    }
 
-    bool found = false;
-    if (!(top_k && nucleus)) {
-      // ---- the steps of the logits that the cut may lie in: by weights below the list, if there is one, down to
-      // where weights are nothing
-      const bool under = sums && all <= kList;
-      for (int x = lane; x < ctas * kWarps; x += 32) lowest = fminf(lowest, value_of((uint32_t)s.first[x] ^ 0x80000000u));
-      lowest = value_of(__reduce_min_sync(0xffffffffu, key_of(lowest)));
-      const float range_hi = under ? threshold : largest;
-      const float range_lo = fmaxf(lowest, largest - (float)((p.scale + 2) * kLn2 * (double)temperature));
-      const float step = (range_hi - range_lo) / kSteps, per_step = kSteps / (range_hi - range_lo);
-      const float range_to = under ? range_hi : INFINITY;  // the largest is at range_hi, and counts
-      float lo = range_lo, hi = range_hi;
-      if (step > 0.f && step < 1e30f && per_step < 1e30f) {
-        cluster.sync();  // the list has been read
-        for (int b = tid; b < kSteps; b += kThreads) s.list.count[b] = 0;
-        if (tid == 0) s.found = s.found_end = UINT32_MAX, s.listed = 0;
-        __syncthreads();
-        row.template each<U>([&](int, const float (&x)[E]) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const int b = min(kSteps - 1, (int)((range_hi - x[e]) * per_step));
-            if (x[e] >= range_lo && x[e] < range_to) atomicAdd(&s.list.count[b], 1u);
-          }
-        });
-        if (ctas > 1) {
-          // A CTA adds up its part of the steps, for all of them (each reading all of eight took 21000 cycles).
-          cluster.sync();
-          for (int x = tid; x < kSteps / 4 / ctas; x += kThreads) {
-            const int at = rank * (kSteps / ctas) + 4 * x;
-            uint32_t n[4] = {0};
-#pragma unroll
-            for (int c = 0; c < kMostCtas; ++c)
-              if (c < ctas) add_words(n, other(c).list.count + at);
-#pragma unroll
-            for (int c = 0; c < kMostCtas; ++c)
-              if (c < ctas) *reinterpret_cast<uint4 *>(other(c).list.count + at) = make_uint4(n[0], n[1], n[2], n[3]);
-          }
-        }
-        cluster.sync();
-        // A thread's consecutive steps: their elements, and the least and the most that their weights (of the
-        // largest's) may come to: of the steps' edges, a little wider for the rounding of a step's number, of
-        // the exponential and of the weights.
-        constexpr int kOwn = kSteps / kThreads;
-        uint32_t n[kOwn] = {0};
-        add_words(n, s.list.count + tid * kOwn);
-        const float unit = exp2f(-(float)p.scale), octaves = (float)(weights.factor / 32);
-        const float wider = exp2f(0.01f * step * octaves) * (1 + 1e-4f);
-        float amounts[2][kOwn];
-        float edge = exp2f(fminf(0.f, (range_hi - (float)(tid * kOwn) * step - largest) * octaves));
-#pragma unroll
-        for (int x = 0; x < kOwn; ++x) {
-          const float next = exp2f(fminf(0.f, (range_hi - (float)(tid * kOwn + x + 1) * step - largest) * octaves));
-          amounts[0][x] = sums ? n[x] * fmaxf(0.f, next / wider - unit) : n[x];
-          amounts[1][x] = sums ? n[x] * (edge * wider + unit) : n[x];
-          edge = next;
-        }
-        float run[2];
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-          float mine = 0.f;
-#pragma unroll
-          for (int x = 0; x < kOwn; ++x) mine += amounts[side][x];
-          run[side] = mine;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const float up = __shfl_up_sync(0xffffffffu, run[side], o);
-            if (lane >= o) run[side] += up;
-          }
-          if (lane == 31) s.scan_steps[side][warp] = run[side];
-          run[side] -= mine;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < kWarps; ++x) {
-          run[0] += x < warp ? s.scan_steps[0][x] : 0.f;
-          run[1] += x < warp ? s.scan_steps[1][x] : 0.f;
-        }
-        // the first step that may hold the cut, and the first by which it is surely reached: f32's sums of weights are
-        // off by 4e-6 or less (40 additions one after the other, and a difference), its counts are exact
-        const float need = sums ? (float)((double)(under ? want_sum - inside : want_sum) * (double)unit) : (float)top_k, off = sums ? 1e-5f : 0.f;
-        uint32_t from = UINT32_MAX, to = UINT32_MAX;
-#pragma unroll
-        for (int x = 0; x < kOwn; ++x) {
-          run[0] += amounts[0][x];
-          run[1] += amounts[1][x];
-          if (n[x] && run[1] * (1 + off) >= need) from = min(from, tid * kOwn + x);
-          if (n[x] && run[0] * (1 - off) >= need) to = min(to, tid * kOwn + x);
-        }
-        from = __reduce_min_sync(0xffffffffu, from);
-        to = __reduce_min_sync(0xffffffffu, to);
-        if (lane == 0 && from != UINT32_MAX) atomicMin(&s.found, from);
-        if (lane == 0 && to != UINT32_MAX) atomicMin(&s.found_end, to);
-        __syncthreads();
-        const uint32_t step_from = s.found, step_to = s.found_end;
-        if (step_from == UINT32_MAX && !sums) {
-          found = true;  // fewer than k elements weigh anything: no cut
-        } else if (step_from != UINT32_MAX) {
-          if (step_from > 0) hi = range_hi - ((float)step_from - 0.01f) * step;
-          if (step_to < kSteps - 1) lo = range_hi - ((float)step_to + 1.01f) * step;
-          // the list of lo .. hi, and the sums of what lies above it
-          list_lo = lo, list_hi = hi;
-          cluster.sync();  // the histogram has been read, in whose place lists may arrive
-          uint64_t mine = 0;  // of this warp's run, of those that min_p leaves
-          total = count = 0;
-          row.template each<1>([&](int v, const float (&x)[E]) {
-            list(v, x, lo, hi);
-            float over[E];
-            bool some = false;
+      if (again) break;
+      {
+        // ---- the steps of the logits that the cut may lie in: by weights below the list, if there is one, down to
+        // where weights are nothing
+        const bool under = sums && all <= kList;
+        for (int x = lane; x < ctas * kWarps; x += 32) lowest = fminf(lowest, value_of((uint32_t)s.first[x] ^ 0x80000000u));
+        lowest = value_of(__reduce_min_sync(0xffffffffu, key_of(lowest)));
+        const float range_hi = under ? threshold : largest;
+        const float range_lo = fmaxf(lowest, largest - (float)((p.scale + 2) * kLn2 * (double)temperature));
+        const float step = (range_hi - range_lo) / kSteps, per_step = kSteps / (range_hi - range_lo);
+        const float range_to = under ? range_hi : INFINITY;  // the largest is at range_hi, and counts
+        float lo = range_lo, hi = range_hi;
+        if (step > 0.f && step < 1e30f && per_step < 1e30f) {
+          cluster.sync();  // the list has been read
+          for (int b = tid; b < kSteps; b += kThreads) s.list.count[b] = 0;
+          if (tid == 0) s.found = s.found_end = UINT32_MAX, s.listed = 0;
+          __syncthreads();
+          row.template each<U>([&](int, const float (&x)[E]) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-              const bool is = x[e] > hi;
-              some |= is;
-              count += is;
-              over[e] = is ? x[e] : -INFINITY;
-            }
-            if (!__any_sync(0xffffffffu, some)) return;
-            total += weigh(over);
-            if (least > hi) {
-#pragma unroll
-              for (int e = 0; e < E; ++e) over[e] = over[e] >= least ? over[e] : -INFINITY;
-              mine += weigh(over);
+              const int b = min(kSteps - 1, (int)((range_hi - x[e]) * per_step));
+              if (x[e] >= range_lo && x[e] < range_to) atomicAdd(&s.list.count[b], 1u);
             }
           });
-          if (!(least > hi)) mine = total;
-          mine = warp_total(mine, 0).sum;
-          if (lane == 0) other(0).run_sum[rank * kWarps + warp] = mine;
-          exchange(true, true);
-          if (all <= kList && (sums ? total < want_sum && total + inside >= want_sum : count < (uint64_t)top_k && count + all >= (uint64_t)top_k)) {
-            found = have_runs = true;
-            if (rank == 0) {
-              for (int x = tid; x < ctas * kWarps; x += kThreads) s.runs[x] = s.run_sum[x];
-              gather();
-            }
-            if (rank == 0 && tid < threads) {
-              if (sums)
-                cut_list(want_sum - total, weight);
-              else
-                cut_list(top_k - count, one);
-              // the kept entries join their runs
-#pragma unroll
-              for (int x = 0; x < kListed; ++x)
-                if (kept[x] && value_of(key[x]) >= least) atomicAdd((unsigned long long *)&s.runs[(index[x] + row.skew) / E / per], (unsigned long long)w[x]);
-              // the last of them is the cut
-              uint32_t last = UINT32_MAX;
-#pragma unroll
-              for (int x = 0; x < kListed; ++x)
-                if (kept[x]) last = min(last, key[x]);
-              if (tid == 0) s.found = UINT32_MAX, s.cut_index = -1;
-              totals(0);
-              last = __reduce_min_sync(0xffffffffu, last);
-              if (lane == 0) atomicMin(&s.found, last);
-              totals(0);
-#pragma unroll
-              for (int x = 0; x < kListed; ++x)
-                if (kept[x] && key[x] == s.found) atomicMax(&s.cut_index, index[x]);
-              totals(0);
-              if (tid == 0) s.cut = s.found;
-            }
-            totals.threads = kThreads;
-            totals.turn = 0;  // the others have not taken part
+          if (ctas > 1) {
+            // A CTA adds up its part of the steps, for all of them (each reading all of eight took 21000 cycles).
             cluster.sync();
-            cut = other(0).cut;
-            cut_index = other(0).cut_index;
+            for (int x = tid; x < kSteps / 4 / ctas; x += kThreads) {
+              const int at = rank * (kSteps / ctas) + 4 * x;
+              uint32_t n[4] = {0};
+#pragma unroll
+              for (int c = 0; c < kMostCtas; ++c)
+                if (c < ctas) add_words(n, other(c).list.count + at);
+#pragma unroll
+              for (int c = 0; c < kMostCtas; ++c)
+                if (c < ctas) *reinterpret_cast<uint4 *>(other(c).list.count + at) = make_uint4(n[0], n[1], n[2], n[3]);
+            }
+          }
+          cluster.sync();
+          // A thread's consecutive steps: their elements, and the least and the most that their weights (of the
+          // largest's) may come to: of the steps' edges, a little wider for the rounding of a step's number, of
+          // the exponential and of the weights.
+          constexpr int kOwn = kSteps / kThreads;
+          uint32_t n[kOwn] = {0};
+          add_words(n, s.list.count + tid * kOwn);
+          const float unit = exp2f(-(float)p.scale), octaves = (float)(weights.factor / 32);
+          const float wider = exp2f(0.01f * step * octaves) * (1 + 1e-4f);
+          float amounts[2][kOwn];
+          float edge = exp2f(fminf(0.f, (range_hi - (float)(tid * kOwn) * step - largest) * octaves));
+#pragma unroll
+          for (int x = 0; x < kOwn; ++x) {
+            const float next = exp2f(fminf(0.f, (range_hi - (float)(tid * kOwn + x + 1) * step - largest) * octaves));
+            amounts[0][x] = sums ? n[x] * fmaxf(0.f, next / wider - unit) : n[x];
+            amounts[1][x] = sums ? n[x] * (edge * wider + unit) : n[x];
+            edge = next;
+          }
+          float run[2];
+#pragma unroll
+          for (int side = 0; side < 2; ++side) {
+            float mine = 0.f;
+#pragma unroll
+            for (int x = 0; x < kOwn; ++x) mine += amounts[side][x];
+            run[side] = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const float up = __shfl_up_sync(0xffffffffu, run[side], o);
+              if (lane >= o) run[side] += up;
+            }
+            if (lane == 31) s.scan_steps[side][warp] = run[side];
+            run[side] -= mine;
+          }
+          __syncthreads();
+#pragma unroll
+          for (int x = 0; x < kWarps; ++x) {
+            run[0] += x < warp ? s.scan_steps[0][x] : 0.f;
+            run[1] += x < warp ? s.scan_steps[1][x] : 0.f;
+          }
+          // the first step that may hold the cut, and the first by which it is surely reached: f32's sums of weights are
+          // off by 4e-6 or less (40 additions one after the other, and a difference), its counts are exact
+          const float need = sums ? (float)((double)(under ? want_sum - inside : want_sum) * (double)unit) : (float)top_k, off = sums ? 1e-5f : 0.f;
+          uint32_t from = UINT32_MAX, to = UINT32_MAX;
+#pragma unroll
+          for (int x = 0; x < kOwn; ++x) {
+            run[0] += amounts[0][x];
+            run[1] += amounts[1][x];
+            if (n[x] && run[1] * (1 + off) >= need) from = min(from, tid * kOwn + x);
+            if (n[x] && run[0] * (1 - off) >= need) to = min(to, tid * kOwn + x);
+          }
+          from = __reduce_min_sync(0xffffffffu, from);
+          to = __reduce_min_sync(0xffffffffu, to);
+          if (lane == 0 && from != UINT32_MAX) atomicMin(&s.found, from);
+          if (lane == 0 && to != UINT32_MAX) atomicMin(&s.found_end, to);
+          __syncthreads();
+          const uint32_t step_from = s.found, step_to = s.found_end;
+          if (step_from == UINT32_MAX && !nucleus) {
+            found = true;  // fewer than k elements weigh anything: no cut
+          } else if (step_from != UINT32_MAX) {
+            if (step_from > 0) hi = range_hi - ((float)step_from - 0.01f) * step;
+            if (step_to < kSteps - 1) lo = range_hi - ((float)step_to + 1.01f) * step;
+            // the list of lo .. hi, and the sums of what lies above it
+            list_lo = lo, list_hi = hi;
+            cluster.sync();  // the histogram has been read, in whose place lists may arrive
+            if (nucleus && !sums) {  // the k and what else the last step holds, as a list of another threshold
+              list_hi = largest;
+              row.template each<1>([&](int v, const float (&x)[E]) { list(v, x, lo, INFINITY); });
+              exchange(false, false);
+              again = true;
+              continue;
+            }
+            uint64_t mine = 0;  // of this warp's run, of those that min_p leaves
+            total = count = 0;
+            row.template each<1>([&](int v, const float (&x)[E]) {
+              list(v, x, lo, hi);
+              float over[E];
+              bool some = false;
+#pragma unroll
+              for (int e = 0; e < E; ++e) {
+                const bool is = x[e] > hi;
+                some |= is;
+                count += is;
+                over[e] = is ? x[e] : -INFINITY;
+              }
+              if (!__any_sync(0xffffffffu, some)) return;
+              total += weigh(over);
+              if (least > hi) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) over[e] = over[e] >= least ? over[e] : -INFINITY;
+                mine += weigh(over);
+              }
+            });
+            if (!(least > hi)) mine = total;
+            mine = warp_total(mine, 0).sum;
+            if (lane == 0) other(0).run_sum[rank * kWarps + warp] = mine;
+            exchange(true, true);
+            if (all <= kList && (sums ? total < want_sum && total + inside >= want_sum : count < (uint64_t)top_k && count + all >= (uint64_t)top_k)) {
+              found = have_runs = true;
+              if (rank == 0) {
+                for (int x = tid; x < ctas * kWarps; x += kThreads) s.runs[x] = s.run_sum[x];
+                gather();
+              }
+              if (rank == 0 && tid < threads) {
+                if (sums)
+                  cut_list(want_sum - total, weight);
+                else
+                  cut_list(top_k - count, one);
+                // the kept entries join their runs
+#pragma unroll
+                for (int x = 0; x < kListed; ++x)
+                  if (kept[x] && value_of(key[x]) >= least) add_word(reinterpret_cast<uint32_t *>(&s.runs[(index[x] + row.skew) / E / per]), 1, w[x]);
+                // the last of them is the cut
+                uint32_t last = UINT32_MAX;
+#pragma unroll
+                for (int x = 0; x < kListed; ++x)
+                  if (kept[x]) last = min(last, key[x]);
+                if (tid == 0) s.found = UINT32_MAX, s.cut_index = -1;
+                totals(0);
+                last = __reduce_min_sync(0xffffffffu, last);
+                if (lane == 0) atomicMin(&s.found, last);
+                totals(0);
+#pragma unroll
+                for (int x = 0; x < kListed; ++x)
+                  if (kept[x] && key[x] == s.found) atomicMax(&s.cut_index, index[x]);
+                totals(0);
+                if (tid == 0) s.cut = s.found;
+              }
+              totals.threads = kThreads;
+              totals.turn = 0;  // the others have not taken part
+              cluster.sync();
+              cut = other(0).cut;
+              cut_index = other(0).cut_index;
+            }
           }
         }
       }
+      break;
     }
     if (!found) {
       // ---- histograms of the keys.  First the k-th key by counts, then the run's end by weights.
@@ -790,11 +810,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
               if (!in) continue;
               const uint32_t b = (hi - key) >> shift;
               atomicAdd(&s.bins.count[b], 1u);
-              if (w != 0) {
-                const uint32_t add = (uint32_t)w, old = atomicAdd(&s.bins.low[b], add);
-                const uint32_t up = (uint32_t)(w >> 32) + (old + add < old);
-                if (up) atomicAdd(&s.bins.high[b], up);
-              }
+              if (w != 0) add_word(&s.bins.low[b], kBins, w);
             }
             __syncwarp();
           });
