@@ -633,11 +633,13 @@ __global__ void __launch_bounds__(kMostThreads, 1) prefixes_kernel(PrefixParams 
     }
   }
   cluster.sync();
+  for (int s = tid; s < p.slots; s += blockDim.x) keys[s] = __ldcg(p.leader + s);
+  __syncthreads();
   constexpr int kPiece = 32 * kCompare;
   const int pieces = (p.width + kPiece - 1) / kPiece;
   for (int64_t x = warp; x < (int64_t)p.slots * pieces; x += warps) {
     const int s = (int)(x / pieces), begin = (int)(x - (int64_t)s * pieces) * kPiece;
-    const int leader = __ldcg(p.leader + s);
+    const int leader = keys[s];
     if (leader == s) continue;
     const int end = min(min(full_pages(s), full_pages(leader)), begin + kPiece);
     if (begin == 0 && lane == 0) atomicMin(p.least + leader, full_pages(s));
@@ -653,8 +655,6 @@ __global__ void __launch_bounds__(kMostThreads, 1) prefixes_kernel(PrefixParams 
     if (other < end && lane == 0) atomicMin(p.least + leader, other);
   }
   cluster.sync();
-  for (int s = tid; s < p.slots; s += blockDim.x) keys[s] = __ldcg(p.leader + s);
-  __syncthreads();
   for (int s = warp; s < p.slots; s += warps) {
     int before = 0, members = 0;
     for (int j = lane; j < p.slots; j += 32) {
