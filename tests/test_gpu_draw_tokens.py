@@ -64,6 +64,18 @@ def test_flat_rows(dtype, vocab):
     check(peaked(len(t), vocab, 1, dtype, bulk=1.0, likely=0), uniforms(len(t), 2), t, k, p, m)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(20, 2100), (20, 32000), (3, 151643), (300, 20011)])
+def test_many_likeliest(dtype, rows, vocab):
+    """Top-k around what a list holds, alone and with what comes behind it; rows of one CTA to eight."""
+    k = [255, 256, 257, 511, 512, 513, 1023, 1025, 1500, 1999, 2040, 2047, 2048, 2049, 2090, 5000, vocab - 1]
+    t, p, m = [1.0, 1.3, 0.7, 5.0], [0.9, 1.0, 0.99, 0.5, 0.999], [0.0, 0.0, 1e-3]
+    ask = [[v[i % len(v)] for i in range(rows)] for v in (t, k, p, m)]
+    if rows == 3:
+        ask[1] = [1500, 2040, 700]
+    check(peaked(rows, vocab, 23, dtype), uniforms(rows, 24), *ask)
+
+
 @pytest.mark.parametrize("vocab", [5, 2048, 2500, 40000])
 def test_equal_logits(vocab):
     """Ties go by index: all equal, two values, and a tie where the list or the cut ends."""
