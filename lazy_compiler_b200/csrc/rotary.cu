@@ -291,7 +291,7 @@ extern "C" int lc_rotate(int dtype, const void *x, void *out, const int32_t *pos
   if (int rc = check_rotary(me, dtype, turns, d, rot, magnitude)) return rc;
   if (batch < 0 || tokens < 0 || heads < 0) return fail(LC_ERR_INVALID, "%s: negative size", me);
   if (!strides) return fail(LC_ERR_INVALID, "%s: null strides", me);
-  if (batch > INT32_MAX || tokens > INT32_MAX / 2 || heads * d > (1 << 22)) return fail(LC_ERR_UNSUPPORTED, "%s: shape too large", me);
+  if (batch > INT32_MAX || tokens > INT32_MAX / 2 || heads > (1 << 22) || heads * d > (1 << 22)) return fail(LC_ERR_UNSUPPORTED, "%s: shape too large", me);
   if (batch == 0 || tokens == 0 || heads == 0) return LC_OK;
   if (!x || !out || !positions) return fail(LC_ERR_INVALID, "%s: null buffer", me);
   const int64_t size = dtype == LC_F32 ? 4 : 2, extent[3] = {batch, tokens, heads};
@@ -320,7 +320,7 @@ extern "C" int lc_cache_append(int dtype, const void *q, const void *k, const vo
     return fail(LC_ERR_INVALID, "%s: negative or zero size", me);
   if (!strides) return fail(LC_ERR_INVALID, "%s: null strides", me);
   if (slots > (1 << 20) || most > (1 << 30) || pages > (1 << 30) || page_size > (1 << 20) || width > (1 << 24) ||
-      width * page_size > (1ll << 30) || (q_heads + 2 * kv_heads) * d > (1 << 22))
+      width * page_size > (1ll << 30) || q_heads > (1 << 22) || kv_heads > (1 << 22) || (q_heads + 2 * kv_heads) * d > (1 << 22))
     return fail(LC_ERR_UNSUPPORTED, "%s: shape too large", me);
   if (slots == 0 || most == 0) return LC_OK;
   if (!k || !v || !lens || !add || (q_heads > 0 && (!q || !out)) || (width > 0 && !table) || (pages > 0 && (!k_pages || !v_pages)))

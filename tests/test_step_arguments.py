@@ -71,6 +71,7 @@ UNSUPPORTED = [
     lambda: append(slots=1 << 21), lambda: append(most=1 << 31), lambda: append(width=1 << 25), lambda: append(hq=1 << 20),
     lambda: append(page=1 << 21), lambda: prefixes(slots=8193), lambda: prefixes(width=1 << 30), lambda: sample(rows=1 << 25),
     lambda: sample(vocab=(1 << 24) + 1), lambda: shared(slots=8193), lambda: shared(d=257), lambda: shared(width=1 << 30),
+    lambda: rotate(heads=1 << 62), lambda: append(hq=1 << 62), lambda: append(h=1 << 61),
 ]
 
 
