@@ -14,7 +14,8 @@
 //      that some hundred elements reach, from the lanes' own largest
 //   2  what reaches the threshold goes to a list; where top-p asks for it, the total
 //   3  one CTA has the list in registers and finds the k-th, the end of the run and the token
-//      by bisection of (logit, index) and of the index, each step a sum over the threads
+//      by bisection of (logit, index) and of the index, each step a sum over the threads; of a
+//      short list by looking through all of it
 // Where the list does not hold what may be kept, the cut is looked for first: a histogram of
 // counts over 4096 equal steps of the logits, the steps that the cut may lie in (a step's weights
 // are nearly one), and the list is of those, with the exact sums of what lies above them; where even
@@ -27,7 +28,7 @@
 // element (measured by itself, 4 elements a clock and SM, 34 us of 256 rows of 151643), the list
 // chains of sums over the CTA; by latencies for few rows. Measured: one row of 32000, f16, top-k and
 // top-p 9 us a call; in a graph, 64 rows of 50257, bf16: top-k 17, top-p 24; 256 rows of 151643,
-// f32: largest only 31 (5 TB/s), top-k 73, top-p of 0.9 107, of 0.99 249, nothing cut 99.
+// f32: largest only 31 (5 TB/s), top-k 69, top-p of 0.9 107, of 0.99 249, nothing cut 99.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -45,6 +46,7 @@ constexpr int kMostCtas = 8;
 constexpr int kListed = 4, kList = kListed * kThreads;  // entries of a thread, of the list
 constexpr int kWanted = 256;                             // entries of a list for top-p alone, at least
 constexpr int kFew = 128;                                // threads that a short list is dealt to
+constexpr int kOwnFew = 2;                               // entries of each of them, at which looking through all pays
 constexpr int kBinBits = 11, kBins = 1 << kBinBits;     // of keys
 constexpr int kSteps = 4096;                             // of logits
 constexpr uint32_t kNone = 0x007fffffu;                  // the key of -infinity
@@ -568,6 +570,62 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (rank != 0) return;
         gather();
         if (tid >= threads) return;
+        if (all <= kOwnFew * kFew) {
+          // So few that each thread looks through all of them for what lies before its own: twice, where bisection
+          // takes some twenty sums a cut (in a graph, with this and without; top-k of 50 with top-p of 0.9: 64 rows of
+          // 50257, bf16, 17.0 and 20.1 us, one of 32000 13.3 and 14.4; top-k alone: 16.8 and 17.8, 13.0 and 12.5).
+          struct Entry {
+            uint64_t place, weight;
+          };
+          Entry *entries = reinterpret_cast<Entry *>(s.list.key);  // (the first CTA's own list has gone to in_key)
+          uint64_t place[kOwnFew], before[kOwnFew], sum = 0;
+          int above[kOwnFew];
+          auto look = [&] {
+#pragma unroll
+            for (int x = 0; x < kOwnFew; ++x) {
+              if (x * kFew + tid < all) entries[x * kFew + tid] = {place[x], kept[x] ? w[x] : 0};
+              before[x] = 0, above[x] = 0;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kFew) : "memory");
+#pragma unroll 4
+            for (int i = 0; i < all; ++i) {
+              const Entry e = entries[i];
+#pragma unroll
+              for (int x = 0; x < kOwnFew; ++x)
+                if (e.place > place[x]) before[x] += e.weight, ++above[x];
+            }
+          };
+#pragma unroll
+          for (int x = 0; x < kOwnFew; ++x) place[x] = order_of(x);
+          look();
+          if (top_k) {
+#pragma unroll
+            for (int x = 0; x < kOwnFew; ++x) kept[x] = kept[x] && above[x] < top_k;
+          }
+          if (nucleus) {
+            if (top_k) {
+#pragma unroll
+              for (int x = 0; x < kOwnFew; ++x) sum += kept[x] ? w[x] : 0;
+              sum = totals(sum).sum;
+            }
+            const uint64_t want = reached(top_p, sums ? row_total : sum);
+#pragma unroll
+            for (int x = 0; x < kOwnFew; ++x) kept[x] = kept[x] && before[x] < want;
+          }
+          sum = 0;
+#pragma unroll
+          for (int x = 0; x < kOwnFew; ++x) {
+            kept[x] = kept[x] && value_of(key[x]) >= least;
+            sum += kept[x] ? w[x] : 0;
+            place[x] = (unsigned)(p.vocab - 1 - index[x]);  // now by the index alone
+          }
+          const uint64_t left = totals(sum).sum, target = passed(uniform, left);
+          look();
+#pragma unroll
+          for (int x = 0; x < kOwnFew; ++x)
+            if (kept[x] && before[x] <= target && target - before[x] < w[x]) answer(index[x], value_of(key[x]), left);
+          return;
+        }
         if (top_k && top_k < all) cut_list(top_k, one);
         uint64_t sum = 0;
         if (nucleus) {
